@@ -12,6 +12,10 @@
 // shift per four codes.  Block scales multiply the fp32 sums of 128 k: two TMEM accumulators in turn, the epilogue warps fetch
 // one and add it to registers while the next fills.
 //
+// Rows that are e4m3 themselves (rows_e4m3.cuh, weights and activations in 8 bits) are one column half instead of two, and a block's sum is
+// scaled with the row's scale of that block too; the gated form can leave its result in that form, since a tile's 128 features are
+// one block of scales.
+//
 // The same pipeline carries W8A8 at decode sizes (int8 weights and activations, `kind::i8`, s32 sums; the parts of a cluster
 // are added as integers).
 //
@@ -27,11 +31,13 @@
 // part in its own shared memory and finishes BN / cluster tokens from all parts.
 #include "gemm_common.cuh"
 
-#include <cuda_fp8.h>
+#include "rows_e4m3.cuh"
+
+#include <cstddef>
 
 namespace xft {
 
-enum { kSrcFp8 = 0, kSrcU4 = 1, kSrcI8 = 2, kSrcBf16 = 3 };
+enum { kSrcFp8 = 0, kSrcU4 = 1, kSrcI8 = 2, kSrcBf16 = 3, kSrcRows = 4 };
 
 struct E4Params {
   int N, T, K;
@@ -53,6 +59,9 @@ struct E4Params {
   // bf16: a folded RMSNorm (W carries its gain): sums are multiplied with 1 / rms of the rows of rms_x, which is X
   const __nv_bfloat16* rms_x; int rms_ldx; float rms_eps;
   const float* rms_ssq;      // [T] their sums of squares, or null: every CTA adds them up for itself
+  // rows in e4m3: x_scale holds a scale per block of 128 k and row, [K / 128, x_ld]; with out_scale the result leaves in that form
+  // too, codes in `out` and out_scale [N / 128, out_ld] (N a multiple of 128)
+  long long x_ld; float* out_scale; long long out_ld;
   int* status;
 };
 
@@ -101,7 +110,7 @@ struct E4Layout {
   static constexpr bool STACK = DUAL && SRC == kSrcU4 && BN <= 32;
   static constexpr int FEAT = STACK ? 64 : 128;
   static constexpr int NACC = DUAL && !STACK ? 2 : 1;
-  static constexpr int A_BYTES = 128 * 128 * NACC, RAW_BYTES = SRC == kSrcU4 ? 128 * 64 * NACC : 0, B_BYTES = (SRC == kSrcI8 || SRC == kSrcBf16 ? 1 : 2) * BN * 128;
+  static constexpr int A_BYTES = 128 * 128 * NACC, RAW_BYTES = SRC == kSrcU4 ? 128 * 64 * NACC : 0, B_BYTES = (SRC == kSrcI8 || SRC == kSrcBf16 || SRC == kSrcRows ? 1 : 2) * BN * 128;
   static constexpr int STAGE = (SRC == kSrcU4 ? RAW_BYTES : A_BYTES) + B_BYTES;       // what TMA fills
   static constexpr int A_RING = SRC == kSrcU4 ? 2 * A_BYTES : 0;                      // expanded codes, two buffers
   // two CTAs per SM where registers allow: one CTA's last accumulators and stores hide behind the other's stream
@@ -122,7 +131,9 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
   using L = E4Layout<BN, DUAL, SRC>;
   constexpr int NACC = L::NACC, STAGES = L::STAGES, FEAT = L::FEAT, HALVES = DUAL ? 2 : 1;
   constexpr bool STACK = L::STACK;
-  constexpr int NB = SRC == kSrcI8 || SRC == kSrcBf16 ? BN : 2 * BN;   // columns of an accumulator: hi [BN], lo [BN]
+  constexpr bool BLOCKS = SRC == kSrcFp8 || SRC == kSrcRows;           // scales per block of k: a block's sum is fetched and scaled
+  constexpr bool ONE_X = SRC == kSrcI8 || SRC == kSrcBf16 || SRC == kSrcRows;      // no lo half
+  constexpr int NB = ONE_X ? BN : 2 * BN;                              // columns of an accumulator: hi [BN], lo [BN]
   constexpr int ACC = NB * NACC;
   // bf16: k in PARTS pieces with an accumulator each.  The tensor core drops bits below an accumulator's last one at every step, so
   // its error grows with the k it adds up: 12288 x 4096 against 64 bits 2.1e-6 (2 CTAs per tile) and 4.4e-6 (one) of the result with
@@ -131,10 +142,10 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
   // 64 rows fetch an accumulator as soon as its k is through, beside the main loop; fewer rows all at once at the end, where a short
   // stream pays for one wait and not for four.
   constexpr bool EARLY = PARTS > 1 && BN == 64;
-  constexpr int BUFS = SRC == kSrcFp8 ? 2 : PARTS;
+  constexpr int BUFS = BLOCKS ? 2 : PARTS;
   constexpr uint32_t TMEM_COLS = BUFS * ACC < 32 ? 32 : BUFS * ACC;
   static_assert(TMEM_COLS * L::CTAS <= 512, "accumulators of the resident CTAs");
-  constexpr uint32_t IDESC = SRC == kSrcI8 ? umma_idesc(128, BN, 1, 1, 2) : SRC == kSrcBf16 ? umma_idesc(128, BN, 1, 1, 1) : umma_idesc(128, 2 * BN, 0, 0, 1);
+  constexpr uint32_t IDESC = SRC == kSrcI8 ? umma_idesc(128, BN, 1, 1, 2) : SRC == kSrcBf16 ? umma_idesc(128, BN, 1, 1, 1) : umma_idesc(128, NB, 0, 0, 1);
   constexpr int HB = BN / 2;                                           // tokens per thread: two warps share a row of the tile
   constexpr int TILE_A = 128 * 128;
 
@@ -149,6 +160,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
   constexpr int NCOL = SRC == kSrcI8 ? 3 : SRC == kSrcU4 ? 2 : 0, NROW = SRC == kSrcI8 ? 3 : SRC == kSrcBf16 ? 1 : 2;
   __shared__ alignas(16) float s_col[NCOL ? NCOL : 1][NACC][NCOL ? 128 : 4];
   __shared__ float s_row[NROW][BN];
+  __shared__ alignas(16) float s_xs[SRC == kSrcRows ? 8 : 1][SRC == kSrcRows ? BN : 4];      // per warp: two lines of its tokens' scales
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int tile_n, tile_t;
@@ -215,7 +227,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       auto load_x = [&](int s, int kb) {
         uint8_t* st = ring + s * L::STAGE + W_TILE * NACC;
         tma_load_2d(st, &tmX, &full_bar[s], SRC == kSrcBf16 ? kb * 64 : kb * 128, x_row0, kEvictLast);
-        if (SRC != kSrcI8 && SRC != kSrcBf16) tma_load_2d(st + BN * 128, &tmX, &full_bar[s], p.x_lo + kb * 128, x_row0, kEvictLast);
+        if (!ONE_X) tma_load_2d(st + BN * 128, &tmX, &full_bar[s], p.x_lo + kb * 128, x_row0, kEvictLast);
       };
       // weights never depend on the previous kernel: the first round is requested before the grid dependency resolves
       const int pre = min(STAGES, kend - kb0);
@@ -238,17 +250,17 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       int in_part = 0, part = 0;                                       // blocks in this accumulator; which it is
       bool ok = true;
       for (int kb = kb0; kb < kend; ++kb, r.next(STAGES), b.next(2)) {
-        if (SRC == kSrcFp8) ok = mbar_wait(&tmem_empty[b.s], b.ph ^ 1, p.status, XFT_ERR_WAIT_TMEM);
+        if (BLOCKS) ok = mbar_wait(&tmem_empty[b.s], b.ph ^ 1, p.status, XFT_ERR_WAIT_TMEM);
         ok = ok && mbar_wait(&full_bar[r.s], r.ph, p.status, XFT_ERR_WAIT_FULL);
         if (SRC == kSrcU4) ok = ok && mbar_wait(&a_ready[b.s], b.ph, p.status, XFT_ERR_WAIT_FULL);
         if (!ok) break;
         tcgen05_fence_after();
         const uint64_t bd = bdesc0 + (uint64_t)(r.s * (L::STAGE / 16));
         const uint64_t ad = a0 + (uint64_t)(SRC == kSrcU4 ? b.s * (L::A_BYTES / 16) : r.s * (L::STAGE / 16));
-        const uint32_t acc = tmem_base + (SRC == kSrcFp8 ? b.s * ACC : PARTS > 1 ? part * ACC : 0);
+        const uint32_t acc = tmem_base + (BLOCKS ? b.s * ACC : PARTS > 1 ? part * ACC : 0);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {                                  // 4 x 32 k
-          const uint32_t on = (SRC != kSrcFp8 && (PARTS > 1 ? in_part > 0 : kb > kb0)) || k > 0;
+          const uint32_t on = (!BLOCKS && (PARTS > 1 ? in_part > 0 : kb > kb0)) || k > 0;
           auto mma = [&](uint32_t d, uint64_t a) {
             if constexpr (SRC == kSrcBf16) umma_bf16(d, a, bd + 2 * k, IDESC, on);
             else if constexpr (SRC == kSrcI8) umma_i8(d, a, bd + 2 * k, IDESC, on);
@@ -264,9 +276,9 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
           in_part = 0;
         }
         if (SRC == kSrcU4) tcgen05_commit(&a_empty[b.s]);
-        if (SRC == kSrcFp8) tcgen05_commit(&tmem_full[b.s]);
+        if (BLOCKS) tcgen05_commit(&tmem_full[b.s]);
       }
-      if (SRC != kSrcFp8 && !EARLY && kend > kb0 && ok) tcgen05_commit(&tmem_full[0]);
+      if (!BLOCKS && !EARLY && kend > kb0 && ok) tcgen05_commit(&tmem_full[0]);
     }
   }
 
@@ -316,10 +328,10 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       if constexpr (SRC == kSrcBf16) {
         s_row[0][e] = in && p.rms_ssq ? p.rms_ssq[t] : 0.f;
       } else {
-        s_row[0][e] = in ? p.x_scale[t] : 0.f;
+        if constexpr (SRC != kSrcRows) s_row[0][e] = in ? p.x_scale[t] : 0.f;
         if constexpr (SRC == kSrcI8) { s_row[1][e] = in ? p.a_zero[t] : 0.f; s_row[2][e] = in ? p.a_qsum[t] : 0.f; }
         if constexpr (SRC == kSrcU4) s_row[1][e] = in ? p.x_sum[t] : 0.f;
-        if constexpr (SRC == kSrcFp8) s_row[1][e] = in && p.col_scale ? p.col_scale[t] : 1.f;
+        if constexpr (BLOCKS) s_row[1][e] = in && p.col_scale ? p.col_scale[t] : 1.f;
       }
     }
   };
@@ -357,6 +369,47 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&tmem_empty[b.s]);
+      }
+    } else if constexpr (SRC == kSrcRows) {
+      // A block's sum of a token is scaled with the row's scale and the weights': a lane holds the scales of one token, two blocks ahead,
+      // and the warp reads them from a line of shared memory of its own (two lines in turn, so one wait of the warp orders both).
+      grid_dep_wait();
+      fetch_rows();
+      const float* sc = p.scale + (size_t)(w_row0 >> 7) * p.scale_ld;
+      const float* sc_up = sc + (size_t)(p.dual_off >> 7) * p.scale_ld;
+      float* line = s_xs[warp - 2];
+      const bool mine = lane < HB && c0 + lane < x_rows;
+      const float* sx = p.x_scale + x_row0 + c0 + lane;
+      auto scale_of = [&](int kb) { return mine && kb < kend ? __ldg(sx + (size_t)kb * p.x_ld) : 0.f; };
+      float x0 = scale_of(kb0), x1 = scale_of(kb0 + 1);
+      float w0 = kb0 < kend ? __ldg(sc + kb0) : 0.f, u0 = DUAL && kb0 < kend ? __ldg(sc_up + kb0) : 0.f;
+      Ring b = {0, 0};
+      for (int kb = kb0; kb < kend && ok; ++kb, b.next(2)) {
+        if (lane < HB) line[b.s * HB + lane] = x0;
+        const float wf = w0, uf = u0;
+        x0 = x1;
+        x1 = scale_of(kb + 2);
+        if (kb + 1 < kend) { w0 = __ldg(sc + kb + 1); u0 = DUAL ? __ldg(sc_up + kb + 1) : 0.f; }
+        ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[b.s], b.ph, p.status, XFT_ERR_WAIT_TMEM));
+        if (!ok) break;
+        tcgen05_fence_after();
+        uint32_t v[NACC][HB];
+#pragma unroll
+        for (int a = 0; a < NACC; ++a) tmem_ld_cols<HB>(taddr + b.s * ACC + a * NB, v[a]);
+        tmem_ld_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tmem_empty[b.s]);
+#pragma unroll
+        for (int j = 0; j < HB; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(line + b.s * HB + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float s = (&f.x)[i];
+            g[0][j + i] = fmaf(s * wf, __uint_as_float(v[0][j + i]), g[0][j + i]);
+            if constexpr (DUAL) g[NACC - 1][j + i] = fmaf(s * uf, __uint_as_float(v[NACC - 1][j + i]), g[NACC - 1][j + i]);
+          }
+        }
       }
     } else if constexpr (SRC == kSrcI8 || SRC == kSrcBf16) {
       grid_dep_wait();
@@ -564,7 +617,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
           else x = act_of(value(x, 0, b), p.act, 1.f);
           if (p.residual) x += p.res_scale * r;
         } else {
-          const float st = s_row[0][c];
+          const float st = SRC == kSrcRows ? 1.f : s_row[0][c];
           if constexpr (SRC == kSrcU4) {
             const float xs = s_row[1][c];
             x = act_of(fmaf(x, st * s_col[0][0][f0 + f], b + s_col[1][0][f0 + f] * xs), p.act, 1.f);
@@ -578,6 +631,20 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
           if (p.residual) x += p.res_scale * r;
         }
         out[f] = x;
+      }
+      if constexpr (SRC == kSrcRows) {
+        if (p.out_scale) {                                             // the warp has a block of 128 features of this token
+          float top = 0.f;
+#pragma unroll
+          for (int f = 0; f < 4; ++f) top = e4m3_top(top, out[f]);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const E4m3Scale s = e4m3_scale(top);
+          reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + t * p.ldo)[n >> 2] =
+              e4m3_codes(out[0], out[1], s.inv) | e4m3_codes(out[2], out[3], s.inv) << 16;
+          if (lane == 0) p.out_scale[(size_t)tile_n * p.out_ld + t] = s.scale;
+          continue;
+        }
       }
       if (p.out_fp32) {
         float* to = reinterpret_cast<float*>(p.out) + t * p.ldo + n;
@@ -813,6 +880,55 @@ extern "C" int xft_gemm_e4m3(const void* xs, int x_rows, const float* x_scale, c
     return gated ? launch_e4<BN_, true, kSrcFp8>(tmW, tmX, p, st) : launch_e4<BN_, false, kSrcFp8>(tmW, tmX, p, st);
   switch (bn) { XFT_E4(16) XFT_E4(32) XFT_E4(64) }
 #undef XFT_E4
+  return -1;
+}
+
+// Size and field offsets of RowsGemm, for the layout check of the Python mirror.
+extern "C" int xft_rows_gemm_layout(long long* out, int n) {
+  const long long v[] = {sizeof(RowsGemm),             offsetof(RowsGemm, x),          offsetof(RowsGemm, x_scale),
+                         offsetof(RowsGemm, w),        offsetof(RowsGemm, w_scale),    offsetof(RowsGemm, out),
+                         offsetof(RowsGemm, out_scale), offsetof(RowsGemm, bias),      offsetof(RowsGemm, residual),
+                         offsetof(RowsGemm, group_tiles), offsetof(RowsGemm, num_group_tiles), offsetof(RowsGemm, col_scale),
+                         offsetof(RowsGemm, status),   offsetof(RowsGemm, x_ld),       offsetof(RowsGemm, out_ld),
+                         offsetof(RowsGemm, x_rows),   offsetof(RowsGemm, ldx),        offsetof(RowsGemm, w_rows),
+                         offsetof(RowsGemm, ldw),      offsetof(RowsGemm, scale_ld),   offsetof(RowsGemm, T),
+                         offsetof(RowsGemm, N),        offsetof(RowsGemm, K),          offsetof(RowsGemm, ldo),
+                         offsetof(RowsGemm, out_fp32), offsetof(RowsGemm, ldr),        offsetof(RowsGemm, act),
+                         offsetof(RowsGemm, gated),    offsetof(RowsGemm, dual_off),   offsetof(RowsGemm, group_w_rows),
+                         offsetof(RowsGemm, max_tiles), offsetof(RowsGemm, bn),        offsetof(RowsGemm, res_scale)};
+  const int m = (int)(sizeof(v) / sizeof(v[0]));
+  for (int i = 0; i < m && i < n; ++i) out[i] = v[i];
+  return m;
+}
+
+// Y = epi(rows · W^T) of e4m3 rows and weights, a scale for each 128 columns of a row ([K / 128, x_ld]) and each 128 x 128 block of W.
+// gated: act(gate) * up of gate rows [0, N) and up rows from dual_off on.  out_scale: the result in e4m3 with scales [N / 128, out_ld].
+// Grouped: tiles of `bn` rows as in xft_qgemm_grouped.
+extern "C" int xft_gemm_rows_e4m3(const RowsGemm* args, cudaStream_t st) {
+  const RowsGemm& a = *args;
+  if (a.T <= 0 || a.N <= 0 || a.K <= 0) return 0;
+  if ((a.ldx & 15) || (a.ldw & 15) || (reinterpret_cast<uintptr_t>(a.x) & 15) || (reinterpret_cast<uintptr_t>(a.w) & 15)) return -2;
+  if ((a.gated && (a.dual_off & 127)) || (a.group_tiles && (a.group_w_rows & 127))) return -4;
+  if (a.out_scale && ((a.N & 127) || (a.ldo & 15) || (reinterpret_cast<uintptr_t>(a.out) & 15) || a.residual || a.col_scale)) return -5;
+  E4Params p{};
+  p.N = a.N; p.T = a.T; p.K = a.K; p.dual_off = a.dual_off; p.out = a.out; p.ldo = a.ldo; p.out_fp32 = a.out_fp32; p.bias = a.bias;
+  p.residual = (const __nv_bfloat16*)a.residual; p.ldr = a.ldr; p.res_scale = a.res_scale; p.act = a.act; p.x_scale = a.x_scale;
+  p.x_ld = a.x_ld; p.scale = a.w_scale; p.scale_ld = a.scale_ld; p.status = a.status; p.col_scale = a.col_scale;
+  p.out_scale = a.out_scale; p.out_ld = a.out_ld;
+  p.group_tiles = reinterpret_cast<const int4*>(a.group_tiles); p.num_group_tiles = a.num_group_tiles; p.group_w_rows = a.group_w_rows;
+  const int bn = a.group_tiles ? a.bn : a.T <= 16 ? 16 : a.T <= 32 ? 32 : 64;
+  p.num_kb = (a.K + 127) / 128;
+  p.n_tiles = (a.N + 127) / 128;
+  p.t_tiles = a.group_tiles ? a.max_tiles : (a.T + bn - 1) / bn;
+  CUtensorMap tmW, tmX;
+  int r = make_tensor_map(&tmW, a.w, (uint64_t)a.w_rows, (uint64_t)a.K, (uint64_t)a.ldw, 128, 1);
+  if (r) return 1000 - r;
+  r = make_tensor_map(&tmX, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, (uint64_t)a.ldx, (uint32_t)bn, 1);
+  if (r) return 2000 - r;
+#define XFT_ROWS(BN_) \
+  case BN_: return a.gated ? launch_e4<BN_, true, kSrcRows>(tmW, tmX, p, st) : launch_e4<BN_, false, kSrcRows>(tmW, tmX, p, st);
+  switch (bn) { XFT_ROWS(16) XFT_ROWS(32) XFT_ROWS(64) }
+#undef XFT_ROWS
   return -1;
 }
 

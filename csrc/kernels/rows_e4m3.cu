@@ -1,0 +1,194 @@
+// Rows on their way into e4m3 products (rows_e4m3.cuh has the form):
+//     h = x + r;  y = h * rsqrt(mean(h^2) + eps) * gain;  codes and scales of y         (norm), or codes and scales of x alone
+// h leaves in bf16 (the stream that goes on, rounded once, and what the norm sees), y on request (a router reads it), codes always.
+//
+// A row stays in registers: x and r are read once, and a block of 128 columns lies with 16 neighbouring threads of eight columns each,
+// so its maximum is four shuffles and only the norm's sum crosses the block.  y is not rounded before its codes are taken.  Bound by
+// bytes where rows are many, by the chain fetch, reduction, store where they are few.
+#include "rows_e4m3.cuh"
+
+namespace xft {
+
+struct RowsE4m3Params {
+  const __nv_bfloat16* x; long long ldx;
+  const void* r; long long ldr;                // bf16 or fp32, or null
+  const float* gain; float eps;                // NORM
+  int K;
+  uint8_t* codes; long long ldc;
+  float* scale; long long lds;                 // [K / 128, lds]
+  __nv_bfloat16* h; long long ldh;             // x + r
+  __nv_bfloat16* y; long long ldy;             // normalised rows, or null
+};
+
+enum { kNoResidual = 0, kResidualBf16 = 1, kResidualFp32 = 2 };
+
+template <int NT, int CH, int RES, bool NORM>
+__global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
+  __shared__ float s_ss[NT / 32];
+  grid_dep_launch();
+  grid_dep_wait();
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x, nch = p.K / 8;
+  uint4 v[CH];
+  const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.ldx);
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = tid + c * NT;
+    v[c] = i < nch ? x[i] : make_uint4(0, 0, 0, 0);
+  }
+  auto pair = [&](int c, int j) { return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&v[c])[j]); };
+  if constexpr (RES != kNoResidual) {
+    float r[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = tid + c * NT;
+      if (i >= nch) continue;
+      if constexpr (RES == kResidualFp32) {
+        const float4* from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.r) + row * p.ldr) + 2 * i;
+        const float4 a = from[0], b = from[1];
+        r[c][0] = a.x; r[c][1] = a.y; r[c][2] = a.z; r[c][3] = a.w; r[c][4] = b.x; r[c][5] = b.y; r[c][6] = b.z; r[c][7] = b.w;
+      } else {
+        const uint4 u = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.r) + row * p.ldr)[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&u)[j]);
+          r[c][2 * j] = f.x; r[c][2 * j + 1] = f.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = tid + c * NT;
+      if (i >= nch) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = pair(c, j);
+        reinterpret_cast<__nv_bfloat162*>(&v[c])[j] = __floats2bfloat162_rn(f.x + r[c][2 * j], f.y + r[c][2 * j + 1]);
+      }
+      reinterpret_cast<uint4*>(p.h + row * p.ldh)[i] = v[c];
+    }
+  }
+  float inv = 1.f;
+  if constexpr (NORM) {
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = pair(c, j);
+        ss += f.x * f.x + f.y * f.y;
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if constexpr (NT > 32) {
+      if ((tid & 31) == 0) s_ss[tid >> 5] = ss;
+      __syncthreads();
+      ss = 0.f;
+#pragma unroll
+      for (int w = 0; w < NT / 32; ++w) ss += s_ss[w];
+    }
+    inv = rsqrtf(__fdiv_rn(ss, (float)p.K) + p.eps);
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = tid + c * NT;
+    float y[8];
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = pair(c, j);
+      y[2 * j] = f.x; y[2 * j + 1] = f.y;
+    }
+    if constexpr (NORM) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+      if (i < nch) { a = __ldg(reinterpret_cast<const float4*>(p.gain) + 2 * i); b = __ldg(reinterpret_cast<const float4*>(p.gain) + 2 * i + 1); }
+      y[0] *= inv * a.x; y[1] *= inv * a.y; y[2] *= inv * a.z; y[3] *= inv * a.w;
+      y[4] *= inv * b.x; y[5] *= inv * b.y; y[6] *= inv * b.z; y[7] *= inv * b.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = e4m3_top(top, y[j]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (i >= nch) continue;
+    const E4m3Scale s = e4m3_scale(top);
+    uint2 q;
+    q.x = e4m3_codes(y[0], y[1], s.inv) | e4m3_codes(y[2], y[3], s.inv) << 16;
+    q.y = e4m3_codes(y[4], y[5], s.inv) | e4m3_codes(y[6], y[7], s.inv) << 16;
+    reinterpret_cast<uint2*>(p.codes + row * p.ldc)[i] = q;
+    if ((i & 15) == 0) p.scale[(i >> 4) * p.lds + row] = s.scale;
+    if constexpr (NORM) {
+      if (p.y) {
+        uint4 u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reinterpret_cast<__nv_bfloat162*>(&u)[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+        reinterpret_cast<uint4*>(p.y + row * p.ldy)[i] = u;
+      }
+    }
+  }
+}
+
+template <int RES, bool NORM>
+static int launch_rows_e4m3(const RowsE4m3Params& p, int rows, cudaStream_t st) {
+  const int nch = p.K / 8;
+  cudaError_t e;
+#define XFT_ROWS_LAUNCH(NT, CH) e = launch_pdl(rows_e4m3_kernel<NT, CH, RES, NORM>, dim3(rows), dim3(NT), 0, st, p)
+  if (nch <= 32) XFT_ROWS_LAUNCH(32, 1);
+  else if (nch <= 64) XFT_ROWS_LAUNCH(64, 1);
+  else if (nch <= 128) XFT_ROWS_LAUNCH(128, 1);
+  else if (nch <= 256) XFT_ROWS_LAUNCH(256, 1);
+  else if (nch <= 512) XFT_ROWS_LAUNCH(256, 2);
+  else if (nch <= 1024) XFT_ROWS_LAUNCH(256, 4);
+  else if (nch <= 2048) XFT_ROWS_LAUNCH(256, 8);
+  else XFT_ROWS_LAUNCH(256, 16);
+#undef XFT_ROWS_LAUNCH
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+// Rows of the experts' products: row r of the output is row src[r] of the input, codes and scales; rows from *used on are left alone.
+__global__ void __launch_bounds__(128) gather_e4m3_kernel(const uint8_t* __restrict__ codes, long long ldc, const float* __restrict__ scale,
+                                                          long long lds, const int* __restrict__ src, const int* __restrict__ used,
+                                                          uint8_t* __restrict__ out, long long ldo, float* __restrict__ out_scale,
+                                                          long long ldos, int K) {
+  grid_dep_launch();
+  grid_dep_wait();
+  const int r = blockIdx.x;
+  if (r >= *used) return;
+  const long long s = src[r];
+  const uint4* from = reinterpret_cast<const uint4*>(codes + s * ldc);
+  uint4* to = reinterpret_cast<uint4*>(out + (long long)r * ldo);
+  for (int i = threadIdx.x; i < (K + 15) / 16; i += 128) to[i] = from[i];
+  for (int i = threadIdx.x; i < (K + 127) / 128; i += 128) out_scale[i * ldos + r] = scale[i * lds + s];
+}
+
+}  // namespace xft
+
+using namespace xft;
+
+// gain null: codes and scales of x [rows, K] (no residual).  K a multiple of 8, at most 32768; rows of x, r, h, y on 16 bytes, rows of
+// codes on 8, gain on 16.  r_kind: 0 none, 1 bf16, 2 fp32.
+extern "C" int xft_rows_e4m3(const void* x, long long ldx, const void* r, long long ldr, int r_kind, const float* gain, float eps, int rows,
+                             int K, void* codes, long long ldc, float* scale, long long lds, void* h, long long ldh, void* y,
+                             long long ldy, cudaStream_t st) {
+  if (rows <= 0) return 0;
+  if (K <= 0 || (K & 7) || K > 32768 || (ldx & 7) || (ldc & 7) || (ldh & 7) || (ldy & 7) || (ldr & (r_kind == 2 ? 3 : 7)) ||
+      (r_kind && (!r || !h || !gain)) ||
+      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(r) | reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(h) |
+        reinterpret_cast<uintptr_t>(y)) & 15) || (reinterpret_cast<uintptr_t>(codes) & 7))
+    return -1;
+  RowsE4m3Params p{};
+  p.x = (const __nv_bfloat16*)x; p.ldx = ldx; p.r = r; p.ldr = ldr; p.gain = gain; p.eps = eps; p.K = K; p.codes = (uint8_t*)codes; p.ldc = ldc;
+  p.scale = scale; p.lds = lds; p.h = (__nv_bfloat16*)h; p.ldh = ldh; p.y = (__nv_bfloat16*)y; p.ldy = ldy;
+  if (!gain) return launch_rows_e4m3<kNoResidual, false>(p, rows, st);
+  if (r_kind == 0) return launch_rows_e4m3<kNoResidual, true>(p, rows, st);
+  return r_kind == 1 ? launch_rows_e4m3<kResidualBf16, true>(p, rows, st) : launch_rows_e4m3<kResidualFp32, true>(p, rows, st);
+}
+
+// Rows of codes on 16 bytes, and as long as K rounded up to 16.
+extern "C" int xft_gather_e4m3(const void* codes, long long ldc, const float* scale, long long lds, const int* src, const int* used,
+                               int max_rows, int K, void* out, long long ldo, float* out_scale, long long ldos, cudaStream_t st) {
+  if (max_rows <= 0) return 0;
+  if (K <= 0 || (ldc & 15) || (ldo & 15) || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
+  const cudaError_t e = launch_pdl(gather_e4m3_kernel, dim3(max_rows), dim3(128), 0, st, (const uint8_t*)codes, ldc, scale, lds, src, used,
+                                   (uint8_t*)out, ldo, out_scale, ldos, K);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}

@@ -12,6 +12,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import reference as R
+from .rows import BLOCK as _BLOCK, RowsE4M3
 
 _native = None
 
@@ -87,13 +88,15 @@ def _timed(kernel: str, x, W, fn):
 
 
 def linear(x, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=None, times=None, out=None):
-    """act(x W^T + bias) + res_scale * residual, or with `times` [T, out] act(x W^T + bias) * times.  `out`: rows to write
-    into.  act "softcap": res_scale * tanh(. / res_scale)."""
+    """act(x W^T + bias) + res_scale * residual, or with `times` [T, out] act(x W^T + bias) * times.  x may be rows in e4m3 where W is
+    (see linear_e4m3).  `out`: rows to write into.  act "softcap": res_scale * tanh(. / res_scale)."""
     if out is not None:
         assert residual is None and times is None
         return (_nat() if _cuda(x) else R).linear_into(x, W, bias, act, out)
     if times is not None:
         return (_nat() if _cuda(x) else R).linear_times(x, W, bias, act, times)
+    if isinstance(x, RowsE4M3):
+        return linear_e4m3(x, W, bias, act, residual, res_scale, out_dtype)
     if _verbose():
         name = "gemm" + ("_bias" if bias is not None else "") + (f"_{act}" if act else "") + \
             ("_residual" if residual is not None else "")
@@ -120,7 +123,14 @@ def linear_rms(x, W, eps, bias=None, act=None, gated=False, out_dtype=None):
 
 
 def norm_linear(x, gain, eps, W, bias=None, act=None, gated=False):
-    """RMSNorm(x; gain) @ W^T: as rmsnorm and linear (or linear_gated) after each other, in fewer launches where the rows are quantised."""
+    """RMSNorm(x; gain) @ W^T: as rmsnorm and linear (or linear_gated) after each other, in fewer launches where the rows are quantised.
+    Weights of kind "fp8a" give the gated form in e4m3 (RowsE4M3) where its halves have a multiple of 128 rows."""
+    if W.kind == "fp8a":
+        q = rmsnorm_e4m3(x, gain, eps)[0]
+        if gated and W.out_features % (2 * _BLOCK) == 0:
+            return linear_gated_e4m3(q, W, act, bias)
+        y = linear_e4m3(q, W, bias, None if gated else act)
+        return gated_act(y, act) if gated else y
     if _verbose() or not _cuda(x):
         h = rmsnorm(x, gain, eps)
         return linear_gated(h, W, act, bias) if gated else linear(h, W, bias, act)
@@ -134,6 +144,130 @@ def linear_gated(x, W, act="silu", bias=None, limit=0.0):
     if _verbose():
         return _timed(f"gemm_gated_{act}", x, W, lambda: impl(x, W, act, bias, limit))
     return impl(x, W, act, bias, limit)
+
+
+# -- 8-bit weights and activations ------------------------------------------------------------
+_ROW_ACTS = (None, "none", "relu", "silu", "gelu", "gelu_tanh", "gelu_new", "gelu_pytorch_tanh", "relu2", "gelu_erf", "tanh", "swiglu")
+
+
+def _native_e4m3():
+    from . import native_e4m3
+    return native_e4m3
+
+
+def _same_device(what, *tensors):
+    d = [t.device for t in tensors if t is not None]
+    if any(x != d[0] for x in d):
+        raise ValueError(f"{what}: tensors on {', '.join(sorted({str(x) for x in d}))}")
+
+
+def _check_rows_e4m3(what, q, W, act):
+    if not isinstance(q, RowsE4M3):
+        raise ValueError(f"{what} multiplies rows in e4m3 (RowsE4M3), not {type(q).__name__}")
+    if W.kind not in ("fp8", "fp8a") or W.block != _BLOCK:
+        raise ValueError(f"{what}: weights are e4m3 with a scale for each block of {_BLOCK}, not {W.kind}")
+    if q.shape[1] != W.in_features:
+        raise ValueError(f"{what}: rows of {q.shape[1]} columns and weights of {W.in_features}")
+    if tuple(W.scale.shape) != (-(-W.out_features // _BLOCK), -(-W.in_features // _BLOCK)):
+        raise ValueError(f"{what}: block scales {tuple(W.scale.shape)} of weights [{W.out_features}, {W.in_features}]")
+    if act not in _ROW_ACTS:
+        raise ValueError(f"{what}: no activation {act!r}")
+
+
+def quantize_e4m3(x) -> RowsE4M3:
+    """Rows x [.., K] in e4m3 with a scale for each 128 columns (`RowsE4M3`, [T, K]): codes e4m3(x * (448 / a)), scales a / 448, a = max
+    |x| of the block, at least 2^-100.  A value that is not finite becomes the code of NaN."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_e4m3: rows of {tuple(x.shape)}")
+    if _cuda(x):
+        return _native_e4m3().rows_e4m3(x)[0]
+    return R.quantize_e4m3(x.reshape(-1, x.shape[-1]))
+
+
+def rmsnorm_e4m3(x, w, eps, residual=None, want_rows=False):
+    """RMSNorm(x + residual) * w on its way into products of 8-bit rows, in one launch: (rows in e4m3, the normalised rows in x's type or
+    None, x + residual or None).  The sum is rounded once, to x's type, and the norm is of what was rounded; codes are taken from the
+    fp32 norm.  `residual`: bf16 or fp32 (CPU: any float type), the shape of x.  `want_rows`: for what reads the norm beside the products."""
+    if x.dim() < 1 or tuple(w.shape) != (x.shape[-1],):
+        raise ValueError(f"rmsnorm_e4m3: gain {tuple(w.shape)} of rows {tuple(x.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"rmsnorm_e4m3: residual {tuple(residual.shape)} of rows {tuple(x.shape)}")
+    _same_device("rmsnorm_e4m3", x, w, residual)
+    if _cuda(x):
+        return _native_e4m3().rows_e4m3(x, w, eps, residual, want_rows)
+    return R.rmsnorm_e4m3(x, w, eps, residual, want_rows)
+
+
+def linear_e4m3(q, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=None):
+    """act(rows W^T + bias) + res_scale * residual of rows in e4m3 and e4m3 weights (kinds "fp8" and "fp8a"): sums of 128 columns are
+    scaled and added in fp32.  `out_dtype`: bf16 or fp32; the activation type of the device by default (bf16 on a GPU)."""
+    _check_rows_e4m3("linear_e4m3", q, W, act)
+    T, N = q.shape[0], W.out_features
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.float32):
+        raise ValueError(f"linear_e4m3: the bias of {N} features is fp32 [{N}], not {tuple(bias.shape)} in {bias.dtype}")
+    if residual is not None and (residual.shape[-1] != N or residual.numel() != T * N):
+        raise ValueError(f"linear_e4m3: residual {tuple(residual.shape)} of a result [{T}, {N}]")
+    if out_dtype not in (None, torch.bfloat16, torch.float32):
+        raise ValueError(f"linear_e4m3: results are bf16 or fp32, not {out_dtype}")
+    _same_device("linear_e4m3", q.codes, W.w, W.scale, bias, residual)
+    if not q.is_cuda:
+        return R.linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype or torch.float32)
+    run = lambda: _native_e4m3().linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
+    return _timed("gemm_e4m3", q, W, run) if _verbose() else run()
+
+
+def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
+    """act(g) * u with (g | u) = rows W^T + bias, as rows in e4m3 for the next product: quantised from fp32, a scale for each 128
+    features.  The two halves of W have a multiple of 128 rows each."""
+    _check_rows_e4m3("linear_gated_e4m3", q, W, act)
+    if W.out_features % (2 * _BLOCK):
+        raise ValueError(f"linear_gated_e4m3: gate and up have a multiple of {_BLOCK} features each, not {W.out_features / 2:g}")
+    if bias is not None and (tuple(bias.shape) != (W.out_features,) or bias.dtype != torch.float32):
+        raise ValueError(f"linear_gated_e4m3: the bias is fp32 [{W.out_features}], not {tuple(bias.shape)} in {bias.dtype}")
+    _same_device("linear_gated_e4m3", q.codes, W.w, W.scale, bias)
+    impl = _native_e4m3().linear_gated_e4m3 if q.is_cuda else R.linear_gated_e4m3
+    return _timed(f"gemm_e4m3_gated_{act}", q, W, lambda: impl(q, W, act, bias)) if _verbose() else impl(q, W, act, bias)
+
+
+def pack_experts_e4m3(experts):
+    """The stacked weights of a list of experts, (gate | up, down) each, that `moe_experts_e4m3` takes as `packed`; made once, the experts'
+    own weights become views of the stacks.  None on a CPU."""
+    if not experts:
+        raise ValueError("pack_experts_e4m3: no experts")
+    for g, d in experts:
+        if any(w.kind not in ("fp8", "fp8a") or w.block != _BLOCK for w in (g, d)):
+            raise ValueError("pack_experts_e4m3: experts' weights are e4m3 with block scales")
+        if d.in_features % _BLOCK or d.out_features % _BLOCK or (g.in_features, g.out_features) != (d.out_features, 2 * d.in_features):
+            raise ValueError(f"pack_experts_e4m3: experts of widths that are multiples of {_BLOCK}, gate and up [2 I, H], down [H, I]; not "
+                             f"[{g.out_features}, {g.in_features}] and [{d.out_features}, {d.in_features}]")
+        if (d.in_features, d.out_features) != (experts[0][1].in_features, experts[0][1].out_features):
+            raise ValueError("pack_experts_e4m3: experts of different sizes")
+    return _native_e4m3().pack_experts(experts) if experts[0][0].w.is_cuda else None
+
+
+def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=None, expected_pairs=None, add=None, out_dtype=torch.float32):
+    """sum_k w[t, k] down_e(act(gate_e q_t) * up_e q_t) (+ `add`, fp32 or bf16) over the local experts e = idx[t, k] - expert_offset of
+    rows in e4m3, the middle rows in e4m3 too; experts outside the list (or -1) add nothing.  `out_dtype`: fp32 or bf16.  Other
+    arguments as in `moe_experts`."""
+    if not isinstance(q, RowsE4M3):
+        raise ValueError(f"moe_experts_e4m3 multiplies rows in e4m3 (RowsE4M3), not {type(q).__name__}")
+    T, H = q.shape
+    if idx.dim() != 2 or idx.shape[0] != T or idx.shape[1] < 1 or idx.shape != w.shape:
+        raise ValueError(f"moe_experts_e4m3: experts {tuple(idx.shape)} and weights {tuple(w.shape)} of {T} rows")
+    if add is not None and (tuple(add.shape) != (T, H) or add.dtype not in (torch.float32, torch.bfloat16)):
+        raise ValueError(f"moe_experts_e4m3: what is added is [{T}, {H}] in fp32 or bf16, not {tuple(add.shape)} in {add.dtype}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"moe_experts_e4m3: results are bf16 or fp32, not {out_dtype}")
+    if act not in _ROW_ACTS:
+        raise ValueError(f"moe_experts_e4m3: no activation {act!r}")
+    if packed is None:
+        packed = pack_experts_e4m3(experts)
+    if experts[0][1].out_features != H:
+        raise ValueError(f"moe_experts_e4m3: rows of {H} columns and experts of {experts[0][1].out_features}")
+    _same_device("moe_experts_e4m3", q.codes, idx, w, add, experts[0][0].w)
+    if not q.is_cuda:
+        return R.moe_experts_e4m3(q, idx, w, experts, act, expert_offset, add, out_dtype)
+    return _native_e4m3().moe_experts_e4m3(q, idx, w, experts, act, expert_offset, packed, expected_pairs, add, out_dtype)
 
 
 def linear_parts(x, W, n, out):
@@ -553,6 +687,8 @@ def route(logits, kind, top_k, bias=None, n_group=1, topk_group=1, routed_scalin
 
 def moe_experts(x, idx, w, experts, act="silu", expert_offset=0, packed=None, expected_pairs=None, gated=True, add=None):
     """Weighted sum of the chosen experts' outputs (see `reference.moe_experts`) in fp32, plus `add` [T, H] fp32."""
+    if gated and experts and experts[0][0].kind == "fp8a":
+        return moe_experts_e4m3(quantize_e4m3(x), idx, w, experts, act, expert_offset, packed, expected_pairs, add)
     if _cuda(x):
         return _nat().moe_experts(x, idx, w, experts, act, expert_offset, packed, expected_pairs, gated, add)
     out = R.moe_experts(x, idx, w, experts, act, expert_offset, gated)

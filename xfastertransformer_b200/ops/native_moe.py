@@ -50,7 +50,7 @@ def pack_experts(experts) -> dict:
     pk = gu0.cache.get("moe_pack")
     if pk is not None and pk["E"] == len(experts) and pk["last"] is experts[-1][0]:
         return pk
-    if all(g.kind == "fp8" and d.kind == "fp8" for g, d in experts) and _fp8_packable(gu0, dn0):
+    if all(g.kind in ("fp8", "fp8a") and d.kind in ("fp8", "fp8a") for g, d in experts) and _fp8_packable(gu0, dn0):
         return _pack_fp8(experts)
     I, H = dn0.in_features, dn0.out_features
     E = len(experts)

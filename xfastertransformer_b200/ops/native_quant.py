@@ -215,6 +215,9 @@ def _w8a8(x, W, rows, bias, act, residual, res_scale, out_dtype, row0=0, norm=No
 def linear(x, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=None, norm=None):
     if W.kind == "w8a8":
         return _w8a8(x, W, W.out_features, bias, act, residual, res_scale, out_dtype, norm=norm)
+    if W.kind == "fp8a":
+        from . import native_e4m3 as E
+        return E.linear_e4m3(E.rows_e4m3(x)[0], W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
     if W.kind in _QT or W.kind in _E4M3:
         return _qgemm(x, W, W.out_features, False, bias, act, residual, res_scale, out_dtype, norm)
     raise N.KernelError(f"no sm_100a GEMM for weight kind {W.kind}")
@@ -233,6 +236,10 @@ def linear_gated(x, W, act="silu", bias=None, norm=None):
                                             N._stream()), "w8a8_gemm_gated")
         ws.launches += 1
         return out
+    if W.kind == "fp8a":
+        from . import native_e4m3 as E
+        q = E.rows_e4m3(x)[0]
+        return N.gated_act(E.linear_e4m3(q, W, bias), act) if I % 128 else E.gated_rows(q, W, act, bias)
     if W.kind == "fp8" and I % 128:
         gu = _qgemm(x, W, 2 * I, False, bias, None, None, 1.0, None)
         return N.gated_act(gu, act)

@@ -15,6 +15,8 @@ from typing import Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
+from .rows import BLOCK, LEAST, TOP, RowsE4M3
+
 # NF4 code book (QLoRA); reference: src/common/normal_float4x2.h
 NF4_CODE = torch.tensor([
     -1.0, -0.6961928009986877, -0.5250730514526367, -0.39491748809814453, -0.28444138169288635,
@@ -168,7 +170,7 @@ def dequant_weight(W) -> torch.Tensor:
         return unpack_nibbles(W.w).float() * W.scale[:, None] + W.zero[:, None]
     if k == "nf4":
         return NF4_CODE.to(W.w.device)[unpack_nibbles(W.w).long()] * W.scale[:, None] + W.zero[:, None]
-    if k == "fp8":
+    if k in ("fp8", "fp8a"):
         o, i = W.w.shape
         b = W.block
         s = W.scale.repeat_interleave(b, 0)[:o].repeat_interleave(b, 1)[:, :i]
@@ -219,6 +221,8 @@ def linear(x: torch.Tensor, W, bias: Optional[torch.Tensor] = None, act: Optiona
     if W.kind == "w8a8":
         q, sa, za = quantize_act_w8a8(x)
         xf = q.float() * sa[..., None] + za[..., None]
+    elif W.kind == "fp8a":
+        xf = quantize_e4m3(x.reshape(-1, x.shape[-1])).values().view(x.shape)
     else:
         xf = x.float()
     y = xf @ dequant_weight(W).t()
@@ -264,6 +268,8 @@ def linear_gated(x: torch.Tensor, W, act: str = "silu", bias: Optional[torch.Ten
     if W.kind == "w8a8":
         q, sa, za = quantize_act_w8a8(x)
         xf = q.float() * sa[..., None] + za[..., None]
+    elif W.kind == "fp8a":
+        xf = quantize_e4m3(x.reshape(-1, x.shape[-1])).values().view(x.shape)
     y = xf @ dequant_weight(W).t()
     if bias is not None:
         y = y + bias.float()
@@ -272,6 +278,56 @@ def linear_gated(x: torch.Tensor, W, act: str = "silu", bias: Optional[torch.Ten
         g, u = y[..., :i].clamp(max=limit), y[..., i:].clamp(-limit, limit)
         return (g * torch.sigmoid(1.702 * g) * (u + 1)).to(x.dtype)
     return (_act(y[..., :i], act) * y[..., i:]).to(x.dtype)
+
+
+# ----------------------------------------------------------------------------------------
+# 8-bit weights and activations: rows in e4m3 with a scale for each 128 columns
+# ----------------------------------------------------------------------------------------
+def quantize_e4m3(y: torch.Tensor) -> RowsE4M3:
+    """Rows y [T, K] as codes e4m3(y * (448 / a)) and scales a / 448, a the block's largest magnitude (at least 2^-100).  A value that
+    is not finite becomes NaN and has no part in a."""
+    T, K = y.shape
+    n = -(-K // BLOCK)
+    b = F.pad(y.float(), (0, n * BLOCK - K)).view(T, n, BLOCK)
+    fine = torch.isfinite(b)
+    a = torch.where(fine, b.abs(), torch.zeros_like(b)).amax(-1).clamp_min(LEAST)
+    inv = torch.full_like(a, TOP) / a                          # one rounding: a number over a tensor would be a reciprocal and a product
+    v = torch.where(fine, (b * inv[..., None]).clamp(-TOP, TOP), torch.full_like(b, float("nan")))
+    return RowsE4M3(v.view(T, -1)[:, :K].to(torch.float8_e4m3fn).contiguous(), (a / TOP).t().contiguous())
+
+
+def rmsnorm_e4m3(x, w, eps, residual=None, want_rows=False):
+    """See `ops.rmsnorm_e4m3`: the normalised row is quantised from fp32, without a rounding in between."""
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    f = h.float()
+    y = f * torch.rsqrt(f.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+    return quantize_e4m3(y.reshape(-1, y.shape[-1])), y.to(x.dtype) if want_rows else None, None if residual is None else h
+
+
+def linear_e4m3(q: RowsE4M3, W, bias=None, act=None, residual=None, res_scale: float = 1.0, out_dtype=torch.float32):
+    y = q.values() @ dequant_weight(W).t()
+    if bias is not None:
+        y = y + bias.float()
+    y = _act(y, act)
+    if residual is not None:
+        y = y + res_scale * residual.reshape(y.shape).float()
+    return y.to(out_dtype)
+
+
+def linear_gated_e4m3(q: RowsE4M3, W, act: str = "silu", bias=None) -> RowsE4M3:
+    y = linear_e4m3(q, W, bias)
+    i = y.shape[-1] // 2
+    return quantize_e4m3(_act(y[:, :i], act) * y[:, i:])
+
+
+def moe_experts_e4m3(q: RowsE4M3, idx, w, experts, act="silu", expert_offset=0, add=None, out_dtype=torch.float32):
+    out = torch.zeros(q.shape[0], experts[0][1].out_features, dtype=torch.float32, device=q.device)
+    for i, (gu, dn) in enumerate(experts):
+        tok, slot = (idx == expert_offset + i).nonzero(as_tuple=True)
+        if tok.numel():
+            h = linear_gated_e4m3(RowsE4M3(q.codes[tok], q.scale[:, tok]), gu, act)
+            out.index_add_(0, tok, linear_e4m3(h, dn) * w[tok, slot].float()[:, None])
+    return (out if add is None else out + add.float()).to(out_dtype)
 
 
 # ----------------------------------------------------------------------------------------

@@ -77,7 +77,8 @@ class LinearWeight:
     kind: bf16|fp16|fp32 (plain), int8|w8a8 (int8 + per-out-channel scale/zero, w = q*s+z;
     w8a8 additionally keeps the row sums for the zero-point correction), int4 / nf4 (two 4-bit
     codes per byte along `in`, low nibble first), fp8 (e4m3 + fp32 scale per 128x128 block,
-    ``scale[out/128, in/128]``).  Reference staging struct: DenseLayerParams
+    ``scale[out/128, in/128]``; activations as they are), fp8a (the same weights, activations in e4m3 too, a scale per row and
+    128 columns: `ops.RowsE4M3`).  Reference staging struct: DenseLayerParams
     (src/common/llm_params.h:21-80).
     """
     kind: str
@@ -149,7 +150,7 @@ def make_linear(w_out_in: torch.Tensor, kind: str, device=None, act_dtype: torch
         else:
             p, s, z = R.quantize_nf4_per_channel(w_out_in)
         return LinearWeight(kind, p, s, z, in_features=p.shape[1] * 2, out_features=o)
-    if kind == "fp8":
+    if kind in ("fp8", "fp8a"):
         if w_out_in.dtype == torch.float8_e4m3fn:
             if scale is None:
                 raise ValueError("fp8 weight needs its block scales")
@@ -165,9 +166,11 @@ def cat_linear(ws: Sequence[LinearWeight]) -> LinearWeight:
     k = ws[0].kind
     assert all(w.kind == k for w in ws)
     cat = lambda name: None if getattr(ws[0], name) is None else torch.cat([getattr(w, name) for w in ws], 0)
-    if k == "fp8":
+    if k in ("fp8", "fp8a"):
         for w in ws[:-1]:
-            assert w.out_features % w.block == 0, "fp8 concat needs 128-aligned out dims"
+            if w.out_features % w.block:
+                raise ValueError(f"e4m3 weights with block scales: {w.out_features} features end inside a block of {w.block}, so no "
+                                 "other weights can follow them")
     return LinearWeight(k, cat("w"), cat("scale"), cat("zero"), cat("wsum"), ws[0].block, ws[0].in_features,
                         sum(w.out_features for w in ws))
 
@@ -238,7 +241,7 @@ class WeightSource:
                 o = sum(e - s for s, e in out_ranges)
             else:
                 o = out_f if out_rng is None else out_rng[1] - out_rng[0]
-            if kind == "fp8" and self.fake != 1:
+            if kind in ("fp8", "fp8a") and self.fake != 1:
                 w = self._fake((o, i), torch.bfloat16, name)
                 return make_linear(w, kind)
             return make_linear(self._fake((o, i), torch.bfloat16 if kind != "fp16" else torch.float16, name), kind)
@@ -279,8 +282,8 @@ class WeightSource:
         self.loaded_bytes += w.numel() + s.numel() * 4
         w = w.to(self.device).view(torch.uint8).t().contiguous().view(torch.float8_e4m3fn)
         s = s.to(self.device).t().contiguous()
-        if kind == "fp8":
-            return make_linear(w, "fp8", scale=s)
+        if kind in ("fp8", "fp8a"):
+            return make_linear(w, kind, scale=s)
         dense = R.dequant_weight(LinearWeight("fp8", w, s, in_features=w.shape[1], out_features=w.shape[0]))
         return make_linear(dense, kind)
 
