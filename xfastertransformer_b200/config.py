@@ -26,6 +26,7 @@ WEIGHT_DTYPES = (
     "fp16", "bf16", "int8", "w8a8", "int4", "nf4",
     "bf16_fp16", "bf16_int8", "bf16_w8a8", "bf16_int4", "bf16_nf4",
     "w8a8_int8", "w8a8_int4", "w8a8_nf4", "fp8_e4m3",
+    "fp8_w8a8",                       # e4m3 weights and activations, a scale per block of 128
     "fp32",                           # everything in 32 bits: layered designs on a GPU, any family on CPU
 )
 KV_DTYPES = ("fp16", "bf16", "int8")
@@ -51,12 +52,12 @@ DENSE_TRAITS = {"dagezen": dict(act="clamped", ff_bias=True)}
 def split_hybrid_dtype(dtype: str) -> Tuple[str, str]:
     """``"bf16_int8"`` -> (prefill dtype, decode dtype); plain names map to themselves.
 
-    ``fp8_e4m3`` contains an underscore but is a single type (reference
+    ``fp8_e4m3`` and ``fp8_w8a8`` contain an underscore but are single types (reference
     ``hybrid_model.h:46-83`` registers only the pairs listed in `WEIGHT_DTYPES`).
     """
     if dtype not in WEIGHT_DTYPES:
         raise ValueError(f"AutoModel don't support {dtype}.")
-    if dtype == "fp8_e4m3" or "_" not in dtype:
+    if dtype in ("fp8_e4m3", "fp8_w8a8") or "_" not in dtype:
         return dtype, dtype
     a, b = dtype.split("_", 1)
     return a, b

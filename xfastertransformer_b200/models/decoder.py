@@ -34,7 +34,7 @@ from ..utils.trace import TimeLine
 from .registry import FamilySpec, family_for
 
 WEIGHT_KIND = {"bf16": "bf16", "fp16": "fp16", "int8": "int8", "w8a8": "w8a8", "int4": "int4", "nf4": "nf4",
-               "fp8_e4m3": "fp8", "fp32": "fp32"}
+               "fp8_e4m3": "fp8", "fp8_w8a8": "fp8a", "fp32": "fp32"}
 
 
 @dataclass
@@ -117,6 +117,7 @@ class Decoder:
         self.first_stage = ctx.pp_rank == 0
         self.last_stage = ctx.pp_rank == ctx.pp_size - 1
         self.pairs_run = 0          # forward_pair calls
+        self._pending = None        # fp32 output of the last experts, which the next norm adds to the stream (see _moe_e4m3)
         self._overlap = False       # True while forward_pair interleaves two batches (all-reduces are started, not awaited)
         self._work = None
 
@@ -286,10 +287,13 @@ class Decoder:
     def _load_mlp_llama(self, L, p, i):
         c = self.cfg
         H, I = c.hidden_size, c.inter_size
-        r = self._ffn_range(I)
-        g = self._lin(p + "mlp.gate_proj", H, I, out_rng=r)
-        u = self._lin(p + "mlp.up_proj", H, I, out_rng=r)
+        r = self._ffn_range(I, 128 if self.kind == "fp8a" else 1)
+        odd = self.kind == "fp8a" and (r[1] - r[0]) % 128 != 0          # up follows gate inside a block of scales: quantised as one matrix
+        g = self._lin(p + "mlp.gate_proj", H, I, out_rng=r, kind="fp32" if odd else None)
+        u = self._lin(p + "mlp.up_proj", H, I, out_rng=r, kind="fp32" if odd else None)
         L.gate_up = cat_linear([g, u])
+        if odd:
+            L.gate_up = make_linear(L.gate_up.w, self.kind)
         L.down = self._lin(p + "mlp.down_proj", I, H, in_rng=r)
         L.act = "gelu" if c.activation_type.startswith("gelu") else c.activation_type
 
@@ -321,7 +325,7 @@ class Decoder:
         if self.ctx.ep_size > 1:
             r = (0, I)
         else:
-            gran = 128 if self.kind == "fp8" else 1
+            gran = 128 if self.kind in ("fp8", "fp8a") else 1
             r = self._ffn_range(I, gran, P.moe_slice_index(self.tpr, self.tp, layer, e, env.moe_split_balance_dim))
         g = self._named_lin(names[0], H, I, out_rng=r)
         u = self._named_lin(names[1], H, I, out_rng=r)
@@ -417,7 +421,7 @@ class Decoder:
         else:
             q = self.src.fp8_linear(p + "self_attn.q_a_proj", H, c.head_num * qk, out_rng=(hs * qk, he * qk),
                                     kind=self.kind)
-            L.qkv_a = cat_linear([q, kv_a]) if (he - hs) * qk % 128 == 0 or self.kind != "fp8" else None
+            L.qkv_a = cat_linear([q, kv_a]) if (he - hs) * qk % 128 == 0 or self.kind not in ("fp8", "fp8a") else None
             L.q_direct, L.kv_a = q, kv_a
             L.q_a_norm = L.q_b = None
         L.kv_a_norm = self.src.vector(p + "self_attn.kv_a_layernorm.weight.bin", kvl, dtype="bf16", fake_ones=True)
@@ -468,7 +472,7 @@ class Decoder:
     # ------------------------------------------------------------------------------------
     def _quantises(self, W) -> bool:
         """Whether the product behind an RMSNorm rewrites its rows as codes, with nothing else reading the normalised state."""
-        return (W is not None and W.kind in ("w8a8", "int4", "fp8") and self.spec.norm == "rms" and not self.spec.resid_from_norm
+        return (W is not None and W.kind in ("w8a8", "int4", "fp8", "fp8a") and self.spec.norm == "rms" and not self.spec.resid_from_norm
                 and Env.get().fuse_norm)
 
     def _norm(self, x, w, b):
@@ -519,7 +523,14 @@ class Decoder:
         h = None
         # the norm in front of a product that quantises its rows goes with that (ops.norm_linear), unless something else reads it
         norm_later = not L.attn_fold and self._quantises(L.qkv_a if s.attention == "mla" else L.qkv)
-        if not L.attn_fold and not norm_later:
+        if self._pending is not None:
+            if norm_later:                # with the experts' output of the layer before, the norm and the codes in one launch
+                with TimeLine("Attention.norm"):
+                    h, _, x = ops.rmsnorm_e4m3(x, L.attn_norm_w, self.eps, self._take_pending())
+                norm_later = False
+            else:
+                x = self._settled(x)
+        if not L.attn_fold and not norm_later and h is None:
             with TimeLine("Attention.norm"):
                 h = self._norm(x, L.attn_norm_w, L.attn_norm_b)
         if s.attention == "mla":
@@ -583,8 +594,11 @@ class Decoder:
         Hl = self.hq
         if ql > 0:
             qa_kv = down(L.qkv_a)                                # [T, ql + kvl + rope]
-            qa = ops.rmsnorm(qa_kv[:, :ql], L.q_a_norm, self.eps)
-            q = ops.linear(qa, L.q_b)
+            if L.q_b.kind == "fp8a":
+                q = ops.norm_linear(qa_kv[:, :ql], L.q_a_norm, self.eps, L.q_b)
+            else:
+                qa = ops.rmsnorm(qa_kv[:, :ql], L.q_a_norm, self.eps)
+                q = ops.linear(qa, L.q_b)
             kv = qa_kv[:, ql:]
         elif L.qkv_a is not None:
             both = down(L.qkv_a)
@@ -608,6 +622,10 @@ class Decoder:
             with TimeLine("LlamaMLP"):
                 g = ops.norm_linear(x, L.mlp_norm_w, self.eps, L.gate_up, None, L.act, gated=True)
                 return self._row_parallel(g, L.down, None, x, 1.0)
+        if k not in ("llama", "gpt") and self.ctx.dp_size == 1 and L.experts and L.experts[0][0].kind == "fp8a" and \
+                self._quantises(L.experts[0][0]):
+            with TimeLine("MoE"):
+                return self._moe_e4m3(L, x)
         with TimeLine("MLP.norm"):
             h = self._norm(x, L.mlp_norm_w, L.mlp_norm_b)
         resid, rs = (h, math.sqrt(2 * self.cfg.num_layer)) if s.resid_from_norm else (x, 1.0)
@@ -698,6 +716,29 @@ class Decoder:
             if L.mlp_kind not in ("llama", "gpt"):
                 self._moe_dp(L, empty, None)
 
+    def _take_pending(self):
+        p, self._pending = self._pending, None
+        return p
+
+    def _settled(self, x):
+        """The stream with what is still to be added to it."""
+        p = self._take_pending()
+        return x if p is None else (x.float() + p).to(x.dtype)
+
+    def _moe_e4m3(self, L: Layer, x):
+        """A layer of routed experts with 8-bit activations: the norm leaves its rows for the router and, in e4m3, for every product.  On one
+        rank their sum stays in 32 bits and joins the stream in the launch of the next layer's norm."""
+        q, h, _ = ops.rmsnorm_e4m3(x, L.mlp_norm_w, self.eps, want_rows=True)
+        idx, w = self._route(L, h)
+        shared = None
+        if getattr(L, "shared", None) is not None:
+            shared = ops.linear_e4m3(ops.linear_gated_e4m3(q, L.shared[0], L.act), L.shared[1], out_dtype=torch.float32)
+        out = ops.moe_experts_e4m3(q, idx, w, L.experts, L.act, L.e0, getattr(L, "packed", None), add=shared)
+        if self.tp == 1 and not self._overlap and not debugger.enabled():
+            self._pending = out
+            return x
+        return self._experts_sum(out, x)
+
     def _moe(self, L: Layer, h, x):
         if self.ctx.dp_size > 1:
             return self._moe_dp(L, h, x)
@@ -714,6 +755,10 @@ class Decoder:
         if getattr(L, "shared", None) is not None:
             g = ops.linear_gated(h, L.shared[0], L.act)
             out = out + ops.linear(g, L.shared[1], out_dtype=torch.float32)
+        return self._experts_sum(out, x)
+
+    def _experts_sum(self, out, x):
+        """The experts' fp32 partial sums with the stream, over the ranks."""
         if self.tpr == 0:
             out = out + x.float()
         if self.tp > 1:
@@ -730,6 +775,7 @@ class Decoder:
         return out.to(x.dtype)
 
     def forward_layers(self, x: torch.Tensor, b: Batch, cache: PagedKVCache) -> torch.Tensor:
+        self._pending = None              # a pass that raised may have left one
         dbg = debugger.enabled()
         step = debugger.next_step() if dbg else 0
         if dbg:
@@ -743,7 +789,7 @@ class Decoder:
                 x = self._mlp(L, x, b)
             if dbg:
                 debugger.dump(f"layer{self.l0 + li}_ffn_out", x, self.ctx.rank, step)
-        return x
+        return self._settled(x)
 
     def _layers_interleaved(self, x: torch.Tensor, b: Batch, cache: PagedKVCache):
         """forward_layers as a generator: after every block whose row-parallel sum was only started, it hands the

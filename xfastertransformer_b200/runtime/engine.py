@@ -79,8 +79,10 @@ class Model:
             raise ValueError("latent attention keeps its cache in the activation type: kv_cache_dtype int8 is not for it")
         if layered and kv_cache_dtype == "int8" and any(m.values_from_keys for l in self.cfg.layers for m in (l.mixer, *l.mixer.parts)):
             raise ValueError("layers whose values are their keys keep them in the activation type: kv_cache_dtype int8 is not for them")
-        if self.cfg.model_type == "deepseek_moe" and d_prefill not in ("bf16", "fp8_e4m3"):
-            raise ValueError("deepseek_moe supports bf16 and fp8_e4m3 only")      # model_factory.h:105-114
+        if self.cfg.model_type == "deepseek_moe" and d_prefill not in ("bf16", "fp8_e4m3", "fp8_w8a8"):
+            raise ValueError("deepseek_moe supports bf16, fp8_e4m3 and fp8_w8a8 only")      # model_factory.h:105-114
+        if d_prefill == "fp8_w8a8" and layered:
+            raise ValueError("layered designs have no fp8_w8a8 form")
         if d_prefill == "fp8_e4m3" and self.cfg.model_type != "deepseek_moe":
             raise ValueError("fp8_e4m3 is supported for deepseek_moe only")
         with TimeLine("Model.load"):
