@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
   constexpr int NCOL = SRC == kSrcI8 ? 3 : SRC == kSrcU4 ? 2 : 0, NROW = SRC == kSrcI8 ? 3 : SRC == kSrcBf16 ? 1 : 2;
   __shared__ alignas(16) float s_col[NCOL ? NCOL : 1][NACC][NCOL ? 128 : 4];
   __shared__ float s_row[NROW][BN];
-  __shared__ alignas(16) float s_xs[SRC == kSrcRows ? 8 : 1][SRC == kSrcRows ? BN : 4];      // per warp: two lines of its tokens' scales
+  __shared__ alignas(16) float s_xs[SRC == kSrcRows ? 8 : 1][SRC == kSrcRows ? 2 * BN : 4];  // per warp: its tokens' scales of four blocks
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int tile_n, tile_t;
@@ -371,44 +371,67 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
         if (lane == 0) mbar_arrive(&tmem_empty[b.s]);
       }
     } else if constexpr (SRC == kSrcRows) {
-      // A block's sum of a token is scaled with the row's scale and the weights': a lane holds the scales of one token, two blocks ahead,
-      // and the warp reads them from a line of shared memory of its own (two lines in turn, so one wait of the warp orders both).
-      grid_dep_wait();
-      fetch_rows();
+      // A block's sum of a token is scaled with the row's scale and the weights'.  Scales come four blocks at a time and are asked for four
+      // blocks ahead (a load from L2 takes longer than a block, and a value that moves between registers waits for its load); a lane holds
+      // a token's, and the warp reads them from lines of shared memory of its own.
       const float* sc = p.scale + (size_t)(w_row0 >> 7) * p.scale_ld;
       const float* sc_up = sc + (size_t)(p.dual_off >> 7) * p.scale_ld;
+      float xs[4], ws[4], us[4];
+      auto fetch_weights = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ws[i] = kb + i < kend ? __ldg(sc + kb + i) : 0.f;
+          if (DUAL) us[i] = kb + i < kend ? __ldg(sc_up + kb + i) : 0.f;
+        }
+      };
       float* line = s_xs[warp - 2];
       const bool mine = lane < HB && c0 + lane < x_rows;
       const float* sx = p.x_scale + x_row0 + c0 + lane;
-      auto scale_of = [&](int kb) { return mine && kb < kend ? __ldg(sx + (size_t)kb * p.x_ld) : 0.f; };
-      float x0 = scale_of(kb0), x1 = scale_of(kb0 + 1);
-      float w0 = kb0 < kend ? __ldg(sc + kb0) : 0.f, u0 = DUAL && kb0 < kend ? __ldg(sc_up + kb0) : 0.f;
+      auto fetch_xs = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xs[i] = mine && kb + i < kend ? __ldg(sx + (size_t)(kb + i) * p.x_ld) : 0.f;
+      };
+      fetch_weights(kb0);
+      grid_dep_wait();
+      fetch_xs(kb0);
+      fetch_rows();
       Ring b = {0, 0};
-      for (int kb = kb0; kb < kend && ok; ++kb, b.next(2)) {
-        if (lane < HB) line[b.s * HB + lane] = x0;
-        const float wf = w0, uf = u0;
-        x0 = x1;
-        x1 = scale_of(kb + 2);
-        if (kb + 1 < kend) { w0 = __ldg(sc + kb + 1); u0 = DUAL ? __ldg(sc_up + kb + 1) : 0.f; }
-        ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[b.s], b.ph, p.status, XFT_ERR_WAIT_TMEM));
-        if (!ok) break;
-        tcgen05_fence_after();
-        uint32_t v[NACC][HB];
-#pragma unroll
-        for (int a = 0; a < NACC; ++a) tmem_ld_cols<HB>(taddr + b.s * ACC + a * NB, v[a]);
-        tmem_ld_wait();
-        tcgen05_fence_before();
+      for (int kb4 = kb0; kb4 < kend && ok; kb4 += 4) {
+        float wf[4], uf[4];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tmem_empty[b.s]);
 #pragma unroll
-        for (int j = 0; j < HB; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(line + b.s * HB + j);
+        for (int i = 0; i < 4; ++i) {
+          if (lane < HB) line[i * HB + lane] = xs[i];
+          wf[i] = ws[i];
+          uf[i] = DUAL ? us[i] : 0.f;
+        }
+        fetch_xs(kb4 + 4);
+        fetch_weights(kb4 + 4);
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float s = (&f.x)[i];
-            g[0][j + i] = fmaf(s * wf, __uint_as_float(v[0][j + i]), g[0][j + i]);
-            if constexpr (DUAL) g[NACC - 1][j + i] = fmaf(s * uf, __uint_as_float(v[NACC - 1][j + i]), g[NACC - 1][j + i]);
+        for (int i = 0; i < 4; ++i) {
+          if (kb4 + i >= kend) break;
+          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[b.s], b.ph, p.status, XFT_ERR_WAIT_TMEM));
+          if (!ok) break;
+          tcgen05_fence_after();
+          uint32_t v[NACC][HB];
+#pragma unroll
+          for (int a = 0; a < NACC; ++a) tmem_ld_cols<HB>(taddr + b.s * ACC + a * NB, v[a]);
+          tmem_ld_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_empty[b.s]);
+#pragma unroll
+          for (int j = 0; j < HB; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(line + i * HB + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float s = (&f.x)[k];
+              g[0][j + k] = fmaf(s * wf[i], __uint_as_float(v[0][j + k]), g[0][j + k]);
+              if constexpr (DUAL) g[NACC - 1][j + k] = fmaf(s * uf[i], __uint_as_float(v[NACC - 1][j + k]), g[NACC - 1][j + k]);
+            }
           }
+          b.next(2);
         }
       }
     } else if constexpr (SRC == kSrcI8 || SRC == kSrcBf16) {
@@ -883,6 +906,13 @@ extern "C" int xft_gemm_e4m3(const void* xs, int x_rows, const float* x_scale, c
   return -1;
 }
 
+namespace xft {
+int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st);  // gemm_rows_e4m3_sm100.cu
+int rows_form(int T, int N, int K, int gated, int sms);
+int encode_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
+                      uint32_t esize);                                 // gemm_sm100.cu
+}
+
 // Size and field offsets of RowsGemm, for the layout check of the Python mirror.
 extern "C" int xft_rows_gemm_layout(long long* out, int n) {
   const long long v[] = {sizeof(RowsGemm),             offsetof(RowsGemm, x),          offsetof(RowsGemm, x_scale),
@@ -895,7 +925,8 @@ extern "C" int xft_rows_gemm_layout(long long* out, int n) {
                          offsetof(RowsGemm, N),        offsetof(RowsGemm, K),          offsetof(RowsGemm, ldo),
                          offsetof(RowsGemm, out_fp32), offsetof(RowsGemm, ldr),        offsetof(RowsGemm, act),
                          offsetof(RowsGemm, gated),    offsetof(RowsGemm, dual_off),   offsetof(RowsGemm, group_w_rows),
-                         offsetof(RowsGemm, max_tiles), offsetof(RowsGemm, bn),        offsetof(RowsGemm, res_scale)};
+                         offsetof(RowsGemm, max_tiles), offsetof(RowsGemm, bn),        offsetof(RowsGemm, form),
+                         offsetof(RowsGemm, res_scale)};
   const int m = (int)(sizeof(v) / sizeof(v[0]));
   for (int i = 0; i < m && i < n; ++i) out[i] = v[i];
   return m;
@@ -910,6 +941,13 @@ extern "C" int xft_gemm_rows_e4m3(const RowsGemm* args, cudaStream_t st) {
   if ((a.ldx & 15) || (a.ldw & 15) || (reinterpret_cast<uintptr_t>(a.x) & 15) || (reinterpret_cast<uintptr_t>(a.w) & 15)) return -2;
   if ((a.gated && (a.dual_off & 127)) || (a.group_tiles && (a.group_w_rows & 127))) return -4;
   if (a.out_scale && ((a.N & 127) || (a.ldo & 15) || (reinterpret_cast<uintptr_t>(a.out) & 15) || a.residual || a.col_scale)) return -5;
+  int form = a.form;
+  if (a.group_tiles) {
+    form = a.bn == 256 ? 1 : a.bn == 128 ? 3 : 0;
+  } else if (form < 0) {
+    form = a.T > 64 ? rows_form(a.T, a.N, a.K, a.gated, 148) : 0;
+  }
+  if (form > 0) return launch_rows_prompt(a, form, st);
   E4Params p{};
   p.N = a.N; p.T = a.T; p.K = a.K; p.dual_off = a.dual_off; p.out = a.out; p.ldo = a.ldo; p.out_fp32 = a.out_fp32; p.bias = a.bias;
   p.residual = (const __nv_bfloat16*)a.residual; p.ldr = a.ldr; p.res_scale = a.res_scale; p.act = a.act; p.x_scale = a.x_scale;
@@ -923,7 +961,7 @@ extern "C" int xft_gemm_rows_e4m3(const RowsGemm* args, cudaStream_t st) {
   CUtensorMap tmW, tmX;
   int r = make_tensor_map(&tmW, a.w, (uint64_t)a.w_rows, (uint64_t)a.K, (uint64_t)a.ldw, 128, 1);
   if (r) return 1000 - r;
-  r = make_tensor_map(&tmX, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, (uint64_t)a.ldx, (uint32_t)bn, 1);
+  r = encode_tensor_map(&tmX, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, (uint64_t)a.ldx, (uint32_t)bn, 1);
   if (r) return 2000 - r;
 #define XFT_ROWS(BN_) \
   case BN_: return a.gated ? launch_e4<BN_, true, kSrcRows>(tmW, tmX, p, st) : launch_e4<BN_, false, kSrcRows>(tmW, tmX, p, st);

@@ -1,0 +1,483 @@
+// Products of e4m3 rows and e4m3 weights above 64 rows (rows_e4m3.cuh has the form of the rows):
+//     Y[t, n] = epilogue( sum_b sx[b, t] sw[n / 128, b] sum_{k in block b} X[t, k] W[n, k] ),
+// plain, gated (act(gate) * up, on request as e4m3 rows for the next product) and grouped by expert.
+//
+// Tokens are the rows of the MMA and features its columns, as in gemm_prefill_tm_kernel (gemm_prefill_sm100.cu), whose pipeline this
+// is: one producer warp, one MMA warp, eight warps behind them; with CG = 2 two CTAs share a tile of 256 tokens and each holds half of
+// its weight rows.  What differs is that a sum may run over one block of 128 k only: its scales are a number per token and block and a
+// number per 128 features and block.  So a block is one accumulator (two in turn), and the eight warps fetch it, scale it and add it to
+// registers while the next fills: a thread has one token and 128 columns, whose factor is one product of two scales.  That is 64
+// two-wide multiply-adds and 128 words from TMEM per thread and block, against 512 cycles of MMAs in the largest tile; the last
+// accumulators of a tile are finished and stored while the next tile's first two fill.
+#include "rows_e4m3.cuh"
+
+namespace xft {
+
+int encode_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
+                      uint32_t esize);                                 // gemm_sm100.cu: make_tensor_map without its table
+
+// Three groups of four warps: the issuing ones (producer, MMA; two idle), and eight warps that add up, to which the first group's registers go
+// (setmaxnreg: 24 and 240 a thread of the 168 that each was launched with).
+constexpr int kRowsThreads = 384;
+constexpr int kRowsRing = 192 * 1024;
+
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// (x, y) += f * (a, b)
+__device__ __forceinline__ void fma_pair(float& x, float& y, float f, uint32_t a, uint32_t b) {
+  asm("{\n"
+      ".reg .b64 c, m, s;\n"
+      "mov.b64 c, {%0, %1};\n"
+      "mov.b64 m, {%2, %2};\n"
+      "mov.b64 s, {%3, %4};\n"
+      "fma.rn.f32x2 c, s, m, c;\n"
+      "mov.b64 {%0, %1}, c;\n"
+      "}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(f), "r"(a), "r"(b));
+}
+// waits for the loads from TMEM under way; nothing that uses v moves in front of it
+__device__ __forceinline__ void rows_ld_wait(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+// A bounded wait that also ends when another role of this CTA has given up
+__device__ __forceinline__ bool rows_wait(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* lost) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*lost) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      if (status) atomicCAS(status, 0, code);
+      *lost = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// What this arrival orders are the warp's loads from TMEM, which have their own fence and wait; no other memory has to be seen, so it is
+// relaxed, and the waits of the issuing threads carry the scope of the CTA also in pairs.  Cluster scope there drops the SM's cached
+// lines at every wait: 256 x 256 tiles of 8192 x 8192 x 28672 took 3778 us with it.
+__device__ __forceinline__ void rows_arrive(uint32_t addr) {           // in the window of the cluster
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// act of 16 values: one branch for all of them
+__device__ __forceinline__ void rows_act(float* x, int act) {
+#define XFT_ROWS_ACT(A)                                    \
+  case A:                                                  \
+    _Pragma("unroll") for (int j = 0; j < 16; ++j) x[j] = apply_act(x[j], A); \
+    break;
+  switch (act) { XFT_ROWS_ACT(1) XFT_ROWS_ACT(2) XFT_ROWS_ACT(3) XFT_ROWS_ACT(4) XFT_ROWS_ACT(kActGeluErf) XFT_ROWS_ACT(kActTanh) default: break; }
+#undef XFT_ROWS_ACT
+}
+
+struct RowsTmParams {
+  RowsGemm g;
+  int n_tiles, t_tiles, num_kb;
+  int gn;                                    // feature tiles that walk the token tiles together
+};
+
+// NCOL: accumulator columns of a tile; gated: half gate, half up (the other way round as many features).
+template <int NCOL, bool DUAL, int CG>
+struct RowsTile {
+  static constexpr int FEAT = DUAL ? NCOL / 2 : NCOL, TOK = 128 * CG;
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = NCOL / CG * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int FIT = kRowsRing / STAGE, STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr int SMEM = STAGES * STAGE + 1024;
+  static constexpr int COLS = NCOL / 2;      // of a thread: two warps share 32 tokens
+  static_assert((NCOL == 256 || (NCOL == 128 && !DUAL)) && (CG == 1 || CG == 2), "tile");
+};
+
+template <int NCOL, bool DUAL, int CG>
+__global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                                       const __grid_constant__ CUtensorMap tmW, const RowsTmParams p) {
+  using L = RowsTile<NCOL, DUAL, CG>;
+  constexpr int FEAT = L::FEAT, TOK = L::TOK, STAGES = L::STAGES, STAGE = L::STAGE, COLS = L::COLS;
+  constexpr uint32_t TMEM_COLS = 2 * NCOL;
+  constexpr uint32_t IDESC = umma_idesc(TOK, NCOL, 0, 0, 1);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full[2], tmem_empty[2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int s_lost_mem;
+  __shared__ float s_top[2][2][DUAL ? 128 : 1];          // gated: largest value of a token over each half of the features, two items in turn
+  volatile int* lost = &s_lost_mem;
+  int* status = p.g.status;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = CG == 2 ? (int)cluster_ctarank() : 0;              // which 128 tokens of a tile are this CTA's
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int4* groups = reinterpret_cast<const int4*>(p.g.group_tiles);
+  const int total = p.n_tiles * (groups ? min(*p.g.num_group_tiles, p.t_tiles) : p.t_tiles);
+  struct Item { int nt, row0, rows, w0; };                             // feature tile, first token row, rows, first weight row of its group
+  auto item_of = [&](int item) {
+    Item r;
+    if (groups) {
+      const int4 e = groups[item / p.n_tiles];
+      r = {item % p.n_tiles, e.y, e.z, e.x * p.g.group_w_rows};
+    } else {
+      const int per = p.gn * p.t_tiles, gr = item / per, at = item % per, gn = min(p.gn, p.n_tiles - gr * p.gn);
+      r = {gr * p.gn + at % gn, at / gn * TOK, p.g.T - at / gn * TOK, 0};
+    }
+    r.row0 += half * 128;
+    r.rows -= half * 128;
+    return r;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 8 * CG); }
+    s_lost_mem = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) { tmem_alloc_pair(&tmem_base_s, TMEM_COLS); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_base_s, TMEM_COLS); tmem_relinquish(); }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) {              // both CTAs' barriers and accumulators exist before either touches the other's
+    cluster_arrive();
+    cluster_wait();
+  }
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+    if (warp == 0) {
+      if (elect_one()) {
+        const uint32_t lead_bar = CG == 2 ? dsmem_addr(smem_u32(full_bar), 0) : 0;      // the first CTA's full barriers
+        Ring r = {0, 0};
+        bool ok = true;
+        for (int item = first; item < total && ok; item += step) {
+          const Item im = item_of(item);
+          const int wrow = im.w0 + im.nt * FEAT + half * (DUAL ? p.g.dual_off : NCOL / 2);
+          for (int kb = 0; kb < p.num_kb; ++kb, r.next(STAGES)) {
+            ok = rows_wait(&empty_bar[r.s], r.ph ^ 1, status, XFT_ERR_WAIT_EMPTY, lost);
+            if (!ok) break;
+            uint8_t* a = smem + r.s * STAGE;
+            if constexpr (CG == 2) {
+              if (half == 0) mbar_expect_tx(&full_bar[r.s], 2 * STAGE);
+              tma_load_2d_pair(a, &tmX, lead_bar + 8 * r.s, kb * 128, im.row0, kEvictNormal);
+              tma_load_2d_pair(a + L::A_BYTES, &tmW, lead_bar + 8 * r.s, kb * 128, wrow, kEvictNormal);
+            } else {
+              mbar_expect_tx(&full_bar[r.s], STAGE);
+              tma_load_2d(a, &tmX, &full_bar[r.s], kb * 128, im.row0, kEvictNormal);
+              tma_load_2d(a + L::A_BYTES, &tmW, &full_bar[r.s], kb * 128, wrow, kEvictNormal);
+              if (DUAL) tma_load_2d(a + L::A_BYTES + FEAT * 128, &tmW, &full_bar[r.s], kb * 128, wrow + p.g.dual_off, kEvictNormal);
+            }
+          }
+        }
+        if (!ok) {                        // copies in flight land before the CTA's shared memory goes
+          const long long t0 = clock64();
+          while (clock64() - t0 < 2000000LL) {}
+        } else if (CG == 2) {
+          // the first CTA's commits also arrive here: stay until every stage has been given back
+          for (int k = 0; k < STAGES; ++k, r.next(STAGES))
+            if (!rows_wait(&empty_bar[r.s], r.ph ^ 1, status, XFT_ERR_WAIT_EMPTY, lost)) break;
+        }
+      }
+    } else if (warp == 1) {
+      if (half == 0 && elect_one()) {
+        const uint64_t adesc0 = umma_desc_k128(smem_u32(smem)), bdesc0 = umma_desc_k128(smem_u32(smem) + L::A_BYTES);
+        Ring r = {0, 0}, b = {0, 0};
+        bool ok = true;
+        for (int item = first; item < total && ok; item += step) {
+          for (int kb = 0; kb < p.num_kb; ++kb, r.next(STAGES), b.next(2)) {
+            ok = rows_wait(&tmem_empty[b.s], b.ph ^ 1, status, XFT_ERR_WAIT_TMEM, lost) &&
+                 rows_wait(&full_bar[r.s], r.ph, status, XFT_ERR_WAIT_FULL, lost);
+            if (!ok) break;
+            tcgen05_fence_after();
+            const uint64_t off = (uint64_t)(r.s * (STAGE / 16));
+            const uint32_t acc = tmem_base + (uint32_t)(b.s * NCOL);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (CG == 2) umma_e4m3_pair(acc, adesc0 + off + 2 * k, bdesc0 + off + 2 * k, IDESC, k > 0);
+              else umma_e4m3(acc, adesc0 + off + 2 * k, bdesc0 + off + 2 * k, IDESC, k > 0);
+            }
+            if constexpr (CG == 2) { tcgen05_commit_pair(&empty_bar[r.s]); tcgen05_commit_pair(&tmem_full[b.s]); }
+            else { tcgen05_commit(&empty_bar[r.s]); tcgen05_commit(&tmem_full[b.s]); }
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
+    // ---- a token and COLS columns per thread; gated: COLS / 2 gate columns, then their up columns
+    const int q = warp & 3, side = warp >= 8, row = q * 32 + lane;
+    constexpr int PART = DUAL ? COLS / 2 : COLS;                       // columns in a row
+    const int col0 = side * PART;
+    const bool vec = p.g.N % 8 == 0 && p.g.ldo % 8 == 0 && (!p.g.residual || p.g.ldr % 8 == 0) &&
+                     ((reinterpret_cast<uintptr_t>(p.g.out) | reinterpret_cast<uintptr_t>(p.g.residual)) & 15) == 0;
+    const bool vec32 = vec && p.g.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
+    Ring b = {0, 0};
+    bool ok = true;
+    int turn = 0;
+    for (int item = first; item < total; item += step, turn ^= 1) {
+      const Item im = item_of(item);
+      const int t = im.row0 + row, n0 = im.nt * FEAT + col0;
+      const bool t_ok = row < im.rows;
+      const float* sx = p.g.x_scale + t;
+      const float* sw = p.g.w_scale + (size_t)((im.w0 + n0) >> 7) * p.g.scale_ld;
+      const float* su = sw + (size_t)(p.g.dual_off >> 7) * p.g.scale_ld;
+      const bool w_ok = n0 < p.g.N;                                    // a last tile may have no features on this side
+      // Scales of two blocks at a time, asked for two blocks ahead: a load from L2 takes longer than a block, and a value that moves
+      // from one register to the next waits for its load.
+      float xs[2], ws[2], us[2];
+      auto fetch_scales = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool in = kb + i < p.num_kb;
+          xs[i] = in && t_ok ? __ldg(sx + (size_t)(kb + i) * p.g.x_ld) : 0.f;
+          ws[i] = in && w_ok ? __ldg(sw + kb + i) : 0.f;
+          if (DUAL) us[i] = in && w_ok ? __ldg(su + kb + i) : 0.f;
+        }
+      };
+      float acc[COLS];
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      fetch_scales(0);
+      for (int kb0 = 0; kb0 < p.num_kb && ok; kb0 += 2) {
+        float f[2], fu[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { f[i] = xs[i] * ws[i]; fu[i] = DUAL ? xs[i] * us[i] : 0.f; }
+        fetch_scales(kb0 + 2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (kb0 + i >= p.num_kb) break;
+          ok = __all_sync(0xffffffffu, rows_wait(&tmem_full[b.s], b.ph, status, XFT_ERR_WAIT_TMEM, lost));
+          if (!ok) break;
+          tcgen05_fence_after();
+          const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + (uint32_t)(b.s * NCOL + col0);
+          auto at = [&](int c) { return taddr + (DUAL && c >= PART ? FEAT - PART + c : c); };
+          auto add = [&](int c, const uint32_t (&v)[32]) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) fma_pair(acc[c + j], acc[c + j + 1], DUAL && c >= PART ? fu[i] : f[i], v[j], v[j + 1]);
+          };
+#pragma unroll
+          for (int c = 0; c < COLS; c += 64) {                         // 64 columns at a time: one wait for two loads
+            uint32_t v0[32], v1[32];
+            tmem_ld32(at(c), v0);
+            tmem_ld32(at(c + 32), v1);
+            rows_ld_wait(v0);
+            rows_ld_wait(v1);
+            if (c + 64 == COLS) {                                      // given back before the last of it is added
+              tcgen05_fence_before();
+              __syncwarp();
+              if (lane == 0) rows_arrive(CG == 2 ? dsmem_addr(smem_u32(&tmem_empty[b.s]), 0) : smem_u32(&tmem_empty[b.s]));
+            }
+            add(c, v0);
+            add(c + 32, v1);
+          }
+          b.next(2);
+        }
+      }
+      // ---- epilogue of the item (all warps come through here, also after a wait that ran out: the barrier below counts them)
+      if constexpr (DUAL) {
+        if (p.g.bias) {
+#pragma unroll
+          for (int j = 0; j < PART; ++j) {
+            acc[j] += __ldg(p.g.bias + min(n0 + j, p.g.N - 1));
+            acc[PART + j] += __ldg(p.g.bias + p.g.dual_off + min(n0 + j, p.g.N - 1));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < PART; c += 16) rows_act(acc + c, p.g.act);
+#pragma unroll
+        for (int j = 0; j < PART; ++j) acc[j] *= acc[PART + j];
+        if (p.g.out_scale) {
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < PART; ++j) top = e4m3_top(top, acc[j]);
+          s_top[turn][side][row] = top;
+          named_bar_sync(1, 256);
+          top = fmaxf(s_top[turn][0][row], s_top[turn][1][row]);
+          if (t_ok && ok) {
+            const E4m3Scale s = e4m3_scale(top);
+            uint8_t* to = reinterpret_cast<uint8_t*>(p.g.out) + (size_t)t * p.g.ldo + n0;
+#pragma unroll
+            for (int j = 0; j < PART; j += 16) {
+              uint32_t c[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                c[i] = e4m3_codes(acc[j + 4 * i], acc[j + 4 * i + 1], s.inv) | e4m3_codes(acc[j + 4 * i + 2], acc[j + 4 * i + 3], s.inv) << 16;
+              *reinterpret_cast<uint4*>(to + j) = make_uint4(c[0], c[1], c[2], c[3]);
+            }
+            if (side == 0) p.g.out_scale[(size_t)im.nt * p.g.out_ld + t] = s.scale;
+          }
+          continue;
+        }
+      }
+      if (!t_ok || !ok) continue;
+      const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr : nullptr;
+      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo;
+      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t * p.g.ldo;
+#pragma unroll
+      for (int c = 0; c < PART; c += 16) {
+        const int n = n0 + c;
+        if (n >= p.g.N) continue;
+        const bool full = vec && n + 16 <= p.g.N;
+        float* x = acc + c;
+        if constexpr (!DUAL) {
+          if (p.g.bias) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
+          }
+          rows_act(x, p.g.act);
+        }
+        if (rrow) {
+          if (full) {
+            uint4 res[2] = {reinterpret_cast<const uint4*>(rrow + n)[0], reinterpret_cast<const uint4*>(rrow + n)[1]};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
+              x[2 * j] += p.g.res_scale * f.x;
+              x[2 * j + 1] += p.g.res_scale * f.y;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (n + j < p.g.N) x[j] += p.g.res_scale * __bfloat162float(rrow[n + j]);
+          }
+        }
+        if (p.g.out_fp32) {
+          if (full) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(frow + n)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) if (n + j < p.g.N) frow[n + j] = x[j];
+          }
+        } else if (full) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const __nv_bfloat162 o = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&o);
+          }
+          if (vec32) {
+            st_global_256(orow + n, w);
+          } else {
+            reinterpret_cast<uint4*>(orow + n)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4*>(orow + n)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) if (n + j < p.g.N) orow[n + j] = __float2bfloat16(x[j]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) {              // neither CTA's shared memory or accumulator goes while the other may still use it
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (warp == 1) {
+    tcgen05_fence_after();
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+template <int NCOL, bool DUAL, int CG>
+static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
+  using L = RowsTile<NCOL, DUAL, CG>;
+  RowsTmParams p{};
+  p.g = g;
+  p.num_kb = (g.K + 127) / 128;
+  p.n_tiles = (g.N + L::FEAT - 1) / L::FEAT;
+  p.t_tiles = g.group_tiles ? g.max_tiles : (g.T + L::TOK - 1) / L::TOK;
+  p.gn = 8;
+  CUtensorMap tmW, tmX;
+  int r = make_tensor_map(&tmW, g.w, (uint64_t)g.w_rows, (uint64_t)g.K, (uint64_t)g.ldw, (uint32_t)(DUAL ? L::FEAT : NCOL / CG), 1);
+  if (r) return 1000 - r;
+  r = encode_tensor_map(&tmX, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.ldx, 128, 1);
+  if (r) return 2000 - r;
+  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return 3000 + (int)e;
+  const long long total = (long long)p.n_tiles * p.t_tiles, slots = sms / CG > 0 ? sms / CG : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((total < slots ? total : slots) * CG));
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = L::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, tmX, tmW, (const RowsTmParams)p);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+// The tile that is expected to take least, or 0 for the weight-stream kernel (gemm_e4m3_sm100.cu), in us: what a launch costs, then rounds of
+// tiles, each of its blocks of k and its finish.  Fitted to a sweep on B200; tiles 1 / 2 / 3 / 4: 389 x 2112 x 7168 41 / 24 / 40 / 23, 512 x
+// 12288 x 4096 49 / 39 / 48 / 38, 4096 x 8192 x 8192 303 / 312 / 340 / 334; gated 600 x 2 x 11008 x 4096 86 / - / 72, 1500 x 2 x 14336 x
+// 4096 205 / - / 224; the other kernel 128 x 4096 x 4096 13.5, here 16.4.
+int rows_form(int T, int N, int K, int gated, int sms) {
+  const int kb = (K + 127) / 128, cols = gated ? 2 * N : N;
+  auto cost = [&](int tok, int ncol, int ctas, float block, float finish) {
+    const long long tiles = (long long)((T + tok - 1) / tok) * ((cols + ncol - 1) / ncol), slots = sms / ctas > 0 ? sms / ctas : 1;
+    return 5.f + (float)((tiles + slots - 1) / slots) * (kb * block + finish);
+  };
+  const long long small = (long long)((T + 63) / 64) * ((N + 127) / 128);
+  int parts = 1;
+  while (parts < 8 && small * parts * 2 <= sms && kb / (parts * 2) >= 4) parts *= 2;
+  float best = 5.f + (float)((small * parts + sms - 1) / sms) * ((float)kb / parts * (gated ? 0.9f : 0.5f) + 1.5f);
+  int form = 0;
+  const float costs[5] = {0.f, cost(256, 256, 2, 0.60f, 2.f), cost(256, 128, 2, 0.345f, 1.2f), cost(128, 256, 1, 0.62f, 2.f), cost(128, 128, 1, 0.34f, 1.f)};
+  for (int i = 1; i <= 4; ++i) {
+    if (gated && (i == 2 || i == 4)) continue;
+    if (costs[i] < best) { best = costs[i]; form = i; }
+  }
+  return form;
+}
+
+// Tiles: 1 = 256 tokens x 256 columns on two CTAs, 2 = 256 x 128 on two, 3 = 128 x 256, 4 = 128 x 128 (gated: 1 and 3).
+int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (sms <= 0) sms = 148;
+  if (g.gated) return form == 1 ? launch_rows_tm<256, true, 2>(g, sms, st) : launch_rows_tm<256, true, 1>(g, sms, st);
+  switch (form) {
+    case 1: return launch_rows_tm<256, false, 2>(g, sms, st);
+    case 2: return launch_rows_tm<128, false, 2>(g, sms, st);
+    case 3: return launch_rows_tm<256, false, 1>(g, sms, st);
+    default: return launch_rows_tm<128, false, 1>(g, sms, st);
+  }
+}
+
+}  // namespace xft

@@ -39,7 +39,8 @@ struct RowsGemm {
   int x_rows, ldx, w_rows, ldw, scale_ld;              // codes: pitches in bytes, multiples of 16
   int T, N, K, ldo, out_fp32, ldr, act;
   int gated, dual_off;
-  int group_w_rows, max_tiles, bn;                     // grouped form
+  int group_w_rows, max_tiles, bn;                     // grouped form: rows of a tile of the table
+  int form;                                            // -1: by size; 0: gemm_e4m3_sm100.cu, else a tile of gemm_rows_e4m3_sm100.cu
   float res_scale;
 };
 

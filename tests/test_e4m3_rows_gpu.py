@@ -1,4 +1,4 @@
-"""Rows in e4m3 and their products on a GPU (csrc/kernels/rows_e4m3.cu, gemm_e4m3_sm100.cu) against 64 bits."""
+"""Rows in e4m3 and their products on a GPU (csrc/kernels/rows_e4m3.cu, gemm_e4m3_sm100.cu, gemm_rows_e4m3_sm100.cu) against 64 bits."""
 import pytest
 import torch
 
@@ -102,6 +102,48 @@ def test_product_matches_64_bits(T, N, K):
         got = ops.linear_e4m3(dq, dW, bias.cuda(), None, res.cuda(), 0.5, out_dtype=dtype)
         assert got.dtype == dtype and bool(((got.cpu().double() - full).abs() <= tol + half * full.abs()).all())
     check_status()
+
+
+# tiles of prompts, whatever the size would choose: one item and several per CTA, rows and features that end inside a tile, one block of k and
+# many, k that ends inside a block
+@pytest.mark.parametrize("form", [1, 2, 3, 4])
+@pytest.mark.parametrize("T,N,K", [(1, 8, 128), (100, 136, 16), (129, 256, 640), (257, 300, 1032), (300, 2112, 2048), (2000, 5000, 264), (9000, 1160, 128)])
+def test_tiles_of_prompts(T, N, K, form):
+    from xfastertransformer_b200.ops import native_e4m3 as E
+    g = gen(T, N, K)
+    q, W = rows(activations(g, T, K)), weight(g, N, K)
+    bias, res = torch.randn(N, generator=g), torch.randn(T, N, generator=g).bfloat16()
+    want, tol = sum_tol(q, W)
+    want = want + bias.double() + 0.5 * res.double()
+    tol = tol + 2.0 ** -23 * (bias.double().abs() + res.double().abs() + want.abs())
+    dq, dW = rows_on(q), on(W)
+    for dtype, half in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8)):
+        out = torch.full((T + 1, N), 7.0, dtype=dtype, device="cuda")
+        E._gemm(dq, dW.w if K % 16 == 0 else E._weight(dW), dW.scale, out[:T], T, N, K, bias=bias.cuda(), residual=res.cuda(), res_scale=0.5, form=form)
+        check_status()
+        assert bool(((out[:T].cpu().double() - want).abs() <= tol + half * want.abs()).all()) and bool((out[T] == 7).all())
+
+
+@pytest.mark.parametrize("form", [1, 3])
+@pytest.mark.parametrize("T,I,K", [(1, 128, 128), (130, 384, 200), (300, 640, 1024), (5000, 1408, 256)])
+def test_gated_tiles_of_prompts(T, I, K, form):
+    from xfastertransformer_b200.ops import native_e4m3 as E
+    g = gen(T, I, K)
+    q, W, bias = rows(torch.randn(T, K, generator=g)), weight(g, 2 * I, K), torch.randn(2 * I, generator=g)
+    y, tol = sum_tol(q, W)
+    y, tol = y + bias.double(), tol + 2.0 ** -23 * (y.abs() + bias.double().abs())
+    a = R._act(y[:, :I], "silu")
+    want = a * y[:, I:]
+    err = 1.2 * tol[:, :I] * (y[:, I:].abs() + tol[:, I:]) + a.abs() * tol[:, I:] + 2.0 ** -18 * y[:, :I].abs() * y[:, I:].abs()
+    out = E.new_rows(T, I, torch.device("cuda", 0))
+    dq, dW = rows_on(q), on(W)
+    E._gemm(dq, E._weight(dW), dW.scale, out.codes, T, I, K, True, I, bias.cuda(), "silu", out_scale=out.scale, form=form)
+    check_status()
+    assert coded_error(out, want, err) <= 0 and scale_error(out, want, err) <= 0
+    plain = torch.empty(T, I, dtype=torch.bfloat16, device="cuda")
+    E._gemm(dq, E._weight(dW), dW.scale, plain, T, I, K, True, I, bias.cuda(), "silu", form=form)
+    check_status()
+    assert bool(((plain.cpu().double() - want).abs() <= err + 2.0 ** -8 * want.abs()).all())
 
 
 @pytest.mark.parametrize("T", [5, 40, 150])

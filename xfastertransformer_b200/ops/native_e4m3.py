@@ -1,5 +1,5 @@
 """Bindings of the block-scaled e4m3 path, 8-bit weights and activations: rows in e4m3 (csrc/kernels/rows_e4m3.cu), their products
-(csrc/kernels/gemm_e4m3_sm100.cu) and the experts' form of both.
+(csrc/kernels/gemm_e4m3_sm100.cu; prompts: csrc/kernels/gemm_rows_e4m3_sm100.cu) and the experts' form of both.
 
 Nothing here keeps scratch between calls, so calls on several streams and captured graphs do not touch one another; the kernels run on
 the device of their rows, on that device's current stream."""
@@ -23,7 +23,7 @@ class RowsGemm(C.Structure):
                 ("out_ld", C.c_longlong), ("x_rows", C.c_int), ("ldx", C.c_int), ("w_rows", C.c_int), ("ldw", C.c_int),
                 ("scale_ld", C.c_int), ("T", C.c_int), ("N", C.c_int), ("K", C.c_int), ("ldo", C.c_int), ("out_fp32", C.c_int),
                 ("ldr", C.c_int), ("act", C.c_int), ("gated", C.c_int), ("dual_off", C.c_int), ("group_w_rows", C.c_int),
-                ("max_tiles", C.c_int), ("bn", C.c_int), ("res_scale", C.c_float)]
+                ("max_tiles", C.c_int), ("bn", C.c_int), ("form", C.c_int), ("res_scale", C.c_float)]
 
 
 _ready = False
@@ -116,7 +116,7 @@ def _weight(W):
 
 
 def _gemm(q, w, w_scale, out, T, n_out, K, gated=False, dual_off=0, bias=None, act=None, residual=None, res_scale=1.0, out_scale=None,
-          tiles=None, n_tiles=None, group_rows=0, max_tiles=0, bn=0, col_scale=None, x_rows=None):
+          tiles=None, n_tiles=None, group_rows=0, max_tiles=0, bn=0, col_scale=None, form=-1):
     codes, scale = _pitched(q.codes), _scales(q.scale)
     ws = N.Workspace.get(codes.device)
     a = RowsGemm()
@@ -128,7 +128,7 @@ def _gemm(q, w, w_scale, out, T, n_out, K, gated=False, dual_off=0, bias=None, a
     a.x_rows, a.ldx, a.w_rows, a.ldw, a.scale_ld = codes.shape[0], _pitch(codes), w.shape[0], _pitch(w), w_scale.shape[1]
     a.T, a.N, a.K, a.ldo, a.out_fp32 = T, n_out, K, _pitch(out) if out_scale is not None else out.stride(0), int(out.dtype == torch.float32)
     a.ldr, a.act = 0 if residual is None else residual.stride(0), N._ACT[act]
-    a.gated, a.dual_off, a.group_w_rows, a.max_tiles, a.bn, a.res_scale = int(gated), dual_off, group_rows, max_tiles, bn, res_scale
+    a.gated, a.dual_off, a.group_w_rows, a.max_tiles, a.bn, a.form, a.res_scale = int(gated), dual_off, group_rows, max_tiles, bn, form, res_scale
     N._check(_lib().xft_gemm_rows_e4m3(C.byref(a), N._stream()), "gemm_rows_e4m3")
     ws.launches += 1
 
@@ -190,7 +190,7 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
     ws, lib = N.Workspace.get(dev), _lib()
     pairs = T * k
     avg = max(1, ((pairs if expected_pairs is None else min(int(expected_pairs), pairs)) + E - 1) // E)
-    bn = 16 if avg <= 16 else 32 if avg <= 32 else 64
+    bn = 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 64 else 128 if avg < 512 else 256
     max_tiles = (pairs + bn - 1) // bn + E
     i32 = lambda *s: torch.empty(*s, dtype=torch.int32, device=dev)
     pos, src, tiles, meta = i32(pairs), i32(pairs), i32(max_tiles, 4), i32(2)
@@ -204,10 +204,17 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
                                  N._p(meta[1:]), pairs, H, N._p(xs.codes), L(_pitch(xs.codes)), N._p(xs.scale), L(pairs), N._stream()), "gather_e4m3")
     group = dict(tiles=tiles, n_tiles=meta, max_tiles=max_tiles, bn=bn)
     _gemm(xs, pk["gu"], pk["gus"], h1.codes, pairs, I, H, True, I, act=act, out_scale=h1.scale, group_rows=2 * I, **group)
-    ys = torch.empty(pairs, H, dtype=torch.float32, device=dev)
-    _gemm(h1, pk["dn"], pk["dns"], ys, pairs, H, I, group_rows=H, col_scale=row_w, **group)
-    add32, add16 = (None, None) if add is None else (add, None) if add.dtype == torch.float32 else (None, add)
+    add32, add16 = (None, None) if add is None else (add.contiguous(), None) if add.dtype == torch.float32 else (None, add.contiguous())
     o16, o32 = (out, None) if out_dtype == torch.bfloat16 else (None, out)
-    N._check(lib.xft_moe_combine(N._p(ys), N._p(pos), k, N._p(add32), N._p(add16), H, N._p(o16), N._p(o32), T, H, N._stream()), "moe_combine")
+    if bn >= 128:
+        # prompts: a pair's row waits for the sum in bf16, half the bytes; the routing weights come in with the fp32 sum
+        ys = torch.empty(pairs, H, dtype=torch.bfloat16, device=dev)
+        _gemm(h1, pk["dn"], pk["dns"], ys, pairs, H, I, group_rows=H, **group)
+        N._check(lib.xft_moe_combine_bf16(N._p(ys), N._p(pos), N._p(w32), k, N._p(add32), N._p(add16), H, N._p(o16), N._p(o32), T, H, N._stream()),
+                 "moe_combine")
+    else:
+        ys = torch.empty(pairs, H, dtype=torch.float32, device=dev)
+        _gemm(h1, pk["dn"], pk["dns"], ys, pairs, H, I, group_rows=H, col_scale=row_w, **group)
+        N._check(lib.xft_moe_combine(N._p(ys), N._p(pos), k, N._p(add32), N._p(add16), H, N._p(o16), N._p(o32), T, H, N._stream()), "moe_combine")
     ws.launches += 3
     return out
