@@ -114,7 +114,7 @@ struct E4Layout {
   static constexpr int STAGE = (SRC == kSrcU4 ? RAW_BYTES : A_BYTES) + B_BYTES;       // what TMA fills
   static constexpr int A_RING = SRC == kSrcU4 ? 2 * A_BYTES : 0;                      // expanded codes, two buffers
   // two CTAs per SM where registers allow: one CTA's last accumulators and stores hide behind the other's stream
-  static constexpr int CTAS = BN <= 32 && A_RING + 3 * STAGE <= 110 * 1024 ? 2 : 1;
+  static constexpr int CTAS = (BN <= 32 || (SRC == kSrcRows && !DUAL)) && A_RING + 3 * STAGE <= 110 * 1024 ? 2 : 1;
   // Registers are left for the CTAs of the kernels behind: with programmatic launches those sit beside this one, their first weights
   // under way.  At 90 registers (16 rows, bf16) instead of 64 the products of a 7B layer were as fast one behind the other, but 31 steps
   // of one row over 16 layers took 48.3 ms instead of 46.3.
@@ -142,7 +142,10 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
   // 64 rows fetch an accumulator as soon as its k is through, beside the main loop; fewer rows all at once at the end, where a short
   // stream pays for one wait and not for four.
   constexpr bool EARLY = PARTS > 1 && BN == 64;
-  constexpr int BUFS = BLOCKS ? 2 : PARTS;
+  // Accumulators in turn: rows in e4m3 are half the columns of split ones, so four fit; fetching one and giving it back takes longer than the
+  // MMAs of a block.  us with two / four: 33 x 7168 x 16384 34.4 / 26.5, 1 x 12288 x 4096 13.1 / 11.9.
+  constexpr int TURN = SRC == kSrcRows ? 4 : 2;
+  constexpr int BUFS = BLOCKS ? TURN : PARTS;
   constexpr uint32_t TMEM_COLS = BUFS * ACC < 32 ? 32 : BUFS * ACC;
   static_assert(TMEM_COLS * L::CTAS <= 512, "accumulators of the resident CTAs");
   constexpr uint32_t IDESC = SRC == kSrcI8 ? umma_idesc(128, BN, 1, 1, 2) : SRC == kSrcBf16 ? umma_idesc(128, BN, 1, 1, 1) : umma_idesc(128, NB, 0, 0, 1);
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full[PARTS > 2 ? PARTS : 2], tmem_empty[2], a_ready[2], a_empty[2];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full[PARTS > TURN ? PARTS : TURN], tmem_empty[TURN], a_ready[2], a_empty[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ int s_group[4];
   __shared__ float s_ssq[SRC == kSrcBf16 ? BN : 1];                    // bf16: sums of squares of the tokens over this CTA's k
@@ -181,7 +184,8 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       mbar_init(&a_ready[a], 8);
       mbar_init(&a_empty[a], 1);
     }
-    for (int a = 2; a < PARTS; ++a) mbar_init(&tmem_full[a], 1);
+    for (int a = 2; a < (PARTS > TURN ? PARTS : TURN); ++a) mbar_init(&tmem_full[a], 1);
+    for (int a = 2; a < TURN; ++a) mbar_init(&tmem_empty[a], 8);
     fence_barrier_init();
     fence_proxy_async();
     tma_prefetch_desc(&tmW);
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       Ring r = {0, 0}, b = {0, 0};                                     // stage; buffer of expanded codes or accumulator
       int in_part = 0, part = 0;                                       // blocks in this accumulator; which it is
       bool ok = true;
-      for (int kb = kb0; kb < kend; ++kb, r.next(STAGES), b.next(2)) {
+      for (int kb = kb0; kb < kend; ++kb, r.next(STAGES), b.next(TURN)) {
         if (BLOCKS) ok = mbar_wait(&tmem_empty[b.s], b.ph ^ 1, p.status, XFT_ERR_WAIT_TMEM);
         ok = ok && mbar_wait(&full_bar[r.s], r.ph, p.status, XFT_ERR_WAIT_FULL);
         if (SRC == kSrcU4) ok = ok && mbar_wait(&a_ready[b.s], b.ph, p.status, XFT_ERR_WAIT_FULL);
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
               if constexpr (DUAL) g[NACC - 1][j + k] = fmaf(s * uf[i], __uint_as_float(v[NACC - 1][j + k]), g[NACC - 1][j + k]);
             }
           }
-          b.next(2);
+          b.next(TURN);
         }
       }
     } else if constexpr (SRC == kSrcI8 || SRC == kSrcBf16) {

@@ -106,11 +106,14 @@ def test_refusals():
 
 def test_mirror_of_the_kernels_parameters():
     from xfastertransformer_b200.ops import native as N
-    from xfastertransformer_b200.ops.native_e4m3 import RowsGemm
+    from xfastertransformer_b200.ops.native_e4m3 import ROWS_GEMM
     fn = N.lib().xft_rows_gemm_layout
     got = (C.c_longlong * 64)()
     n = fn(got, 64)
-    assert list(got[:n]) == [C.sizeof(RowsGemm)] + [getattr(RowsGemm, f).offset for f, _ in RowsGemm._fields_]
+    sizes = [8] * 12 + [8] * 2 + [4] * 18 + [4]                       # pointers, pitches, sizes, a factor: what ROWS_GEMM packs
+    assert n == 1 + len(sizes) and ROWS_GEMM.format == "@12P2q18if"
+    assert list(got[1:n]) == [sum(sizes[:i]) for i in range(len(sizes))]
+    assert ROWS_GEMM.size == sum(sizes) and ROWS_GEMM.size <= got[0] <= ROWS_GEMM.size + 4      # the struct may be padded at its end
 
 
 # -- models -----------------------------------------------------------------------------------------------------------

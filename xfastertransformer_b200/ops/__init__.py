@@ -150,26 +150,33 @@ def linear_gated(x, W, act="silu", bias=None, limit=0.0):
 _ROW_ACTS = (None, "none", "relu", "silu", "gelu", "gelu_tanh", "gelu_new", "gelu_pytorch_tanh", "relu2", "gelu_erf", "tanh", "swiglu")
 
 
+_e4m3 = None
+
+
 def _native_e4m3():
-    from . import native_e4m3
-    return native_e4m3
+    global _e4m3
+    if _e4m3 is None:
+        from . import native_e4m3 as _e4m3
+    return _e4m3
 
 
-def _same_device(what, *tensors):
-    d = [t.device for t in tensors if t is not None]
-    if any(x != d[0] for x in d):
-        raise ValueError(f"{what}: tensors on {', '.join(sorted({str(x) for x in d}))}")
+def _same_device(what, first, *tensors):
+    d = first.device
+    for t in tensors:
+        if t is not None and t.device != d:
+            raise ValueError(f"{what}: tensors on {d} and on {t.device}")
 
 
 def _check_rows_e4m3(what, q, W, act):
     if not isinstance(q, RowsE4M3):
         raise ValueError(f"{what} multiplies rows in e4m3 (RowsE4M3), not {type(q).__name__}")
+    n, k = W.out_features, W.in_features
     if W.kind not in ("fp8", "fp8a") or W.block != _BLOCK:
         raise ValueError(f"{what}: weights are e4m3 with a scale for each block of {_BLOCK}, not {W.kind}")
-    if q.shape[1] != W.in_features:
-        raise ValueError(f"{what}: rows of {q.shape[1]} columns and weights of {W.in_features}")
-    if tuple(W.scale.shape) != (-(-W.out_features // _BLOCK), -(-W.in_features // _BLOCK)):
-        raise ValueError(f"{what}: block scales {tuple(W.scale.shape)} of weights [{W.out_features}, {W.in_features}]")
+    if q.codes.shape[1] != k:
+        raise ValueError(f"{what}: rows of {q.shape[1]} columns and weights of {k}")
+    if W.scale.shape != (-(-n // _BLOCK), -(-k // _BLOCK)):
+        raise ValueError(f"{what}: block scales {tuple(W.scale.shape)} of weights [{n}, {k}]")
     if act not in _ROW_ACTS:
         raise ValueError(f"{what}: no activation {act!r}")
 
@@ -188,7 +195,7 @@ def rmsnorm_e4m3(x, w, eps, residual=None, want_rows=False):
     """RMSNorm(x + residual) * w on its way into products of 8-bit rows, in one launch: (rows in e4m3, the normalised rows in x's type or
     None, x + residual or None).  The sum is rounded once, to x's type, and the norm is of what was rounded; codes are taken from the
     fp32 norm.  `residual`: bf16 or fp32 (CPU: any float type), the shape of x.  `want_rows`: for what reads the norm beside the products."""
-    if x.dim() < 1 or tuple(w.shape) != (x.shape[-1],):
+    if x.dim() < 1 or w.shape != x.shape[-1:]:
         raise ValueError(f"rmsnorm_e4m3: gain {tuple(w.shape)} of rows {tuple(x.shape)}")
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"rmsnorm_e4m3: residual {tuple(residual.shape)} of rows {tuple(x.shape)}")
@@ -202,18 +209,19 @@ def linear_e4m3(q, W, bias=None, act=None, residual=None, res_scale=1.0, out_dty
     """act(rows W^T + bias) + res_scale * residual of rows in e4m3 and e4m3 weights (kinds "fp8" and "fp8a"): sums of 128 columns are
     scaled and added in fp32.  `out_dtype`: bf16 or fp32; the activation type of the device by default (bf16 on a GPU)."""
     _check_rows_e4m3("linear_e4m3", q, W, act)
-    T, N = q.shape[0], W.out_features
-    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.float32):
+    T, N = q.codes.shape[0], W.out_features
+    if bias is not None and (bias.shape != (N,) or bias.dtype is not torch.float32):
         raise ValueError(f"linear_e4m3: the bias of {N} features is fp32 [{N}], not {tuple(bias.shape)} in {bias.dtype}")
     if residual is not None and (residual.shape[-1] != N or residual.numel() != T * N):
         raise ValueError(f"linear_e4m3: residual {tuple(residual.shape)} of a result [{T}, {N}]")
     if out_dtype not in (None, torch.bfloat16, torch.float32):
         raise ValueError(f"linear_e4m3: results are bf16 or fp32, not {out_dtype}")
     _same_device("linear_e4m3", q.codes, W.w, W.scale, bias, residual)
-    if not q.is_cuda:
+    if not q.codes.is_cuda:
         return R.linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype or torch.float32)
-    run = lambda: _native_e4m3().linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
-    return _timed("gemm_e4m3", q, W, run) if _verbose() else run()
+    if _verbose():
+        return _timed("gemm_e4m3", q, W, lambda: _native_e4m3().linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype or torch.bfloat16))
+    return _native_e4m3().linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
 
 
 def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
@@ -222,7 +230,7 @@ def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
     _check_rows_e4m3("linear_gated_e4m3", q, W, act)
     if W.out_features % (2 * _BLOCK):
         raise ValueError(f"linear_gated_e4m3: gate and up have a multiple of {_BLOCK} features each, not {W.out_features / 2:g}")
-    if bias is not None and (tuple(bias.shape) != (W.out_features,) or bias.dtype != torch.float32):
+    if bias is not None and (bias.shape != (W.out_features,) or bias.dtype is not torch.float32):
         raise ValueError(f"linear_gated_e4m3: the bias is fp32 [{W.out_features}], not {tuple(bias.shape)} in {bias.dtype}")
     _same_device("linear_gated_e4m3", q.codes, W.w, W.scale, bias)
     impl = _native_e4m3().linear_gated_e4m3 if q.is_cuda else R.linear_gated_e4m3

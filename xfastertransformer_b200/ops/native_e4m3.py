@@ -2,10 +2,12 @@
 (csrc/kernels/gemm_e4m3_sm100.cu; prompts: csrc/kernels/gemm_rows_e4m3_sm100.cu) and the experts' form of both.
 
 Nothing here keeps scratch between calls, so calls on several streams and captured graphs do not touch one another; the kernels run on
-the device of their rows, on that device's current stream."""
+the device of their rows, on that device's current stream.  A step of a small model is bound by the host, so arguments go over as one
+packed struct or as plain numbers."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -14,53 +16,59 @@ from .rows import BLOCK, RowsE4M3
 
 MAX_COLS = 32768               # of a row that is quantised: it stays in registers
 
+# csrc/kernels/rows_e4m3.cuh:RowsGemm, field after field: x, x_scale, w, w_scale, out, out_scale, bias, residual, group_tiles, num_group_tiles,
+# col_scale, status | x_ld, out_ld | x_rows, ldx, w_rows, ldw, scale_ld, T, N, K, ldo, out_fp32, ldr, act, gated, dual_off, group_w_rows,
+# max_tiles, bn, form | res_scale
+ROWS_GEMM = struct.Struct("@12P2q18if")
+_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+_ARGS = {"xft_rows_e4m3": [_P, _L, _P, _L, _I, _P, _F, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P],
+         "xft_gather_e4m3": [_P, _L, _P, _L, _P, _P, _I, _I, _P, _L, _P, _L, _P],
+         "xft_gemm_rows_e4m3": [C.c_char_p, _P]}
+_fns = None
 
-class RowsGemm(C.Structure):
-    """Mirror of the struct of the same name in csrc/kernels/rows_e4m3.cuh."""
-    _fields_ = [("x", C.c_void_p), ("x_scale", C.c_void_p), ("w", C.c_void_p), ("w_scale", C.c_void_p), ("out", C.c_void_p),
-                ("out_scale", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("group_tiles", C.c_void_p),
-                ("num_group_tiles", C.c_void_p), ("col_scale", C.c_void_p), ("status", C.c_void_p), ("x_ld", C.c_longlong),
-                ("out_ld", C.c_longlong), ("x_rows", C.c_int), ("ldx", C.c_int), ("w_rows", C.c_int), ("ldw", C.c_int),
-                ("scale_ld", C.c_int), ("T", C.c_int), ("N", C.c_int), ("K", C.c_int), ("ldo", C.c_int), ("out_fp32", C.c_int),
-                ("ldr", C.c_int), ("act", C.c_int), ("gated", C.c_int), ("dual_off", C.c_int), ("group_w_rows", C.c_int),
-                ("max_tiles", C.c_int), ("bn", C.c_int), ("form", C.c_int), ("res_scale", C.c_float)]
 
+class _Lib:
+    """Entry points of the library with their argument types; the experts' plan and sum under names of their own, since others call them with
+    wrapped arguments."""
 
-_ready = False
+    def __init__(self):
+        lib = N.lib()
+        for name, args in _ARGS.items():
+            f = getattr(lib, name)
+            f.restype, f.argtypes = _I, args
+            setattr(self, name, f)
+        plain = lambda name, *args: C.CFUNCTYPE(_I, *args)((name, lib))
+        self.plan = plain("xft_moe_plan", _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _P)
+        self.combine = plain("xft_moe_combine", _P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P)
+        self.combine_bf16 = plain("xft_moe_combine_bf16", _P, _P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P)
 
 
 def _lib():
-    global _ready
-    lib = N.lib()
-    if not _ready:
-        for fn in ("xft_rows_e4m3", "xft_gather_e4m3", "xft_gemm_rows_e4m3", "xft_moe_plan", "xft_moe_combine", "xft_moe_combine_bf16"):
-            getattr(lib, fn).restype = C.c_int
-        _ready = True
-    return lib
+    global _fns
+    if _fns is None:
+        _fns = _Lib()
+    return _fns
 
 
-def _on(device):
-    """The device of the rows as the current one, for launches, allocations and the stream."""
-    return torch.cuda.device(device)
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def _foreign(t) -> bool:
-    return t.device.index != torch._C._cuda_getDevice()
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _foreign(device) -> bool:
+    """Whether `device` is another than the current one, which allocations, stream and launches would go to."""
+    return device.index != torch._C._cuda_getDevice()
 
 
 def new_rows(T, K, device) -> RowsE4M3:
     """Room for rows: codes on a pitch of 16 bytes, which the products' copies want."""
-    codes = torch.empty(T, (K + 15) // 16 * 16, dtype=torch.float8_e4m3fn, device=device)
-    return RowsE4M3(codes if K % 16 == 0 else codes[:, :K], torch.empty(-(-K // BLOCK), T, dtype=torch.float32, device=device))
+    codes = torch.empty((T, (K + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
+    return RowsE4M3.of(codes if K % 16 == 0 else codes[:, :K], torch.empty((-(-K // BLOCK), T), dtype=torch.float32, device=device))
 
 
 def _pitched(codes):
     """Codes whose rows start on 16 bytes (a copy where they do not)."""
-    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.data_ptr() % 16 == 0:
+    ld, one = codes.stride()
+    if one == 1 and ld % 16 == 0 and codes.data_ptr() % 16 == 0:
         return codes
     T, K = codes.shape
     own = torch.zeros(T, (K + 15) // 16 * 16, dtype=torch.uint8, device=codes.device)
@@ -78,36 +86,40 @@ def _scales(scale):
 
 def rows_e4m3(x, gain=None, eps=0.0, residual=None, want_rows=False):
     """(rows, normalised bf16 rows or None, x + residual or None), see ops.quantize_e4m3 and ops.rmsnorm_e4m3."""
-    if _foreign(x):
-        with _on(x.device):
+    dev = x.device
+    if _foreign(dev):
+        with torch.cuda.device(dev):
             return rows_e4m3(x, gain, eps, residual, want_rows)
+    K = x.shape[-1]
+    if x.dtype is not torch.bfloat16 or K % 8 or not 0 < K <= MAX_COLS:
+        raise N.KernelError(f"rows in e4m3 are made of bf16 rows of up to {MAX_COLS} columns, a multiple of 8 (got {K} in {x.dtype})")
     x2, ldx = N._rows2d(x)
-    T, K = x2.shape
-    if x2.dtype != torch.bfloat16 or K % 8 or not 0 < K <= MAX_COLS:
-        raise N.KernelError(f"rows in e4m3 are made of bf16 rows of up to {MAX_COLS} columns, a multiple of 8 (got {K} in {x2.dtype})")
-    q = new_rows(T, K, x.device)
-    y = torch.empty(T, K, dtype=torch.bfloat16, device=x.device) if want_rows else None
+    T = x2.shape[0]
+    q = new_rows(T, K, dev)
+    y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if want_rows else None
     h, r2, ldr, kind = None, None, 0, 0
     if residual is not None:
         if residual.dtype not in (torch.bfloat16, torch.float32):
             raise N.KernelError(f"a residual is bf16 or fp32, not {residual.dtype}")
         r2, ldr = N._rows2d(residual)
-        kind = 2 if r2.dtype == torch.float32 else 1
-        h = torch.empty(T, K, dtype=torch.bfloat16, device=x.device)
-    if gain is not None and (gain.dtype != torch.float32 or not gain.is_contiguous() or gain.data_ptr() % 16):
+        kind = 2 if r2.dtype is torch.float32 else 1
+        h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+    if gain is not None and (gain.dtype is not torch.float32 or not gain.is_contiguous() or gain.data_ptr() % 16):
         gain = gain.float().clone(memory_format=torch.contiguous_format)
-    L = C.c_longlong
-    N._check(_lib().xft_rows_e4m3(N._p(x2), L(ldx), N._p(r2), L(ldr), kind, N._p(gain), C.c_float(eps), T, K, N._p(q.codes), L(_pitch(q.codes)),
-                                  N._p(q.scale), L(T), N._p(h), L(K), N._p(y), L(K), N._stream()), "rows_e4m3")
-    N.Workspace.get(x.device).launches += 1
-    shape = x.shape
-    return q, y if y is None else y.view(shape), h if h is None else h.view(shape)
+    rc = _lib().xft_rows_e4m3(x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, kind, None if gain is None else gain.data_ptr(), eps,
+                              T, K, q.codes.data_ptr(), _pitch(q.codes), q.scale.data_ptr(), T, None if h is None else h.data_ptr(), K,
+                              None if y is None else y.data_ptr(), K, _stream())
+    if rc:
+        N._check(rc, "rows_e4m3")
+    N.Workspace.get(dev).launches += 1
+    return q, y, h
 
 
 def _weight(W):
     """The codes of W with rows on 16 bytes; the copy that this may take is kept with the weight."""
     w = W.w
-    if w.stride(0) % 16 or w.data_ptr() % 16 or w.stride(1) != 1:
+    ld, one = w.stride()
+    if ld % 16 or one != 1 or w.data_ptr() % 16:
         kept = W.cache.get("w_pitch16")
         if kept is None:
             kept = W.cache["w_pitch16"] = _pitched(w)
@@ -119,44 +131,46 @@ def _gemm(q, w, w_scale, out, T, n_out, K, gated=False, dual_off=0, bias=None, a
           tiles=None, n_tiles=None, group_rows=0, max_tiles=0, bn=0, col_scale=None, form=-1):
     codes, scale = _pitched(q.codes), _scales(q.scale)
     ws = N.Workspace.get(codes.device)
-    a = RowsGemm()
-    a.x, a.x_scale, a.w, a.w_scale = codes.data_ptr(), scale.data_ptr(), w.data_ptr(), w_scale.data_ptr()
-    a.out, a.out_scale, a.bias, a.residual = out.data_ptr(), _ptr(out_scale), _ptr(bias), _ptr(residual)
-    a.group_tiles, a.num_group_tiles, a.col_scale, a.status = _ptr(tiles), _ptr(n_tiles), _ptr(col_scale), ws.status.data_ptr()
-    a.x_ld = scale.stride(0) if scale.shape[0] > 1 else scale.shape[1]
-    a.out_ld = 0 if out_scale is None else out_scale.shape[1]
-    a.x_rows, a.ldx, a.w_rows, a.ldw, a.scale_ld = codes.shape[0], _pitch(codes), w.shape[0], _pitch(w), w_scale.shape[1]
-    a.T, a.N, a.K, a.ldo, a.out_fp32 = T, n_out, K, _pitch(out) if out_scale is not None else out.stride(0), int(out.dtype == torch.float32)
-    a.ldr, a.act = 0 if residual is None else residual.stride(0), N._ACT[act]
-    a.gated, a.dual_off, a.group_w_rows, a.max_tiles, a.bn, a.form, a.res_scale = int(gated), dual_off, group_rows, max_tiles, bn, form, res_scale
-    N._check(_lib().xft_gemm_rows_e4m3(C.byref(a), N._stream()), "gemm_rows_e4m3")
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    a = ROWS_GEMM.pack(codes.data_ptr(), scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), out.data_ptr(), ptr(out_scale), ptr(bias),
+                       ptr(residual), ptr(tiles), ptr(n_tiles), ptr(col_scale), ws.status.data_ptr(),
+                       scale.stride(0) if scale.shape[0] > 1 else scale.shape[1], 0 if out_scale is None else out_scale.shape[1],
+                       codes.shape[0], _pitch(codes), w.shape[0], _pitch(w), w_scale.shape[1], T, n_out, K,
+                       out.stride(0) if out_scale is None else _pitch(out), out.dtype is torch.float32,
+                       0 if residual is None else residual.stride(0), N._ACT[act], gated, dual_off, group_rows, max_tiles, bn, form, res_scale)
+    rc = _lib().xft_gemm_rows_e4m3(a, _stream())
+    if rc:
+        N._check(rc, "gemm_rows_e4m3")
     ws.launches += 1
 
 
 def linear_e4m3(q, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=torch.bfloat16):
-    if _foreign(q):
-        with _on(q.device):
+    dev = q.codes.device
+    if _foreign(dev):
+        with torch.cuda.device(dev):
             return linear_e4m3(q, W, bias, act, residual, res_scale, out_dtype)
-    T, K = q.shape
+    T, K = q.codes.shape
     if residual is not None:
-        residual = residual.reshape(-1, residual.shape[-1])
-        if residual.dtype != torch.bfloat16:
+        if residual.dtype is not torch.bfloat16:
             raise N.KernelError(f"the residual of a product is bf16, not {residual.dtype}")
+        if residual.dim() != 2:
+            residual = residual.reshape(-1, residual.shape[-1])
         if residual.stride(1) != 1:
             residual = residual.contiguous()
-    out = torch.empty(T, W.out_features, dtype=out_dtype, device=q.device)
+    out = torch.empty((T, W.out_features), dtype=out_dtype, device=dev)
     if T:
         _gemm(q, _weight(W), W.scale, out, T, W.out_features, K, False, 0, bias, act, residual, res_scale)
     return out
 
 
 def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
-    if _foreign(q):
-        with _on(q.device):
+    dev = q.codes.device
+    if _foreign(dev):
+        with torch.cuda.device(dev):
             return linear_gated_e4m3(q, W, act, bias)
-    T, K = q.shape
+    T, K = q.codes.shape
     I = W.out_features // 2
-    out = new_rows(T, I, q.device)
+    out = new_rows(T, I, dev)
     if T:
         _gemm(q, _weight(W), W.scale, out.codes, T, I, K, True, I, bias, act, out_scale=out.scale)
     return out
@@ -178,43 +192,54 @@ def pack_experts(experts) -> dict:
 
 
 def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=None, expected_pairs=None, add=None, out_dtype=torch.float32):
-    if _foreign(q):
-        with _on(q.device):
+    dev = q.codes.device
+    if _foreign(dev):
+        with torch.cuda.device(dev):
             return moe_experts_e4m3(q, idx, w, experts, act, expert_offset, packed, expected_pairs, add, out_dtype)
     pk = packed or pack_experts(experts)
-    (T, H), k, dev = q.shape, idx.shape[1], q.device
+    (T, H), k = q.codes.shape, idx.shape[1]
     E, I = pk["E"], pk["I"]
-    out = torch.empty(T, H, dtype=out_dtype, device=dev)
+    out = torch.empty((T, H), dtype=out_dtype, device=dev)
     if T == 0:
         return out
-    ws, lib = N.Workspace.get(dev), _lib()
+    ws, lib, st = N.Workspace.get(dev), _lib(), _stream()
     pairs = T * k
     avg = max(1, ((pairs if expected_pairs is None else min(int(expected_pairs), pairs)) + E - 1) // E)
     bn = 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 64 else 128 if avg < 512 else 256
     max_tiles = (pairs + bn - 1) // bn + E
-    i32 = lambda *s: torch.empty(*s, dtype=torch.int32, device=dev)
-    pos, src, tiles, meta = i32(pairs), i32(pairs), i32(max_tiles, 4), i32(2)
-    row_w = torch.empty(pairs, dtype=torch.float32, device=dev)
-    idx32, w32 = (idx if idx.dtype == torch.int32 else idx.int()).contiguous(), w.float().contiguous()
-    N._check(lib.xft_moe_plan(N._p(idx32), N._p(w32), T, k, expert_offset, expert_offset + E, bn, N._p(pos), N._p(src), N._p(row_w),
-                              N._p(tiles), N._p(meta), max_tiles, pairs, N._stream()), "moe_plan")
-    codes, scale, L = _pitched(q.codes), _scales(q.scale), C.c_longlong
-    xs, h1 = new_rows(pairs, H, dev), new_rows(pairs, I, dev)
-    N._check(lib.xft_gather_e4m3(N._p(codes), L(_pitch(codes)), N._p(scale), L(scale.stride(0) if scale.shape[0] > 1 else T), N._p(src),
-                                 N._p(meta[1:]), pairs, H, N._p(xs.codes), L(_pitch(xs.codes)), N._p(xs.scale), L(pairs), N._stream()), "gather_e4m3")
-    group = dict(tiles=tiles, n_tiles=meta, max_tiles=max_tiles, bn=bn)
-    _gemm(xs, pk["gu"], pk["gus"], h1.codes, pairs, I, H, True, I, act=act, out_scale=h1.scale, group_rows=2 * I, **group)
-    add32, add16 = (None, None) if add is None else (add.contiguous(), None) if add.dtype == torch.float32 else (None, add.contiguous())
-    o16, o32 = (out, None) if out_dtype == torch.bfloat16 else (None, out)
-    if bn >= 128:
-        # prompts: a pair's row waits for the sum in bf16, half the bytes; the routing weights come in with the fp32 sum
-        ys = torch.empty(pairs, H, dtype=torch.bfloat16, device=dev)
-        _gemm(h1, pk["dn"], pk["dns"], ys, pairs, H, I, group_rows=H, **group)
-        N._check(lib.xft_moe_combine_bf16(N._p(ys), N._p(pos), N._p(w32), k, N._p(add32), N._p(add16), H, N._p(o16), N._p(o32), T, H, N._stream()),
-                 "moe_combine")
+    # one allocation for everything between the rows and the sum (a step of a small model is bound by the host): the plan's tiles, positions,
+    # sources, weights and counts, the gathered rows, the middle rows and the pairs' results
+    prompt = bn >= 128
+    places, size = [], 0
+    for n in (16 * max_tiles, 4 * pairs, 4 * pairs, 4 * pairs, 8, pairs * H, 4 * pairs * (H // BLOCK), pairs * I, 4 * pairs * (I // BLOCK),
+              (2 if prompt else 4) * pairs * H):
+        places.append(size)
+        size += (n + 255) // 256 * 256
+    room = torch.empty(size, dtype=torch.uint8, device=dev)
+    base = room.data_ptr()
+    tiles, pos, src, row_w, meta, xc, xs, hc, hs, ys = [base + p for p in places]
+    idx32, w32 = (idx if idx.dtype is torch.int32 else idx.int()).contiguous(), w.float().contiguous()
+    N._check(lib.plan(idx32.data_ptr(), w32.data_ptr(), T, k, expert_offset, expert_offset + E, bn, pos, src, row_w, tiles, meta, max_tiles, pairs, st),
+             "moe_plan")
+    codes, scale = _pitched(q.codes), _scales(q.scale)
+    N._check(lib.xft_gather_e4m3(codes.data_ptr(), _pitch(codes), scale.data_ptr(), scale.stride(0) if scale.shape[0] > 1 else T, src, meta + 4,
+                                 pairs, H, xc, H, xs, pairs, st), "gather_e4m3")
+    gu, gus, dn, dns, status = pk["gu"], pk["gus"], pk["dn"], pk["dns"], ws.status.data_ptr()
+    a = ROWS_GEMM.pack(xc, xs, gu.data_ptr(), gus.data_ptr(), hc, hs, 0, 0, tiles, meta, 0, status, pairs, pairs, pairs, H, gu.shape[0], H,
+                       gus.shape[1], pairs, I, H, I, 0, 0, N._ACT[act], 1, I, 2 * I, max_tiles, bn, -1, 1.0)
+    N._check(lib.xft_gemm_rows_e4m3(a, st), "experts' gate_up")
+    # prompts: a pair's row waits for the sum in bf16, half the bytes; the routing weights come in with the fp32 sum
+    a = ROWS_GEMM.pack(hc, hs, dn.data_ptr(), dns.data_ptr(), ys, 0, 0, 0, tiles, meta, 0 if prompt else row_w, status, pairs, 0, pairs, I,
+                       dn.shape[0], I, dns.shape[1], pairs, H, I, H, not prompt, 0, 0, 0, 0, H, max_tiles, bn, -1, 1.0)
+    N._check(lib.xft_gemm_rows_e4m3(a, st), "experts' down")
+    if add is not None and not add.is_contiguous():
+        add = add.contiguous()
+    add32, add16 = (0, 0) if add is None else (add.data_ptr(), 0) if add.dtype is torch.float32 else (0, add.data_ptr())
+    o16, o32 = (out.data_ptr(), 0) if out_dtype is torch.bfloat16 else (0, out.data_ptr())
+    if prompt:
+        rc = lib.combine_bf16(ys, pos, w32.data_ptr(), k, add32, add16, H, o16, o32, T, H, st)
     else:
-        ys = torch.empty(pairs, H, dtype=torch.float32, device=dev)
-        _gemm(h1, pk["dn"], pk["dns"], ys, pairs, H, I, group_rows=H, col_scale=row_w, **group)
-        N._check(lib.xft_moe_combine(N._p(ys), N._p(pos), k, N._p(add32), N._p(add16), H, N._p(o16), N._p(o32), T, H, N._stream()), "moe_combine")
-    ws.launches += 3
+        rc = lib.combine(ys, pos, k, add32, add16, H, o16, o32, T, H, st)
+    N._check(rc, "moe_combine")
+    ws.launches += 5
     return out

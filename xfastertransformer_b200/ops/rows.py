@@ -18,12 +18,19 @@ class RowsE4M3:
     scale: torch.Tensor
 
     def __post_init__(self):
-        if self.codes.dim() != 2 or self.codes.dtype != torch.float8_e4m3fn:
+        if self.codes.dim() != 2 or self.codes.dtype is not torch.float8_e4m3fn:
             raise ValueError(f"rows in e4m3 have codes [T, K] in float8_e4m3fn, not {tuple(self.codes.shape)} in {self.codes.dtype}")
         T, K = self.codes.shape
-        if tuple(self.scale.shape) != (-(-K // BLOCK), T) or self.scale.dtype != torch.float32 or self.scale.device != self.codes.device:
+        if self.scale.shape != (-(-K // BLOCK), T) or self.scale.dtype is not torch.float32 or self.scale.device != self.codes.device:
             raise ValueError(f"{T} rows of {K} columns need fp32 scales [{-(-K // BLOCK)}, {T}] on their device, not "
                              f"{tuple(self.scale.shape)} in {self.scale.dtype}")
+
+    @classmethod
+    def of(cls, codes, scale) -> "RowsE4M3":
+        """Rows that were made to fit, unchecked."""
+        q = cls.__new__(cls)
+        q.codes, q.scale = codes, scale
+        return q
 
     @property
     def shape(self):
