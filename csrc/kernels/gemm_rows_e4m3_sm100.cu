@@ -133,10 +133,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
   const int4* groups = reinterpret_cast<const int4*>(p.g.group_tiles);
   const int total = p.n_tiles * (groups ? min(*p.g.num_group_tiles, p.t_tiles) : p.t_tiles);
   struct Item { int nt, row0, rows, w0; };                             // feature tile, first token row, rows, first weight row of its group
-  auto item_of = [&](int item) {
+  auto entry_of = [&](int item) { return groups && item < total ? __ldg(groups + item / p.n_tiles) : make_int4(0, 0, 0, 0); };
+  auto item_of = [&](int item, int4 e) {
     Item r;
     if (groups) {
-      const int4 e = groups[item / p.n_tiles];
       r = {item % p.n_tiles, e.y, e.z, e.x * p.g.group_w_rows};
     } else {
       const int per = p.gn * p.t_tiles, gr = item / per, at = item % per, gn = min(p.gn, p.n_tiles - gr * p.gn);
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         Ring r = {0, 0};
         bool ok = true;
         for (int item = first; item < total && ok; item += step) {
-          const Item im = item_of(item);
+          const Item im = item_of(item, entry_of(item));
           const int wrow = im.w0 + im.nt * FEAT + half * (DUAL ? p.g.dual_off : NCOL / 2);
           for (int kb = 0; kb < p.num_kb; ++kb, r.next(STAGES)) {
             ok = rows_wait(&empty_bar[r.s], r.ph ^ 1, status, XFT_ERR_WAIT_EMPTY, lost);
@@ -240,30 +240,39 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     Ring b = {0, 0};
     bool ok = true;
     int turn = 0;
-    for (int item = first; item < total; item += step, turn ^= 1) {
-      const Item im = item_of(item);
-      const int t = im.row0 + row, n0 = im.nt * FEAT + col0;
-      const bool t_ok = row < im.rows;
-      const float* sx = p.g.x_scale + t;
-      const float* sw = p.g.w_scale + (size_t)((im.w0 + n0) >> 7) * p.g.scale_ld;
-      const float* su = sw + (size_t)(p.g.dual_off >> 7) * p.g.scale_ld;
-      const bool w_ok = n0 < p.g.N;                                    // a last tile may have no features on this side
-      // Scales of two blocks at a time, asked for two blocks ahead: a load from L2 takes longer than a block, and a value that moves
-      // from one register to the next waits for its load.
-      float xs[2], ws[2], us[2];
-      auto fetch_scales = [&](int kb) {
+    // Scales of two blocks at a time, asked for two blocks ahead: a load from L2 takes longer than a block, and a value that moves from one
+    // register to the next waits for its load.  The first ones of an item are asked for before the item in front of it is finished.
+    int t = 0, n0 = 0, nt = 0;
+    bool t_ok = false, w_ok = false;
+    const float *sx = nullptr, *sw = nullptr, *su = nullptr;
+    float xs[2], ws[2], us[2];
+    auto fetch_scales = [&](int kb) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bool in = kb + i < p.num_kb;
-          xs[i] = in && t_ok ? __ldg(sx + (size_t)(kb + i) * p.g.x_ld) : 0.f;
-          ws[i] = in && w_ok ? __ldg(sw + kb + i) : 0.f;
-          if (DUAL) us[i] = in && w_ok ? __ldg(su + kb + i) : 0.f;
-        }
-      };
+      for (int i = 0; i < 2; ++i) {
+        const bool in = kb + i < p.num_kb;
+        xs[i] = in && t_ok ? __ldg(sx + (size_t)(kb + i) * p.g.x_ld) : 0.f;
+        ws[i] = in && w_ok ? __ldg(sw + kb + i) : 0.f;
+        if (DUAL) us[i] = in && w_ok ? __ldg(su + kb + i) : 0.f;
+      }
+    };
+    auto begin = [&](int item, int4 e) {
+      const Item im = item_of(item, e);
+      nt = im.nt;
+      t = im.row0 + row;
+      n0 = nt * FEAT + col0;
+      t_ok = row < im.rows;
+      w_ok = n0 < p.g.N;                                               // a last tile may have no features on this side
+      sx = p.g.x_scale + t;
+      sw = p.g.w_scale + (size_t)((im.w0 + n0) >> 7) * p.g.scale_ld;
+      su = sw + (size_t)(p.g.dual_off >> 7) * p.g.scale_ld;
+      fetch_scales(0);
+    };
+    if (first < total) begin(first, entry_of(first));
+    for (int item = first; item < total; item += step, turn ^= 1) {
+      const int4 e_next = entry_of(item + step);
       float acc[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
-      fetch_scales(0);
       for (int kb0 = 0; kb0 < p.num_kb && ok; kb0 += 2) {
         float f[2], fu[2];
 #pragma unroll
@@ -300,12 +309,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
       }
       // ---- epilogue of the item (all warps come through here, also after a wait that ran out: the barrier below counts them)
+      const int t_now = t, n_now = n0, nt_now = nt;
+      const bool t_in = t_ok;
+      if (item + step < total) begin(item + step, e_next);
       if constexpr (DUAL) {
         if (p.g.bias) {
 #pragma unroll
           for (int j = 0; j < PART; ++j) {
-            acc[j] += __ldg(p.g.bias + min(n0 + j, p.g.N - 1));
-            acc[PART + j] += __ldg(p.g.bias + p.g.dual_off + min(n0 + j, p.g.N - 1));
+            acc[j] += __ldg(p.g.bias + min(n_now + j, p.g.N - 1));
+            acc[PART + j] += __ldg(p.g.bias + p.g.dual_off + min(n_now + j, p.g.N - 1));
           }
         }
 #pragma unroll
@@ -319,9 +331,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
           s_top[turn][side][row] = top;
           named_bar_sync(1, 256);
           top = fmaxf(s_top[turn][0][row], s_top[turn][1][row]);
-          if (t_ok && ok) {
+          if (t_in && ok) {
             const E4m3Scale s = e4m3_scale(top);
-            uint8_t* to = reinterpret_cast<uint8_t*>(p.g.out) + (size_t)t * p.g.ldo + n0;
+            uint8_t* to = reinterpret_cast<uint8_t*>(p.g.out) + (size_t)t_now * p.g.ldo + n_now;
 #pragma unroll
             for (int j = 0; j < PART; j += 16) {
               uint32_t c[4];
@@ -330,18 +342,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
                 c[i] = e4m3_codes(acc[j + 4 * i], acc[j + 4 * i + 1], s.inv) | e4m3_codes(acc[j + 4 * i + 2], acc[j + 4 * i + 3], s.inv) << 16;
               *reinterpret_cast<uint4*>(to + j) = make_uint4(c[0], c[1], c[2], c[3]);
             }
-            if (side == 0) p.g.out_scale[(size_t)im.nt * p.g.out_ld + t] = s.scale;
+            if (side == 0) p.g.out_scale[(size_t)nt_now * p.g.out_ld + t_now] = s.scale;
           }
           continue;
         }
       }
-      if (!t_ok || !ok) continue;
-      const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr : nullptr;
-      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo;
-      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t * p.g.ldo;
+      if (!t_in || !ok) continue;
+      const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t_now * p.g.ldr : nullptr;
+      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t_now * p.g.ldo;
+      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t_now * p.g.ldo;
 #pragma unroll
       for (int c = 0; c < PART; c += 16) {
-        const int n = n0 + c;
+        const int n = n_now + c;
         if (n >= p.g.N) continue;
         const bool full = vec && n + 16 <= p.g.N;
         float* x = acc + c;

@@ -144,22 +144,6 @@ static int launch_rows_e4m3(const RowsE4m3Params& p, int rows, cudaStream_t st) 
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-// Rows of the experts' products: row r of the output is row src[r] of the input, codes and scales; rows from *used on are left alone.
-__global__ void __launch_bounds__(128) gather_e4m3_kernel(const uint8_t* __restrict__ codes, long long ldc, const float* __restrict__ scale,
-                                                          long long lds, const int* __restrict__ src, const int* __restrict__ used,
-                                                          uint8_t* __restrict__ out, long long ldo, float* __restrict__ out_scale,
-                                                          long long ldos, int K) {
-  grid_dep_launch();
-  grid_dep_wait();
-  const int r = blockIdx.x;
-  if (r >= *used) return;
-  const long long s = src[r];
-  const uint4* from = reinterpret_cast<const uint4*>(codes + s * ldc);
-  uint4* to = reinterpret_cast<uint4*>(out + (long long)r * ldo);
-  for (int i = threadIdx.x; i < (K + 15) / 16; i += 128) to[i] = from[i];
-  for (int i = threadIdx.x; i < (K + 127) / 128; i += 128) out_scale[i * ldos + r] = scale[i * lds + s];
-}
-
 }  // namespace xft
 
 using namespace xft;
@@ -181,14 +165,4 @@ extern "C" int xft_rows_e4m3(const void* x, long long ldx, const void* r, long l
   if (!gain) return launch_rows_e4m3<kNoResidual, false>(p, rows, st);
   if (r_kind == 0) return launch_rows_e4m3<kNoResidual, true>(p, rows, st);
   return r_kind == 1 ? launch_rows_e4m3<kResidualBf16, true>(p, rows, st) : launch_rows_e4m3<kResidualFp32, true>(p, rows, st);
-}
-
-// Rows of codes on 16 bytes, and as long as K rounded up to 16.
-extern "C" int xft_gather_e4m3(const void* codes, long long ldc, const float* scale, long long lds, const int* src, const int* used,
-                               int max_rows, int K, void* out, long long ldo, float* out_scale, long long ldos, cudaStream_t st) {
-  if (max_rows <= 0) return 0;
-  if (K <= 0 || (ldc & 15) || (ldo & 15) || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
-  const cudaError_t e = launch_pdl(gather_e4m3_kernel, dim3(max_rows), dim3(128), 0, st, (const uint8_t*)codes, ldc, scale, lds, src, used,
-                                   (uint8_t*)out, ldo, out_scale, ldos, K);
-  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }

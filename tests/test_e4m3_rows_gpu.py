@@ -135,8 +135,8 @@ def test_gated_tiles_of_prompts(T, I, K, form):
     a = R._act(y[:, :I], "silu")
     want = a * y[:, I:]
     err = 1.2 * tol[:, :I] * (y[:, I:].abs() + tol[:, I:]) + a.abs() * tol[:, I:] + 2.0 ** -18 * y[:, :I].abs() * y[:, I:].abs()
-    out = E.new_rows(T, I, torch.device("cuda", 0))
     dq, dW = rows_on(q), on(W)
+    out = E.new_rows(T, I, dq.codes)
     E._gemm(dq, E._weight(dW), dW.scale, out.codes, T, I, K, True, I, bias.cuda(), "silu", out_scale=out.scale, form=form)
     check_status()
     assert coded_error(out, want, err) <= 0 and scale_error(out, want, err) <= 0
@@ -287,6 +287,39 @@ def test_experts_of_a_part(T):
     assert torch.equal(got[0].cpu(), torch.zeros(H)) and torch.equal(got[1].cpu(), torch.zeros(H))
     bound = tol + 8 * 2.0 ** -24 * want.abs().amax(1, keepdim=True) + experts_half_step(q, idx, w, experts, 3)
     assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+# one CTA and a cluster of them, one round of pairs and several, an expert and 256, tiles of every size, indexes on both sides of the local ones
+@pytest.mark.parametrize("T,k,E,bn", [(1, 1, 1, 16), (5, 3, 4, 16), (31, 8, 256, 32), (1024, 2, 8, 64), (1025, 2, 8, 64), (2049, 1, 3, 128), (4096, 6, 64, 128),
+                                      (9000, 8, 32, 256), (40000, 2, 2, 256)])
+def test_plan_of_rows(T, k, E, bn):
+    from xfastertransformer_b200.ops import native_e4m3 as E4
+    g = gen(T, k, E)
+    e0, n = 5, T * k
+    idx = torch.randint(3, E + 7, (T, k), generator=g).int()
+    idx[torch.rand(T, k, generator=g) < 0.1] = -1
+    w = torch.rand(T, k, generator=g)
+    most = (n + bn - 1) // bn + E
+    i32 = lambda *s: torch.full(s, -7, dtype=torch.int32, device="cuda")
+    pos, src, tiles, meta, row_w = i32(n), i32(n), i32(most, 4), i32(2), torch.full((n,), -7.0, device="cuda")
+    di, dw = idx.cuda(), w.cuda()
+    assert E4._lib().xft_plan_rows(di.data_ptr(), dw.data_ptr(), T, k, e0, e0 + E, bn, pos.data_ptr(), src.data_ptr(), row_w.data_ptr(), tiles.data_ptr(),
+                                   meta.data_ptr(), most, E4._stream()) == 0
+    pos, src, row_w, tiles, meta = (t.cpu() for t in (pos, src, row_w, tiles, meta))
+    flat = idx.view(-1)
+    local = (flat >= e0) & (flat < e0 + E)
+    rows_ = int(local.sum())
+    counts = torch.bincount((flat[local] - e0).long(), minlength=E)
+    assert meta.tolist() == [int(((counts + bn - 1) // bn).sum()), rows_]
+    assert bool((pos[~local] == -1).all()) and torch.equal(pos[local].sort()[0], torch.arange(rows_, dtype=torch.int32))
+    start = torch.cumsum(counts, 0) - counts
+    e = (flat[local] - e0).long()
+    assert bool((pos[local] >= start[e]).all()) and bool((pos[local] < start[e] + counts[e]).all())
+    pair = local.nonzero()[:, 0]
+    at = pos[local].long()
+    assert torch.equal(src[at], (pair // k).int()) and torch.equal(row_w[at], w.view(-1)[pair])
+    want = [[i, int(start[i]) + j, min(bn, int(counts[i]) - j), 0] for i in range(E) for j in range(0, int(counts[i]), bn)]
+    assert tiles[:len(want)].tolist() == want and bool((src[rows_:] == -7).all())
 
 
 def test_experts_that_nobody_asks():

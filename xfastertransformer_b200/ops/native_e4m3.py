@@ -1,5 +1,6 @@
 """Bindings of the block-scaled e4m3 path, 8-bit weights and activations: rows in e4m3 (csrc/kernels/rows_e4m3.cu), their products
-(csrc/kernels/gemm_e4m3_sm100.cu; prompts: csrc/kernels/gemm_rows_e4m3_sm100.cu) and the experts' form of both.
+(csrc/kernels/gemm_e4m3_sm100.cu; prompts: csrc/kernels/gemm_rows_e4m3_sm100.cu) and what stands around those of experts
+(csrc/kernels/experts_e4m3.cu).
 
 Nothing here keeps scratch between calls, so calls on several streams and captured graphs do not touch one another; the kernels run on
 the device of their rows, on that device's current stream.  A step of a small model is bound by the host, so arguments go over as one
@@ -22,31 +23,20 @@ MAX_COLS = 32768               # of a row that is quantised: it stays in registe
 ROWS_GEMM = struct.Struct("@12P2q18if")
 _P, _I, _L, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
 _ARGS = {"xft_rows_e4m3": [_P, _L, _P, _L, _I, _P, _F, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P],
+         "xft_plan_rows": [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P],
+         "xft_sum_rows": [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _I, _P],
          "xft_gather_e4m3": [_P, _L, _P, _L, _P, _P, _I, _I, _P, _L, _P, _L, _P],
          "xft_gemm_rows_e4m3": [C.c_char_p, _P]}
 _fns = None
 
 
-class _Lib:
-    """Entry points of the library with their argument types; the experts' plan and sum under names of their own, since others call them with
-    wrapped arguments."""
-
-    def __init__(self):
-        lib = N.lib()
-        for name, args in _ARGS.items():
-            f = getattr(lib, name)
-            f.restype, f.argtypes = _I, args
-            setattr(self, name, f)
-        plain = lambda name, *args: C.CFUNCTYPE(_I, *args)((name, lib))
-        self.plan = plain("xft_moe_plan", _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _P)
-        self.combine = plain("xft_moe_combine", _P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P)
-        self.combine_bf16 = plain("xft_moe_combine_bf16", _P, _P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _P)
-
-
 def _lib():
     global _fns
     if _fns is None:
-        _fns = _Lib()
+        _fns = N.lib()
+        for name, args in _ARGS.items():
+            f = getattr(_fns, name)
+            f.restype, f.argtypes = _I, args
     return _fns
 
 
@@ -59,10 +49,10 @@ def _foreign(device) -> bool:
     return device.index != torch._C._cuda_getDevice()
 
 
-def new_rows(T, K, device) -> RowsE4M3:
-    """Room for rows: codes on a pitch of 16 bytes, which the products' copies want."""
-    codes = torch.empty((T, (K + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
-    return RowsE4M3.of(codes if K % 16 == 0 else codes[:, :K], torch.empty((-(-K // BLOCK), T), dtype=torch.float32, device=device))
+def new_rows(T, K, beside) -> RowsE4M3:
+    """Room for rows on the device of `beside`: codes on a pitch of 16 bytes, which the products' copies want."""
+    codes = beside.new_empty((T, (K + 15) // 16 * 16), dtype=torch.float8_e4m3fn)
+    return RowsE4M3.of(codes if K % 16 == 0 else codes[:, :K], beside.new_empty((-(-K // BLOCK), T), dtype=torch.float32))
 
 
 def _pitched(codes):
@@ -95,15 +85,16 @@ def rows_e4m3(x, gain=None, eps=0.0, residual=None, want_rows=False):
         raise N.KernelError(f"rows in e4m3 are made of bf16 rows of up to {MAX_COLS} columns, a multiple of 8 (got {K} in {x.dtype})")
     x2, ldx = N._rows2d(x)
     T = x2.shape[0]
-    q = new_rows(T, K, dev)
-    y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev) if want_rows else None
+    like = (lambda: torch.empty_like(x)) if x.is_contiguous() else (lambda: x.new_empty(x.shape))       # the cheapest of torch's ways
+    q = new_rows(T, K, x2)
+    y = like() if want_rows else None
     h, r2, ldr, kind = None, None, 0, 0
     if residual is not None:
         if residual.dtype not in (torch.bfloat16, torch.float32):
             raise N.KernelError(f"a residual is bf16 or fp32, not {residual.dtype}")
         r2, ldr = N._rows2d(residual)
         kind = 2 if r2.dtype is torch.float32 else 1
-        h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        h = like()
     if gain is not None and (gain.dtype is not torch.float32 or not gain.is_contiguous() or gain.data_ptr() % 16):
         gain = gain.float().clone(memory_format=torch.contiguous_format)
     rc = _lib().xft_rows_e4m3(x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, kind, None if gain is None else gain.data_ptr(), eps,
@@ -157,7 +148,7 @@ def linear_e4m3(q, W, bias=None, act=None, residual=None, res_scale=1.0, out_dty
             residual = residual.reshape(-1, residual.shape[-1])
         if residual.stride(1) != 1:
             residual = residual.contiguous()
-    out = torch.empty((T, W.out_features), dtype=out_dtype, device=dev)
+    out = q.codes.new_empty((T, W.out_features), dtype=out_dtype)
     if T:
         _gemm(q, _weight(W), W.scale, out, T, W.out_features, K, False, 0, bias, act, residual, res_scale)
     return out
@@ -170,7 +161,7 @@ def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
             return linear_gated_e4m3(q, W, act, bias)
     T, K = q.codes.shape
     I = W.out_features // 2
-    out = new_rows(T, I, dev)
+    out = new_rows(T, I, q.codes)
     if T:
         _gemm(q, _weight(W), W.scale, out.codes, T, I, K, True, I, bias, act, out_scale=out.scale)
     return out
@@ -199,7 +190,7 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
     pk = packed or pack_experts(experts)
     (T, H), k = q.codes.shape, idx.shape[1]
     E, I = pk["E"], pk["I"]
-    out = torch.empty((T, H), dtype=out_dtype, device=dev)
+    out = q.codes.new_empty((T, H), dtype=out_dtype)
     if T == 0:
         return out
     ws, lib, st = N.Workspace.get(dev), _lib(), _stream()
@@ -215,12 +206,12 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
               (2 if prompt else 4) * pairs * H):
         places.append(size)
         size += (n + 255) // 256 * 256
-    room = torch.empty(size, dtype=torch.uint8, device=dev)
+    room = q.codes.new_empty(size, dtype=torch.uint8)
     base = room.data_ptr()
     tiles, pos, src, row_w, meta, xc, xs, hc, hs, ys = [base + p for p in places]
     idx32, w32 = (idx if idx.dtype is torch.int32 else idx.int()).contiguous(), w.float().contiguous()
-    N._check(lib.plan(idx32.data_ptr(), w32.data_ptr(), T, k, expert_offset, expert_offset + E, bn, pos, src, row_w, tiles, meta, max_tiles, pairs, st),
-             "moe_plan")
+    N._check(lib.xft_plan_rows(idx32.data_ptr(), w32.data_ptr(), T, k, expert_offset, expert_offset + E, bn, pos, src, row_w, tiles, meta, max_tiles, st),
+             "plan_rows")
     codes, scale = _pitched(q.codes), _scales(q.scale)
     N._check(lib.xft_gather_e4m3(codes.data_ptr(), _pitch(codes), scale.data_ptr(), scale.stride(0) if scale.shape[0] > 1 else T, src, meta + 4,
                                  pairs, H, xc, H, xs, pairs, st), "gather_e4m3")
@@ -232,14 +223,10 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
     a = ROWS_GEMM.pack(hc, hs, dn.data_ptr(), dns.data_ptr(), ys, 0, 0, 0, tiles, meta, 0 if prompt else row_w, status, pairs, 0, pairs, I,
                        dn.shape[0], I, dns.shape[1], pairs, H, I, H, not prompt, 0, 0, 0, 0, H, max_tiles, bn, -1, 1.0)
     N._check(lib.xft_gemm_rows_e4m3(a, st), "experts' down")
-    if add is not None and not add.is_contiguous():
-        add = add.contiguous()
+    if add is not None and (not add.is_contiguous() or add.data_ptr() % 16):
+        add = add.clone(memory_format=torch.contiguous_format)
     add32, add16 = (0, 0) if add is None else (add.data_ptr(), 0) if add.dtype is torch.float32 else (0, add.data_ptr())
     o16, o32 = (out.data_ptr(), 0) if out_dtype is torch.bfloat16 else (0, out.data_ptr())
-    if prompt:
-        rc = lib.combine_bf16(ys, pos, w32.data_ptr(), k, add32, add16, H, o16, o32, T, H, st)
-    else:
-        rc = lib.combine(ys, pos, k, add32, add16, H, o16, o32, T, H, st)
-    N._check(rc, "moe_combine")
+    N._check(lib.xft_sum_rows(ys, not prompt, pos, w32.data_ptr() if prompt else 0, k, add32, add16, o32, o16, T, H, st), "sum_rows")
     ws.launches += 5
     return out
