@@ -111,7 +111,7 @@ struct RowsTile {
   static_assert((NCOL == 256 || (NCOL == 128 && !DUAL)) && (CG == 1 || CG == 2), "tile");
 };
 
-template <int NCOL, bool DUAL, int CG>
+template <int NCOL, bool DUAL, int CG, int SPLIT>
 __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                        const __grid_constant__ CUtensorMap tmW, const RowsTmParams p) {
   using L = RowsTile<NCOL, DUAL, CG>;
@@ -129,19 +129,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = CG == 2 ? (int)cluster_ctarank() : 0;              // which 128 tokens of a tile are this CTA's
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int part = SPLIT > 1 ? (int)cluster_ctarank() : 0;             // which part of k
+  const int first = blockIdx.x / (CG * SPLIT), step = gridDim.x / (CG * SPLIT);
+  const int k_lo = part * p.num_kb / SPLIT, k_hi = (part + 1) * p.num_kb / SPLIT;
   const int4* groups = reinterpret_cast<const int4*>(p.g.group_tiles);
   const int total = p.n_tiles * (groups ? min(*p.g.num_group_tiles, p.t_tiles) : p.t_tiles);
   struct Item { int nt, row0, rows, w0; };                             // feature tile, first token row, rows, first weight row of its group
-  auto entry_of = [&](int item) { return groups && item < total ? __ldg(groups + item / p.n_tiles) : make_int4(0, 0, 0, 0); };
+  // `gn` feature tiles walk all token tiles together (the tiles of an expert follow one another, so its weights are read once)
+  const int per = p.gn * (groups ? min(*p.g.num_group_tiles, p.t_tiles) : p.t_tiles);
+  auto entry_of = [&](int item) {
+    if (!groups || item >= total) return make_int4(0, 0, 0, 0);
+    const int gr = item / per;
+    return __ldg(groups + (item - gr * per) / min(p.gn, p.n_tiles - gr * p.gn));
+  };
   auto item_of = [&](int item, int4 e) {
     Item r;
-    if (groups) {
-      r = {item % p.n_tiles, e.y, e.z, e.x * p.g.group_w_rows};
-    } else {
-      const int per = p.gn * p.t_tiles, gr = item / per, at = item % per, gn = min(p.gn, p.n_tiles - gr * p.gn);
-      r = {gr * p.gn + at % gn, at / gn * TOK, p.g.T - at / gn * TOK, 0};
-    }
+    const int gr = item / per, at = item - gr * per, gn = min(p.gn, p.n_tiles - gr * p.gn), tt = at / gn;
+    if (groups) r = {gr * p.gn + at - tt * gn, e.y, e.z, e.x * p.g.group_w_rows};
+    else r = {gr * p.gn + at - tt * gn, tt * TOK, p.g.T - tt * TOK, 0};
     r.row0 += half * 128;
     r.rows -= half * 128;
     return r;
@@ -179,7 +184,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         for (int item = first; item < total && ok; item += step) {
           const Item im = item_of(item, entry_of(item));
           const int wrow = im.w0 + im.nt * FEAT + half * (DUAL ? p.g.dual_off : NCOL / 2);
-          for (int kb = 0; kb < p.num_kb; ++kb, r.next(STAGES)) {
+          for (int kb = k_lo; kb < k_hi; ++kb, r.next(STAGES)) {
             ok = rows_wait(&empty_bar[r.s], r.ph ^ 1, status, XFT_ERR_WAIT_EMPTY, lost);
             if (!ok) break;
             uint8_t* a = smem + r.s * STAGE;
@@ -210,7 +215,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         Ring r = {0, 0}, b = {0, 0};
         bool ok = true;
         for (int item = first; item < total && ok; item += step) {
-          for (int kb = 0; kb < p.num_kb; ++kb, r.next(STAGES), b.next(2)) {
+          for (int kb = k_lo; kb < k_hi; ++kb, r.next(STAGES), b.next(2)) {
             ok = rows_wait(&tmem_empty[b.s], b.ph ^ 1, status, XFT_ERR_WAIT_TMEM, lost) &&
                  rows_wait(&full_bar[r.s], r.ph, status, XFT_ERR_WAIT_FULL, lost);
             if (!ok) break;
@@ -228,6 +233,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
       }
     }
+    if constexpr (SPLIT > 1) {          // the parts lie in shared memory
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
     // ---- a token and COLS columns per thread; gated: COLS / 2 gate columns, then their up columns
@@ -237,6 +247,60 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     const bool vec = p.g.N % 8 == 0 && p.g.ldo % 8 == 0 && (!p.g.residual || p.g.ldr % 8 == 0) &&
                      ((reinterpret_cast<uintptr_t>(p.g.out) | reinterpret_cast<uintptr_t>(p.g.residual)) & 15) == 0;
     const bool vec32 = vec && p.g.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
+    // 16 columns from n on of token t on their way out
+    auto store16 = [&](float* x, int t, int n) {
+      const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr : nullptr;
+      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo;
+      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t * p.g.ldo;
+      const bool full = vec && n + 16 <= p.g.N;
+      if constexpr (!DUAL) {
+        if (p.g.bias) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
+        }
+        rows_act(x, p.g.act);
+      }
+      if (rrow) {
+        if (full) {
+          uint4 res[2] = {reinterpret_cast<const uint4*>(rrow + n)[0], reinterpret_cast<const uint4*>(rrow + n)[1]};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
+            x[2 * j] += p.g.res_scale * f.x;
+            x[2 * j + 1] += p.g.res_scale * f.y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (n + j < p.g.N) x[j] += p.g.res_scale * __bfloat162float(rrow[n + j]);
+        }
+      }
+      if (p.g.out_fp32) {
+        if (full) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(frow + n)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) if (n + j < p.g.N) frow[n + j] = x[j];
+        }
+      } else if (full) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const __nv_bfloat162 o = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&o);
+        }
+        if (vec32) {
+          st_global_256(orow + n, w);
+        } else {
+          reinterpret_cast<uint4*>(orow + n)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          reinterpret_cast<uint4*>(orow + n)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) if (n + j < p.g.N) orow[n + j] = __float2bfloat16(x[j]);
+      }
+    };
     Ring b = {0, 0};
     bool ok = true;
     int turn = 0;
@@ -249,7 +313,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     auto fetch_scales = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const bool in = kb + i < p.num_kb;
+        const bool in = kb + i < k_hi;
         xs[i] = in && t_ok ? __ldg(sx + (size_t)(kb + i) * p.g.x_ld) : 0.f;
         ws[i] = in && w_ok ? __ldg(sw + kb + i) : 0.f;
         if (DUAL) us[i] = in && w_ok ? __ldg(su + kb + i) : 0.f;
@@ -265,7 +329,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
       sx = p.g.x_scale + t;
       sw = p.g.w_scale + (size_t)((im.w0 + n0) >> 7) * p.g.scale_ld;
       su = sw + (size_t)(p.g.dual_off >> 7) * p.g.scale_ld;
-      fetch_scales(0);
+      fetch_scales(k_lo);
     };
     if (first < total) begin(first, entry_of(first));
     for (int item = first; item < total; item += step, turn ^= 1) {
@@ -273,14 +337,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
       float acc[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
-      for (int kb0 = 0; kb0 < p.num_kb && ok; kb0 += 2) {
+      for (int kb0 = k_lo; kb0 < k_hi && ok; kb0 += 2) {
         float f[2], fu[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) { f[i] = xs[i] * ws[i]; fu[i] = DUAL ? xs[i] * us[i] : 0.f; }
         fetch_scales(kb0 + 2);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (kb0 + i >= p.num_kb) break;
+          if (kb0 + i >= k_hi) break;
           ok = __all_sync(0xffffffffu, rows_wait(&tmem_full[b.s], b.ph, status, XFT_ERR_WAIT_TMEM, lost));
           if (!ok) break;
           tcgen05_fence_after();
@@ -347,70 +411,42 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
           continue;
         }
       }
-      if (!t_in || !ok) continue;
-      const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t_now * p.g.ldr : nullptr;
-      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t_now * p.g.ldo;
-      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t_now * p.g.ldo;
+      if constexpr (SPLIT > 1) {
+        // One tile per cluster: every CTA leaves its part of the sums in its shared memory, whose stages the MMAs have all read, [column][token],
+        // and finishes NCOL / SPLIT columns from all parts, in the order of k.
+        float* mine = reinterpret_cast<float*>(smem);
 #pragma unroll
-      for (int c = 0; c < PART; c += 16) {
-        const int n = n_now + c;
-        if (n >= p.g.N) continue;
-        const bool full = vec && n + 16 <= p.g.N;
-        float* x = acc + c;
-        if constexpr (!DUAL) {
-          if (p.g.bias) {
+        for (int j = 0; j < COLS; ++j) mine[(col0 + j) * 128 + row] = acc[j];
+        cluster_arrive();
+        cluster_wait();
+        constexpr int OWN = NCOL / SPLIT / 2;                          // columns of a thread
+        const int c0 = part * (NCOL / SPLIT) + side * OWN;
+        const uint32_t at = smem_u32(mine) + (uint32_t)(c0 * 128 + row) * 4;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
-          }
-          rows_act(x, p.g.act);
+        for (int j = 0; j < OWN; ++j) acc[j] = 0.f;
+#pragma unroll
+        for (int r = 0; r < SPLIT; ++r) {
+          const uint32_t from = dsmem_addr(at, r);
+#pragma unroll
+          for (int j = 0; j < OWN; ++j) acc[j] += ld_dsmem(from + j * 512);
         }
-        if (rrow) {
-          if (full) {
-            uint4 res[2] = {reinterpret_cast<const uint4*>(rrow + n)[0], reinterpret_cast<const uint4*>(rrow + n)[1]};
+        if (t_in && ok) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
-              x[2 * j] += p.g.res_scale * f.x;
-              x[2 * j + 1] += p.g.res_scale * f.y;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (n + j < p.g.N) x[j] += p.g.res_scale * __bfloat162float(rrow[n + j]);
-          }
+          for (int c = 0; c < OWN; c += 16)
+            if (nt_now * FEAT + c0 + c < p.g.N) store16(acc + c, t_now, nt_now * FEAT + c0 + c);
         }
-        if (p.g.out_fp32) {
-          if (full) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(frow + n)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) if (n + j < p.g.N) frow[n + j] = x[j];
-          }
-        } else if (full) {
-          uint32_t w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const __nv_bfloat162 o = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&o);
-          }
-          if (vec32) {
-            st_global_256(orow + n, w);
-          } else {
-            reinterpret_cast<uint4*>(orow + n)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            reinterpret_cast<uint4*>(orow + n)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) if (n + j < p.g.N) orow[n + j] = __float2bfloat16(x[j]);
-        }
+        continue;
       }
+      if (!t_in || !ok) continue;
+#pragma unroll
+      for (int c = 0; c < PART; c += 16)
+        if (n_now + c < p.g.N) store16(acc + c, t_now, n_now + c);
     }
   }
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) {              // neither CTA's shared memory or accumulator goes while the other may still use it
+  if constexpr (CG == 2 || SPLIT > 1) { // no CTA's shared memory or accumulator goes while another may still use it
     cluster_arrive();
     cluster_wait();
   }
@@ -421,7 +457,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
   }
 }
 
-template <int NCOL, bool DUAL, int CG>
+template <int NCOL, bool DUAL, int CG, int SPLIT = 1>
 static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
   using L = RowsTile<NCOL, DUAL, CG>;
   RowsTmParams p{};
@@ -429,55 +465,63 @@ static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
   p.num_kb = (g.K + 127) / 128;
   p.n_tiles = (g.N + L::FEAT - 1) / L::FEAT;
   p.t_tiles = g.group_tiles ? g.max_tiles : (g.T + L::TOK - 1) / L::TOK;
-  p.gn = 8;
+  p.gn = g.group_tiles && p.n_tiles <= 16 ? p.n_tiles : 8;
   CUtensorMap tmW, tmX;
   int r = make_tensor_map(&tmW, g.w, (uint64_t)g.w_rows, (uint64_t)g.K, (uint64_t)g.ldw, (uint32_t)(DUAL ? L::FEAT : NCOL / CG), 1);
   if (r) return 1000 - r;
   r = encode_tensor_map(&tmX, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.ldx, 128, 1);
   if (r) return 2000 - r;
-  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG>;
+  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG, SPLIT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return 3000 + (int)e;
-  const long long total = (long long)p.n_tiles * p.t_tiles, slots = sms / CG > 0 ? sms / CG : 1;
+  const long long total = (long long)p.n_tiles * p.t_tiles, slots = SPLIT > 1 ? total : sms / CG > 0 ? sms / CG : 1;      // parts: a tile per cluster
+  if (total * CG * SPLIT > 0x7fffffffLL || (SPLIT > 1 && p.num_kb < SPLIT)) return -6;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((total < slots ? total : slots) * CG));
+  cfg.gridDim = dim3((unsigned)((total < slots ? total : slots) * CG * SPLIT));
   cfg.blockDim = dim3(kRowsThreads);
   cfg.dynamicSmemBytes = L::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.x = CG * SPLIT;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
+  cfg.numAttrs = CG * SPLIT > 1 ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, kernel, tmX, tmW, (const RowsTmParams)p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 // The tile that is expected to take least, or 0 for the weight-stream kernel (gemm_e4m3_sm100.cu), in us: what a launch costs, then rounds of
-// tiles, each of its blocks of k and its finish.  Fitted to a sweep on B200; tiles 1 / 2 / 3 / 4: 389 x 2112 x 7168 41 / 24 / 40 / 23, 512 x
-// 12288 x 4096 49 / 39 / 48 / 38, 4096 x 8192 x 8192 303 / 312 / 340 / 334; gated 600 x 2 x 11008 x 4096 86 / - / 72, 1500 x 2 x 14336 x
-// 4096 205 / - / 224; the other kernel 128 x 4096 x 4096 13.5, here 16.4.
+// tiles, each of its blocks of k and its finish.  Fitted to sweeps on B200; us of tiles 1 / 2 / 3 / 4: 512 x 12288 x 4096 49 / 39 / 48 / 38,
+// 4096 x 8192 x 8192 303 / 312 / 340 / 334; gated 600 x 2 x 11008 x 4096 86 / - / 72, 1500 x 2 x 14336 x 4096 205 / - / 224; of 0 / 4 / 5 / 6:
+// 128 x 4096 x 4096 12.1 / 14.2 / 12.1 / 11.3, 389 x 2112 x 7168 25.3 / 20.9 / 15.6 / 31.4, 389 x 1024 x 7168 15.8 / 21.3 / 15.1 / 12.3,
+// 600 x 4096 x 1024 20.1 / 12.2 / 21.7 / 36.8.
 int rows_form(int T, int N, int K, int gated, int sms) {
   const int kb = (K + 127) / 128, cols = gated ? 2 * N : N;
+  auto tiles = [&](int tok, int ncol) { return (long long)((T + tok - 1) / tok) * ((cols + ncol - 1) / ncol); };
   auto cost = [&](int tok, int ncol, int ctas, float block, float finish) {
-    const long long tiles = (long long)((T + tok - 1) / tok) * ((cols + ncol - 1) / ncol), slots = sms / ctas > 0 ? sms / ctas : 1;
-    return 5.f + (float)((tiles + slots - 1) / slots) * (kb * block + finish);
+    const long long slots = sms / ctas > 0 ? sms / ctas : 1;
+    return 3.5f + (float)((tiles(tok, ncol) + slots - 1) / slots) * (kb * block + finish);
   };
   const long long small = (long long)((T + 63) / 64) * ((N + 127) / 128);
   int parts = 1;
   while (parts < 8 && small * parts * 2 <= sms && kb / (parts * 2) >= 4) parts *= 2;
-  float best = 5.f + (float)((small * parts + sms - 1) / sms) * ((float)kb / parts * (gated ? 0.9f : 0.5f) + 1.5f);
+  float best = 4.5f + (float)((small * parts + sms - 1) / sms) * ((float)kb / parts * (gated ? 0.7f : 0.35f) + 1.7f);
   int form = 0;
-  const float costs[5] = {0.f, cost(256, 256, 2, 0.60f, 2.f), cost(256, 128, 2, 0.345f, 1.2f), cost(128, 256, 1, 0.62f, 2.f), cost(128, 128, 1, 0.34f, 1.f)};
-  for (int i = 1; i <= 4; ++i) {
-    if (gated && (i == 2 || i == 4)) continue;
-    if (costs[i] < best) { best = costs[i]; form = i; }
+  auto take = [&](int f, float c) { if (c < best) { best = c; form = f; } };
+  take(1, cost(256, 256, 2, 0.60f, 2.f));
+  take(3, cost(128, 256, 1, 0.62f, 2.f));
+  if (!gated) {
+    take(2, cost(256, 128, 2, 0.345f, 1.2f));
+    take(4, cost(128, 128, 1, 0.34f, 1.f));
+    if (tiles(128, 128) * 2 <= sms && kb >= 4) take(5, 6.7f + kb * 0.17f);
+    if (tiles(128, 128) * 4 <= sms && kb >= 8) take(6, 7.5f + kb * 0.085f);
   }
   return form;
 }
 
-// Tiles: 1 = 256 tokens x 256 columns on two CTAs, 2 = 256 x 128 on two, 3 = 128 x 256, 4 = 128 x 128 (gated: 1 and 3).
+// Tiles: 1 = 256 tokens x 256 columns on two CTAs, 2 = 256 x 128 on two, 3 = 128 x 256, 4 = 128 x 128 (gated: 1 and 3); 5 and 6 = 128 x 128 with k cut into
+// two and four parts over a cluster.
 int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st) {
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
@@ -488,6 +532,8 @@ int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st) {
     case 1: return launch_rows_tm<256, false, 2>(g, sms, st);
     case 2: return launch_rows_tm<128, false, 2>(g, sms, st);
     case 3: return launch_rows_tm<256, false, 1>(g, sms, st);
+    case 5: return launch_rows_tm<128, false, 1, 2>(g, sms, st);
+    case 6: return launch_rows_tm<128, false, 1, 4>(g, sms, st);
     default: return launch_rows_tm<128, false, 1>(g, sms, st);
   }
 }

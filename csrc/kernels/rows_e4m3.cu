@@ -102,15 +102,26 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
     if constexpr (NORM) {
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
       if (i < nch) { a = __ldg(reinterpret_cast<const float4*>(p.gain) + 2 * i); b = __ldg(reinterpret_cast<const float4*>(p.gain) + 2 * i + 1); }
-      y[0] *= inv * a.x; y[1] *= inv * a.y; y[2] *= inv * a.z; y[3] *= inv * a.w;
-      y[4] *= inv * b.x; y[5] *= inv * b.y; y[6] *= inv * b.z; y[7] *= inv * b.w;
+      y[0] *= a.x; y[1] *= a.y; y[2] *= a.z; y[3] *= a.w;
+      y[4] *= b.x; y[5] *= b.y; y[6] *= b.z; y[7] *= b.w;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = e4m3_top(top, y[j]);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (i >= nch) continue;
-    const E4m3Scale s = e4m3_scale(top);
+    // The row's factor 1 / rms is in the scale alone where the block lies above the floor: it cancels in a code, whose rounding then sees one
+    // rounding of the product with the gain and two of the scaling.
+    E4m3Scale s;
+    if constexpr (!NORM) {
+      s = e4m3_scale(top);
+    } else if (top * inv < kE4m3Least) {
+      s = e4m3_scale(0.f);
+      s.inv *= inv;
+    } else {
+      s = e4m3_scale_of(top);
+      s.scale = __fdiv_rn(top * inv, kE4m3Top);
+    }
     uint2 q;
     q.x = e4m3_codes(y[0], y[1], s.inv) | e4m3_codes(y[2], y[3], s.inv) << 16;
     q.y = e4m3_codes(y[4], y[5], s.inv) | e4m3_codes(y[6], y[7], s.inv) << 16;
@@ -120,7 +131,7 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
       if (p.y) {
         uint4 u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) reinterpret_cast<__nv_bfloat162*>(&u)[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) reinterpret_cast<__nv_bfloat162*>(&u)[j] = __floats2bfloat162_rn(y[2 * j] * inv, y[2 * j + 1] * inv);
         reinterpret_cast<uint4*>(p.y + row * p.ldy)[i] = u;
       }
     }

@@ -18,10 +18,8 @@ __device__ __forceinline__ float e4m3_top(float top, float y) {
   const float a = fabsf(y);
   return a <= 3.4e38f ? fmaxf(top, a) : top;
 }
-__device__ __forceinline__ E4m3Scale e4m3_scale(float top) {
-  top = fmaxf(top, kE4m3Least);
-  return {__fdiv_rn(top, kE4m3Top), __fdiv_rn(kE4m3Top, top)};
-}
+__device__ __forceinline__ E4m3Scale e4m3_scale_of(float top) { return {__fdiv_rn(top, kE4m3Top), __fdiv_rn(kE4m3Top, top)}; }
+__device__ __forceinline__ E4m3Scale e4m3_scale(float top) { return e4m3_scale_of(fmaxf(top, kE4m3Least)); }
 // two codes, the first in the low byte
 __device__ __forceinline__ uint32_t e4m3_codes(float a, float b, float inv) {
   uint32_t v = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);

@@ -106,13 +106,15 @@ def test_product_matches_64_bits(T, N, K):
 
 # tiles of prompts, whatever the size would choose: one item and several per CTA, rows and features that end inside a tile, one block of k and
 # many, k that ends inside a block
-@pytest.mark.parametrize("form", [1, 2, 3, 4])
-@pytest.mark.parametrize("T,N,K", [(1, 8, 128), (100, 136, 16), (129, 256, 640), (257, 300, 1032), (300, 2112, 2048), (2000, 5000, 264), (9000, 1160, 128)])
+@pytest.mark.parametrize("form", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("T,N,K", [(1, 8, 128), (100, 136, 16), (65, 200, 520), (131, 256, 3000), (129, 256, 640), (257, 300, 1032), (300, 2112, 2048), (2000, 5000, 264), (9000, 1160, 128)])
 def test_tiles_of_prompts(T, N, K, form):
     from xfastertransformer_b200.ops import native_e4m3 as E
     g = gen(T, N, K)
     q, W = rows(activations(g, T, K)), weight(g, N, K)
     bias, res = torch.randn(N, generator=g), torch.randn(T, N, generator=g).bfloat16()
+    if form > 4 and -(-K // 128) < 2 * form - 8:
+        pytest.skip("fewer blocks of k than parts")
     want, tol = sum_tol(q, W)
     want = want + bias.double() + 0.5 * res.double()
     tol = tol + 2.0 ** -23 * (bias.double().abs() + res.double().abs() + want.abs())

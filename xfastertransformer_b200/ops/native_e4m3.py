@@ -182,6 +182,15 @@ def pack_experts(experts) -> dict:
     return native_moe.pack_experts(experts)
 
 
+def _tile_rows(avg) -> int:
+    """Rows of a tile for experts of `avg` rows on average: 16 and 32 rows on the weight stream, 128 and 256 on the kernel of prompts.  A tile
+    with fewer rows reads an expert's weights more often, one with more multiplies rows that are not there.  B200, us with 16 / 32 / 128 / 256
+    (64 lies between its neighbours everywhere): 64 experts of 1408 x 2048, average 0.8: 56 / 59 / 86 / 116, 6: 108 / 103 / 135 / 196, 19: 148 /
+    126 / 156 / 218, 66: 318 / 224 / 185 / 247, 384: 1630 / 1034 / 431 / 486; 8 of 14336 x 4096, 16: 275 / 273 / 274 / 381, 50: 458 / 330 / 283 /
+    394, 1024: - / - / 1712 / 1750, 2048: - / - / 3253 / 3183."""
+    return 16 if avg <= 4 else 32 if avg <= 32 else 128 if avg < 1536 else 256
+
+
 def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=None, expected_pairs=None, add=None, out_dtype=torch.float32):
     dev = q.codes.device
     if _foreign(dev):
@@ -196,7 +205,7 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
     ws, lib, st = N.Workspace.get(dev), _lib(), _stream()
     pairs = T * k
     avg = max(1, ((pairs if expected_pairs is None else min(int(expected_pairs), pairs)) + E - 1) // E)
-    bn = 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 64 else 128 if avg < 512 else 256
+    bn = _tile_rows(avg)
     max_tiles = (pairs + bn - 1) // bn + E
     # one allocation for everything between the rows and the sum (a step of a small model is bound by the host): the plan's tiles, positions,
     # sources, weights and counts, the gathered rows, the middle rows and the pairs' results
