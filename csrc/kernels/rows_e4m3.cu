@@ -7,6 +7,8 @@
 // bytes where rows are many, by the chain fetch, reduction, store where they are few.
 #include "rows_e4m3.cuh"
 
+#include <cstddef>
+
 namespace xft {
 
 struct RowsE4m3Params {
@@ -159,21 +161,38 @@ static int launch_rows_e4m3(const RowsE4m3Params& p, int rows, cudaStream_t st) 
 
 using namespace xft;
 
+// Arguments of xft_rows_e4m3 (packed by ops/native_e4m3.py).
+struct RowsArgs {
+  const void* x; const void* r; const float* gain; void* codes; float* scale; void* h; void* y;
+  long long ldx, ldr, ldc, lds, ldh, ldy;
+  int rows, K, r_kind; float eps;                // r_kind: 0 none, 1 bf16, 2 fp32
+};
+
+// Size and field offsets of RowsArgs, for the layout check of the Python side.
+extern "C" int xft_rows_args_layout(long long* out, int n) {
+  const long long v[] = {sizeof(RowsArgs),         offsetof(RowsArgs, x),     offsetof(RowsArgs, r),    offsetof(RowsArgs, gain),
+                         offsetof(RowsArgs, codes), offsetof(RowsArgs, scale), offsetof(RowsArgs, h),    offsetof(RowsArgs, y),
+                         offsetof(RowsArgs, ldx),  offsetof(RowsArgs, ldr),   offsetof(RowsArgs, ldc),  offsetof(RowsArgs, lds),
+                         offsetof(RowsArgs, ldh),  offsetof(RowsArgs, ldy),   offsetof(RowsArgs, rows), offsetof(RowsArgs, K),
+                         offsetof(RowsArgs, r_kind), offsetof(RowsArgs, eps)};
+  const int m = (int)(sizeof(v) / sizeof(v[0]));
+  for (int i = 0; i < m && i < n; ++i) out[i] = v[i];
+  return m;
+}
+
 // gain null: codes and scales of x [rows, K] (no residual).  K a multiple of 8, at most 32768; rows of x, r, h, y on 16 bytes, rows of
-// codes on 8, gain on 16.  r_kind: 0 none, 1 bf16, 2 fp32.
-extern "C" int xft_rows_e4m3(const void* x, long long ldx, const void* r, long long ldr, int r_kind, const float* gain, float eps, int rows,
-                             int K, void* codes, long long ldc, float* scale, long long lds, void* h, long long ldh, void* y,
-                             long long ldy, cudaStream_t st) {
-  if (rows <= 0) return 0;
-  if (K <= 0 || (K & 7) || K > 32768 || (ldx & 7) || (ldc & 7) || (ldh & 7) || (ldy & 7) || (ldr & (r_kind == 2 ? 3 : 7)) ||
-      (r_kind && (!r || !h || !gain)) ||
-      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(r) | reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(h) |
-        reinterpret_cast<uintptr_t>(y)) & 15) || (reinterpret_cast<uintptr_t>(codes) & 7))
+// codes on 8, gain on 16.
+extern "C" int xft_rows_e4m3(const RowsArgs* args, cudaStream_t st) {
+  const RowsArgs& a = *args;
+  auto on = [](const void* q, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(q) & (bytes - 1)) == 0; };
+  if (a.rows <= 0) return 0;
+  if (a.K <= 0 || (a.K & 7) || a.K > 32768 || (a.ldx & 7) || (a.ldc & 7) || (a.ldh & 7) || (a.ldy & 7) || (a.ldr & (a.r_kind == 2 ? 3 : 7)) ||
+      (a.r_kind && (!a.r || !a.h || !a.gain)) || !on(a.x, 16) || !on(a.r, 16) || !on(a.gain, 16) || !on(a.h, 16) || !on(a.y, 16) || !on(a.codes, 8))
     return -1;
   RowsE4m3Params p{};
-  p.x = (const __nv_bfloat16*)x; p.ldx = ldx; p.r = r; p.ldr = ldr; p.gain = gain; p.eps = eps; p.K = K; p.codes = (uint8_t*)codes; p.ldc = ldc;
-  p.scale = scale; p.lds = lds; p.h = (__nv_bfloat16*)h; p.ldh = ldh; p.y = (__nv_bfloat16*)y; p.ldy = ldy;
-  if (!gain) return launch_rows_e4m3<kNoResidual, false>(p, rows, st);
-  if (r_kind == 0) return launch_rows_e4m3<kNoResidual, true>(p, rows, st);
-  return r_kind == 1 ? launch_rows_e4m3<kResidualBf16, true>(p, rows, st) : launch_rows_e4m3<kResidualFp32, true>(p, rows, st);
+  p.x = (const __nv_bfloat16*)a.x; p.ldx = a.ldx; p.r = a.r; p.ldr = a.ldr; p.gain = a.gain; p.eps = a.eps; p.K = a.K; p.codes = (uint8_t*)a.codes;
+  p.ldc = a.ldc; p.scale = a.scale; p.lds = a.lds; p.h = (__nv_bfloat16*)a.h; p.ldh = a.ldh; p.y = (__nv_bfloat16*)a.y; p.ldy = a.ldy;
+  if (!a.gain) return launch_rows_e4m3<kNoResidual, false>(p, a.rows, st);
+  if (a.r_kind == 0) return launch_rows_e4m3<kNoResidual, true>(p, a.rows, st);
+  return a.r_kind == 1 ? launch_rows_e4m3<kResidualBf16, true>(p, a.rows, st) : launch_rows_e4m3<kResidualFp32, true>(p, a.rows, st);
 }

@@ -106,13 +106,18 @@ def test_refusals():
 
 def test_mirror_of_the_kernels_parameters():
     from xfastertransformer_b200.ops import native as N
-    from xfastertransformer_b200.ops.native_e4m3 import ROWS_GEMM
+    from xfastertransformer_b200.ops.native_e4m3 import ROWS_ARGS, ROWS_GEMM
     fn = N.lib().xft_rows_gemm_layout
     got = (C.c_longlong * 64)()
     n = fn(got, 64)
     sizes = [8] * 12 + [8] * 2 + [4] * 18 + [4]                       # pointers, pitches, sizes, a factor: what ROWS_GEMM packs
     assert n == 1 + len(sizes) and ROWS_GEMM.format == "@12P2q18if"
     assert list(got[1:n]) == [sum(sizes[:i]) for i in range(len(sizes))]
+    n = N.lib().xft_rows_args_layout(got, 64)
+    rows = [8] * 13 + [4] * 4
+    assert n == 1 + len(rows) and ROWS_ARGS.format == "@7P6q3if" and got[0] == ROWS_ARGS.size == sum(rows)
+    assert list(got[1:n]) == [sum(rows[:i]) for i in range(len(rows))]
+    n = fn(got, 64)
     assert ROWS_GEMM.size == sum(sizes) and ROWS_GEMM.size <= got[0] <= ROWS_GEMM.size + 4      # the struct may be padded at its end
 
 

@@ -64,9 +64,14 @@ def residual_norm(x, y, post, nxt, eps, kind="layer", rows=None, h_dtype=torch.b
 
 
 # -- GEMMs ---------------------------------------------------------------------------------
+_Env = None
+
+
 def _verbose() -> bool:
-    from ..utils.flags import Env
-    return Env.get().verbose >= 1
+    global _Env
+    if _Env is None:
+        from ..utils.flags import Env as _Env
+    return _Env.get().verbose >= 1
 
 
 def _timed(kernel: str, x, W, fn):

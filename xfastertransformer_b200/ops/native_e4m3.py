@@ -21,8 +21,10 @@ MAX_COLS = 32768               # of a row that is quantised: it stays in registe
 # col_scale, status | x_ld, out_ld | x_rows, ldx, w_rows, ldw, scale_ld, T, N, K, ldo, out_fp32, ldr, act, gated, dual_off, group_w_rows,
 # max_tiles, bn, form | res_scale
 ROWS_GEMM = struct.Struct("@12P2q18if")
-_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
-_ARGS = {"xft_rows_e4m3": [_P, _L, _P, _L, _I, _P, _F, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P],
+_P, _I, _L = C.c_void_p, C.c_int, C.c_longlong
+# csrc/kernels/rows_e4m3.cu:RowsArgs: x, r, gain, codes, scale, h, y | ldx, ldr, ldc, lds, ldh, ldy | rows, K, r_kind | eps
+ROWS_ARGS = struct.Struct("@7P6q3if")
+_ARGS = {"xft_rows_e4m3": [C.c_char_p, _P],
          "xft_plan_rows": [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P],
          "xft_sum_rows": [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _I, _P],
          "xft_gather_e4m3": [_P, _L, _P, _L, _P, _P, _I, _I, _P, _L, _P, _L, _P],
@@ -83,23 +85,25 @@ def rows_e4m3(x, gain=None, eps=0.0, residual=None, want_rows=False):
     K = x.shape[-1]
     if x.dtype is not torch.bfloat16 or K % 8 or not 0 < K <= MAX_COLS:
         raise N.KernelError(f"rows in e4m3 are made of bf16 rows of up to {MAX_COLS} columns, a multiple of 8 (got {K} in {x.dtype})")
-    x2, ldx = N._rows2d(x)
-    T = x2.shape[0]
-    like = (lambda: torch.empty_like(x)) if x.is_contiguous() else (lambda: x.new_empty(x.shape))       # the cheapest of torch's ways
+    whole = x.is_contiguous()
+    x2, ldx = (x, K) if whole and x.data_ptr() % 16 == 0 else N._rows2d(x)
+    T = x2.numel() // K
     q = new_rows(T, K, x2)
-    y = like() if want_rows else None
-    h, r2, ldr, kind = None, None, 0, 0
+    codes, y, h, r, ldr, kind = q.codes, None, None, 0, 0, 0
+    if want_rows:
+        y = torch.empty_like(x) if whole else x.new_empty(x.shape)           # (the cheaper of torch's ways where it gives whole rows)
     if residual is not None:
-        if residual.dtype not in (torch.bfloat16, torch.float32):
+        kind = 2 if residual.dtype is torch.float32 else 1
+        if kind == 1 and residual.dtype is not torch.bfloat16:
             raise N.KernelError(f"a residual is bf16 or fp32, not {residual.dtype}")
-        r2, ldr = N._rows2d(residual)
-        kind = 2 if r2.dtype is torch.float32 else 1
-        h = like()
+        r2, ldr = (residual, K) if residual.is_contiguous() and residual.data_ptr() % 16 == 0 else N._rows2d(residual)
+        r = r2.data_ptr()
+        h = torch.empty_like(x) if whole else x.new_empty(x.shape)
     if gain is not None and (gain.dtype is not torch.float32 or not gain.is_contiguous() or gain.data_ptr() % 16):
         gain = gain.float().clone(memory_format=torch.contiguous_format)
-    rc = _lib().xft_rows_e4m3(x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, kind, None if gain is None else gain.data_ptr(), eps,
-                              T, K, q.codes.data_ptr(), _pitch(q.codes), q.scale.data_ptr(), T, None if h is None else h.data_ptr(), K,
-                              None if y is None else y.data_ptr(), K, _stream())
+    a = ROWS_ARGS.pack(x2.data_ptr(), r, 0 if gain is None else gain.data_ptr(), codes.data_ptr(), q.scale.data_ptr(), 0 if h is None else h.data_ptr(),
+                       0 if y is None else y.data_ptr(), ldx, ldr, (K + 15) // 16 * 16, T, K, K, T, K, kind, eps)
+    rc = _lib().xft_rows_e4m3(a, _stream())
     if rc:
         N._check(rc, "rows_e4m3")
     N.Workspace.get(dev).launches += 1
