@@ -661,14 +661,12 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       }
       if constexpr (SRC == kSrcRows) {
         if (p.out_scale) {                                             // the warp has a block of 128 features of this token
-          float top = 0.f;
-#pragma unroll
-          for (int f = 0; f < 4; ++f) top = e4m3_top(top, out[f]);
+          bool odd;
+          float top = e4m3_top<4>(out, odd);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const E4m3Scale s = e4m3_scale(top);
-          reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + t * p.ldo)[n >> 2] =
-              e4m3_codes(out[0], out[1], s.inv) | e4m3_codes(out[2], out[3], s.inv) << 16;
+          reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + t * p.ldo)[n >> 2] = e4m3_codes(out, s.inv, odd);
           if (lane == 0) p.out_scale[(size_t)tile_n * p.out_ld + t] = s.scale;
           continue;
         }

@@ -389,9 +389,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
 #pragma unroll
         for (int j = 0; j < PART; ++j) acc[j] *= acc[PART + j];
         if (p.g.out_scale) {
-          float top = 0.f;
-#pragma unroll
-          for (int j = 0; j < PART; ++j) top = e4m3_top(top, acc[j]);
+          bool odd;
+          float top = e4m3_top<PART>(acc, odd);
           s_top[turn][side][row] = top;
           named_bar_sync(1, 256);
           top = fmaxf(s_top[turn][0][row], s_top[turn][1][row]);
@@ -402,8 +401,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
             for (int j = 0; j < PART; j += 16) {
               uint32_t c[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                c[i] = e4m3_codes(acc[j + 4 * i], acc[j + 4 * i + 1], s.inv) | e4m3_codes(acc[j + 4 * i + 2], acc[j + 4 * i + 3], s.inv) << 16;
+              for (int i = 0; i < 4; ++i) c[i] = e4m3_codes(acc + j + 4 * i, s.inv, odd);
               *reinterpret_cast<uint4*>(to + j) = make_uint4(c[0], c[1], c[2], c[3]);
             }
             if (side == 0) p.g.out_scale[(size_t)nt_now * p.g.out_ld + t_now] = s.scale;

@@ -95,7 +95,6 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
   for (int c = 0; c < CH; ++c) {
     const int i = tid + c * NT;
     float y[8];
-    float top = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = pair(c, j);
@@ -107,8 +106,8 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
       y[0] *= a.x; y[1] *= a.y; y[2] *= a.z; y[3] *= a.w;
       y[4] *= b.x; y[5] *= b.y; y[6] *= b.z; y[7] *= b.w;
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = e4m3_top(top, y[j]);
+    bool odd;
+    float top = e4m3_top<8>(y, odd);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (i >= nch) continue;
@@ -125,8 +124,8 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
       s.scale = __fdiv_rn(top * inv, kE4m3Top);
     }
     uint2 q;
-    q.x = e4m3_codes(y[0], y[1], s.inv) | e4m3_codes(y[2], y[3], s.inv) << 16;
-    q.y = e4m3_codes(y[4], y[5], s.inv) | e4m3_codes(y[6], y[7], s.inv) << 16;
+    q.x = e4m3_codes(y, s.inv, odd);
+    q.y = e4m3_codes(y + 4, s.inv, odd);
     reinterpret_cast<uint2*>(p.codes + row * p.ldc)[i] = q;
     if ((i & 15) == 0) p.scale[(i >> 4) * p.lds + row] = s.scale;
     if constexpr (NORM) {

@@ -14,18 +14,33 @@ constexpr float kE4m3Top = 448.f, kE4m3Least = 7.8886090522101181e-31f;       //
 
 struct E4m3Scale { float scale, inv; };
 
-__device__ __forceinline__ float e4m3_top(float top, float y) {
-  const float a = fabsf(y);
-  return a <= 3.4e38f ? fmaxf(top, a) : top;
+// max |v| over N values that are finite.  `odd`: there is an infinity among them (a NaN needs no care: maxima pass it over, and it converts to
+// its code).
+template <int N>
+__device__ __forceinline__ float e4m3_top(const float* v, bool& odd) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(v[j]));
+  odd = top > 3.4e38f;
+  if (odd) {
+    top = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(v[j]) <= 3.4e38f ? fabsf(v[j]) : 0.f);
+  }
+  return top;
 }
 __device__ __forceinline__ E4m3Scale e4m3_scale_of(float top) { return {__fdiv_rn(top, kE4m3Top), __fdiv_rn(kE4m3Top, top)}; }
 __device__ __forceinline__ E4m3Scale e4m3_scale(float top) { return e4m3_scale_of(fmaxf(top, kE4m3Least)); }
-// two codes, the first in the low byte
-__device__ __forceinline__ uint32_t e4m3_codes(float a, float b, float inv) {
-  uint32_t v = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
-  if (!(fabsf(a) <= 3.4e38f)) v = (v & 0xFF00u) | 0x7Fu;                      // the conversion saturates infinities
-  if (!(fabsf(b) <= 3.4e38f)) v = (v & 0x00FFu) | 0x7F00u;
-  return v;
+// four codes, the first in the low byte
+__device__ __forceinline__ uint32_t e4m3_codes(const float* v, float inv, bool odd) {
+  uint32_t q = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, __NV_E4M3) |
+               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2] * inv, v[3] * inv), __NV_SATFINITE, __NV_E4M3) << 16;
+  if (odd) {                                                                  // the conversion saturates infinities
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (!(fabsf(v[j]) <= 3.4e38f)) q = (q & ~(0xFFu << 8 * j)) | 0x7Fu << 8 * j;
+  }
+  return q;
 }
 
 // Arguments of xft_gemm_rows_e4m3 (mirrored in ops/native_e4m3.py).
