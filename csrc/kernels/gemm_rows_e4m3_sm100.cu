@@ -106,7 +106,8 @@ struct RowsTile {
   static constexpr int FEAT = DUAL ? NCOL / 2 : NCOL, TOK = 128 * CG;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = NCOL / CG * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int FIT = kRowsRing / STAGE, STAGES = FIT > 8 ? 8 : FIT;
-  static constexpr int SMEM = STAGES * STAGE + 1024;
+  static constexpr int LINES = DUAL ? 0 : 8 * 4096;                  // 32 tokens x 128 bytes of output per summing warp, behind the ring
+  static constexpr int SMEM = STAGES * STAGE + LINES + 1024;
   static constexpr int COLS = NCOL / 2;      // of a thread: two warps share 32 tokens
   static_assert((NCOL == 256 || (NCOL == 128 && !DUAL)) && (CG == 1 || CG == 2), "tile");
 };
@@ -246,7 +247,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     const int col0 = side * PART;
     const bool vec = p.g.N % 8 == 0 && p.g.ldo % 8 == 0 && (!p.g.residual || p.g.ldr % 8 == 0) &&
                      ((reinterpret_cast<uintptr_t>(p.g.out) | reinterpret_cast<uintptr_t>(p.g.residual)) & 15) == 0;
+    const bool codes32 = p.g.ldo % 32 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
     const bool vec32 = vec && p.g.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
+    const bool quick = vec && !p.g.out_fp32 && !p.g.bias && !p.g.act;
     // 16 columns from n on of token t on their way out
     auto store16 = [&](float* x, int t, int n) {
       const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr : nullptr;
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     int turn = 0;
     // Scales of two blocks at a time, asked for two blocks ahead: a load from L2 takes longer than a block, and a value that moves from one
     // register to the next waits for its load.  The first ones of an item are asked for before the item in front of it is finished.
-    int t = 0, n0 = 0, nt = 0;
+    int t = 0, n0 = 0, nt = 0, rows = 0;
     bool t_ok = false, w_ok = false;
     const float *sx = nullptr, *sw = nullptr, *su = nullptr;
     float xs[2], ws[2], us[2];
@@ -324,7 +327,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
       nt = im.nt;
       t = im.row0 + row;
       n0 = nt * FEAT + col0;
-      t_ok = row < im.rows;
+      rows = im.rows;
+      t_ok = row < rows;
       w_ok = n0 < p.g.N;                                               // a last tile may have no features on this side
       sx = p.g.x_scale + t;
       sw = p.g.w_scale + (size_t)((im.w0 + n0) >> 7) * p.g.scale_ld;
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
       }
       // ---- epilogue of the item (all warps come through here, also after a wait that ran out: the barrier below counts them)
-      const int t_now = t, n_now = n0, nt_now = nt;
+      const int t_now = t, n_now = n0, nt_now = nt, rows_now = rows;
       const bool t_in = t_ok;
       if (item + step < total) begin(item + step, e_next);
       if constexpr (DUAL) {
@@ -398,11 +402,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
             const E4m3Scale s = e4m3_scale(top);
             uint8_t* to = reinterpret_cast<uint8_t*>(p.g.out) + (size_t)t_now * p.g.ldo + n_now;
 #pragma unroll
-            for (int j = 0; j < PART; j += 16) {
-              uint32_t c[4];
+            for (int j = 0; j < PART; j += 32) {
+              uint32_t c[8];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) c[i] = e4m3_codes(acc + j + 4 * i, s.inv, odd);
-              *reinterpret_cast<uint4*>(to + j) = make_uint4(c[0], c[1], c[2], c[3]);
+              for (int i = 0; i < 8; ++i) c[i] = e4m3_codes(acc + j + 4 * i, s.inv, odd);
+              if (codes32) {                                           // whole sectors
+                st_global_256(to + j, c);
+              } else {
+                reinterpret_cast<uint4*>(to + j)[0] = make_uint4(c[0], c[1], c[2], c[3]);
+                reinterpret_cast<uint4*>(to + j)[1] = make_uint4(c[4], c[5], c[6], c[7]);
+              }
             }
             if (side == 0) p.g.out_scale[(size_t)nt_now * p.g.out_ld + t_now] = s.scale;
           }
@@ -434,6 +443,50 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
             if (nt_now * FEAT + c0 + c < p.g.N) store16(acc + c, t_now, nt_now * FEAT + c0 + c);
         }
         continue;
+      }
+      if constexpr (!DUAL) {
+        // bf16 rows without bias or activation, the whole run of columns: 64 columns of the warp's 32 tokens at a time through shared memory, so
+        // that a store fills 128-byte lines; all of the residual is on its way before the first value waits for it.  us of 24576 x 2048 x 1408
+        // as generic rows, one 16-column piece after the other / so: 110 / 90 (69 without any store).
+        if (quick && n_now + PART <= p.g.N) {
+          uint4 res[PART / 8];
+          if (p.g.residual && t_in) {
+            const uint4* r = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t_now * p.g.ldr + n_now);
+#pragma unroll
+            for (int j = 0; j < PART / 8; ++j) res[j] = __ldg(r + j);
+          }
+          uint8_t* line = smem + STAGES * STAGE + (warp - 4) * 4096;
+          const int most = ok ? rows_now - q * 32 : 0;                  // tokens of this warp
+          __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)(t_now - lane) * p.g.ldo + n_now;
+#pragma unroll
+          for (int c = 0; c < PART; c += 64) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float* x = acc + c + 8 * j;
+              if (p.g.residual && t_in) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&res[(c + 8 * j) / 8])[i]);
+                  x[2 * i] += p.g.res_scale * f.x;
+                  x[2 * i + 1] += p.g.res_scale * f.y;
+                }
+              }
+              uint4 w;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&w)[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+              *reinterpret_cast<uint4*>(line + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3), j = lane & 7;
+              const uint4 w = *reinterpret_cast<const uint4*>(line + r * 128 + ((j ^ (r & 7)) << 4));
+              if (r < most) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + c + 8 * j) = w;
+            }
+            __syncwarp();
+          }
+          continue;
+        }
       }
       if (!t_in || !ok) continue;
 #pragma unroll
@@ -490,10 +543,10 @@ static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
 }
 
 // The tile that is expected to take least, or 0 for the weight-stream kernel (gemm_e4m3_sm100.cu), in us: what a launch costs, then rounds of
-// tiles, each of its blocks of k and its finish.  Fitted to sweeps on B200; us of tiles 1 / 2 / 3 / 4: 512 x 12288 x 4096 49 / 39 / 48 / 38,
-// 4096 x 8192 x 8192 303 / 312 / 340 / 334; gated 600 x 2 x 11008 x 4096 86 / - / 72, 1500 x 2 x 14336 x 4096 205 / - / 224; of 0 / 4 / 5 / 6:
-// 128 x 4096 x 4096 12.1 / 14.2 / 12.1 / 11.3, 389 x 2112 x 7168 25.3 / 20.9 / 15.6 / 31.4, 389 x 1024 x 7168 15.8 / 21.3 / 15.1 / 12.3,
-// 600 x 4096 x 1024 20.1 / 12.2 / 21.7 / 36.8.
+// tiles, each of its blocks of k and its finish.  Fitted to sweeps on B200; us of tiles 1 / 2 / 3 / 4: 512 x 12288 x 4096 42 / 42 / 39 / 40,
+// 4096 x 8192 x 8192 261 / 334 / 254 / 341, 24576 x 2048 x 1408 97 / 119 / 90 / 112; gated 600 x 2 x 11008 x 4096 86 / - / 72, 1500 x 2 x 14336 x
+// 4096 205 / - / 224; of 0 / 4 / 5 / 6: 128 x 4096 x 4096 12.1 / 14.2 / 12.1 / 11.3, 389 x 2112 x 7168 25.3 / 20.9 / 15.6 / 31.4, 389 x 1024 x
+// 7168 15.8 / 21.3 / 15.1 / 12.3, 600 x 4096 x 1024 20.1 / 12.2 / 21.7 / 36.8.  Under the power cap 1 and 3 are within 4 % of each other.
 int rows_form(int T, int N, int K, int gated, int sms) {
   const int kb = (K + 127) / 128, cols = gated ? 2 * N : N;
   auto tiles = [&](int tok, int ncol) { return (long long)((T + tok - 1) / tok) * ((cols + ncol - 1) / ncol); };
@@ -507,11 +560,11 @@ int rows_form(int T, int N, int K, int gated, int sms) {
   float best = 4.5f + (float)((small * parts + sms - 1) / sms) * ((float)kb / parts * (gated ? 0.7f : 0.35f) + 1.7f);
   int form = 0;
   auto take = [&](int f, float c) { if (c < best) { best = c; form = f; } };
-  take(1, cost(256, 256, 2, 0.60f, 2.f));
-  take(3, cost(128, 256, 1, 0.62f, 2.f));
+  take(1, cost(256, 256, 2, 0.56f, 1.5f));
+  take(3, cost(128, 256, 1, 0.55f, 1.5f));
   if (!gated) {
-    take(2, cost(256, 128, 2, 0.345f, 1.2f));
-    take(4, cost(128, 128, 1, 0.34f, 1.f));
+    take(2, cost(256, 128, 2, 0.35f, 1.2f));
+    take(4, cost(128, 128, 1, 0.35f, 1.2f));
     if (tiles(128, 128) * 2 <= sms && kb >= 4) take(5, 6.7f + kb * 0.17f);
     if (tiles(128, 128) * 4 <= sms && kb >= 8) take(6, 7.5f + kb * 0.085f);
   }
