@@ -11,6 +11,8 @@
 // accumulators of a tile are finished and stored while the next tile's first two fill.
 #include "rows_e4m3.cuh"
 
+#include <type_traits>
+
 namespace xft {
 
 int encode_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
@@ -249,35 +251,43 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
                      ((reinterpret_cast<uintptr_t>(p.g.out) | reinterpret_cast<uintptr_t>(p.g.residual)) & 15) == 0;
     const bool codes32 = p.g.ldo % 32 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
     const bool vec32 = vec && p.g.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
-    const bool quick = vec && !p.g.out_fp32 && !p.g.bias && !p.g.act;
-    // 16 columns from n on of token t on their way out
-    auto store16 = [&](float* x, int t, int n) {
-      const __nv_bfloat16* rrow = p.g.residual ? reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr : nullptr;
-      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo;
-      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t * p.g.ldo;
-      const bool full = vec && n + 16 <= p.g.N;
+    // bias, activation (the gated form has its own) and residual on C columns from n on of token t; all of the residual is on its way before the
+    // first value waits for it
+    auto apply = [&](auto count, float* x, int t, int n, bool in) {
+      constexpr int C = decltype(count)::value;
       if constexpr (!DUAL) {
         if (p.g.bias) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
+          for (int j = 0; j < C; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
         }
-        rows_act(x, p.g.act);
-      }
-      if (rrow) {
-        if (full) {
-          uint4 res[2] = {reinterpret_cast<const uint4*>(rrow + n)[0], reinterpret_cast<const uint4*>(rrow + n)[1]};
+        if (p.g.act) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
-            x[2 * j] += p.g.res_scale * f.x;
-            x[2 * j + 1] += p.g.res_scale * f.y;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (n + j < p.g.N) x[j] += p.g.res_scale * __bfloat162float(rrow[n + j]);
+          for (int c = 0; c < C; c += 16) rows_act(x + c, p.g.act);
         }
       }
+      if (!p.g.residual || !in) return;
+      const __nv_bfloat16* rrow = reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr + n;
+      if (vec && n + C <= p.g.N) {
+        uint4 res[C / 8];
+#pragma unroll
+        for (int j = 0; j < C / 8; ++j) res[j] = __ldg(reinterpret_cast<const uint4*>(rrow) + j);
+#pragma unroll
+        for (int j = 0; j < C / 2; ++j) {
+          const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
+          x[2 * j] += p.g.res_scale * f.x;
+          x[2 * j + 1] += p.g.res_scale * f.y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (n + j < p.g.N) x[j] += p.g.res_scale * __bfloat162float(rrow[j]);
+      }
+    };
+    // 16 columns from n on of token t on their way out
+    auto store16 = [&](float* x, int t, int n) {
+      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo;
+      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t * p.g.ldo;
+      const bool full = vec && n + 16 <= p.g.N;
       if (p.g.out_fp32) {
         if (full) {
 #pragma unroll
@@ -437,6 +447,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
 #pragma unroll
           for (int j = 0; j < OWN; ++j) acc[j] += ld_dsmem(from + j * 512);
         }
+        apply(std::integral_constant<int, OWN>(), acc, t_now, nt_now * FEAT + c0, t_in);
         if (t_in && ok) {
 #pragma unroll
           for (int c = 0; c < OWN; c += 16)
@@ -444,46 +455,49 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
         continue;
       }
+      apply(std::integral_constant<int, PART>(), acc, t_now, n_now, t_in);
       if constexpr (!DUAL) {
-        // bf16 rows without bias or activation, the whole run of columns: 64 columns of the warp's 32 tokens at a time through shared memory, so
-        // that a store fills 128-byte lines; all of the residual is on its way before the first value waits for it.  us of 24576 x 2048 x 1408
-        // as generic rows, one 16-column piece after the other / so: 110 / 90 (69 without any store).
-        if (quick && n_now + PART <= p.g.N) {
-          uint4 res[PART / 8];
-          if (p.g.residual && t_in) {
-            const uint4* r = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t_now * p.g.ldr + n_now);
-#pragma unroll
-            for (int j = 0; j < PART / 8; ++j) res[j] = __ldg(r + j);
-          }
+        // The whole run of columns: 128 bytes of each of the warp's 32 tokens at a time through shared memory, so that a store fills lines.  us of
+        // 24576 x 2048 x 1408 with a lane's own 32 bytes per store, residual and branches piece by piece / so: 110 / 90 (69 without any store).
+        if (vec && n_now + PART <= p.g.N) {
           uint8_t* line = smem + STAGES * STAGE + (warp - 4) * 4096;
           const int most = ok ? rows_now - q * 32 : 0;                  // tokens of this warp
-          __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)(t_now - lane) * p.g.ldo + n_now;
-#pragma unroll
-          for (int c = 0; c < PART; c += 64) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              float* x = acc + c + 8 * j;
-              if (p.g.residual && t_in) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&res[(c + 8 * j) / 8])[i]);
-                  x[2 * i] += p.g.res_scale * f.x;
-                  x[2 * i + 1] += p.g.res_scale * f.y;
-                }
-              }
-              uint4 w;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&w)[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-              *reinterpret_cast<uint4*>(line + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
-            }
+          const size_t size = p.g.out_fp32 ? 4 : 2;
+          uint8_t* out = reinterpret_cast<uint8_t*>(p.g.out) + ((size_t)(t_now - lane) * p.g.ldo + n_now) * size;
+          auto leave = [&](int byte0) {                                // the line of every token, from byte0 of its run on
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = 4 * i + (lane >> 3), j = lane & 7;
               const uint4 w = *reinterpret_cast<const uint4*>(line + r * 128 + ((j ^ (r & 7)) << 4));
-              if (r < most) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + c + 8 * j) = w;
+              if (r < most) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo * size + byte0 + 16 * j) = w;
             }
             __syncwarp();
+          };
+          auto piece = [&](int j, uint4 w) { *reinterpret_cast<uint4*>(line + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; };
+          if (p.g.out_fp32) {
+#pragma unroll
+            for (int c = 0; c < PART; c += 32) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float* x = acc + c + 4 * j;
+                piece(j, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
+              }
+              leave(4 * c);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < PART; c += 64) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float* x = acc + c + 8 * j;
+                uint4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&w)[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                piece(j, w);
+              }
+              leave(2 * c);
+            }
           }
           continue;
         }
