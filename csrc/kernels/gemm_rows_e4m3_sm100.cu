@@ -108,13 +108,14 @@ struct RowsTile {
   static constexpr int FEAT = DUAL ? NCOL / 2 : NCOL, TOK = 128 * CG;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = NCOL / CG * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int FIT = kRowsRing / STAGE, STAGES = FIT > 8 ? 8 : FIT;
-  static constexpr int LINES = DUAL ? 0 : 8 * 4096;                  // 32 tokens x 128 bytes of output per summing warp, behind the ring
+  static constexpr int LINES = 8 * 4096;     // 32 tokens x 128 bytes of output per summing warp, behind the ring
   static constexpr int SMEM = STAGES * STAGE + LINES + 1024;
   static constexpr int COLS = NCOL / 2;      // of a thread: two warps share 32 tokens
   static_assert((NCOL == 256 || (NCOL == 128 && !DUAL)) && (CG == 1 || CG == 2), "tile");
 };
 
-template <int NCOL, bool DUAL, int CG, int SPLIT>
+// CODES: the gated form's result leaves as e4m3 rows.
+template <int NCOL, bool DUAL, int CG, int SPLIT, bool CODES>
 __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                        const __grid_constant__ CUtensorMap tmW, const RowsTmParams p) {
   using L = RowsTile<NCOL, DUAL, CG>;
@@ -126,7 +127,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], tmem_full[2], tmem_empty[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ int s_lost_mem;
-  __shared__ float s_top[2][2][DUAL ? 128 : 1];          // gated: largest value of a token over each half of the features, two items in turn
   volatile int* lost = &s_lost_mem;
   int* status = p.g.status;
 
@@ -250,10 +250,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     const bool vec = p.g.N % 8 == 0 && p.g.ldo % 8 == 0 && (!p.g.residual || p.g.ldr % 8 == 0) &&
                      ((reinterpret_cast<uintptr_t>(p.g.out) | reinterpret_cast<uintptr_t>(p.g.residual)) & 15) == 0;
     const bool codes32 = p.g.ldo % 32 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
-    const bool vec32 = vec && p.g.ldo % 16 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0;
-    // bias, activation (the gated form has its own) and residual on C columns from n on of token t; all of the residual is on its way before the
-    // first value waits for it
-    auto apply = [&](auto count, float* x, int t, int n, bool in) {
+    uint8_t* line = smem + STAGES * STAGE + (warp - 4) * 4096;        // 128 bytes of each of the warp's tokens, their 16-byte pieces interchanged
+    auto line_at = [&](int r, int byte) { return line + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15); };
+    // bias, activation (the gated form has its own) and residual on C columns from n on of token t, the warp's first `most` tokens being there; all of
+    // the residual is on its way before the first value waits for it
+    auto apply = [&](auto count, float* x, int t, int n, int most) {
+      const bool in = lane < most;
       constexpr int C = decltype(count)::value;
       if constexpr (!DUAL) {
         if (p.g.bias) {
@@ -265,9 +267,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
           for (int c = 0; c < C; c += 16) rows_act(x + c, p.g.act);
         }
       }
-      if (!p.g.residual || !in) return;
+      if (!p.g.residual) return;
       const __nv_bfloat16* rrow = reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr + n;
       if (vec && n + C <= p.g.N) {
+        if (!in) return;
         uint4 res[C / 8];
 #pragma unroll
         for (int j = 0; j < C / 8; ++j) res[j] = __ldg(reinterpret_cast<const uint4*>(rrow) + j);
@@ -278,40 +281,97 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
           x[2 * j + 1] += p.g.res_scale * f.y;
         }
       } else {
+        // rows that do not start on 16 bytes, or end inside the run: read along the row into the warp's lines, 64 columns at a time
+        const __nv_bfloat16* r0 = rrow - (size_t)lane * p.g.ldr;
 #pragma unroll
-        for (int j = 0; j < C; ++j)
-          if (n + j < p.g.N) x[j] += p.g.res_scale * __bfloat162float(rrow[j]);
+        for (int c = 0; c < C; c += 64) {
+          constexpr int W = C < 64 ? C : 64;
+          __syncwarp();
+#pragma unroll 1
+          for (int r8 = 0; r8 < 32; r8 += 8) {                         // eight tokens' loads under way together
+            __nv_bfloat16 v[8][(W + 31) / 32];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+              for (int h = 0; h < W; h += 32) {
+                const int col = h + lane;
+                v[r][h / 32] = col < W && r8 + r < most && n + c + col < p.g.N ? r0[(size_t)(r8 + r) * p.g.ldr + c + col] : __float2bfloat16(0.f);
+              }
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+              for (int h = 0; h < W; h += 32)
+                if (h + lane < W) *reinterpret_cast<__nv_bfloat16*>(line_at(r8 + r, 2 * (h + lane))) = v[r][h / 32];
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < W / 8; ++j) {
+            const uint4 u = *reinterpret_cast<const uint4*>(line_at(lane, 16 * j));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&u)[i]);
+              x[c + 8 * j + 2 * i] += p.g.res_scale * f.x;
+              x[c + 8 * j + 2 * i + 1] += p.g.res_scale * f.y;
+            }
+          }
+        }
+        __syncwarp();
       }
     };
-    // 16 columns from n on of token t on their way out
-    auto store16 = [&](float* x, int t, int n) {
-      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo;
-      float* frow = reinterpret_cast<float*>(p.g.out) + (size_t)t * p.g.ldo;
-      const bool full = vec && n + 16 <= p.g.N;
+    // C columns from n on of token t on their way out: 128 bytes of each token at a time through shared memory, so that a store fills lines; rows
+    // that do not start on 16 bytes, or end inside the run, leave element by element, along the row all the same.  us of 24576 x 2048 x 1408
+    // with a lane's own 32 bytes per store, residual and branches piece by piece / so: 110 / 90 (69 without any store).
+    auto leave = [&](auto count, const float* x, int t, int n, int most) {
+      constexpr int C = decltype(count)::value;
+      const bool whole = vec && n + C <= p.g.N;
+      auto pieces = [&](auto type, int c0) {                           // the lines hold columns c0 on, W of them
+        using OT = decltype(type);
+        constexpr int W = C < 128 / (int)sizeof(OT) ? C : 128 / (int)sizeof(OT), PIECES = W * (int)sizeof(OT) / 16;
+        OT* out = reinterpret_cast<OT*>(p.g.out) + (size_t)(t - lane) * p.g.ldo + n + c0;
+        __syncwarp();
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) {
+            const int r = 32 / PIECES * i + lane / PIECES, j = lane % PIECES;
+            const uint4 w = *reinterpret_cast<const uint4*>(line_at(r, 16 * j));
+            if (r < most) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + j * (16 / (int)sizeof(OT))) = w;
+          }
+        } else {
+#pragma unroll 4
+          for (int r = 0; r < 32; ++r)
+#pragma unroll
+            for (int h = 0; h < W; h += 32) {
+              const int col = h + lane;
+              if (col < W && r < most && n + c0 + col < p.g.N)
+                out[(size_t)r * p.g.ldo + col] = *reinterpret_cast<const OT*>(line_at(r, col * (int)sizeof(OT)));
+            }
+        }
+        __syncwarp();
+      };
       if (p.g.out_fp32) {
-        if (full) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(frow + n)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-        } else {
+        for (int c = 0; c < C; c += 32) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) if (n + j < p.g.N) frow[n + j] = x[j];
-        }
-      } else if (full) {
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const __nv_bfloat162 o = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&o);
-        }
-        if (vec32) {
-          st_global_256(orow + n, w);
-        } else {
-          reinterpret_cast<uint4*>(orow + n)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          reinterpret_cast<uint4*>(orow + n)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          for (int j = 0; j < (C < 32 ? C : 32) / 4; ++j) {
+            const float* v = x + c + 4 * j;
+            *reinterpret_cast<uint4*>(line_at(lane, 16 * j)) =
+                make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          }
+          pieces(float(), c);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) if (n + j < p.g.N) orow[n + j] = __float2bfloat16(x[j]);
+        for (int c = 0; c < C; c += 64) {
+#pragma unroll
+          for (int j = 0; j < (C < 64 ? C : 64) / 8; ++j) {
+            const float* v = x + c + 8 * j;
+            uint4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&w)[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            *reinterpret_cast<uint4*>(line_at(lane, 16 * j)) = w;
+          }
+          pieces(__nv_bfloat16(), c);
+        }
       }
     };
     Ring b = {0, 0};
@@ -402,12 +462,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         for (int c = 0; c < PART; c += 16) rows_act(acc + c, p.g.act);
 #pragma unroll
         for (int j = 0; j < PART; ++j) acc[j] *= acc[PART + j];
-        if (p.g.out_scale) {
+        if constexpr (CODES) {
           bool odd;
           float top = e4m3_top<PART>(acc, odd);
-          s_top[turn][side][row] = top;
+          float* tops = reinterpret_cast<float*>(smem + STAGES * STAGE);      // [two items in turn][side][token], where lines would be
+          tops[(turn * 2 + side) * 128 + row] = top;
           named_bar_sync(1, 256);
-          top = fmaxf(s_top[turn][0][row], s_top[turn][1][row]);
+          top = fmaxf(tops[turn * 256 + row], tops[turn * 256 + 128 + row]);
           if (t_in && ok) {
             const E4m3Scale s = e4m3_scale(top);
             uint8_t* to = reinterpret_cast<uint8_t*>(p.g.out) + (size_t)t_now * p.g.ldo + n_now;
@@ -447,65 +508,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
 #pragma unroll
           for (int j = 0; j < OWN; ++j) acc[j] += ld_dsmem(from + j * 512);
         }
-        apply(std::integral_constant<int, OWN>(), acc, t_now, nt_now * FEAT + c0, t_in);
-        if (t_in && ok) {
-#pragma unroll
-          for (int c = 0; c < OWN; c += 16)
-            if (nt_now * FEAT + c0 + c < p.g.N) store16(acc + c, t_now, nt_now * FEAT + c0 + c);
+        if (nt_now * FEAT + c0 < p.g.N) {
+          const int most = ok ? rows_now - q * 32 : 0;
+          apply(std::integral_constant<int, OWN>(), acc, t_now, nt_now * FEAT + c0, most);
+          leave(std::integral_constant<int, OWN>(), acc, t_now, nt_now * FEAT + c0, most);
         }
         continue;
       }
-      apply(std::integral_constant<int, PART>(), acc, t_now, n_now, t_in);
-      if constexpr (!DUAL) {
-        // The whole run of columns: 128 bytes of each of the warp's 32 tokens at a time through shared memory, so that a store fills lines.  us of
-        // 24576 x 2048 x 1408 with a lane's own 32 bytes per store, residual and branches piece by piece / so: 110 / 90 (69 without any store).
-        if (vec && n_now + PART <= p.g.N) {
-          uint8_t* line = smem + STAGES * STAGE + (warp - 4) * 4096;
-          const int most = ok ? rows_now - q * 32 : 0;                  // tokens of this warp
-          const size_t size = p.g.out_fp32 ? 4 : 2;
-          uint8_t* out = reinterpret_cast<uint8_t*>(p.g.out) + ((size_t)(t_now - lane) * p.g.ldo + n_now) * size;
-          auto leave = [&](int byte0) {                                // the line of every token, from byte0 of its run on
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + (lane >> 3), j = lane & 7;
-              const uint4 w = *reinterpret_cast<const uint4*>(line + r * 128 + ((j ^ (r & 7)) << 4));
-              if (r < most) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo * size + byte0 + 16 * j) = w;
-            }
-            __syncwarp();
-          };
-          auto piece = [&](int j, uint4 w) { *reinterpret_cast<uint4*>(line + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; };
-          if (p.g.out_fp32) {
-#pragma unroll
-            for (int c = 0; c < PART; c += 32) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float* x = acc + c + 4 * j;
-                piece(j, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
-              }
-              leave(4 * c);
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < PART; c += 64) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float* x = acc + c + 8 * j;
-                uint4 w;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&w)[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                piece(j, w);
-              }
-              leave(2 * c);
-            }
-          }
-          continue;
-        }
+      if constexpr (!CODES) {
+        if (n_now >= p.g.N) continue;
+        const int most = ok ? rows_now - q * 32 : 0;                      // tokens of this warp
+        apply(std::integral_constant<int, PART>(), acc, t_now, n_now, most);
+        leave(std::integral_constant<int, PART>(), acc, t_now, n_now, most);
       }
-      if (!t_in || !ok) continue;
-#pragma unroll
-      for (int c = 0; c < PART; c += 16)
-        if (n_now + c < p.g.N) store16(acc + c, t_now, n_now + c);
     }
   }
   __syncwarp();
@@ -522,7 +537,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
   }
 }
 
-template <int NCOL, bool DUAL, int CG, int SPLIT = 1>
+template <int NCOL, bool DUAL, int CG, int SPLIT = 1, bool CODES = false>
 static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
   using L = RowsTile<NCOL, DUAL, CG>;
   RowsTmParams p{};
@@ -536,7 +551,7 @@ static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
   if (r) return 1000 - r;
   r = encode_tensor_map(&tmX, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.ldx, 128, 1);
   if (r) return 2000 - r;
-  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG, SPLIT>;
+  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG, SPLIT, CODES>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return 3000 + (int)e;
   const long long total = (long long)p.n_tiles * p.t_tiles, slots = SPLIT > 1 ? total : sms / CG > 0 ? sms / CG : 1;      // parts: a tile per cluster
@@ -574,7 +589,7 @@ int rows_form(int T, int N, int K, int gated, int sms) {
   float best = 4.5f + (float)((small * parts + sms - 1) / sms) * ((float)kb / parts * (gated ? 0.7f : 0.35f) + 1.7f);
   int form = 0;
   auto take = [&](int f, float c) { if (c < best) { best = c; form = f; } };
-  take(1, cost(256, 256, 2, 0.56f, 1.5f));
+  take(1, cost(256, 256, 2, 0.60f, 1.5f));
   take(3, cost(128, 256, 1, 0.55f, 1.5f));
   if (!gated) {
     take(2, cost(256, 128, 2, 0.35f, 1.2f));
@@ -592,7 +607,10 @@ int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (sms <= 0) sms = 148;
+  if (g.gated && g.out_scale)
+    return form == 1 ? launch_rows_tm<256, true, 2, 1, true>(g, sms, st) : launch_rows_tm<256, true, 1, 1, true>(g, sms, st);
   if (g.gated) return form == 1 ? launch_rows_tm<256, true, 2>(g, sms, st) : launch_rows_tm<256, true, 1>(g, sms, st);
+  if (g.out_scale) return -5;
   switch (form) {
     case 1: return launch_rows_tm<256, false, 2>(g, sms, st);
     case 2: return launch_rows_tm<128, false, 2>(g, sms, st);

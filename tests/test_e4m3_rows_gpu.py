@@ -83,7 +83,8 @@ def test_norm_of_strided_rows():
 
 # token tiles and one past them, features and k that end inside a block, k that wants a pitch of its own, few and many tiles, parts of k
 SHAPES = [(1, 128, 128), (1, 2112, 4096), (16, 136, 8), (17, 384, 200), (32, 1000, 1032), (33, 200, 4096), (64, 264, 2056), (65, 512, 1152),
-          (129, 136, 640), (200, 4096, 520), (257, 300, 1024), (300, 2112, 7168), (1000, 1544, 264), (2100, 640, 512)]
+          (129, 136, 640), (200, 4096, 520), (257, 300, 1024), (300, 2112, 7168), (1000, 1544, 264), (2100, 640, 512), (150, 901, 1000), (333, 2049, 256),
+          (2000, 1283, 136), (1, 33, 72)]
 
 
 @pytest.mark.parametrize("T,N,K", SHAPES)
@@ -107,7 +108,8 @@ def test_product_matches_64_bits(T, N, K):
 # tiles of prompts, whatever the size would choose: one item and several per CTA, rows and features that end inside a tile, one block of k and
 # many, k that ends inside a block
 @pytest.mark.parametrize("form", [1, 2, 3, 4, 5, 6])
-@pytest.mark.parametrize("T,N,K", [(1, 8, 128), (100, 136, 16), (65, 200, 520), (131, 256, 3000), (129, 256, 640), (257, 300, 1032), (300, 2112, 2048), (2000, 5000, 264), (9000, 1160, 128)])
+@pytest.mark.parametrize("T,N,K", [(1, 8, 128), (100, 136, 16), (65, 200, 520), (131, 256, 3000), (129, 256, 640), (257, 300, 1032), (300, 2112, 2048), (2000, 5000, 264), (9000, 1160, 128), (140, 777, 1024),
+                                   (513, 515, 640)])
 def test_tiles_of_prompts(T, N, K, form):
     from xfastertransformer_b200.ops import native_e4m3 as E
     g = gen(T, N, K)
@@ -374,10 +376,11 @@ def test_rows_and_weights_as_they_lie(T):
         ww[:, :400] = W.w.view(torch.uint8)
         V = LinearWeight("fp8a", ww.view(torch.float8_e4m3fn)[:, :400], W.scale, in_features=400, out_features=264)
         assert torch.equal(ops.linear_e4m3(q, V, out_dtype=torch.float32), want)
-    out = torch.randn(T, 300, generator=g).bfloat16().cuda()
-    for at in (0, 1, 4):
-        res = out[:, at:at + 264]
-        assert torch.equal(ops.linear_e4m3(q, W, None, None, res, 0.5), ops.linear_e4m3(q, W, None, None, res.clone(), 0.5))
+    for cols in (300, 301):
+        out = torch.randn(T, cols, generator=g).bfloat16().cuda()
+        for at in (0, 1, 4):
+            res = out[:, at:at + 264]
+            assert torch.equal(ops.linear_e4m3(q, W, None, None, res, 0.5), ops.linear_e4m3(q, W, None, None, res.clone(), 0.5))
     check_status()
 
 
