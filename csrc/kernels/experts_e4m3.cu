@@ -10,7 +10,7 @@ namespace xft {
 //
 // One pass counts and one places, the pairs of a warp that ask for the same expert together (one addition in shared memory for all of them).
 // A cluster shares the pairs: its CTAs read each other's counts and know where their rows start.  Bound by the chain of two passes, a scan
-// and a barrier; us, one CTA for all as in moe_plan_kernel / here: 24576 pairs 64 experts 37 / PLAN1, 48 pairs 9 / PLAN0.
+// and a barrier; us, one CTA for all as in moe_plan_kernel / here: 24576 pairs 64 experts 37 / 12, 48 pairs 9 / 9.
 struct PlanRows {
   const int* idx; const float* w; int pairs, k, e0, E, bn;
   int* pos; int* src; float* row_w; int4* tiles; int* meta; int max_tiles;

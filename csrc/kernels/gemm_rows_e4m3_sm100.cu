@@ -114,8 +114,10 @@ struct RowsTile {
   static_assert((NCOL == 256 || (NCOL == 128 && !DUAL)) && (CG == 1 || CG == 2), "tile");
 };
 
-// CODES: the gated form's result leaves as e4m3 rows.
-template <int NCOL, bool DUAL, int CG, int SPLIT, bool CODES>
+// OUT: how a result leaves.  Each has a kernel of its own: what the others need at the end of a tile takes registers that the sums and their
+// scales lack in front of it (8192 x 8192 x 28672 on pairs under the power cap, us: 2285 with kRowsAny for all, 1974 with kRowsPlain).
+enum { kRowsCodes = 0, kRowsPlain = 1, kRowsAny = 2 };                // e4m3 rows (gated); bf16 in 16-byte pieces, no bias or activation; anything
+template <int NCOL, bool DUAL, int CG, int SPLIT, int OUT>
 __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                        const __grid_constant__ CUtensorMap tmW, const RowsTmParams p) {
   using L = RowsTile<NCOL, DUAL, CG>;
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     auto apply = [&](auto count, float* x, int t, int n, int most) {
       const bool in = lane < most;
       constexpr int C = decltype(count)::value;
-      if constexpr (!DUAL) {
+      if constexpr (!DUAL && OUT == kRowsAny) {
         if (p.g.bias) {
 #pragma unroll
           for (int j = 0; j < C; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
@@ -269,18 +271,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
       }
       if (!p.g.residual) return;
       const __nv_bfloat16* rrow = reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr + n;
-      if (vec && n + C <= p.g.N) {
+      if (OUT == kRowsPlain || (vec && n + C <= p.g.N)) {
         if (!in) return;
         uint4 res[C / 8];
 #pragma unroll
-        for (int j = 0; j < C / 8; ++j) res[j] = __ldg(reinterpret_cast<const uint4*>(rrow) + j);
+        for (int j = 0; j < C / 8; ++j)
+          res[j] = OUT == kRowsAny || n + 8 * j < p.g.N ? __ldg(reinterpret_cast<const uint4*>(rrow) + j) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < C / 2; ++j) {
           const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
           x[2 * j] += p.g.res_scale * f.x;
           x[2 * j + 1] += p.g.res_scale * f.y;
         }
-      } else {
+      } else if constexpr (OUT == kRowsAny) {
         // rows that do not start on 16 bytes, or end inside the run: read along the row into the warp's lines, 64 columns at a time
         const __nv_bfloat16* r0 = rrow - (size_t)lane * p.g.ldr;
 #pragma unroll
@@ -329,14 +332,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         constexpr int W = C < 128 / (int)sizeof(OT) ? C : 128 / (int)sizeof(OT), PIECES = W * (int)sizeof(OT) / 16;
         OT* out = reinterpret_cast<OT*>(p.g.out) + (size_t)(t - lane) * p.g.ldo + n + c0;
         __syncwarp();
-        if (whole) {
+        if (OUT == kRowsPlain || whole) {
 #pragma unroll
           for (int i = 0; i < PIECES; ++i) {
             const int r = 32 / PIECES * i + lane / PIECES, j = lane % PIECES;
             const uint4 w = *reinterpret_cast<const uint4*>(line_at(r, 16 * j));
-            if (r < most) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + j * (16 / (int)sizeof(OT))) = w;
+            const int col = j * (16 / (int)sizeof(OT));
+            if (r < most && (OUT == kRowsAny || n + c0 + col < p.g.N)) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + col) = w;
           }
-        } else {
+        } else if constexpr (OUT == kRowsAny) {
 #pragma unroll 4
           for (int r = 0; r < 32; ++r)
 #pragma unroll
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
         __syncwarp();
       };
-      if (p.g.out_fp32) {
+      if (OUT == kRowsAny && p.g.out_fp32) {
 #pragma unroll
         for (int c = 0; c < C; c += 32) {
 #pragma unroll
@@ -462,7 +466,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         for (int c = 0; c < PART; c += 16) rows_act(acc + c, p.g.act);
 #pragma unroll
         for (int j = 0; j < PART; ++j) acc[j] *= acc[PART + j];
-        if constexpr (CODES) {
+        if constexpr (OUT == kRowsCodes) {
           bool odd;
           float top = e4m3_top<PART>(acc, odd);
           float* tops = reinterpret_cast<float*>(smem + STAGES * STAGE);      // [two items in turn][side][token], where lines would be
@@ -515,7 +519,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
         continue;
       }
-      if constexpr (!CODES) {
+      if constexpr (OUT != kRowsCodes) {
         if (n_now >= p.g.N) continue;
         const int most = ok ? rows_now - q * 32 : 0;                      // tokens of this warp
         apply(std::integral_constant<int, PART>(), acc, t_now, n_now, most);
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
   }
 }
 
-template <int NCOL, bool DUAL, int CG, int SPLIT = 1, bool CODES = false>
+template <int NCOL, bool DUAL, int CG, int SPLIT, int OUT>
 static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
   using L = RowsTile<NCOL, DUAL, CG>;
   RowsTmParams p{};
@@ -551,7 +555,7 @@ static int launch_rows_tm(const RowsGemm& g, int sms, cudaStream_t st) {
   if (r) return 1000 - r;
   r = encode_tensor_map(&tmX, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.ldx, 128, 1);
   if (r) return 2000 - r;
-  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG, SPLIT, CODES>;
+  const auto kernel = gemm_rows_tm_kernel<NCOL, DUAL, CG, SPLIT, OUT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return 3000 + (int)e;
   const long long total = (long long)p.n_tiles * p.t_tiles, slots = SPLIT > 1 ? total : sms / CG > 0 ? sms / CG : 1;      // parts: a tile per cluster
@@ -608,17 +612,22 @@ int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st) {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (sms <= 0) sms = 148;
   if (g.gated && g.out_scale)
-    return form == 1 ? launch_rows_tm<256, true, 2, 1, true>(g, sms, st) : launch_rows_tm<256, true, 1, 1, true>(g, sms, st);
-  if (g.gated) return form == 1 ? launch_rows_tm<256, true, 2>(g, sms, st) : launch_rows_tm<256, true, 1>(g, sms, st);
+    return form == 1 ? launch_rows_tm<256, true, 2, 1, kRowsCodes>(g, sms, st) : launch_rows_tm<256, true, 1, 1, kRowsCodes>(g, sms, st);
+  if (g.gated) return launch_rows_tm<256, true, 1, 1, kRowsAny>(g, sms, st);
   if (g.out_scale) return -5;
+  const bool plain = !g.bias && !g.act && !g.out_fp32 && g.N % 8 == 0 && g.ldo % 8 == 0 && (!g.residual || g.ldr % 8 == 0) &&
+                     ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.residual)) & 15) == 0;
+#define XFT_ROWS_TM(NCOL, CG, SPLIT) \
+  (plain ? launch_rows_tm<NCOL, false, CG, SPLIT, kRowsPlain>(g, sms, st) : launch_rows_tm<NCOL, false, CG, SPLIT, kRowsAny>(g, sms, st))
   switch (form) {
-    case 1: return launch_rows_tm<256, false, 2>(g, sms, st);
-    case 2: return launch_rows_tm<128, false, 2>(g, sms, st);
-    case 3: return launch_rows_tm<256, false, 1>(g, sms, st);
-    case 5: return launch_rows_tm<128, false, 1, 2>(g, sms, st);
-    case 6: return launch_rows_tm<128, false, 1, 4>(g, sms, st);
-    default: return launch_rows_tm<128, false, 1>(g, sms, st);
+    case 1: return XFT_ROWS_TM(256, 2, 1);
+    case 2: return XFT_ROWS_TM(128, 2, 1);
+    case 3: return XFT_ROWS_TM(256, 1, 1);
+    case 5: return XFT_ROWS_TM(128, 1, 2);
+    case 6: return XFT_ROWS_TM(128, 1, 4);
+    default: return XFT_ROWS_TM(128, 1, 1);
   }
+#undef XFT_ROWS_TM
 }
 
 }  // namespace xft
