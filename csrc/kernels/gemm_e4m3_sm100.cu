@@ -33,6 +33,7 @@
 
 #include "rows_e4m3.cuh"
 
+#include <atomic>
 #include <cstddef>
 
 namespace xft {
@@ -825,11 +826,14 @@ template <int BN, bool DUAL, int SRC>
 static int launch_e4(const CUtensorMap& tmW, const CUtensorMap& tmX, E4Params p, cudaStream_t st) {
   using L = E4Layout<BN, DUAL, SRC>;
   const auto kernel = gemm_e4m3_kernel<BN, DUAL, SRC>;
-  static bool attr_set = false;
-  if (!attr_set) {
+  static std::atomic<uint64_t> attr_set{0};                            // a bit for each device, whose kernel has its own
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (!(attr_set.load(std::memory_order_relaxed) & bit)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) != cudaSuccess)
       return 3000 + (int)cudaGetLastError();
-    attr_set = true;
+    attr_set.fetch_or(bit, std::memory_order_relaxed);
   }
   // stacked tiles: as many parts as tiles of 128 features on an SM each would have (64 rows have those), so a row's sums do not depend on
   // how many rows stand beside it
@@ -943,6 +947,7 @@ extern "C" int xft_gemm_rows_e4m3(const RowsGemm* args, cudaStream_t st) {
   if ((a.ldx & 15) || (a.ldw & 15) || (reinterpret_cast<uintptr_t>(a.x) & 15) || (reinterpret_cast<uintptr_t>(a.w) & 15)) return -2;
   if ((a.gated && (a.dual_off & 127)) || (a.group_tiles && (a.group_w_rows & 127))) return -4;
   if (a.out_scale && (!a.gated || (a.N & 127) || (a.ldo & 15) || (reinterpret_cast<uintptr_t>(a.out) & 15) || a.residual || a.col_scale)) return -5;
+  if (a.group_tiles && a.gated && !a.out_scale) return -5;
   int form = a.form;
   if (a.group_tiles) {
     form = a.bn == 256 ? 1 : a.bn == 128 ? 3 : 0;
