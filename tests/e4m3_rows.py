@@ -2,7 +2,7 @@
 import torch
 
 from xfastertransformer_b200 import ops
-from xfastertransformer_b200.runtime.loader import make_linear
+from xfastertransformer_b200.runtime.loader import LinearWeight, make_linear
 
 TOP, LEAST = 448.0, 2.0 ** -100
 
@@ -23,6 +23,11 @@ def activations(g, T, K, dtype=torch.bfloat16):
 def weight(g, N, K, kind="fp8a", std=0.05):
     w = torch.randn(N, K, generator=g) * std * torch.exp(0.5 * torch.randn(N, 1, generator=g))
     return make_linear(w, kind)
+
+
+def scaled(W, scale):
+    """The weight with other scales."""
+    return LinearWeight(W.kind, W.w, scale, block=W.block, in_features=W.in_features, out_features=W.out_features)
 
 
 def rows(x):

@@ -5,11 +5,11 @@ import pytest
 import torch
 
 import xfastertransformer_b200 as xft
-from e4m3_rows import activations, coded_error, gen, rows, scale_error, sum_tol, values64, weight
+from e4m3_rows import activations, coded_error, gen, rows, scale_error, scaled, sum_tol, values64, weight
 from xfastertransformer_b200 import ops
 from xfastertransformer_b200.ops import reference as R
 from xfastertransformer_b200.config import ModelConfig, RopeConfig
-from xfastertransformer_b200.runtime.loader import cat_linear, make_linear
+from xfastertransformer_b200.runtime.loader import LinearWeight, cat_linear, make_linear
 from xfastertransformer_b200.tools.synthetic import preset, write_synthetic_checkpoint
 from xfastertransformer_b200.utils.flags import Env
 
@@ -58,6 +58,17 @@ def test_chain_of_a_layer():
     assert bool(((out.double() - want).abs() <= tol + 2.0 ** -22 * (want.abs() + x.double().abs())).all())
 
 
+def test_an_empty_share_of_the_columns_adds_nothing():
+    """What a rank without features of a gated product, or without columns of a row-parallel one, has to do."""
+    g = gen(4)
+    q, r, b = rows(torch.randn(3, 128, generator=g)), torch.randn(3, 64, generator=g), torch.randn(64, generator=g)
+    none = ops.linear_gated_e4m3(q, LinearWeight("fp8a", torch.zeros(0, 128).to(torch.float8_e4m3fn), torch.zeros(0, 1), in_features=128, out_features=0))
+    assert none.shape == (3, 0) and none.scale.shape == (0, 3)
+    W = LinearWeight("fp8a", torch.zeros(64, 0).to(torch.float8_e4m3fn), torch.zeros(1, 0), in_features=0, out_features=64)
+    assert torch.equal(ops.linear_e4m3(none, W), torch.zeros(3, 64))
+    assert torch.equal(ops.linear_e4m3(none, W, b, "relu", r, 0.5), b.clamp_min(0) + 0.5 * r)
+
+
 def test_refusals():
     g = gen(3)
     q, W = rows(torch.randn(4, 256, generator=g)), weight(g, 512, 256)
@@ -93,13 +104,20 @@ def test_refusals():
         ops.quantize_e4m3(torch.zeros(4, 0))
     with pytest.raises(ValueError, match="end inside a block"):
         cat_linear([odd, W])
+    for scale in (W.scale[:, :1], W.scale.double(), W.scale.t().contiguous().t(), W.scale[:1]):
+        with pytest.raises(ValueError, match="scales"):
+            ops.linear_e4m3(q, scaled(W, scale))
+    for kw in (dict(times=torch.zeros(4, 512)), dict(out=torch.zeros(4, 512))):
+        with pytest.raises(ValueError, match="no `out` and no `times`"):
+            ops.linear(q, W, **kw)
     e = [(W, weight(g, 256, 256))]
     idx, w = torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, 2)
     for bad, match in ((dict(q=rows(torch.zeros(4, 128))), "columns"), (dict(idx=idx[:3]), "experts"), (dict(w=w[:, :1]), "weights"),
                        (dict(idx=idx[:, :0], w=w[:, :0]), "experts"), (dict(add=torch.zeros(4, 128)), "added"), (dict(experts=[]), "no experts"),
                        (dict(out_dtype=torch.float16), "bf16 or fp32"), (dict(act="clamped"), "activation"),
                        (dict(experts=[(odd, weight(g, 256, 160))]), "multiples of 128"),
-                       (dict(experts=e + [(weight(g, 256, 256), weight(g, 256, 128))]), "different sizes")):
+                       (dict(experts=e + [(weight(g, 256, 256), weight(g, 256, 128))]), "different sizes"), (dict(packed={}), "packed"),
+                       (dict(packed=dict(gus=None, E=2)), "packed"), (dict(experts=[(scaled(W, W.scale[:1, :1]), e[0][1])]), "scales")):
         with pytest.raises(ValueError, match=match):
             ops.moe_experts_e4m3(**{**dict(q=q, idx=idx, w=w, experts=e), **bad})
 

@@ -250,7 +250,7 @@ def test_experts_match_64_bits(T, E, k, H, I):
     dev = [(on(a), on(b)) for a, b in experts]
     got = ops.moe_experts_e4m3(rows_on(q), idx.cuda(), w.cuda(), dev, "relu")
     check_status()
-    big = tol + 2.0 ** -8 * 0 + (k + 2) * 2.0 ** -24 * want.abs().amax(1, keepdim=True)
+    big = tol + (k + 2) * 2.0 ** -24 * want.abs().amax(1, keepdim=True)
     half = experts_half_step(q, idx, w, experts)                    # prompts hold a pair's row in bf16 on its way into the sum
     assert bool(((got.cpu().double() - want).abs() <= big + half).all())
     add = torch.randn(T, H, generator=g)
@@ -344,6 +344,66 @@ def test_no_rows():
     assert n[0].shape == (0, 128) and n[1].shape == n[2].shape == (0, 128)
     e = [(W, on(weight(g, 128, 128)))]
     assert ops.moe_experts_e4m3(q, torch.zeros(0, 1, dtype=torch.int32, device="cuda"), torch.zeros(0, 1, device="cuda"), e).shape == (0, 128)
+
+
+def test_an_empty_share_of_the_columns_adds_nothing():
+    g = gen(4)
+    q = rows_on(whole_rows(g, 3, 128))
+    none = ops.linear_gated_e4m3(q, LinearWeight("fp8a", torch.zeros(0, 128).to(torch.float8_e4m3fn), torch.zeros(0, 1), in_features=128,
+                                                 out_features=0).to("cuda"))
+    assert none.shape == (3, 0) and none.scale.shape == (0, 3)
+    W = LinearWeight("fp8a", torch.zeros(64, 0).to(torch.float8_e4m3fn), torch.zeros(1, 0), in_features=0, out_features=64).to("cuda")
+    r, b = torch.randn(3, 64, generator=g).bfloat16(), torch.randn(64, generator=g)
+    assert torch.equal(ops.linear_e4m3(none, W).cpu(), torch.zeros(3, 64).bfloat16())
+    got = ops.linear_e4m3(none, W, b.cuda(), "relu", r.cuda(), 0.5, torch.float32)
+    assert torch.equal(got.cpu(), b.clamp_min(0) + 0.5 * r.float())
+
+
+def test_lists_of_experts_that_share_their_ends():
+    """Stacks belong to the very experts that were asked for: another list with the same first and last one, a part of a list, and the whole
+    again, each gives what its experts give."""
+    g = gen(5)
+    a, b, c, d = [(on(whole(g, 256, 128)), on(whole(g, 128, 128))) for _ in range(4)]
+    q = whole_rows(g, 9, 128)
+    idx, w = torch.arange(9, dtype=torch.int32).view(9, 1) % 3, torch.ones(9, 1)
+    first = [a, b, c]
+    kept = ops.pack_experts_e4m3(first)
+    for experts in (first, [a, d, c], [b, c, a], [a, b], first):
+        want, tol = experts64(q, idx, w, experts)
+        got = ops.moe_experts_e4m3(rows_on(q), idx.cuda(), w.cuda(), experts, "relu")
+        assert bool(((got.cpu().double() - want).abs() <= tol + 3 * 2.0 ** -24 * want.abs().amax(1, keepdim=True)).all())
+    assert ops.pack_experts_e4m3(first) is kept
+    check_status()
+
+
+def test_copies_of_weights_and_captured_graphs():
+    """A copy that a graph makes of a weight with odd rows is the graph's own; stacks are made before a capture or not at all."""
+    from xfastertransformer_b200.ops import native as N
+    g = gen(6)
+    host = weight(g, 64, 200)
+    W, x = on(host), activations(g, 3, 200).cuda()
+    assert W.w.stride(0) % 16
+    ops.quantize_e4m3(x)
+    stream = torch.cuda.Stream()
+    q = ops.quantize_e4m3(x)
+    ops.linear_e4m3(q, on(host))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        y = ops.linear_e4m3(q, W)
+    eager = ops.linear_e4m3(q, W)                                   # before the graph's copy has been made once
+    graph.replay()
+    want, tol = sum_tol(q, host)
+    for got in (eager, y):
+        assert bool(((got.cpu().double() - want).abs() <= tol * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()).all())
+    experts = [(on(whole(g, 256, 128)), on(whole(g, 128, 128)))]
+    qe, idx, w = rows_on(whole_rows(g, 2, 128)), torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, 1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(N.KernelError, match="before a graph"):
+            ops.moe_experts_e4m3(qe, idx, w, experts, "relu")
+        ops.linear_e4m3(q, W)
+    check_status()
 
 
 @pytest.mark.parametrize("T", [20, 100, 300])

@@ -733,7 +733,9 @@ class Decoder:
         shared = None
         if getattr(L, "shared", None) is not None:
             shared = ops.linear_e4m3(ops.linear_gated_e4m3(q, L.shared[0], L.act), L.shared[1], out_dtype=torch.float32)
-        out = ops.moe_experts_e4m3(q, idx, w, L.experts, L.act, L.e0, getattr(L, "packed", None), add=shared)
+        if getattr(L, "packed", None) is None:
+            L.packed = ops.pack_experts_e4m3(L.experts)
+        out = ops.moe_experts_e4m3(q, idx, w, L.experts, L.act, L.e0, L.packed, add=shared)
         if self.tp == 1 and not self._overlap and not debugger.enabled():
             self._pending = out
             return x

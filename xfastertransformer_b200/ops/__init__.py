@@ -95,13 +95,15 @@ def _timed(kernel: str, x, W, fn):
 def linear(x, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=None, times=None, out=None):
     """act(x W^T + bias) + res_scale * residual, or with `times` [T, out] act(x W^T + bias) * times.  x may be rows in e4m3 where W is
     (see linear_e4m3).  `out`: rows to write into.  act "softcap": res_scale * tanh(. / res_scale)."""
+    if isinstance(x, RowsE4M3):
+        if out is not None or times is not None:
+            raise ValueError("linear: products of rows in e4m3 have no `out` and no `times`")
+        return linear_e4m3(x, W, bias, act, residual, res_scale, out_dtype)
     if out is not None:
         assert residual is None and times is None
         return (_nat() if _cuda(x) else R).linear_into(x, W, bias, act, out)
     if times is not None:
         return (_nat() if _cuda(x) else R).linear_times(x, W, bias, act, times)
-    if isinstance(x, RowsE4M3):
-        return linear_e4m3(x, W, bias, act, residual, res_scale, out_dtype)
     if _verbose():
         name = "gemm" + ("_bias" if bias is not None else "") + (f"_{act}" if act else "") + \
             ("_residual" if residual is not None else "")
@@ -175,15 +177,21 @@ def _same_device(what, first, *tensors):
 def _check_rows_e4m3(what, q, W, act):
     if not isinstance(q, RowsE4M3):
         raise ValueError(f"{what} multiplies rows in e4m3 (RowsE4M3), not {type(q).__name__}")
-    n, k = W.out_features, W.in_features
-    if W.kind not in ("fp8", "fp8a") or W.block != _BLOCK:
-        raise ValueError(f"{what}: weights are e4m3 with a scale for each block of {_BLOCK}, not {W.kind}")
-    if q.codes.shape[1] != k:
-        raise ValueError(f"{what}: rows of {q.shape[1]} columns and weights of {k}")
-    if W.scale.shape != (-(-n // _BLOCK), -(-k // _BLOCK)):
-        raise ValueError(f"{what}: block scales {tuple(W.scale.shape)} of weights [{n}, {k}]")
+    _check_e4m3_weight(what, W)
+    if q.codes.shape[1] != W.in_features:
+        raise ValueError(f"{what}: rows of {q.shape[1]} columns and weights of {W.in_features}")
     if act not in _ROW_ACTS:
         raise ValueError(f"{what}: no activation {act!r}")
+
+
+def _check_e4m3_weight(what, W):
+    if W.kind not in ("fp8", "fp8a") or W.block != _BLOCK:
+        raise ValueError(f"{what}: weights are e4m3 with a scale for each block of {_BLOCK}, not {W.kind}")
+    n, k, s = W.out_features, W.in_features, W.scale
+    if s.shape != (-(-n // _BLOCK), -(-k // _BLOCK)) or s.dtype is not torch.float32 or not s.is_contiguous() or W.w.shape != (n, k) \
+            or W.w.dtype is not torch.float8_e4m3fn:
+        raise ValueError(f"{what}: weights {tuple(W.w.shape)} in {W.w.dtype} with block scales {tuple(s.shape)} in {s.dtype} (contiguous: "
+                         f"{s.is_contiguous()}) for [{n}, {k}] in e4m3")
 
 
 def quantize_e4m3(x) -> RowsE4M3:
@@ -248,8 +256,9 @@ def pack_experts_e4m3(experts):
     if not experts:
         raise ValueError("pack_experts_e4m3: no experts")
     for g, d in experts:
-        if any(w.kind not in ("fp8", "fp8a") or w.block != _BLOCK for w in (g, d)):
-            raise ValueError("pack_experts_e4m3: experts' weights are e4m3 with block scales")
+        _check_e4m3_weight("pack_experts_e4m3", g)
+        _check_e4m3_weight("pack_experts_e4m3", d)
+        _same_device("pack_experts_e4m3", experts[0][0].w, g.w, g.scale, d.w, d.scale)
         if d.in_features % _BLOCK or d.out_features % _BLOCK or (g.in_features, g.out_features) != (d.out_features, 2 * d.in_features):
             raise ValueError(f"pack_experts_e4m3: experts of widths that are multiples of {_BLOCK}, gate and up [2 I, H], down [H, I]; not "
                              f"[{g.out_features}, {g.in_features}] and [{d.out_features}, {d.in_features}]")
@@ -273,12 +282,17 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
         raise ValueError(f"moe_experts_e4m3: results are bf16 or fp32, not {out_dtype}")
     if act not in _ROW_ACTS:
         raise ValueError(f"moe_experts_e4m3: no activation {act!r}")
-    if packed is None:
-        packed = pack_experts_e4m3(experts)
+    if not experts:
+        raise ValueError("moe_experts_e4m3: no experts")
+    cuda = q.is_cuda
+    if packed is None:                                   # packed before: the experts were looked at then
+        packed = cuda and _native_e4m3().packed_before(experts) or pack_experts_e4m3(experts)
+    elif "gus" not in packed or packed["E"] != len(experts):
+        raise ValueError("moe_experts_e4m3: `packed` is not of these e4m3 experts (pack_experts_e4m3)")
     if experts[0][1].out_features != H:
         raise ValueError(f"moe_experts_e4m3: rows of {H} columns and experts of {experts[0][1].out_features}")
     _same_device("moe_experts_e4m3", q.codes, idx, w, add, experts[0][0].w)
-    if not q.is_cuda:
+    if not cuda:
         return R.moe_experts_e4m3(q, idx, w, experts, act, expert_offset, add, out_dtype)
     return _native_e4m3().moe_experts_e4m3(q, idx, w, experts, act, expert_offset, packed, expected_pairs, add, out_dtype)
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import weakref
 
 import torch
 
@@ -114,13 +115,16 @@ def rows_e4m3(x, gain=None, eps=0.0, residual=None, want_rows=False):
 
 
 def _weight(W):
-    """The codes of W with rows on 16 bytes; the copy that this may take is kept with the weight."""
+    """The codes of W with rows on 16 bytes; the copy that this may take is kept with the weight (inside a capture it is part of the graph)."""
     w = W.w
     ld, one = w.stride()
     if ld % 16 or one != 1 or w.data_ptr() % 16:
         kept = W.cache.get("w_pitch16")
         if kept is None:
-            kept = W.cache["w_pitch16"] = _pitched(w)
+            kept = _pitched(w)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(w.device).synchronize()       # other streams may read it from now on
+                W.cache["w_pitch16"] = kept
         w = kept
     return w
 
@@ -155,6 +159,12 @@ def linear_e4m3(q, W, bias=None, act=None, residual=None, res_scale=1.0, out_dty
             residual = residual.reshape(-1, residual.shape[-1])
         if residual.stride(1) != 1:
             residual = residual.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if not K:                                            # a rank's empty share of a row-parallel product
+        from . import reference as R
+        y = R._act(torch.zeros((T, W.out_features), device=dev) + (0 if bias is None else bias), act)
+        return (y if residual is None else y + res_scale * residual.float()).to(out_dtype)
     out = q.codes.new_empty((T, W.out_features), dtype=out_dtype)
     if T:
         _gemm(q, _weight(W), W.scale, out, T, W.out_features, K, False, 0, bias, act, residual, res_scale)
@@ -168,8 +178,10 @@ def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
             return linear_gated_e4m3(q, W, act, bias)
     T, K = q.codes.shape
     I = W.out_features // 2
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     out = new_rows(T, I, q.codes)
-    if T:
+    if T and I:
         _gemm(q, _weight(W), W.scale, out.codes, T, I, K, True, I, bias, act, out_scale=out.scale)
     return out
 
@@ -184,9 +196,35 @@ def gated_rows(q, W, act, bias=None):
     return out
 
 
+def packed_before(experts):
+    """The stacks that an earlier call made of these very experts, kept with the first one's weight; None where there are none."""
+    for of, pk in experts[0][0].cache.get("e4m3_packs", ()):
+        if len(of) == len(experts) and all(a() is g and b() is d for (a, b), (g, d) in zip(of, experts)):
+            return pk
+    return None
+
+
 def pack_experts(experts) -> dict:
-    from . import native_moe
-    return native_moe.pack_experts(experts)
+    """Stacks of these experts, made once: what a captured graph reads stays, also when another list with the same first expert comes."""
+    pk = packed_before(experts)
+    if pk is None:
+        from . import native_moe
+        cache, dev = experts[0][0].cache, experts[0][0].w.device
+        if torch.cuda.is_current_stream_capturing():
+            raise N.KernelError("experts' weights are stacked before a graph is captured (pack_experts_e4m3), not inside it")
+        old = cache.get("moe_pack")
+        step = lambda s, n: s.data_ptr() + n * s.shape[1]
+        if old is not None and "gus" in old and old["E"] == len(experts) and all(
+                g.w.data_ptr() == step(old["gu"], e * 2 * old["I"]) and d.w.data_ptr() == step(old["dn"], e * old["H"])
+                for e, (g, d) in enumerate(experts)):
+            pk = old
+        else:
+            pk = native_moe._pack_fp8(experts)
+            if old is not None:
+                cache["moe_pack"] = old
+        cache.setdefault("e4m3_packs", []).append(([(weakref.ref(g), weakref.ref(d)) for g, d in experts], pk))
+        torch.cuda.current_stream(dev).synchronize()                    # other streams may read them from now on
+    return pk
 
 
 def _tile_rows(avg) -> int:

@@ -217,6 +217,8 @@ def linear(x, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=No
         return _w8a8(x, W, W.out_features, bias, act, residual, res_scale, out_dtype, norm=norm)
     if W.kind == "fp8a":
         from . import native_e4m3 as E
+        if N._ACT.get(act, 9) > 5 and act != "tanh":
+            raise N.KernelError(f"no product of {W.kind} weights with activation {act!r}")
         return E.linear_e4m3(E.rows_e4m3(x)[0], W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
     if W.kind in _QT or W.kind in _E4M3:
         return _qgemm(x, W, W.out_features, False, bias, act, residual, res_scale, out_dtype, norm)
@@ -238,6 +240,8 @@ def linear_gated(x, W, act="silu", bias=None, norm=None):
         return out
     if W.kind == "fp8a":
         from . import native_e4m3 as E
+        if N._ACT.get(act, 9) > 5 and act != "tanh":
+            raise N.KernelError(f"no gated product of {W.kind} weights with activation {act!r}")
         q = E.rows_e4m3(x)[0]
         return N.gated_act(E.linear_e4m3(q, W, bias), act) if I % 128 else E.gated_rows(q, W, act, bias)
     if W.kind == "fp8" and I % 128:
