@@ -184,6 +184,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     if (warp == 0) {
       if (elect_one()) {
         const uint32_t lead_bar = CG == 2 ? dsmem_addr(smem_u32(full_bar), 0) : 0;      // the first CTA's full barriers
+        // weights that are read about once leave L2 first: 64 experts of 1408 x 2048, 38 rows each, 136 us and 124 so, 8 of 14336 x 4096, 75 rows each,
+        // 275 and 266; with three token tiles each the former 366 and 372
+        const bool once = groups ? p.n_tiles * (p.g.w_rows / p.g.group_w_rows) * 2 >= total : p.t_tiles == 1;
+        const uint64_t hint_w = once ? kEvictFirst : kEvictNormal;
         Ring r = {0, 0};
         bool ok = true;
         for (int item = first; item < total && ok; item += step) {
@@ -196,12 +200,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
             if constexpr (CG == 2) {
               if (half == 0) mbar_expect_tx(&full_bar[r.s], 2 * STAGE);
               tma_load_2d_pair(a, &tmX, lead_bar + 8 * r.s, kb * 128, im.row0, kEvictNormal);
-              tma_load_2d_pair(a + L::A_BYTES, &tmW, lead_bar + 8 * r.s, kb * 128, wrow, kEvictNormal);
+              tma_load_2d_pair(a + L::A_BYTES, &tmW, lead_bar + 8 * r.s, kb * 128, wrow, hint_w);
             } else {
               mbar_expect_tx(&full_bar[r.s], STAGE);
               tma_load_2d(a, &tmX, &full_bar[r.s], kb * 128, im.row0, kEvictNormal);
-              tma_load_2d(a + L::A_BYTES, &tmW, &full_bar[r.s], kb * 128, wrow, kEvictNormal);
-              if (DUAL) tma_load_2d(a + L::A_BYTES + FEAT * 128, &tmW, &full_bar[r.s], kb * 128, wrow + p.g.dual_off, kEvictNormal);
+              tma_load_2d(a + L::A_BYTES, &tmW, &full_bar[r.s], kb * 128, wrow, hint_w);
+              if (DUAL) tma_load_2d(a + L::A_BYTES + FEAT * 128, &tmW, &full_bar[r.s], kb * 128, wrow + p.g.dual_off, hint_w);
             }
           }
         }
