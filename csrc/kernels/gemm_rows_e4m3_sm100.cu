@@ -96,6 +96,28 @@ __device__ __forceinline__ void rows_act(float* x, int act) {
 #undef XFT_ROWS_ACT
 }
 
+// elements in front of the first 16-byte boundary of a row
+template <typename T>
+__device__ __forceinline__ int rows_head(const T* p) {
+  return (int)((0u - (uint32_t)(reinterpret_cast<uintptr_t>(p) / sizeof(T))) & (16 / sizeof(T) - 1));
+}
+// N words turned by so many bytes, a multiple of UNIT below 16: left, so that what lay `bytes` behind the start lies at the start, or back
+template <int UNIT, bool LEFT, int N>
+__device__ __forceinline__ void rows_rotate(uint32_t (&w)[N], int bytes) {
+  uint32_t v[N];
+#pragma unroll
+  for (int s = UNIT; s < 16; s *= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int by = s / 4;                                            // words
+      if (LEFT) v[i] = s == 2 ? __funnelshift_r(w[i], w[(i + 1) % N], 16) : w[(i + by) % N];
+      else v[i] = s == 2 ? __funnelshift_l(w[(i + N - 1) % N], w[i], 16) : w[(i + N - by) % N];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = bytes & s ? v[i] : w[i];
+  }
+}
+
 struct RowsTmParams {
   RowsGemm g;
   int n_tiles, t_tiles, num_kb;
@@ -261,12 +283,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
     // bias, activation (the gated form has its own) and residual on C columns from n on of token t, the warp's first `most` tokens being there; all of
     // the residual is on its way before the first value waits for it
     auto apply = [&](auto count, float* x, int t, int n, int most) {
-      const bool in = lane < most;
       constexpr int C = decltype(count)::value;
       if constexpr (!DUAL && OUT == kRowsAny) {
         if (p.g.bias) {
+          if (n + C <= p.g.N && (reinterpret_cast<uintptr_t>(p.g.bias) & 15) == 0) {
 #pragma unroll
-          for (int j = 0; j < C; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
+            for (int j = 0; j < C; j += 4) {
+              const float4 b = __ldg(reinterpret_cast<const float4*>(p.g.bias + n + j));
+              x[j] += b.x; x[j + 1] += b.y; x[j + 2] += b.z; x[j + 3] += b.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < C; ++j) x[j] += __ldg(p.g.bias + min(n + j, p.g.N - 1));
+          }
         }
         if (p.g.act) {
 #pragma unroll
@@ -274,110 +303,183 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
         }
       }
       if (!p.g.residual) return;
-      const __nv_bfloat16* rrow = reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr + n;
-      if (OUT == kRowsPlain || (vec && n + C <= p.g.N)) {
-        if (!in) return;
-        uint4 res[C / 8];
+      const __nv_bfloat16* r0 = reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)(t - lane) * p.g.ldr + n;
+      constexpr int W = C < 64 ? C : 64;
+      auto add_line = [&](int c) {                                     // W columns of the residual lie in the warp's lines
 #pragma unroll
-        for (int j = 0; j < C / 8; ++j)
-          res[j] = OUT == kRowsAny || n + 8 * j < p.g.N ? __ldg(reinterpret_cast<const uint4*>(rrow) + j) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < W / 8; ++j) {
+          const uint4 u = *reinterpret_cast<const uint4*>(line_at(lane, 16 * j));
 #pragma unroll
-        for (int j = 0; j < C / 2; ++j) {
-          const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(res)[j]);
-          x[2 * j] += p.g.res_scale * f.x;
-          x[2 * j + 1] += p.g.res_scale * f.y;
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&u)[i]);
+            x[c + 8 * j + 2 * i] += p.g.res_scale * f.x;
+            x[c + 8 * j + 2 * i + 1] += p.g.res_scale * f.y;
+          }
         }
-      } else if constexpr (OUT == kRowsAny) {
-        // rows that do not start on 16 bytes, or end inside the run: read along the row into the warp's lines, 64 columns at a time
-        const __nv_bfloat16* r0 = rrow - (size_t)lane * p.g.ldr;
+      };
+      if (OUT == kRowsPlain || vec) {
+        // along the rows as well: a lane's own 16 bytes of a row each would touch 32 lines a load (8192 x 28672 x 256 with residual: 320 us,
+        // and 228 so)
+        constexpr int PIECES = W / 8;
+        uint4 v[C / 8];
 #pragma unroll
-        for (int c = 0; c < C; c += 64) {
-          constexpr int W = C < 64 ? C : 64;
+        for (int c = 0; c < C; c += W)
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) {
+            const int r = 32 / PIECES * i + lane / PIECES, col = c + lane % PIECES * 8;
+            v[c / 8 + i] = r < most && n + col < p.g.N
+                               ? __ldg(reinterpret_cast<const uint4*>(r0 + (size_t)r * p.g.ldr + col)) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+        for (int c = 0; c < C; c += W) {
           __syncwarp();
-#pragma unroll 1
-          for (int r8 = 0; r8 < 32; r8 += 8) {                         // eight tokens' loads under way together
-            __nv_bfloat16 v[8][(W + 31) / 32];
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+          for (int i = 0; i < PIECES; ++i)
+            *reinterpret_cast<uint4*>(line_at(32 / PIECES * i + lane / PIECES, lane % PIECES * 16)) = v[c / 8 + i];
+          __syncwarp();
+          add_line(c);
+        }
+        __syncwarp();
+      } else if constexpr (OUT == kRowsAny) {
+        // rows that do not start on 16 bytes: their 16-byte pieces go into the lines and the elements around those behind them, that is the run
+        // rotated, which its lane turns back
+        constexpr int PIECES = W / 8, ES = 8 / PIECES;                 // ES: elements of the ends per lane and row
 #pragma unroll
-              for (int h = 0; h < W; h += 32) {
-                const int col = h + lane;
-                v[r][h / 32] = col < W && r8 + r < most && n + c + col < p.g.N ? r0[(size_t)(r8 + r) * p.g.ldr + c + col] : __float2bfloat16(0.f);
-              }
+        for (int c = 0; c < C; c += W) {
+          const int cols = p.g.N - n - c;
+          if (cols <= 0) break;
+          uint4 v[PIECES];
+          __nv_bfloat16 e[PIECES][ES];
+          if (cols >= W) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+            for (int i = 0; i < PIECES; ++i) {
+              const int r = 32 / PIECES * i + lane / PIECES, j = lane % PIECES;
+              const __nv_bfloat16* from = r0 + (size_t)r * p.g.ldr + c;
+              const int head = rows_head(from);
+              v[i] = make_uint4(0, 0, 0, 0);
+              if (r < most && (j < PIECES - 1 || !head)) v[i] = __ldg(reinterpret_cast<const uint4*>(from + head) + j);
 #pragma unroll
-              for (int h = 0; h < W; h += 32)
-                if (h + lane < W) *reinterpret_cast<__nv_bfloat16*>(line_at(r8 + r, 2 * (h + lane))) = v[r][h / 32];
+              for (int h = 0; h < ES; ++h)
+                e[i][h] = r < most && head ? __ldg(from + ((head + W - 8 + j + h * PIECES) & (W - 1))) : __float2bfloat16(0.f);
+            }
           }
           __syncwarp();
+          if (cols >= W) {
 #pragma unroll
-          for (int j = 0; j < W / 8; ++j) {
-            const uint4 u = *reinterpret_cast<const uint4*>(line_at(lane, 16 * j));
+            for (int i = 0; i < PIECES; ++i) {
+              const int r = 32 / PIECES * i + lane / PIECES, j = lane % PIECES, head = rows_head(r0 + (size_t)r * p.g.ldr + c);
+              if (j < PIECES - 1 || !head) *reinterpret_cast<uint4*>(line_at(r, 16 * j)) = v[i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&u)[i]);
-              x[c + 8 * j + 2 * i] += p.g.res_scale * f.x;
-              x[c + 8 * j + 2 * i + 1] += p.g.res_scale * f.y;
+              for (int h = 0; h < ES; ++h)
+                if (head) *reinterpret_cast<__nv_bfloat16*>(line_at(r, 2 * (W - 8 + j + h * PIECES))) = e[i][h];
             }
+          } else {                                                     // the last features: one by one, sixteen rows under way
+#pragma unroll 1
+            for (int r16 = 0; r16 < 32; r16 += 16) {
+              constexpr int LC = (W + 31) / 32;                        // columns of a lane
+              __nv_bfloat16 u[16][LC];
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int h = 0; h < LC; ++h) {
+                  const int col = 32 * h + lane;
+                  u[r][h] = r16 + r < most && col < cols && col < W ? __ldg(r0 + (size_t)(r16 + r) * p.g.ldr + c + col) : __float2bfloat16(0.f);
+                }
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int h = 0; h < LC; ++h) {
+                  const int col = 32 * h + lane, head = rows_head(r0 + (size_t)(r16 + r) * p.g.ldr + c);
+                  if (col < W) *reinterpret_cast<__nv_bfloat16*>(line_at(r16 + r, 2 * ((col - head) & (W - 1)))) = u[r][h];
+                }
+            }
+          }
+          __syncwarp();
+          uint32_t w[W / 2];
+#pragma unroll
+          for (int j = 0; j < W / 8; ++j) reinterpret_cast<uint4*>(w)[j] = *reinterpret_cast<const uint4*>(line_at(lane, 16 * j));
+          rows_rotate<2, false>(w, 2 * rows_head(r0 + (size_t)lane * p.g.ldr + c));
+#pragma unroll
+          for (int j = 0; j < W / 2; ++j) {
+            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(w)[j]);
+            x[c + 2 * j] += p.g.res_scale * f.x;
+            x[c + 2 * j + 1] += p.g.res_scale * f.y;
           }
         }
         __syncwarp();
       }
     };
     // C columns from n on of token t on their way out: 128 bytes of each token at a time through shared memory, so that a store fills lines; rows
-    // that do not start on 16 bytes, or end inside the run, leave element by element, along the row all the same.  us of 24576 x 2048 x 1408
-    // with a lane's own 32 bytes per store, residual and branches piece by piece / so: 110 / 90 (69 without any store).
+    // that do not start on 16 bytes are rotated in their line, so that what leaves in 16 bytes lies so, and the elements around that leave one by one
+    // (8192 x 28671 x 256 all one by one 360 us, so 304).  us of 24576 x 2048 x 1408 with a lane's own 32 bytes per store, residual and branches
+    // piece by piece / so: 110 / 90 (69 without any store).
     auto leave = [&](auto count, const float* x, int t, int n, int most) {
       constexpr int C = decltype(count)::value;
-      const bool whole = vec && n + C <= p.g.N;
       auto pieces = [&](auto type, int c0) {                           // the lines hold columns c0 on, W of them
         using OT = decltype(type);
         constexpr int W = C < 128 / (int)sizeof(OT) ? C : 128 / (int)sizeof(OT), PIECES = W * (int)sizeof(OT) / 16;
         OT* out = reinterpret_cast<OT*>(p.g.out) + (size_t)(t - lane) * p.g.ldo + n + c0;
         __syncwarp();
-        if (OUT == kRowsPlain || whole) {
+        if (OUT == kRowsPlain || vec) {
 #pragma unroll
           for (int i = 0; i < PIECES; ++i) {
             const int r = 32 / PIECES * i + lane / PIECES, j = lane % PIECES;
             const uint4 w = *reinterpret_cast<const uint4*>(line_at(r, 16 * j));
             const int col = j * (16 / (int)sizeof(OT));
-            if (r < most && (OUT == kRowsAny || n + c0 + col < p.g.N)) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + col) = w;
+            if (r < most && n + c0 + col < p.g.N) *reinterpret_cast<uint4*>(out + (size_t)r * p.g.ldo + col) = w;
           }
         } else if constexpr (OUT == kRowsAny) {
-#pragma unroll 4
-          for (int r = 0; r < 32; ++r)
+          constexpr int E = 16 / (int)sizeof(OT), ES = E / PIECES < 1 ? 1 : E / PIECES;      // elements of a piece; of the ends per lane and row
+          const int cols = p.g.N - n - c0;
+          if (cols >= W) {
 #pragma unroll
-            for (int h = 0; h < W; h += 32) {
-              const int col = h + lane;
-              if (col < W && r < most && n + c0 + col < p.g.N)
-                out[(size_t)r * p.g.ldo + col] = *reinterpret_cast<const OT*>(line_at(r, col * (int)sizeof(OT)));
+            for (int i = 0; i < PIECES; ++i) {
+              const int r = 32 / PIECES * i + lane / PIECES, j = lane % PIECES;
+              OT* to = out + (size_t)r * p.g.ldo;
+              const int head = rows_head(to);
+              if (r >= most) continue;
+              if (j < PIECES - 1 || !head) reinterpret_cast<uint4*>(to + head)[j] = *reinterpret_cast<const uint4*>(line_at(r, 16 * j));
+#pragma unroll
+              for (int h = 0; h < ES; ++h) {
+                const int k = W - E + j + h * PIECES;
+                if (head && k < W) to[(head + k) & (W - 1)] = *reinterpret_cast<const OT*>(line_at(r, k * (int)sizeof(OT)));
+              }
             }
+          } else {                                                     // the last features: one by one
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+              OT* to = out + (size_t)r * p.g.ldo;
+              const int head = rows_head(to);
+#pragma unroll
+              for (int col = lane; col < W; col += 32)
+                if (r < most && col < cols) to[col] = *reinterpret_cast<const OT*>(line_at(r, ((col - head) & (W - 1)) * (int)sizeof(OT)));
+            }
+          }
         }
         __syncwarp();
       };
       if (OUT == kRowsAny && p.g.out_fp32) {
 #pragma unroll
         for (int c = 0; c < C; c += 32) {
+          constexpr int W = C < 32 ? C : 32;
+          uint32_t w[W];
 #pragma unroll
-          for (int j = 0; j < (C < 32 ? C : 32) / 4; ++j) {
-            const float* v = x + c + 4 * j;
-            *reinterpret_cast<uint4*>(line_at(lane, 16 * j)) =
-                make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-          }
+          for (int j = 0; j < W; ++j) w[j] = __float_as_uint(x[c + j]);
+          if (!vec) rows_rotate<4, true>(w, 4 * rows_head(reinterpret_cast<const float*>(p.g.out) + (size_t)t * p.g.ldo + n + c));
+#pragma unroll
+          for (int j = 0; j < W / 4; ++j) *reinterpret_cast<uint4*>(line_at(lane, 16 * j)) = reinterpret_cast<const uint4*>(w)[j];
           pieces(float(), c);
         }
       } else {
 #pragma unroll
         for (int c = 0; c < C; c += 64) {
+          constexpr int W = C < 64 ? C : 64;
+          uint32_t w[W / 2];
 #pragma unroll
-          for (int j = 0; j < (C < 64 ? C : 64) / 8; ++j) {
-            const float* v = x + c + 8 * j;
-            uint4 w;
+          for (int j = 0; j < W / 2; ++j) reinterpret_cast<__nv_bfloat162*>(w)[j] = __floats2bfloat162_rn(x[c + 2 * j], x[c + 2 * j + 1]);
+          if (OUT == kRowsAny && !vec) rows_rotate<2, true>(w, 2 * rows_head(reinterpret_cast<const __nv_bfloat16*>(p.g.out) + (size_t)t * p.g.ldo + n + c));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162*>(&w)[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<uint4*>(line_at(lane, 16 * j)) = w;
-          }
+          for (int j = 0; j < W / 8; ++j) *reinterpret_cast<uint4*>(line_at(lane, 16 * j)) = reinterpret_cast<const uint4*>(w)[j];
           pieces(__nv_bfloat16(), c);
         }
       }
@@ -411,6 +513,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) gemm_rows_tm_kernel(const __g
       sx = p.g.x_scale + t;
       sw = p.g.w_scale + (size_t)((im.w0 + n0) >> 7) * p.g.scale_ld;
       su = sw + (size_t)(p.g.dual_off >> 7) * p.g.scale_ld;
+      if (!DUAL && SPLIT == 1 && p.g.residual && t_ok && w_ok) {       // on its way to L2 while the item's sums run
+        const __nv_bfloat16* r = reinterpret_cast<const __nv_bfloat16*>(p.g.residual) + (size_t)t * p.g.ldr;
+#pragma unroll
+        for (int c = 0; c < PART; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + min(n0 + c, p.g.N - 1)));
+        if (OUT == kRowsAny) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + min(n0 + PART - 1, p.g.N - 1)));
+      }
       fetch_scales(k_lo);
     };
     if (first < total) begin(first, entry_of(first));
@@ -619,6 +727,9 @@ int launch_rows_prompt(const RowsGemm& g, int form, cudaStream_t st) {
     return form == 1 ? launch_rows_tm<256, true, 2, 1, kRowsCodes>(g, sms, st) : launch_rows_tm<256, true, 1, 1, kRowsCodes>(g, sms, st);
   if (g.gated) return launch_rows_tm<256, true, 1, 1, kRowsAny>(g, sms, st);
   if (g.out_scale) return -5;
+  // A residual whose rows start between 16 bytes takes its time in front of the stores, and narrow tiles finish in fewer registers: 8192 x 28671 x 256
+  // with tiles of 256 and 128 columns 921 and 588 us, 8192 x 28671 x 1024 1078 and 819, 2000 x 5001 x 5000 127 and 111.
+  if ((form == 1 || form == 3) && g.residual && g.K <= 5120 && ((g.ldr & 7) || (reinterpret_cast<uintptr_t>(g.residual) & 15))) form = 4;
   const bool plain = !g.bias && !g.act && !g.out_fp32 && g.N % 8 == 0 && g.ldo % 8 == 0 && (!g.residual || g.ldr % 8 == 0) &&
                      ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.residual)) & 15) == 0;
 #define XFT_ROWS_TM(NCOL, CG, SPLIT) \

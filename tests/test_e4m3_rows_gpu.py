@@ -128,6 +128,29 @@ def test_tiles_of_prompts(T, N, K, form):
         assert bool(((out[:T].cpu().double() - want).abs() <= tol + half * want.abs()).all()) and bool((out[T] == 7).all())
 
 
+# rows of the result and of the residual that start anywhere between 16 bytes, each at its own place
+@pytest.mark.parametrize("form", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("N,pitch,off", [(641, 647, 1), (642, 645, 3), (516, 520, 4), (768, 769, 0), (513, 520, 8), (70, 77, 5), (135, 135, 0)])
+def test_rows_between_16_bytes(N, pitch, off, form):
+    from xfastertransformer_b200.ops import native_e4m3 as E
+    T, K = 261, 1024
+    g = gen(N, pitch, off)
+    q, W, bias = rows(activations(g, T, K)), weight(g, N, K), torch.randn(N, generator=g)
+    wide = torch.randn(T, pitch + 8, generator=g).bfloat16()
+    want, tol = sum_tol(q, W)
+    want = (want + bias.double()).clamp_min(0) + 0.5 * wide[:, off:off + N].double()
+    tol = tol + 2.0 ** -23 * (bias.double().abs() + wide[:, off:off + N].double().abs() + want.abs())
+    dq, dW, dres = rows_on(q), on(W), wide.cuda()[:, off:off + N]
+    for dtype, half in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8)):
+        room = torch.full((T + 1, pitch), 7.0, dtype=dtype, device="cuda")
+        out = room.view(-1)[1:1 + T * pitch].view(T, pitch)[:, :N]
+        E._gemm(dq, dW.w, dW.scale, out, T, N, K, bias=bias.cuda(), act="relu", residual=dres, res_scale=0.5, form=form)
+        check_status()
+        assert bool(((out.cpu().double() - want).abs() <= tol + half * want.abs()).all())
+        out.fill_(7)
+        assert bool((room == 7).all())
+
+
 @pytest.mark.parametrize("form", [1, 3])
 @pytest.mark.parametrize("T,I,K", [(1, 128, 128), (130, 384, 200), (300, 640, 1024), (5000, 1408, 256)])
 def test_gated_tiles_of_prompts(T, I, K, form):
