@@ -118,8 +118,9 @@ struct E4Layout {
   static constexpr int CTAS = (BN <= 32 || (SRC == kSrcRows && !DUAL)) && A_RING + 3 * STAGE <= 110 * 1024 ? 2 : 1;
   // Registers are left for the CTAs of the kernels behind: with programmatic launches those sit beside this one, their first weights
   // under way.  At 90 registers (16 rows, bf16) instead of 64 the products of a 7B layer were as fast one behind the other, but 31 steps
-  // of one row over 16 layers took 48.3 ms instead of 46.3.
-  static constexpr int MIN_CTAS = CTAS == 2 && (BN == 16 || SRC == kSrcI8) ? 3 : CTAS;
+  // of one row over 16 layers took 48.3 ms instead of 46.3.  Gated e4m3 rows have two sums and their scales to keep and would spill at 64: us at 64 /
+  // 96, 16 rows of 2 x 11008 x 4096 21.6 / 20.2, of 2 x 22016 x 4096 35.1 / 32.9, 8 tokens on 64 experts of 1408 x 2048, products in turn, 69.7 / 66.1.
+  static constexpr int MIN_CTAS = CTAS == 2 && ((BN == 16 && !(SRC == kSrcRows && DUAL)) || SRC == kSrcI8) ? 3 : CTAS;
   static constexpr int FIT = ((CTAS == 2 ? 110 : 222) * 1024 - A_RING) / STAGE;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = A_RING + STAGES * STAGE + 1024;
