@@ -118,9 +118,8 @@ struct E4Layout {
   static constexpr int CTAS = (BN <= 32 || (SRC == kSrcRows && !DUAL)) && A_RING + 3 * STAGE <= 110 * 1024 ? 2 : 1;
   // Registers are left for the CTAs of the kernels behind: with programmatic launches those sit beside this one, their first weights
   // under way.  At 90 registers (16 rows, bf16) instead of 64 the products of a 7B layer were as fast one behind the other, but 31 steps
-  // of one row over 16 layers took 48.3 ms instead of 46.3.  Gated e4m3 rows have two sums and their scales to keep and would spill at 64: us at 64 /
-  // 96, 16 rows of 2 x 11008 x 4096 21.6 / 20.2, of 2 x 22016 x 4096 35.1 / 32.9, 8 tokens on 64 experts of 1408 x 2048, products in turn, 69.7 / 66.1.
-  static constexpr int MIN_CTAS = CTAS == 2 && ((BN == 16 && !(SRC == kSrcRows && DUAL)) || SRC == kSrcI8) ? 3 : CTAS;
+  // of one row over 16 layers took 48.3 ms instead of 46.3.
+  static constexpr int MIN_CTAS = CTAS == 2 && (BN == 16 || SRC == kSrcI8) ? 3 : CTAS;
   static constexpr int FIT = ((CTAS == 2 ? 110 : 222) * 1024 - A_RING) / STAGE;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = A_RING + STAGES * STAGE + 1024;
@@ -165,7 +164,7 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
   constexpr int NCOL = SRC == kSrcI8 ? 3 : SRC == kSrcU4 ? 2 : 0, NROW = SRC == kSrcI8 ? 3 : SRC == kSrcBf16 ? 1 : 2;
   __shared__ alignas(16) float s_col[NCOL ? NCOL : 1][NACC][NCOL ? 128 : 4];
   __shared__ float s_row[NROW][BN];
-  __shared__ alignas(16) float s_xs[SRC == kSrcRows ? 8 : 1][SRC == kSrcRows ? 2 * BN : 4];  // per warp: its tokens' scales of four blocks
+  __shared__ alignas(16) float s_xs[SRC == kSrcRows ? 8 : 1][SRC == kSrcRows ? 2 * BN + 8 : 4];  // per warp: scales of four blocks, its tokens' and the weights'
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int tile_n, tile_t;
@@ -379,23 +378,22 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
     } else if constexpr (SRC == kSrcRows) {
       // A block's sum of a token is scaled with the row's scale and the weights'.  Scales come four blocks at a time and are asked for four
       // blocks ahead (a load from L2 takes longer than a block, and a value that moves between registers waits for its load); a lane holds
-      // a token's, and the warp reads them from lines of shared memory of its own.
-      const float* sc = p.scale + (size_t)(w_row0 >> 7) * p.scale_ld;
-      const float* sc_up = sc + (size_t)(p.dual_off >> 7) * p.scale_ld;
-      float xs[4], ws[4], us[4];
-      auto fetch_weights = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ws[i] = kb + i < kend ? __ldg(sc + kb + i) : 0.f;
-          if (DUAL) us[i] = kb + i < kend ? __ldg(sc_up + kb + i) : 0.f;
-        }
-      };
+      // its share of them, and the warp reads them from lines of shared memory of its own: [block][token], then gate and up of the weights.
+      // (Each lane holding all of a block's numbers spilled: 16 rows of 2 x 11008 x 4096 21.7 us and 20.4 so, 64 rows 30.5 and 27.1, 33 rows of 7168 x
+      // 16384 26.2 and 25.3; the same without spills at 96 registers 20.1, but one token on two of 8 experts of 14336 x 4096 94.7 and not 88.5.)
+      const float* sc = p.scale + (size_t)(w_row0 >> 7) * p.scale_ld + (DUAL && lane & 4 ? (size_t)(p.dual_off >> 7) * p.scale_ld : 0) + (lane & 3);
+      constexpr int XR = HB / 8;
+      float xs[XR], ws;
+      auto fetch_weights = [&](int kb) { ws = lane < 8 && kb + (lane & 3) < kend ? __ldg(sc + kb) : 0.f; };
       float* line = s_xs[warp - 2];
-      const bool mine = lane < HB && c0 + lane < x_rows;
-      const float* sx = p.x_scale + x_row0 + c0 + lane;
+      const bool mine = c0 + lane % HB < x_rows;
+      const float* sx = p.x_scale + x_row0 + c0 + lane % HB;
       auto fetch_xs = [&](int kb) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xs[i] = mine && kb + i < kend ? __ldg(sx + (size_t)(kb + i) * p.x_ld) : 0.f;
+        for (int r = 0; r < XR; ++r) {
+          const int at = kb + (lane + 32 * r) / HB;
+          xs[r] = mine && at < kend ? __ldg(sx + (size_t)at * p.x_ld) : 0.f;
+        }
       };
       fetch_weights(kb0);
       grid_dep_wait();
@@ -403,14 +401,10 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
       fetch_rows();
       Ring b = {0, 0};
       for (int kb4 = kb0; kb4 < kend && ok; kb4 += 4) {
-        float wf[4], uf[4];
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (lane < HB) line[i * HB + lane] = xs[i];
-          wf[i] = ws[i];
-          uf[i] = DUAL ? us[i] : 0.f;
-        }
+        for (int r = 0; r < XR; ++r) line[lane + 32 * r] = xs[r];
+        if (lane < 8) line[4 * HB + lane] = ws;
         fetch_xs(kb4 + 4);
         fetch_weights(kb4 + 4);
         __syncwarp();
@@ -427,14 +421,15 @@ __global__ void __launch_bounds__(kE4Threads, E4Layout<BN, DUAL, SRC>::MIN_CTAS)
           tcgen05_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&tmem_empty[b.s]);
+          const float wf = line[4 * HB + i], uf = DUAL ? line[4 * HB + 4 + i] : 0.f;
 #pragma unroll
           for (int j = 0; j < HB; j += 4) {
             const float4 f = *reinterpret_cast<const float4*>(line + i * HB + j);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float s = (&f.x)[k];
-              g[0][j + k] = fmaf(s * wf[i], __uint_as_float(v[0][j + k]), g[0][j + k]);
-              if constexpr (DUAL) g[NACC - 1][j + k] = fmaf(s * uf[i], __uint_as_float(v[NACC - 1][j + k]), g[NACC - 1][j + k]);
+              g[0][j + k] = fmaf(s * wf, __uint_as_float(v[0][j + k]), g[0][j + k]);
+              if constexpr (DUAL) g[NACC - 1][j + k] = fmaf(s * uf, __uint_as_float(v[NACC - 1][j + k]), g[NACC - 1][j + k]);
             }
           }
           b.next(TURN);
