@@ -112,16 +112,22 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (i >= nch) continue;
     // The row's factor 1 / rms is in the scale alone where the block lies above the floor: it cancels in a code, whose rounding then sees one
-    // rounding of the product with the gain and two of the scaling.
+    // rounding of the product with the gain and two of the scaling.  Below the floor, with that factor or without it, the values are
+    // multiplied by it first: 448 / 2^-100 times a factor above 6e5 (eps below 2.8e-12) leaves 32 bits, and so does 448 over such a maximum.
+    // So they are where the factor is no number.
     E4m3Scale s;
+    float lacks = inv;                                                 // what y has still to be multiplied by
     if constexpr (!NORM) {
       s = e4m3_scale(top);
-    } else if (top * inv < kE4m3Least) {
-      s = e4m3_scale(0.f);
-      s.inv *= inv;
-    } else {
+    } else if (const float a = top * inv; top >= kE4m3Least && a >= kE4m3Least && a <= 3.4e38f) {
       s = e4m3_scale_of(top);
-      s.scale = __fdiv_rn(top * inv, kE4m3Top);
+      s.scale = __fdiv_rn(a, kE4m3Top);
+    } else {
+      s = e4m3_scale(a <= 3.4e38f ? a : 0.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] *= inv;
+      odd = odd || inv > 3.4e38f;
+      lacks = 1.f;
     }
     uint2 q;
     q.x = e4m3_codes(y, s.inv, odd);
@@ -132,7 +138,7 @@ __global__ void __launch_bounds__(NT) rows_e4m3_kernel(const RowsE4m3Params p) {
       if (p.y) {
         uint4 u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) reinterpret_cast<__nv_bfloat162*>(&u)[j] = __floats2bfloat162_rn(y[2 * j] * inv, y[2 * j + 1] * inv);
+        for (int j = 0; j < 4; ++j) reinterpret_cast<__nv_bfloat162*>(&u)[j] = __floats2bfloat162_rn(y[2 * j] * lacks, y[2 * j + 1] * lacks);
         reinterpret_cast<uint4*>(p.y + row * p.ldy)[i] = u;
       }
     }
