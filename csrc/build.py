@@ -24,8 +24,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "--use_fast_math", "-Xptxas", "-v"]
 
-# sources that need the accurate division, expf and tanhf
-ACCURATE = {"plain.cu", "latent.cu", "head_prep.cu", "gla.cu", "ssd.cu", "talking.cu", "talking_mma.cu"}
+# sources that need the accurate division, expf and tanhf, or numbers below 2^-126 (rows_e4m3.cu)
+ACCURATE = {"plain.cu", "latent.cu", "head_prep.cu", "gla.cu", "ssd.cu", "talking.cu", "talking_mma.cu", "rows_e4m3.cu"}
 # what a layered model calls: GEMMs, attention, norms, rotary + cache append, experts, arg-max, and what these link against
 LAYERED = ["attention.cu", "attention_prefill_sm100.cu", "elementwise.cu", "gemm_decode_sm100.cu", "gemm_e4m3_sm100.cu",
            "gemm_prefill_sm100.cu", "gemm_rows_e4m3_sm100.cu",
