@@ -939,7 +939,8 @@ extern "C" int xft_rows_gemm_layout(long long* out, int n) {
 // Grouped: tiles of `bn` rows as in xft_qgemm_grouped.
 extern "C" int xft_gemm_rows_e4m3(const RowsGemm* args, cudaStream_t st) {
   const RowsGemm& a = *args;
-  if (a.T <= 0 || a.N <= 0 || a.K <= 0) return 0;
+  if (a.T <= 0 || a.N <= 0) return 0;
+  if (a.K <= 0) return -3;                                             // the result would stay unwritten
   if ((a.ldx & 15) || (a.ldw & 15) || (reinterpret_cast<uintptr_t>(a.x) & 15) || (reinterpret_cast<uintptr_t>(a.w) & 15)) return -2;
   if ((a.gated && (a.dual_off & 127)) || (a.group_tiles && (a.group_w_rows <= 0 || (a.group_w_rows & 127)))) return -4;
   if (a.out_scale && (!a.gated || (a.N & 127) || (a.ldo & 15) || (reinterpret_cast<uintptr_t>(a.out) & 15) || a.residual || a.col_scale)) return -5;

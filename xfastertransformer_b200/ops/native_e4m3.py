@@ -180,6 +180,9 @@ def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
     I = W.out_features // 2
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
+    if not K:                                            # no columns, as in linear_e4m3
+        from . import reference as R
+        return R.linear_gated_e4m3(q, W, act, bias)
     out = new_rows(T, I, q.codes)
     if T and I:
         _gemm(q, _weight(W), W.scale, out.codes, T, I, K, True, I, bias, act, out_scale=out.scale)
@@ -247,6 +250,8 @@ def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=Non
     out = q.codes.new_empty((T, H), dtype=out_dtype)
     if T == 0:
         return out
+    if I == 0:                                           # a rank's empty share of the experts' features
+        return out.zero_() if add is None else out.copy_(add)
     ws, lib, st = N.Workspace.get(dev), _lib(), _stream()
     pairs = T * k
     avg = max(1, ((pairs if expected_pairs is None else min(int(expected_pairs), pairs)) + E - 1) // E)

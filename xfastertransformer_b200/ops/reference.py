@@ -291,9 +291,9 @@ def quantize_e4m3(y: torch.Tensor) -> RowsE4M3:
     b = F.pad(y.float(), (0, n * BLOCK - K)).view(T, n, BLOCK)
     fine = torch.isfinite(b)
     a = torch.where(fine, b.abs(), torch.zeros_like(b)).amax(-1).clamp_min(LEAST)
-    inv = torch.full_like(a, TOP) / a                          # one rounding: a number over a tensor would be a reciprocal and a product
+    inv = torch.full_like(a, TOP) / a                          # one rounding: with a number, a GPU takes a reciprocal and a product
     v = torch.where(fine, (b * inv[..., None]).clamp(-TOP, TOP), torch.full_like(b, float("nan")))
-    return RowsE4M3(v.view(T, -1)[:, :K].to(torch.float8_e4m3fn).contiguous(), (a / TOP).t().contiguous())
+    return RowsE4M3(v.view(T, -1)[:, :K].to(torch.float8_e4m3fn).contiguous(), (a / torch.full_like(a, TOP)).t().contiguous())
 
 
 def rmsnorm_e4m3(x, w, eps, residual=None, want_rows=False):
