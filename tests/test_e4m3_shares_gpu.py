@@ -56,3 +56,12 @@ def test_a_product_without_columns_is_refused_by_the_kernel():
     q, W = rows_on(rows(torch.randn(4, 128, generator=gen(3)))), on(weight(gen(4), 128, 128))
     with pytest.raises(N.KernelError):
         E._gemm(q, W.w, W.scale, torch.empty(4, 128, device="cuda"), 4, 128, 0)
+
+
+def test_products_of_no_columns_and_of_no_rows():
+    """Activations that are not rows in e4m3 yet."""
+    W, r = no_weight(64, 0), torch.randn(3, 64, generator=gen(2)).bfloat16().cuda()
+    soil()
+    assert torch.equal(ops.linear(torch.zeros(3, 0, dtype=torch.bfloat16, device="cuda"), W, residual=r), r)
+    V, none = on(weight(gen(3), 256, 200)), torch.zeros(0, 200, dtype=torch.bfloat16, device="cuda")
+    assert ops.linear(none, V).shape == (0, 256) and ops.linear_gated(none, V).shape == (0, 128)

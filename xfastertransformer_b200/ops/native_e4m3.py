@@ -8,6 +8,7 @@ packed struct or as plain numbers."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 import weakref
 
@@ -112,6 +113,11 @@ def rows_e4m3(x, gain=None, eps=0.0, residual=None, want_rows=False):
         N._check(rc, "rows_e4m3")
     N.Workspace.get(dev).launches += 1
     return q, y, h
+
+
+def rows_of(x) -> RowsE4M3:
+    """What a product of 8-bit rows reads of x; a rank's empty share of the columns has no rows to launch for."""
+    return rows_e4m3(x)[0] if x.shape[-1] else new_rows(math.prod(x.shape[:-1]), 0, x)
 
 
 def _weight(W):

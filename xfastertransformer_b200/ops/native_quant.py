@@ -219,7 +219,7 @@ def linear(x, W, bias=None, act=None, residual=None, res_scale=1.0, out_dtype=No
         from . import native_e4m3 as E
         if N._ACT.get(act, 9) > 5 and act != "tanh":
             raise N.KernelError(f"no product of {W.kind} weights with activation {act!r}")
-        return E.linear_e4m3(E.rows_e4m3(x)[0], W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
+        return E.linear_e4m3(E.rows_of(x), W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
     if W.kind in _QT or W.kind in _E4M3:
         return _qgemm(x, W, W.out_features, False, bias, act, residual, res_scale, out_dtype, norm)
     raise N.KernelError(f"no sm_100a GEMM for weight kind {W.kind}")
@@ -242,7 +242,7 @@ def linear_gated(x, W, act="silu", bias=None, norm=None):
         from . import native_e4m3 as E
         if N._ACT.get(act, 9) > 5 and act != "tanh":
             raise N.KernelError(f"no gated product of {W.kind} weights with activation {act!r}")
-        q = E.rows_e4m3(x)[0]
+        q = E.rows_of(x)
         return N.gated_act(E.linear_e4m3(q, W, bias), act) if I % 128 else E.gated_rows(q, W, act, bias)
     if W.kind == "fp8" and I % 128:
         gu = _qgemm(x, W, 2 * I, False, bias, None, None, 1.0, None)

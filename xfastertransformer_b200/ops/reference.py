@@ -222,7 +222,7 @@ def linear(x: torch.Tensor, W, bias: Optional[torch.Tensor] = None, act: Optiona
         q, sa, za = quantize_act_w8a8(x)
         xf = q.float() * sa[..., None] + za[..., None]
     elif W.kind == "fp8a":
-        xf = quantize_e4m3(x.reshape(-1, x.shape[-1])).values().view(x.shape)
+        xf = quantize_e4m3(x.reshape(math.prod(x.shape[:-1]), x.shape[-1])).values().view(x.shape)
     else:
         xf = x.float()
     y = xf @ dequant_weight(W).t()
@@ -269,7 +269,7 @@ def linear_gated(x: torch.Tensor, W, act: str = "silu", bias: Optional[torch.Ten
         q, sa, za = quantize_act_w8a8(x)
         xf = q.float() * sa[..., None] + za[..., None]
     elif W.kind == "fp8a":
-        xf = quantize_e4m3(x.reshape(-1, x.shape[-1])).values().view(x.shape)
+        xf = quantize_e4m3(x.reshape(math.prod(x.shape[:-1]), x.shape[-1])).values().view(x.shape)
     y = xf @ dequant_weight(W).t()
     if bias is not None:
         y = y + bias.float()
@@ -293,7 +293,7 @@ def quantize_e4m3(y: torch.Tensor) -> RowsE4M3:
     a = torch.where(fine, b.abs(), torch.zeros_like(b)).amax(-1).clamp_min(LEAST)
     inv = torch.full_like(a, TOP) / a                          # one rounding: with a number, a GPU takes a reciprocal and a product
     v = torch.where(fine, (b * inv[..., None]).clamp(-TOP, TOP), torch.full_like(b, float("nan")))
-    return RowsE4M3(v.view(T, -1)[:, :K].to(torch.float8_e4m3fn).contiguous(), (a / torch.full_like(a, TOP)).t().contiguous())
+    return RowsE4M3(v.view(T, n * BLOCK)[:, :K].to(torch.float8_e4m3fn).contiguous(), (a / torch.full_like(a, TOP)).t().contiguous())
 
 
 def rmsnorm_e4m3(x, w, eps, residual=None, want_rows=False):
