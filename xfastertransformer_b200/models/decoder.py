@@ -281,7 +281,7 @@ class Decoder:
     def _ffn_range(self, inter: int, gran: int = 1, split_idx: Optional[int] = None):
         idx = self.tpr if split_idx is None else split_idx
         if gran > 1 and inter % gran == 0:
-            return P.task_range_gran(inter, gran, self.tp, idx)
+            return (P.block_range if self.kind == "fp8a" else P.task_range_gran)(inter, gran, self.tp, idx)
         return P.task_range(inter, self.tp, idx)
 
     def _load_mlp_llama(self, L, p, i):
@@ -486,7 +486,7 @@ class Decoder:
         sum.  Otherwise: partial GEMM with residual/bias on rank 0 only, then a collective."""
         peer = getattr(self.ctx, "peer", None)
         if self.tp > 1 and peer is not None and h.is_cuda:
-            T = h.numel() // h.shape[-1]
+            T = math.prod(h.shape[:-1])                                # (a rank's share of the columns may be empty)
             if peer.can_fuse(T, W.out_features, W.kind):
                 return peer.gemm_ar(h, W, bias, None, residual, res_scale)
             if peer.can_fuse_bulk(T, W.out_features, h.shape[-1], W.kind):      # prefill sizes, opt-in

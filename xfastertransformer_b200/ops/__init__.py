@@ -78,6 +78,7 @@ def _timed(kernel: str, x, W, fn):
     """XFT_VERBOSE >= 1: run one GEMM-shaped op between two time stamps (device-synchronised on a GPU) and print the
     reference's per-call line ``xft_verbose,exec,<dev>,api,<kernel>,m<M>n<N>k<K>,<ms>`` (src/utils/verbose.h:24-83).
     The decode graph runner steps aside while this is on, so every call is a real launch."""
+    import math
     import time
     from ..utils import log
     cuda = _cuda(x)
@@ -88,7 +89,7 @@ def _timed(kernel: str, x, W, fn):
     if cuda:
         torch.cuda.synchronize(x.device)
     ms = (time.perf_counter() - t0) * 1e3
-    log.verbose_line("gpu" if cuda else "cpu", kernel, x.numel() // x.shape[-1], W.out_features, x.shape[-1], ms)
+    log.verbose_line("gpu" if cuda else "cpu", kernel, math.prod(x.shape[:-1]), W.out_features, x.shape[-1], ms)
     return y
 
 

@@ -6,6 +6,8 @@ tensor exactly where the reference would (``src/utils/split_util.h:8-99``):
 * `task_range(N, splits, idx)` — even split when ``N % (splits*64) == 0``; otherwise the
   coarsest granularity of 64/16/2 that divides N, with the remainder going to low ranks
   (FFN 11008 over 8 ranks -> 4x1408 + 4x1344; 688 over 2 -> 352 + 336).
+* `block_range(N, gran, splits, idx)` — blocks shared out evenly (e4m3 weights with e4m3 activations, which
+  the reference does not have).
 * `head_range(q, kv, splits, idx)` — contiguous query-head range and the covering KV range.
 * PP stage layer ranges (``src/layers/decoder_block.h:33-40``) and the MoE slice rotation
   (``src/layers/mlp_llama.h:70-79``).  Expert-parallel placement is new (the reference
@@ -43,6 +45,18 @@ def task_range_gran(n: int, gran: int, splits: int, idx: int) -> Tuple[int, int]
         raise ValueError(f"N ({n}) need to be multiple of granularity ({gran}).")
     s, e = task_range(n // gran, splits, idx)
     return s * gran, e * gran
+
+
+def block_range(n: int, gran: int, splits: int, idx: int) -> Tuple[int, int]:
+    """Blocks of `gran` shared out evenly, one more on the first ranks: a share is empty only where there are fewer blocks than ranks.
+    (`task_range_gran` groups the blocks again: 2048 in blocks of 128 over 2 ranks are 2048 and 0 there.)"""
+    if n % gran:
+        raise ValueError(f"N ({n}) need to be multiple of granularity ({gran}).")
+    if splits <= 0 or not (0 <= idx < splits):
+        raise ValueError(f"bad split {idx}/{splits}")
+    base, rem = divmod(n // gran, splits)
+    start = idx * base + min(idx, rem)
+    return start * gran, (start + base + (idx < rem)) * gran
 
 
 def head_range(q_heads: int, kv_heads: int, splits: int, idx: int):
