@@ -270,8 +270,9 @@ def pack_experts_e4m3(experts):
 
 def moe_experts_e4m3(q, idx, w, experts, act="silu", expert_offset=0, packed=None, expected_pairs=None, add=None, out_dtype=torch.float32):
     """sum_k w[t, k] down_e(act(gate_e q_t) * up_e q_t) (+ `add`, fp32 or bf16) over the local experts e = idx[t, k] - expert_offset of
-    rows in e4m3, the middle rows in e4m3 too; experts outside the list (or -1) add nothing.  `out_dtype`: fp32 or bf16.  Other
-    arguments as in `moe_experts`."""
+    rows in e4m3, the middle rows in e4m3 too; experts outside the list (or -1) add nothing.  `out_dtype`: fp32, with sums and the experts'
+    parts of them in fp32, or bf16, where a GPU rounds a part to bf16 before it is weighted and added if an expert has more than 32 rows on
+    average.  That average comes from `expected_pairs` where that is given.  Other arguments as in `moe_experts`."""
     if not isinstance(q, RowsE4M3):
         raise ValueError(f"moe_experts_e4m3 multiplies rows in e4m3 (RowsE4M3), not {type(q).__name__}")
     T, H = q.shape
