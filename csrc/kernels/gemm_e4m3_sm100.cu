@@ -818,8 +818,9 @@ static int e4_splits(int tiles, int num_kb, int per_sm) {
   return 1 << i;
 }
 
+// early: the launch may begin beside the one in front of it, whose results it waits for in all but the weights
 template <int BN, bool DUAL, int SRC>
-static int launch_e4(const CUtensorMap& tmW, const CUtensorMap& tmX, E4Params p, cudaStream_t st) {
+static int launch_e4(const CUtensorMap& tmW, const CUtensorMap& tmX, E4Params p, cudaStream_t st, bool early = true) {
   using L = E4Layout<BN, DUAL, SRC>;
   const auto kernel = gemm_e4m3_kernel<BN, DUAL, SRC>;
   static std::atomic<uint64_t> attr_set{0};                            // a bit for each device, whose kernel has its own
@@ -847,7 +848,7 @@ static int launch_e4(const CUtensorMap& tmW, const CUtensorMap& tmX, E4Params p,
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = g_xft_pdl ? 2 : 1;
+  cfg.numAttrs = g_xft_pdl && early ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
@@ -968,7 +969,9 @@ extern "C" int xft_gemm_rows_e4m3(const RowsGemm* args, cudaStream_t st) {
   r = encode_tensor_map(&tmX, a.x, (uint64_t)a.x_rows, (uint64_t)a.K, (uint64_t)a.ldx, (uint32_t)bn, 1);
   if (r) return 2000 - r;
 #define XFT_ROWS(BN_) \
-  case BN_: return a.gated ? launch_e4<BN_, true, kSrcRows>(tmW, tmX, p, st) : launch_e4<BN_, false, kSrcRows>(tmW, tmX, p, st);
+  case BN_:                                                                                          \
+    return a.gated ? launch_e4<BN_, true, kSrcRows>(tmW, tmX, p, st, a.form != kRowsFormAfterCopy)   \
+                   : launch_e4<BN_, false, kSrcRows>(tmW, tmX, p, st, a.form != kRowsFormAfterCopy);
   switch (bn) { XFT_ROWS(16) XFT_ROWS(32) XFT_ROWS(64) }
 #undef XFT_ROWS
   return -1;

@@ -43,6 +43,10 @@ __device__ __forceinline__ uint32_t e4m3_codes(const float* v, float inv, bool o
   return q;
 }
 
+// By size, and the launch in front of this one writes the weights: a step's kernel, which asks for weights before it waits for that launch, is
+// then not started beside it.
+constexpr int kRowsFormAfterCopy = -2;
+
 // Arguments of xft_gemm_rows_e4m3 (mirrored in ops/native_e4m3.py).
 struct RowsGemm {
   const void* x; const float* x_scale; const void* w; const float* w_scale;
@@ -53,7 +57,7 @@ struct RowsGemm {
   int T, N, K, ldo, out_fp32, ldr, act;
   int gated, dual_off;
   int group_w_rows, max_tiles, bn;                     // grouped form: rows of a tile of the table
-  int form;                                            // -1: by size; 0: gemm_e4m3_sm100.cu, else a tile of gemm_rows_e4m3_sm100.cu
+  int form;                                            // -1: by size; kRowsFormAfterCopy; 0: gemm_e4m3_sm100.cu, else a tile of gemm_rows_e4m3_sm100.cu
   float res_scale;
 };
 

@@ -120,8 +120,17 @@ def rows_of(x) -> RowsE4M3:
     return rows_e4m3(x)[0] if x.shape[-1] else new_rows(math.prod(x.shape[:-1]), 0, x)
 
 
+AFTER_COPY = -2                # csrc/kernels/rows_e4m3.cuh:kRowsFormAfterCopy
+
+
+def _form(W, w) -> int:
+    """How a product of `_weight`'s codes w is launched: a copy that is not kept was made by the launch in front of it."""
+    return -1 if w is W.w or W.cache.get("w_pitch16") is w else AFTER_COPY
+
+
 def _weight(W):
-    """The codes of W with rows on 16 bytes; the copy that this may take is kept with the weight (inside a capture it is part of the graph)."""
+    """The codes of W with rows on 16 bytes; the copy that this may take is kept with the weight (inside a capture it is part of the graph, and
+    the product behind it says so, see `_form`)."""
     w = W.w
     ld, one = w.stride()
     if ld % 16 or one != 1 or w.data_ptr() % 16:
@@ -173,7 +182,8 @@ def linear_e4m3(q, W, bias=None, act=None, residual=None, res_scale=1.0, out_dty
         return (y if residual is None else y + res_scale * residual.float()).to(out_dtype)
     out = q.codes.new_empty((T, W.out_features), dtype=out_dtype)
     if T:
-        _gemm(q, _weight(W), W.scale, out, T, W.out_features, K, False, 0, bias, act, residual, res_scale)
+        w = _weight(W)
+        _gemm(q, w, W.scale, out, T, W.out_features, K, False, 0, bias, act, residual, res_scale, form=_form(W, w))
     return out
 
 
@@ -191,7 +201,8 @@ def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
         return R.linear_gated_e4m3(q, W, act, bias)
     out = new_rows(T, I, q.codes)
     if T and I:
-        _gemm(q, _weight(W), W.scale, out.codes, T, I, K, True, I, bias, act, out_scale=out.scale)
+        w = _weight(W)
+        _gemm(q, w, W.scale, out.codes, T, I, K, True, I, bias, act, out_scale=out.scale, form=_form(W, w))
     return out
 
 
@@ -201,7 +212,8 @@ def gated_rows(q, W, act, bias=None):
     I = W.out_features // 2
     out = torch.empty(T, I, dtype=torch.bfloat16, device=q.device)
     if T:
-        _gemm(q, _weight(W), W.scale, out, T, I, K, True, I, bias, act)
+        w = _weight(W)
+        _gemm(q, w, W.scale, out, T, I, K, True, I, bias, act, form=_form(W, w))
     return out
 
 
