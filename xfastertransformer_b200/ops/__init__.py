@@ -253,7 +253,8 @@ def linear_gated_e4m3(q, W, act="silu", bias=None) -> RowsE4M3:
 
 def pack_experts_e4m3(experts):
     """The stacked weights of a list of experts, (gate | up, down) each, that `moe_experts_e4m3` takes as `packed`; made once, the experts'
-    own weights become views of the stacks.  None on a CPU."""
+    own weights become views of the stacks.  They are kept with the first expert for as long as all experts of the list live; a graph that was
+    captured over them needs those, or this result, for as long.  None on a CPU."""
     if not experts:
         raise ValueError("pack_experts_e4m3: no experts")
     for g, d in experts:

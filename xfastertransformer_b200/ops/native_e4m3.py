@@ -226,13 +226,20 @@ def packed_before(experts):
 
 
 def pack_experts(experts) -> dict:
-    """Stacks of these experts, made once: what a captured graph reads stays, also when another list with the same first expert comes."""
+    """Stacks of these experts, made once: what a captured graph reads stays, also when another list with the same first expert comes, for as long
+    as all of its experts do.  (Each list that lives has stacks of its own; who holds the result holds them longer.)"""
     pk = packed_before(experts)
     if pk is None:
         from . import native_moe
         cache, dev = experts[0][0].cache, experts[0][0].w.device
         if torch.cuda.is_current_stream_capturing():
             raise N.KernelError("experts' weights are stacked before a graph is captured (pack_experts_e4m3), not inside it")
+        whole = lambda of: all(a() is not None and b() is not None for a, b in of)
+        packs = cache.setdefault("e4m3_packs", [])
+        gone = [p for of, p in packs if not whole(of)]                      # nobody can ask for these again
+        packs[:] = [(of, p) for of, p in packs if whole(of)]
+        if any(p is cache.get("moe_pack") for p in gone):
+            del cache["moe_pack"]
         old = cache.get("moe_pack")
         step = lambda s, n: s.data_ptr() + n * s.shape[1]
         if old is not None and "gus" in old and old["E"] == len(experts) and all(
@@ -243,7 +250,7 @@ def pack_experts(experts) -> dict:
             pk = native_moe._pack_fp8(experts)
             if old is not None:
                 cache["moe_pack"] = old
-        cache.setdefault("e4m3_packs", []).append(([(weakref.ref(g), weakref.ref(d)) for g, d in experts], pk))
+        packs.append(([(weakref.ref(g), weakref.ref(d)) for g, d in experts], pk))
         torch.cuda.current_stream(dev).synchronize()                    # other streams may read them from now on
     return pk
 
