@@ -9,8 +9,8 @@ from xfastertransformer_b200 import ops
 from xfastertransformer_b200.runtime.loader import LinearWeight
 
 
-def no_weight(n, k):
-    return LinearWeight("fp8a", torch.zeros(n, k).to(torch.float8_e4m3fn), torch.zeros(-(-n // 128), -(-k // 128)), in_features=k, out_features=n).to("cuda")
+def no_weight(n, k, kind="fp8a"):
+    return LinearWeight(kind, torch.zeros(n, k).to(torch.float8_e4m3fn), torch.zeros(-(-n // 128), -(-k // 128)), in_features=k, out_features=n).to("cuda")
 
 
 def soil():
@@ -65,3 +65,24 @@ def test_products_of_no_columns_and_of_no_rows():
     assert torch.equal(ops.linear(torch.zeros(3, 0, dtype=torch.bfloat16, device="cuda"), W, residual=r), r)
     V, none = on(weight(gen(3), 256, 200)), torch.zeros(0, 200, dtype=torch.bfloat16, device="cuda")
     assert ops.linear(none, V).shape == (0, 256) and ops.linear_gated(none, V).shape == (0, 128)
+
+
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_weights_alone_in_e4m3(T):
+    """The type that keeps activations in bf16 has empty shares too."""
+    g = gen(T, 2)
+    H, E = 256, 3
+    x, r, b = torch.randn(T, H, generator=g).bfloat16().cuda(), torch.randn(T, H, generator=g).bfloat16().cuda(), torch.randn(H, generator=g).cuda()
+    experts = [(no_weight(0, H, "fp8"), no_weight(H, 0, "fp8")) for _ in range(E)]
+    idx, w = torch.randint(0, E, (T, 2), generator=g).int().cuda(), torch.rand(T, 2, generator=g).cuda()
+    for add in (None, torch.randn(T, H, generator=g).cuda(), torch.randn(T, H, generator=g).cuda().bfloat16()):
+        soil()
+        got = ops.moe_experts(x, idx, w, experts, add=add)
+        assert got.dtype == torch.float32 and torch.equal(got, torch.zeros(T, H, device="cuda") if add is None else add.float())
+        assert add is None or got.data_ptr() != add.data_ptr()
+    mid = ops.linear_gated(x, experts[0][0])
+    assert mid.shape == (T, 0)
+    soil()
+    assert torch.equal(ops.linear(mid, experts[0][1], out_dtype=torch.float32), torch.zeros(T, H, device="cuda"))
+    assert torch.equal(ops.linear(mid, experts[0][1], residual=r), r)
+    assert torch.equal(ops.linear(mid, experts[0][1], b, "relu", r, 0.5, torch.float32), b.clamp_min(0) + 0.5 * r.float())

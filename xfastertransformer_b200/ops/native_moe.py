@@ -147,6 +147,8 @@ def moe_experts(x, idx, w, experts, act="silu", expert_offset=0, packed=None, ex
     E, I = pk["E"], pk["I"]
     up = 2 * I if gated else I                       # weight rows of one expert's first product
     dev = x.device
+    if I == 0:                                       # a rank's empty share of the experts' features
+        return torch.zeros(T, H, dtype=torch.float32, device=dev) if add is None else add.float().reshape(T, H).clone()
     ws = N.Workspace.get(dev)
     lib = _lib()
     avg = max(1, ((T * k if expected_pairs is None else min(int(expected_pairs), T * k)) + E - 1) // E)

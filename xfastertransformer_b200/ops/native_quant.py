@@ -99,6 +99,9 @@ def _qgemm(x, W, n_out, gated, bias, act, residual, res_scale, out_dtype, norm=N
     T, K = x2.shape
     if K % 8:
         raise N.KernelError(f"quantised GEMM needs K % 8 == 0 (got {K})")
+    if not K and not gated:                              # a rank's empty share of a row-parallel product
+        from . import reference as R
+        return R.linear(x2, W, bias, act, residual, res_scale, out_dtype or torch.bfloat16)
     fp32 = out_dtype == torch.float32
     out = torch.empty(T, n_out, dtype=torch.float32 if fp32 else torch.bfloat16, device=x.device)
     ws = N.Workspace.get(x.device)
