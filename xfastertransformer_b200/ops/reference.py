@@ -198,7 +198,7 @@ def _act(y: torch.Tensor, act: Optional[str]) -> torch.Tensor:
         return y
     if act == "relu":
         return F.relu(y)
-    if act == "silu":
+    if act in ("silu", "swiglu"):
         return F.silu(y)
     if act in ("gelu", "gelu_tanh", "gelu_new", "gelu_pytorch_tanh"):
         return F.gelu(y, approximate="tanh")
