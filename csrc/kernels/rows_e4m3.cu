@@ -4,7 +4,8 @@
 //
 // A row stays in registers: x and r are read once, and a block of 128 columns lies with 16 neighbouring threads of eight columns each,
 // so its maximum is four shuffles and only the norm's sum crosses the block.  y is not rounded before its codes are taken.  Bound by
-// bytes where rows are many, by the chain fetch, reduction, store where they are few.
+// bytes where rows are many, by the chain fetch, reduction, store where they are few.  us on B200: norm of 16384 x 8192 with a bf16 residual 164 (0.88 of
+// the copy rate), codes alone 76 (0.82), 33 x 16384 8, one row of 4096 6.
 #include "rows_e4m3.cuh"
 
 #include <cstddef>
