@@ -118,7 +118,12 @@ def _qgemm(x, W, n_out, gated, bias, act, residual, res_scale, out_dtype, norm=N
             cols = w.shape[1]
             pad = (-cols * w.element_size()) % 16 // w.element_size()
             wp = torch.nn.functional.pad(w, (0, pad)).contiguous()[:, :cols]
-            W.cache["w_pitch16"] = wp
+            if torch.cuda.is_current_stream_capturing():
+                # the graph's own; and a plain launch in front of the product, which asks for weights before it waits for the launch before it
+                wp.new_zeros(1)
+            else:
+                torch.cuda.current_stream(w.device).synchronize()       # other streams may read it from now on
+                W.cache["w_pitch16"] = wp
         w = wp
     zero = W.zero
     copy = _codes_copy(W, n_out, w.shape[0], K, T, gated, ws, x.device)
