@@ -212,8 +212,11 @@ def prepare(case, seed):
         s["pools"] = [None if s[x] is None else list(s[x].unbind()) for x in ("kc", "vc", "ks", "vs")]
         tokens, sampled = _drafts(case, seed, trees)
         s["tokens"], s["sampled"] = torch.tensor(tokens, device="cuda"), torch.tensor(sampled, device="cuda")
-    if own:                                                  # the batch that a program's step has made for all of its layers
+    if own:                                                  # the batch that a program's step has made for all of its layers, and its pools
+        from xfastertransformer_b200 import ops
         from xfastertransformer_b200.models.decoder import Batch
+        if "pools" in s:
+            s["handle"] = ops.cache_pools(*s["pools"])
         s["batch"] = Batch(ids=s.get("tokens"), positions=s.get("pos"), slots=None, cu_q=s["cu_q"], kv_lens=s["kv_lens"],
                            block_table=s["table"], cu_q_dev=s["cu_dev"], kv_lens_dev=s["kv_dev"], max_q=max(n for n, _ in lens),
                            max_kv=max(s["kv_lens"]))
@@ -359,7 +362,7 @@ def _calls(s):
         return ops.tree_attention(s["q"], s["kc"], s["vc"], s["table"], s["cu_q"], s["kv_lens"], s["mask"], s["D"] ** -0.5, ks=s["ks"],
                                   vs=s["vs"], meta=s["batch"], softcap=s["softcap"], window=s["window"], keep_first=s["keep"],
                                   sinks=s["sink"], positions=s["pos"])
-    emitted, path, count = ops.tree_accept(s["tokens"], s["parents"], s["sampled"], s["cu_q"], s["kv_lens"], s["table"], *s["pools"],
+    emitted, path, count = ops.tree_accept(s["tokens"], s["parents"], s["sampled"], s["cu_q"], s["kv_lens"], s["table"], s["handle"],
                                            meta=s["batch"])
     return emitted, path, count, s["kc"], s["vc"], s["ks"], s["vs"]
 
