@@ -380,6 +380,131 @@ def paged_attention(q, kc, vc, block_table, cu_q, kv_lens, scale, ks=None, vs=No
                              prefix_lm_lens, group, q_off, softcap, window, keep_first, sinks)
 
 
+# -- trees of drafted tokens -------------------------------------------------------------------
+# One step scores several candidate continuations of each sequence at once.  Sequence b's nodes are rows cu_q[b]:cu_q[b+1], node 0 its last
+# token, a parent before its children; their keys and values are appended to the cache in that order, so they are the last positions of
+# kv_lens[b].  tree_mask, then per layer qkv_rope_cache (with the mask's positions) and tree_attention, then sample, then tree_accept.
+# `cu_q` and `kv_lens` come as lists; with `meta` (cu_q_dev, kv_lens_dev, max_q, max_kv, as a model's batch has them) nothing of them is copied.
+MAX_TREE_NODES = 256
+
+
+def _native_tree():
+    from . import native_tree
+    return native_tree
+
+
+def _check_trees(what, T, cu_q, kv_lens, meta, device):
+    if meta is not None and getattr(meta, "cu_q_dev", None) is not None:
+        cu, kv = meta.cu_q_dev, meta.kv_lens_dev
+        if cu.dtype is not torch.int32 or kv.dtype is not torch.int32 or cu.numel() != kv.numel() + 1 or not cu.is_contiguous() \
+                or not kv.is_contiguous() or cu.device != device or kv.device != device:
+            raise ValueError(f"{what}: cu_q_dev and kv_lens_dev are int32 on {device}, B + 1 and B of them")
+        if meta.max_q and meta.max_kv:
+            if meta.max_q > MAX_TREE_NODES:
+                raise ValueError(f"{what}: trees of up to {MAX_TREE_NODES} nodes, not {meta.max_q}")
+            return
+    if len(cu_q) != len(kv_lens) + 1 or cu_q[0] < 0 or cu_q[-1] > T:
+        raise ValueError(f"{what}: cu_q {list(cu_q)} of {len(kv_lens)} sequences and {T} rows")
+    for b, n_kv in enumerate(kv_lens):
+        n = cu_q[b + 1] - cu_q[b]
+        if not 0 <= n <= min(n_kv, MAX_TREE_NODES):
+            raise ValueError(f"{what}: sequence {b} has {n} nodes and {n_kv} cache positions; trees have up to {MAX_TREE_NODES} nodes")
+
+
+def tree_mask(parents, cu_q, kv_lens, meta=None):
+    """What the nodes of trees see of each other, and where they stand: (mask int64 [T, words], bit j of word j // 64 for every node j on the
+    way from a node to its root, itself included; positions int32 [T], context + distance from the root).  `parents` [T]: index of a node's
+    parent in its own tree, before the node; below zero: a root.  A GPU reports a parent that comes later in the status word and takes the
+    node as a root."""
+    if parents.dim() != 1 or parents.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"tree_mask: parents are int32 or int64 [T], not {tuple(parents.shape)} in {parents.dtype}")
+    _check_trees("tree_mask", parents.numel(), cu_q, kv_lens, meta, parents.device)
+    if _cuda(parents):
+        return _native_tree().tree_mask(parents, cu_q, kv_lens, meta)
+    return R.tree_mask(parents, cu_q, kv_lens)
+
+
+def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, vs=None, group=None, q_off=0, meta=None, softcap=0.0,
+                   window=0, keep_first=0, sinks=None, positions=None):
+    """Attention of trees' nodes q [T, Hq, D] over the paged cache: a node sees the context before the tree and the nodes that its `mask`
+    (int64 [T, words], see tree_mask; any other choice of nodes will do) has; one that sees nothing gives zeros.  Other arguments as in
+    paged_attention; `window` counts in `positions` (int32 [T], needed with it).  A GPU takes bf16 queries over bf16 or int8 caches, D
+    64, 128 or 256.  Of keys that some node sees, the values are finite.  Rows behind the last sequence hold nothing of use."""
+    if q.dim() != 3 or kc.dim() != 4 or vc.shape != kc.shape or q.shape[2] != kc.shape[3]:
+        raise ValueError(f"tree_attention: queries {tuple(q.shape)} over keys {tuple(kc.shape)} and values {tuple(vc.shape)}")
+    T, hq, D = q.shape
+    nb, hkv, bs, _ = kc.shape
+    group = group or max(hq // hkv, 1)
+    if group < 1 or q_off < 0 or (hq and (hq - 1 + q_off) // group >= hkv):
+        raise ValueError(f"tree_attention: {hq} query heads from {q_off} on in groups of {group} over {hkv} heads of keys")
+    if not kc.is_contiguous() or not vc.is_contiguous() or kc.dtype != vc.dtype:
+        raise ValueError("tree_attention: caches are contiguous and of one type")
+    if (ks is None) != (vs is None) or (ks is None) != (kc.dtype is not torch.int8):
+        raise ValueError("tree_attention: an int8 cache comes with ks and vs, another without")
+    for s in (ks, vs):
+        if s is not None and (s.shape != kc.shape[:3] or s.dtype is not torch.float32 or not s.is_contiguous()):
+            raise ValueError(f"tree_attention: scales are fp32 {tuple(kc.shape[:3])}, contiguous")
+    _check_trees("tree_attention", T, cu_q, kv_lens, meta, q.device)
+    if mask.dim() != 2 or mask.shape[0] != T or mask.dtype is not torch.int64 or not 1 <= mask.shape[1] <= MAX_TREE_NODES // 64:
+        raise ValueError(f"tree_attention: the mask is int64 [{T}, words], up to {MAX_TREE_NODES // 64} of them, not {tuple(mask.shape)} in {mask.dtype}")
+    most = meta.max_q if meta is not None and getattr(meta, "max_q", 0) else max([b - a for a, b in zip(cu_q, cu_q[1:])], default=0)
+    if most > 64 * mask.shape[1]:
+        raise ValueError(f"tree_attention: a mask of {mask.shape[1]} words for trees of {most} nodes")
+    B = meta.kv_lens_dev.numel() if meta is not None and getattr(meta, "kv_lens_dev", None) is not None else len(kv_lens)
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] < B:
+        raise ValueError(f"tree_attention: the block table is int32 [{B}, blocks], not {tuple(block_table.shape)} in {block_table.dtype}")
+    if window < 0 or keep_first < 0 or softcap < 0:
+        raise ValueError("tree_attention: window, keep_first and softcap are not negative")
+    if window > 0 and (positions is None or positions.shape != (T,) or positions.dtype is not torch.int32 or not positions.is_contiguous()):
+        raise ValueError(f"tree_attention: a window needs the positions, int32 [{T}]")
+    if sinks is not None and (sinks.shape != (hq,) or sinks.dtype is not torch.float32 or not sinks.is_contiguous()):
+        raise ValueError(f"tree_attention: sinks are fp32 [{hq}]")
+    _same_device("tree_attention", q, kc, vc, block_table, mask, ks, vs, sinks, positions if window > 0 else None)
+    if _cuda(q):
+        return _native_tree().tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks, vs, group, q_off, meta, softcap, window,
+                                             keep_first, sinks, positions)
+    return R.tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks, vs, group, q_off, softcap, window, keep_first, sinks,
+                            positions)
+
+
+def cache_pools(k, v=None, ks=None, vs=None):
+    """The pools of all layers as `tree_accept` takes them: lists of keys and values [blocks, heads, block, D] (None or a None entry: a layer
+    without) and of an int8 cache's scales [blocks, heads, block].  Made once; it holds the pools, and belongs to them for as long as they
+    stay where they are (`PagedKVCache.pools` makes one for a cache)."""
+    pools = [p for group in (k, v, ks, vs) for p in (group or []) if p is not None]
+    if not pools:
+        raise ValueError("cache_pools: no pools")
+    for p in pools:
+        if p.dim() not in (3, 4) or not p.is_contiguous():
+            raise ValueError(f"cache_pools: pools are contiguous [blocks, heads, block, D], scales [blocks, heads, block], not {tuple(p.shape)}")
+        if p.shape[0] != pools[0].shape[0] or p.shape[2] != pools[0].shape[2]:
+            raise ValueError("cache_pools: pools of different numbers or sizes of blocks")
+        if p.element_size() * (p.shape[3] if p.dim() == 4 else 1) % 2:
+            raise ValueError(f"cache_pools: rows of an even number of bytes, not {tuple(p.shape)} in {p.dtype}")
+    _same_device("cache_pools", *pools)
+    return _native_tree().CachePools(pools)
+
+
+def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table=None, pools=None, meta=None):
+    """The path through each tree that the tokens `sampled` at its nodes agree with, from node 0 on to the lowest child whose token
+    (`tokens` [T]) is the one sampled at its parent: (emitted int64 [B, most nodes], the sampled tokens of the path, path int32, its nodes,
+    both padded with -1; count int32 [B], how many).  With `pools` (see cache_pools) the accepted nodes' rows move to the positions
+    behind the context, in place; the sequences then hold kv_lens[b] - nodes + count[b] positions, and the last token emitted is in none."""
+    T = tokens.numel()
+    for name, t in (("tokens", tokens), ("parents", parents), ("sampled", sampled)):
+        if t.shape != (T,) or t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"tree_accept: {name} are int32 or int64 [{T}], not {tuple(t.shape)} in {t.dtype}")
+    _check_trees("tree_accept", T, cu_q, kv_lens, meta, tokens.device)
+    if pools is not None:
+        B = meta.kv_lens_dev.numel() if meta is not None and getattr(meta, "kv_lens_dev", None) is not None else len(kv_lens)
+        if block_table is None or block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] < B:
+            raise ValueError(f"tree_accept: moving rows needs the block table, int32 [{B}, blocks]")
+    _same_device("tree_accept", tokens, parents, sampled, block_table, None if pools is None else pools.pools[0])
+    if _cuda(tokens):
+        return _native_tree().tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table, pools, meta)
+    return R.tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table, None if pools is None else pools.pools)
+
+
 def mla_attention(q_nope, q_rope, latent_cache, block_table, cu_q, kv_lens, w_uk, w_uv, scale, absorbed=True,
                   meta=None):
     if _cuda(q_nope):
@@ -744,3 +869,26 @@ def sample_top_k_top_p(logits, top_k, top_p, temperature, uniform):
     if _cuda(logits):
         return _nat().sample_top_k_top_p(logits, top_k, top_p, temperature, uniform)
     return R.sample_top_k_top_p(logits, top_k, top_p, temperature, uniform)
+
+
+MAX_SAMPLE_VOCAB = 1 << 24
+
+
+def sample(logits, temperature, top_k, top_p, min_p, uniform):
+    """A token id (int64) per row of `logits` [.., V], every row with its own parameters (tensors with one number per row, or one number
+    for all, taken as fp32 and int32).  A row is ordered by logit, equal ones by index, and weighed w = exp((x - max) / temperature).  Kept
+    are the first `top_k` (<= 0: all), of these the ones with less than `top_p` of their mass in front of them (>= 1: all), of these the
+    ones with w >= `min_p` (<= 0: all), the first in any case; the token is the first one up to which more than `uniform` (in [0, 1)) of the
+    kept mass lies.  A temperature <= 0 gives the first of the row.  A logit that is NaN counts as -inf; a row without another gives -1."""
+    V = logits.shape[-1] if logits.dim() else 0
+    if not 1 <= V <= MAX_SAMPLE_VOCAB or not logits.is_floating_point():
+        raise ValueError(f"sample: rows of 1 to {MAX_SAMPLE_VOCAB} logits, not {tuple(logits.shape)} in {logits.dtype}")
+    rows = logits.numel() // V
+    for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("uniform", uniform)):
+        if isinstance(v, torch.Tensor) and v.numel() not in (1, rows):
+            raise ValueError(f"sample: {name} of {v.numel()} rows for {rows}")
+    if not isinstance(uniform, torch.Tensor):
+        raise ValueError("sample: `uniform` is a tensor with a number per row")
+    if _cuda(logits):
+        return _native_tree().sample(logits, temperature, top_k, top_p, min_p, uniform)
+    return R.sample(logits, temperature, top_k, top_p, min_p, uniform)

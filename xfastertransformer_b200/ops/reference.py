@@ -549,6 +549,103 @@ def paged_attention(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_t
 
 
 # ----------------------------------------------------------------------------------------
+# Trees of drafted tokens: sequence b owns rows cu_q[b]:cu_q[b+1] (its nodes) and the last positions of its cache
+# ----------------------------------------------------------------------------------------
+def tree_mask(parents: torch.Tensor, cu_q: Sequence[int], kv_lens: Sequence[int]):
+    """(mask int64 [T, words]: bit j of word j // 64 for every node j on the way from a node to its root, itself included;
+    positions int32 [T]: context + distance from the root)."""
+    most = max([b - a for a, b in zip(cu_q, cu_q[1:])] + [1])
+    mask = torch.zeros(parents.numel(), -(-most // 64), dtype=torch.int64)
+    positions = torch.zeros(parents.numel(), dtype=torch.int32)
+    up = parents.tolist()
+    for b, n_kv in enumerate(kv_lens):
+        q0, n = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b])
+        for i in range(n):
+            at, depth = i, -1
+            bits = [0] * mask.shape[1]
+            while at >= 0:
+                bits[at // 64] |= 1 << at % 64
+                depth += 1
+                if up[q0 + at] >= at:
+                    raise ValueError(f"tree_mask: node {at} of sequence {b} comes before its parent {up[q0 + at]}")
+                at = up[q0 + at]
+            mask[q0 + i] = torch.tensor([x - (1 << 64) if x >> 63 else x for x in bits])
+            positions[q0 + i] = int(n_kv) - n + depth
+    return mask.to(parents.device), positions.to(parents.device)
+
+
+def tree_attention(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, cu_q: Sequence[int],
+                   kv_lens: Sequence[int], mask: torch.Tensor, scale: float, ks: Optional[torch.Tensor] = None,
+                   vs: Optional[torch.Tensor] = None, group: int = 1, q_off: int = 0, softcap: float = 0.0, window: int = 0,
+                   keep_first: int = 0, sinks: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                   dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Attention over a paged cache that ends with the nodes of a tree: a node sees the context before them and the nodes
+    that its mask has; arguments as in `paged_attention`.  A node that sees nothing gives zeros.  `dtype`: of the arithmetic."""
+    T, Hq, D = q.shape
+    hmap = (torch.arange(Hq) + q_off) // group
+    out = torch.zeros(T, Hq, vc.shape[3], dtype=dtype, device=q.device)
+    for b in range(len(kv_lens)):
+        q0, q1, n = int(cu_q[b]), int(cu_q[b + 1]), int(kv_lens[b])
+        m, c = q1 - q0, n - (q1 - q0)
+        if m == 0:
+            continue
+        K = _gather_kv(kc, ks, block_table[b], n).to(dtype)[hmap]
+        V = _gather_kv(vc, vs, block_table[b], n).to(dtype)[hmap]
+        s = torch.matmul(q[q0:q1].to(dtype).permute(1, 0, 2), K.transpose(1, 2)) * scale
+        if softcap > 0:
+            s = softcap * torch.tanh(s / softcap)
+        sees = torch.ones(m, n, dtype=torch.bool, device=q.device)
+        bits = (mask[q0:q1, :, None] >> torch.arange(64, device=q.device) & 1).reshape(m, -1)
+        sees[:, c:] = bits[:, :m].bool()
+        if window > 0:
+            at = positions[q0:q1].long()
+            key = torch.cat([torch.arange(c, device=q.device), at])
+            sees &= (at[:, None] - key < window) | (key < keep_first)
+        s = s.masked_fill(~sees, float("-inf"))
+        if sinks is not None:
+            s = torch.cat([s, sinks.to(dtype)[:, None, None].expand(Hq, m, 1)], dim=-1)
+        p = torch.softmax(s, dim=-1)[..., :n].masked_fill(~sees.any(1)[:, None], 0)
+        # a value that a node does not see is no part of its sum, whatever it is
+        o = torch.matmul(p, V.masked_fill(~torch.isfinite(V), 0))
+        odd = (~torch.isfinite(V)).any(0).any(-1).nonzero()[:, 0].tolist()
+        for j in odd:
+            o = o + torch.where(sees[:, j, None] & ~torch.isfinite(V[:, j, None]), p[:, :, j, None] * V[:, j, None], torch.zeros((), dtype=dtype))
+        out[q0:q1] = o.permute(1, 0, 2)
+    return out.to(q.dtype) if dtype is torch.float32 else out
+
+
+def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table=None, pools=None):
+    """(emitted tokens int64, accepted nodes int32 [B, most nodes], padded with -1, and their number int32 [B]): from node 0 on
+    to the lowest child that carries the token sampled at its parent.  The accepted nodes' rows of every pool move up to
+    follow the context."""
+    B = len(kv_lens)
+    most = max([b - a for a, b in zip(cu_q, cu_q[1:])], default=0)
+    emitted = torch.full((B, most), -1, dtype=torch.int64)
+    path = torch.full((B, most), -1, dtype=torch.int32)
+    count = torch.zeros(B, dtype=torch.int32)
+    tok, up, says = tokens.tolist(), parents.tolist(), sampled.tolist()
+    for b in range(B):
+        q0, n = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b])
+        line = [0] if n else []
+        while line:
+            at = line[-1]
+            fits = [i for i in range(at + 1, n) if up[q0 + i] == at and tok[q0 + i] == says[q0 + at]]
+            if not fits:
+                break
+            line.append(fits[0])
+        count[b] = len(line)
+        for j, i in enumerate(line):
+            path[b, j], emitted[b, j] = i, says[q0 + i]
+        c = int(kv_lens[b]) - n
+        for pool in pools or []:
+            bs = pool.shape[2]
+            for j, i in enumerate(line):
+                if i != j:
+                    pool[int(block_table[b, (c + j) // bs]), :, (c + j) % bs] = pool[int(block_table[b, (c + i) // bs]), :, (c + i) % bs]
+    return emitted, path, count
+
+
+# ----------------------------------------------------------------------------------------
 # MLA (DeepSeek) — latent cache [num_blocks, 1, block, kv_lora + rope]
 # ----------------------------------------------------------------------------------------
 def mla_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_cache: torch.Tensor,
@@ -856,6 +953,30 @@ def sample_top_k_top_p(logits: torch.Tensor, top_k: int, top_p: float, temperatu
     u = uniform.to(c.device).float().clamp(0, 1 - 1e-7)[:, None]
     choice = (c <= u).sum(-1).clamp_max(k - 1)
     return idx.gather(1, choice[:, None]).squeeze(1)
+
+
+def sample(logits: torch.Tensor, temperature, top_k, top_p, min_p, uniform) -> torch.Tensor:
+    """See `ops.sample`; everything in 64 bits, parameters as fp32."""
+    V = logits.shape[-1]
+    l2 = logits.reshape(-1, V).float()
+    rows = l2.shape[0]
+    row = lambda v, t: torch.as_tensor(v, dtype=t).reshape(-1, 1).expand(rows, 1)
+    T, p, m, u = (row(v, torch.float32).double() for v in (temperature, top_p, min_p, uniform))
+    k = row(top_k, torch.int64)
+    x, idx = torch.sort(torch.where(l2.isnan(), -torch.inf, l2).double() + 0.0, dim=1, descending=True, stable=True)
+    top = x[:, :1]
+    z = (x - top) / torch.where(T > 0, T, 1.0)
+    w = torch.where(x == top, 1.0, torch.where((x == -torch.inf) | (top == torch.inf), 0.0, torch.exp(z)))
+    j = torch.arange(V)
+    w = torch.where((j < k) | (k <= 0), w, 0.0)
+    before = torch.cumsum(w, 1) - w
+    keep = ~(p < 1) | (before < p.clamp_min(0) * w.sum(1, keepdim=True)) | (j == 0)
+    keep &= ~(m > 0) | (w >= m.clamp_max(1)) | (j == 0)
+    c = torch.cumsum(torch.where(keep, w, 0.0), 1)
+    u = torch.where(u > 0, u, 0.0).clamp_max(1 - 2.0 ** -24)
+    pick = (c <= u * c[:, -1:]).sum(1, keepdim=True).clamp_max(V - 1)
+    tok = idx.gather(1, torch.where(T > 0, pick, 0))
+    return torch.where(top == -torch.inf, -1, tok)[:, 0].view(logits.shape[:-1])
 
 
 def log_softmax(logits: torch.Tensor) -> torch.Tensor:

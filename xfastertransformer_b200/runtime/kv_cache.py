@@ -271,6 +271,11 @@ class PagedKVCache:
                 self.v[l] = None
         self.k, self.v, self.ks, self.vs = nk, nv, nks, nvs
 
+    def pools(self):
+        """Every layer's pools for `ops.tree_accept`; good until `version` changes, which happens when the pools are replaced."""
+        from .. import ops
+        return ops.cache_pools(self.k, self.v, self.ks, self.vs)
+
     def blocks_for(self, n_tokens: int) -> int:
         return (n_tokens + self.block - 1) // self.block
 
