@@ -308,8 +308,9 @@ extern "C" int xft_tree_attention(const char* packed, cudaStream_t st) {
     return -1;
   int rc = -1;
   const bool i8 = a.ks != nullptr;
-  if (a.D == 64) rc = i8 ? launch<64, true>(a, st) : launch<64, false>(a, st);
-  if (a.D == 128) rc = i8 ? launch<128, true>(a, st) : launch<128, false>(a, st);
-  if (a.D == 256) rc = i8 ? launch<256, true>(a, st) : launch<256, false>(a, st);
+  if (a.form) rc = launch_tree_attention_tc(a, st);
+  else if (a.D == 64) rc = i8 ? launch<64, true>(a, st) : launch<64, false>(a, st);
+  else if (a.D == 128) rc = i8 ? launch<128, true>(a, st) : launch<128, false>(a, st);
+  else if (a.D == 256) rc = i8 ? launch<256, true>(a, st) : launch<256, false>(a, st);
   return rc || a.nsplit == 1 ? rc : launch_tree_join(a, st);
 }

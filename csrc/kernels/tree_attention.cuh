@@ -23,6 +23,7 @@ struct TreeAttnArgs {
   long long table_ld;
   int B, T, max_q, hq, hkv, group, q_off, D, bs, num_blocks, table_w, words, nsplit, window, keep;
   float scale, softcap;
+  int form;                                  // row tiles of a CTA in tree_attention_sm100.cu, 0: tree_attention.cu
 };
 
 // One sequence's rows and keys, cut to what the arrays hold; n = 0 where the lengths cannot be right
@@ -58,6 +59,7 @@ __device__ __forceinline__ int tree_block(const TreeAttnArgs& p, int b, int i) {
 
 constexpr float kTreeLog2e = 1.4426950408889634f;
 
-int launch_tree_join(const TreeAttnArgs& a, cudaStream_t st);       // tree_attention.cu
+int launch_tree_join(const TreeAttnArgs& a, cudaStream_t st);                 // tree_attention.cu
+int launch_tree_attention_tc(const TreeAttnArgs& a, cudaStream_t st);         // tree_attention_sm100.cu
 
 }  // namespace xft

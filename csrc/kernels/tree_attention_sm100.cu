@@ -1,0 +1,419 @@
+// Attention of the nodes of trees of drafted tokens on the 5th-generation tensor cores: bf16 cache in blocks of a multiple of 64, heads of
+// 64 or 128, no window and no cap (those: tree_attention.cu, where the formula is).
+//
+// The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile (two CTAs per
+// SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of 128 keys
+//
+//   S = Q K^T   tcgen05.mma, both operands from shared memory; the keys come by TMA, two blocks of 64 by the block table
+//   P = exp2(S - m) as bf16 over S, whole rows in registers; the sum of a row beside it
+//   O += P V    tcgen05.mma, P from TMEM, V as it lies in the cache (MN-major)
+//
+// O stays in TMEM.  m is the largest score only up to a factor of 2^8: O is multiplied again when a row's maximum has grown by more than
+// that, in the time between S and P when no product with V is under way, which after the first tiles hardly ever happens; P and its sum
+// stay below 2^8 per key, and their quotient does not depend on m.
+//
+// The masks matter only in the last tiles, where the nodes' keys are: 128 bits of a row, shifted to the tile's place.  There two more
+// warps clear the values of keys that no node sees and of slots behind the last key, since 0 x NaN is NaN.
+//
+// Every wait is bounded and reports through the status word.
+#include "tree_attention.cuh"
+
+namespace xft {
+
+int make_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t esize);
+
+namespace {
+
+constexpr int kTgKeys = 128, kTgRows = 128;
+
+// R row tiles of heads of 64 * H
+template <int H, int R>
+struct TgShape {
+  static constexpr int kHalf = kTgKeys * 128;            // 64 features of a tile's 128 rows
+  static constexpr int kTile = H * kHalf;
+  static constexpr int kStages = R == 1 ? 4 / H : 10 / H;            // 64 KB (two CTAs an SM), 160 KB
+  static constexpr int kSmem = (R + kStages) * kTile + 1024;
+  static constexpr int kThreads = 128 + 128 * R;
+};
+
+__device__ __forceinline__ float tg_max3(float a, float b, float c) {
+  float d;
+  asm("max.ftz.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 tg_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 tg_add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ uint32_t tg_pack(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ void tg_ld_wait32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+
+// Bits of 32 keys from key `first` on that a node with mask `m` (32-bit words) sees: the context's all, then the nodes'
+__device__ __forceinline__ uint32_t tg_sees(const uint32_t* m, int first, int ctx, int n) {
+  const int o = first - ctx;
+  if (o <= -32) return 0xffffffffu;
+  auto word = [&](int i) -> uint32_t {
+    const int left = n - 32 * i;
+    if (left <= 0) return 0;
+    return left >= 32 ? m[i] : m[i] & ((1u << left) - 1);
+  };
+  if (o < 0) return (word(0) << -o) | ((1u << -o) - 1);
+  return __funnelshift_r(word(o >> 5), word((o >> 5) + 1), o & 31);
+}
+
+template <int H, int R>
+__global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs p) {
+  using S = TgShape<H, R>;
+  constexpr int D = 64 * H, ST = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                                    // R tiles
+  uint8_t* sT = smem + R * S::kTile;                     // ring: keys and values of the tiles in turn
+  __shared__ uint64_t q_full, full[ST], empty[ST], v_here, v_clean, s_full[R], p_half[R], p_full[R], o_full[R];
+  __shared__ uint32_t tmem_base_s, s_union[kTreeWords * 2];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 4 * R);
+    for (int s = 0; s < ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(&v_here, 1);
+    mbar_init(&v_clean, 2);
+    for (int g = 0; g < R; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_half[g], 4); mbar_init(&p_full[g], 4); mbar_init(&o_full[g], 1); }
+    fence_barrier_init();
+    fence_proxy_async();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base_s, 256 * R);                   // of a row tile: S, whose first half becomes P, and O
+    tmem_relinquish();
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  const TreeSeq s(p, b);
+  int h0;
+  const int heads = tree_heads(p, kvh, h0), rows = s.n * heads;
+  const int n_rt = (p.max_q * p.group + R * kTgRows - 1) / (R * kTgRows);
+  const int row0 = (blockIdx.x % n_rt) * (R * kTgRows), slice = blockIdx.x / n_rt;
+  const int all = (s.kv + kTgKeys - 1) / kTgKeys, per = (all + p.nsplit - 1) / p.nsplit;
+  const int t0 = min(all, slice * per), nt = row0 < rows ? min(all, t0 + per) - t0 : 0;
+  const int tail = s.ctx / kTgKeys;                      // from this tile on there are keys that are not the context's
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+
+  // registers at launch: R = 1 256 x 128, R = 2 384 x 168; from here on 128 x 40 + 128 x 216, 128 x 72 + 256 x 216
+  if (warp < 4) {
+    if (R == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------------------ TMA producer
+      if (elect_one()) {
+        const int n_pieces = (s.kv + 63) / 64;
+        Ring ring{0, 1};
+        bool ok = true;
+        for (int j = 0; j < nt && ok; ++j) {
+          int at[2];
+          for (int i = 0; i < 2; ++i) {                  // past the last keys they are read again
+            const int piece = min(2 * (t0 + j) + i, n_pieces - 1), first = piece * 64;
+            at[i] = (tree_block(p, b, first / p.bs) * p.hkv + kvh) * p.bs + first % p.bs;
+          }
+          for (int v = 0; v < 2; ++v) {
+            ok = mbar_wait(&empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY);
+            if (!ok) break;
+            uint8_t* to = sT + ring.s * S::kTile;
+            mbar_expect_tx(&full[ring.s], S::kTile);
+            for (int i = 0; i < 2; ++i)
+              for (int h = 0; h < H; ++h)
+                tma_load_2d(to + h * S::kHalf + i * 8192, v ? &tmV : &tmK, &full[ring.s], h * 64, at[i], kEvictNormal);
+            ring.next(ST);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (nt > 0 && elect_one()) {
+        constexpr uint32_t IDESC_S = umma_idesc(128, kTgKeys, 1, 1, 1);
+        constexpr uint32_t IDESC_O = umma_idesc(128, D, 1, 1, 1) | (1u << 16);       // B = V, MN-major
+        Ring ring{0, 0};
+        bool ok = mbar_wait(&q_full, 0, p.status, XFT_ERR_WAIT_FULL) && mbar_wait(&full[0], 0, p.status, XFT_ERR_WAIT_FULL);
+        auto scores = [&](int g, int st) {
+          const uint64_t qd = umma_desc_k128(smem_u32(sQ + g * S::kTile)), kd = umma_desc_k128(smem_u32(sT + st * S::kTile));
+          tcgen05_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4 * H; ++k) {
+            const uint32_t off = ((k >> 2) * S::kHalf + (k & 3) * 32) / 16;
+            umma_bf16(tmem_base + g * 256, qd + off, kd + off, IDESC_S, k > 0);
+          }
+          tcgen05_commit(&s_full[g]);
+        };
+        if (ok) {
+          for (int g = 0; g < R; ++g) scores(g, 0);
+          tcgen05_commit(&empty[0]);
+          ring.next(ST);
+        }
+        int cleaned = 0;
+        for (int j = 0; j < nt && ok; ++j) {
+          const Ring vr = ring;
+          ring.next(ST);
+          const Ring kr = ring;
+          ok = mbar_wait(&full[vr.s], vr.ph, p.status, XFT_ERR_WAIT_FULL);
+          if (ok && t0 + j >= tail) {
+            mbar_arrive(&v_here);
+            ok = mbar_wait(&v_clean, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL);
+          }
+          if (!ok) break;
+          const uint64_t vd = umma_desc_mn128(smem_u32(sT + vr.s * S::kTile), S::kHalf);
+          for (int g = 0; g < R && ok; ++g) {
+            const uint32_t pa = tmem_base + g * 256, oa = pa + 128;
+            ok = mbar_wait(&p_half[g], j & 1, p.status, XFT_ERR_WAIT_TMEM);
+            if (!ok) break;
+            tcgen05_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, j > 0 || k > 0);
+            ok = mbar_wait(&p_full[g], j & 1, p.status, XFT_ERR_WAIT_TMEM);
+            if (!ok) break;
+            tcgen05_fence_after();
+#pragma unroll
+            for (int k = 4; k < 8; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, 1);
+            if (g == R - 1) tcgen05_commit(&empty[vr.s]);
+            if (j + 1 < nt) {                            // the next S goes over P, behind the product that reads P
+              if (g == 0) ok = mbar_wait(&full[kr.s], kr.ph, p.status, XFT_ERR_WAIT_FULL);
+              if (!ok) break;
+              scores(g, kr.s);
+              if (g == R - 1) tcgen05_commit(&empty[kr.s]);
+            } else {
+              tcgen05_commit(&o_full[g]);
+            }
+          }
+          ring.next(ST);
+        }
+      }
+    } else {
+      // ------------------------------------------------------------------ values that no node sees
+      if (t0 + nt > tail && nt > 0) {
+        uint32_t seen[kTreeWords * 2] = {};
+        const uint32_t* m = reinterpret_cast<const uint32_t*>(p.mask + (long long)s.q0 * p.words);
+        for (int i = lane; i < s.n; i += 32)
+#pragma unroll
+          for (int w = 0; w < kTreeWords * 2; ++w)
+            if (w < 2 * p.words) seen[w] |= m[(long long)i * p.words * 2 + w];
+#pragma unroll
+        for (int w = 0; w < kTreeWords * 2; ++w) {
+          const uint32_t x = __reduce_or_sync(0xffffffffu, seen[w]);
+          if (lane == 0 && warp == 2) s_union[w] = x;
+        }
+      }
+      named_bar_sync(1, 64);
+      Ring ring{0, 0};
+      for (int j = 0, cleaned = 0; j < nt; ++j) {
+        ring.next(ST);
+        const int st = ring.s;
+        const uint32_t ph = ring.ph;
+        ring.next(ST);
+        if (t0 + j < tail) continue;
+        // (these warps do not hold the ring back, so they ask the issuer which round it is in)
+        if (!mbar_wait(&v_here, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL)) break;
+        const int key = (warp - 2) * 64 + lane * 2;      // two keys a lane
+        const int k0 = (t0 + j) * kTgKeys;
+        const uint32_t sees = tg_sees(s_union, k0 + (key & ~31), s.ctx, s.n) >> (key & 31);
+        if (!mbar_wait(&full[st], ph, p.status, XFT_ERR_WAIT_FULL)) break;
+        uint8_t* v = sT + st * S::kTile;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (!(sees >> e & 1))
+#pragma unroll
+            for (int c = 0; c < 8 * H; ++c)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * S::kHalf + (key + e) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax: one row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int g = (warp - 4) >> 2, qd = warp & 3;
+    const int r = qd * 32 + lane, row = row0 + g * kTgRows + r;
+    const bool mine = row < rows, busy = row0 + g * kTgRows + qd * 32 < rows;          // the row, some row of the warp
+    const int node = mine ? row / heads : 0, h = h0 + (mine ? row - node * heads : 0);
+    const long long at = (long long)(s.q0 + node) * p.hq + h;
+    if (nt > 0) {
+      // this row of queries in the order that the product reads: 16-byte pieces exchanged with the row's low bits
+      uint8_t* to = sQ + g * S::kTile + r * 128;
+      uint4 v[8];
+#pragma unroll
+      for (int half = 0; half < H; ++half) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = mine ? *reinterpret_cast<const uint4*>(p.q + at * D + half * 64 + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(to + half * S::kHalf + ((c ^ (r & 7)) << 4)) = v[c];
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    }
+    const uint32_t sa = tmem_base + g * 256 + (uint32_t(qd * 32) << 16), oa = sa + 128;
+    const float scale = p.scale * kTreeLog2e;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      if (!mbar_wait(&s_full[g], j & 1, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
+      tcgen05_fence_after();
+      if (!busy) {
+        if (lane == 0) { mbar_arrive(&p_half[g]); mbar_arrive(&p_full[g]); }
+        continue;
+      }
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(sa + 32 * c, x[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tg_ld_wait32(x[c]);
+      if (t0 + j >= tail) {
+        const uint32_t* bits = reinterpret_cast<const uint32_t*>(p.mask + (long long)(s.q0 + node) * p.words);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t sees = tg_sees(bits, (t0 + j) * kTgKeys + 32 * c, s.ctx, s.n);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(sees >> i & 1)) x[c][i] = 0xff800000u;
+        }
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = tg_max3(top[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+      const float mx = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale);
+      const bool grown = mx > m + 8.f;
+      if (__any_sync(0xffffffffu, grown)) {
+        const float f = grown ? exp2f(m - mx) : 1.f;     // 0 where nothing has been seen yet
+        if (grown) m = mx;
+        l *= f;
+        if (j > 0) {
+          uint32_t y[32];
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            tmem_ld32(oa + c, y);
+            tg_ld_wait32(y);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tmem_st32(oa + c, y);
+          }
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : -m;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float2 e = tg_fma2(make_float2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), make_float2(scale, scale), make_float2(off, off));
+          e.x = exp2f(e.x);
+          e.y = exp2f(e.y);
+          w[i >> 1] = tg_pack(e.x, e.y);
+          sum[(i >> 1) & 1] = tg_add2(sum[(i >> 1) & 1], e);
+        }
+        tmem_st16(sa + 16 * c, w);
+        if (c == 1) {                                    // the product may begin with the first 64 keys
+          tmem_st_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[g]);
+        }
+      }
+      const float2 t = tg_add2(sum[0], sum[1]);
+      l += t.x + t.y;
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[g]);
+    }
+    if (nt > 0 && ok && busy && mbar_wait(&o_full[g], 0, p.status, XFT_ERR_WAIT_TMEM)) {
+      tcgen05_fence_after();
+      float f = 1.f;
+      if (p.nsplit == 1) {
+        float sum = l;
+        if (p.sinks) {
+          const float sink = p.sinks[h] * kTreeLog2e, mx = fmaxf(m, sink);
+          f = exp2f(m - mx);
+          sum = sum * f + exp2f(sink - mx);
+        }
+        f = l == 0.f ? 0.f : __fdividef(f, sum);         // a row that sees nothing
+      }
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t y[32];
+        tmem_ld32(oa + c, y);
+        tg_ld_wait32(y);
+        if (mine && p.nsplit == 1) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = tg_pack(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
+          st_global_256(p.out + at * D + c, w);
+          st_global_256(p.out + at * D + c + 16, w + 8);
+        } else if (mine) {
+          float* o = p.part_o + (at * p.nsplit + slice) * D + c;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) st_global_256(o + i, y + i);
+        }
+      }
+    }
+    if (mine && p.nsplit > 1) *reinterpret_cast<float2*>(p.part_ml + (at * p.nsplit + slice) * 2) = ok ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem_base, 256 * R);
+  }
+}
+
+template <int H, int R>
+int launch(const TreeAttnArgs& a, cudaStream_t st) {
+  using S = TgShape<H, R>;
+  CUtensorMap tmK, tmV;
+  const uint64_t rows = (uint64_t)a.num_blocks * a.hkv * a.bs;
+  if (make_tensor_map(&tmK, a.kc, rows, a.D, a.D, 64, 2) || make_tensor_map(&tmV, a.vc, rows, a.D, a.D, 64, 2)) return -4;
+  auto k = tree_attention_tc_kernel<H, R>;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return 3000 + (int)cudaGetLastError();
+  const int n_rt = (a.max_q * a.group + R * kTgRows - 1) / (R * kTgRows);
+  const cudaError_t e = launch_pdl(k, dim3(n_rt * a.nsplit, a.hkv, a.B), dim3(S::kThreads), (size_t)S::kSmem, st, tmK, tmV, a);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// 0, -1 where the shape is not one of this kernel's, or an error
+int launch_tree_attention_tc(const TreeAttnArgs& a, cudaStream_t st) {
+  if (a.ks || a.bs % 64 || a.window > 0 || a.softcap > 0.f || !(a.scale > 0.f) || (a.D != 64 && a.D != 128)) return -1;
+  if ((long long)a.num_blocks * a.hkv * a.bs > 0x7fffffffll) return -1;
+  if (a.D == 64) return a.form == 2 ? launch<1, 2>(a, st) : launch<1, 1>(a, st);
+  return a.form == 2 ? launch<2, 2>(a, st) : launch<2, 1>(a, st);
+}
+
+}  // namespace xft

@@ -20,8 +20,8 @@ MASK_ARGS = struct.Struct("@2P2i4Pi4x")
 # table_ld | table_w, n_pools, bs, num_blocks, width
 ACCEPT_ARGS = struct.Struct("@2P2i9Pq5i4x")
 # csrc/kernels/tree_attention.cuh:TreeAttnArgs: q, out, kc, vc, ks, vs, table, cu_q, kv_lens, mask, positions, sinks, part_o, part_ml, status |
-# table_ld | B, T, max_q, hq, hkv, group, q_off, D, bs, num_blocks, table_w, words, nsplit, window, keep | scale, softcap
-ATTN_ARGS = struct.Struct("@15Pq15i2f4x")
+# table_ld | B, T, max_q, hq, hkv, group, q_off, D, bs, num_blocks, table_w, words, nsplit, window, keep | scale, softcap | form
+ATTN_ARGS = struct.Struct("@15Pq15i2fi")
 # csrc/kernels/sample_rows.cu:SampleArgs: x, temperature, top_k, top_p, min_p, uniform, out | ld | rows, V, bf16, k0 | t0, p0, m0
 SAMPLE_ARGS = struct.Struct("@7Pq4i3f4x")
 _P, _I = C.c_void_p, C.c_int
@@ -92,11 +92,21 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
     return mask, positions
 
 
-def _slices(B, hkv, rows, D, max_kv):
-    """Slices that the keys are cut into: enough for two CTAs on each of the 148 SMs, four tiles of keys a slice at least."""
-    ctas = B * hkv * -(-rows // 64)
-    tiles = -(-max_kv // (32 if D == 256 else 64))
-    return max(1, min(296 // max(ctas, 1), tiles // 4, 64))
+def _plan(B, hkv, rows, D, max_kv, tensor):
+    """(form, slices that the keys are cut into): the kernel of csrc/kernels/tree_attention_sm100.cu with one or two tiles of 128 rows per
+    CTA, or (form 0) that of tree_attention.cu."""
+    form = 0 if not tensor else 1 if rows <= 128 else 2
+    keys, tall, slots = ((32 if D == 256 else 64), 64, 296) if not form else (128, 128 * form, 296 // form)
+    ctas = B * hkv * -(-rows // tall)
+    tiles = -(-max_kv // keys)
+    most = max(1, min(tiles // (1 if form else 4), 64))
+    best = None
+    for waves in (1, 2, 3):                               # slices that fill the SMs once, twice, ...; a CTA costs as much as two tiles beside its own
+        n = max(1, min(waves * slots // ctas, most))
+        cost = -(-ctas * n // slots) * (-(-tiles // n) + 2) + (2 if n > 1 else 0)
+        if best is None or cost < best[0]:
+            best = cost, n
+    return form, best[1]
 
 
 def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, vs=None, group=1, q_off=0, meta=None, softcap=0.0, window=0,
@@ -120,13 +130,14 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     if not (T and B and most):
         return out
     ws = N.Workspace.get(dev)
-    n = _slices(B, hkv, most * group, D, longest)
+    form, n = _plan(B, hkv, most * group, D, longest,
+                    ks is None and D <= 128 and bs % 64 == 0 and window == 0 and softcap == 0 and scale > 0 and nb * hkv * bs < 2 ** 31)
     part = torch.empty(T * hq * n * (D + 2), dtype=torch.float32, device=dev) if n > 1 else None
     po = _ptr(part)
     a = ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), _ptr(ks), _ptr(vs), block_table.data_ptr(), cu.data_ptr(),
                        kv.data_ptr(), mask.data_ptr(), _ptr(positions), _ptr(sinks), po, po + T * hq * n * D * 4, ws.status.data_ptr(),
                        block_table.stride(0), B, T, most, hq, hkv, group, q_off, D, bs, nb, block_table.shape[1], mask.shape[1], n, window,
-                       keep_first, scale, softcap)
+                       keep_first, scale, softcap, form)
     rc = _lib().xft_tree_attention(a, _stream())
     if rc:
         N._check(rc, "tree_attention")
