@@ -246,35 +246,72 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
   }
 }
 
-// Joins the slices: one warp per row
+// Joins the slices: a warp per row, a slice's weight per lane and 4 columns of four slices at a time
+template <int D>
 __global__ void __launch_bounds__(128) tree_join_kernel(const TreeAttnArgs p) {
   grid_dep_launch();
   grid_dep_wait();
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= (long long)min(p.T, p.cu_q[p.B]) * p.hq) return;
-  const float* ml = p.part_ml + row * p.nsplit * 2;
+  float2 ml[2];                                          // slices lane and lane + 32
   float mx = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) mx = fmaxf(mx, ml[2 * s]);
-  const float seen = mx;
-  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int s = lane + 32 * e;
+    ml[e] = s < p.nsplit ? *reinterpret_cast<const float2*>(p.part_ml + (row * p.nsplit + s) * 2) : make_float2(-INFINITY, 0.f);
+    mx = fmaxf(mx, ml[e].x);
+  }
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const bool any = mx != -INFINITY;
+  float extra = 0.f;
   if (p.sinks) {
     const float sink = p.sinks[row % p.hq] * kTreeLog2e;
     mx = fmaxf(mx, sink);
-    sum = exp2f(sink - mx);
+    extra = exp2f(sink - mx);
   }
-  for (int s = 0; s < p.nsplit; ++s) sum += ml[2 * s + 1] == 0.f ? 0.f : ml[2 * s + 1] * exp2f(ml[2 * s] - mx);
-  const float inv = seen == -INFINITY ? 0.f : 1.f / sum;
-  for (int d = lane * 2; d < p.D; d += 64) {
-    float2 o = make_float2(0.f, 0.f);
-    for (int s = 0; s < p.nsplit; ++s) {
-      if (ml[2 * s + 1] == 0.f) continue;
-      const float f = exp2f(ml[2 * s] - mx);
-      const float2 v = *reinterpret_cast<const float2*>(p.part_o + (row * p.nsplit + s) * p.D + d);
-      o.x += f * v.x;
-      o.y += f * v.y;
+  float f[2], sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    f[e] = ml[e].y == 0.f ? 0.f : exp2f(ml[e].x - mx);   // (a slice without keys for this row has written no sums)
+    sum += ml[e].y == 0.f ? 0.f : ml[e].y * f[e];
+  }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = any || sum != 0.f ? 1.f / (sum + extra) : 0.f;       // (a sum that is NaN: any is false where every score was)
+  const float* part = p.part_o + row * p.nsplit * D;
+  constexpr int C = D < 128 ? 2 : D / 32;                // columns of a lane
+  float o[C] = {};
+  for (int s0 = 0; s0 < p.nsplit; s0 += 4) {
+    float v[4][C], w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int s = s0 + e;
+      w[e] = __shfl_sync(0xffffffffu, s < 32 ? f[0] : f[1], s & 31);
+      const float y = __shfl_sync(0xffffffffu, s < 32 ? ml[0].y : ml[1].y, s & 31);
+      if (s >= p.nsplit || y == 0.f) {
+        w[e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[e][c] = 0.f;
+      } else if constexpr (C == 2) {
+        *reinterpret_cast<float2*>(v[e]) = *reinterpret_cast<const float2*>(part + (long long)s * D + 2 * lane);
+      } else {
+#pragma unroll
+        for (int c = 0; c < C; c += 4)
+          *reinterpret_cast<float4*>(v[e] + c) = *reinterpret_cast<const float4*>(part + (long long)s * D + c * 32 + 4 * lane);
+      }
     }
-    *reinterpret_cast<uint32_t*>(p.out + row * p.D + d) = gl_pack(o.x * inv, o.y * inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] += w[e] * v[e][c];
+  }
+  __nv_bfloat16* out = p.out + row * D;
+  if constexpr (C == 2) {
+    *reinterpret_cast<uint32_t*>(out + 2 * lane) = gl_pack(o[0] * inv, o[1] * inv);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; c += 4)
+      *reinterpret_cast<uint2*>(out + c * 32 + 4 * lane) = make_uint2(gl_pack(o[c] * inv, o[c + 1] * inv), gl_pack(o[c + 2] * inv, o[c + 3] * inv));
   }
 }
 
@@ -290,7 +327,8 @@ int launch(const TreeAttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int launch_tree_join(const TreeAttnArgs& a, cudaStream_t st) {
-  const cudaError_t e = launch_pdl(tree_join_kernel, dim3((unsigned)(((long long)a.T * a.hq + 3) / 4)), dim3(128), 0, st, a);
+  auto k = a.D == 64 ? tree_join_kernel<64> : a.D == 128 ? tree_join_kernel<128> : tree_join_kernel<256>;
+  const cudaError_t e = launch_pdl(k, dim3((unsigned)(((long long)a.T * a.hq + 3) / 4)), dim3(128), 0, st, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
@@ -303,7 +341,7 @@ extern "C" int xft_tree_attention(const char* packed, cudaStream_t st) {
   TreeAttnArgs a;
   memcpy(&a, packed, sizeof(a));
   if (a.B <= 0 || a.T <= 0 || a.max_q <= 0) return 0;
-  if (a.max_q > 64 * a.words || a.words > kTreeWords || a.group < 1 || a.nsplit < 1 || (a.nsplit > 1 && (!a.part_o || !a.part_ml)) ||
+  if (a.max_q > 64 * a.words || a.words > kTreeWords || a.group < 1 || a.nsplit < 1 || a.nsplit > 64 || (a.nsplit > 1 && (!a.part_o || !a.part_ml)) ||
       (a.window > 0 && !a.positions) || a.bs < 1)
     return -1;
   int rc = -1;

@@ -20,7 +20,7 @@
 
 namespace xft {
 
-int make_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t esize);
+int encode_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t esize);
 
 namespace {
 
@@ -58,6 +58,11 @@ __device__ __forceinline__ float2 tg_add2(float2 a, float2 b) {
 __device__ __forceinline__ uint32_t tg_pack(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
+}
+// Two weights (not negative) in bf16, rounded to the nearest, halves up.  Whole-number instructions: a conversion takes the unit of the
+// exponentials, which bounds the softmax, as long as one of those.  (A NaN may come out as a number: the row's sum has it.)
+__device__ __forceinline__ uint32_t tg_round(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
 }
 __device__ __forceinline__ void tg_ld_wait32(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
           float2 e = tg_fma2(make_float2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), make_float2(scale, scale), make_float2(off, off));
           e.x = exp2f(e.x);
           e.y = exp2f(e.y);
-          w[i >> 1] = tg_pack(e.x, e.y);
+          w[i >> 1] = tg_round(e.x, e.y);
           sum[(i >> 1) & 1] = tg_add2(sum[(i >> 1) & 1], e);
         }
         tmem_st16(sa + 16 * c, w);
@@ -398,7 +403,7 @@ int launch(const TreeAttnArgs& a, cudaStream_t st) {
   using S = TgShape<H, R>;
   CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)a.num_blocks * a.hkv * a.bs;
-  if (make_tensor_map(&tmK, a.kc, rows, a.D, a.D, 64, 2) || make_tensor_map(&tmV, a.vc, rows, a.D, a.D, 64, 2)) return -4;
+  if (encode_tensor_map(&tmK, a.kc, rows, a.D, a.D, 64, 2) || encode_tensor_map(&tmV, a.vc, rows, a.D, a.D, 64, 2)) return -4;
   auto k = tree_attention_tc_kernel<H, R>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return 3000 + (int)cudaGetLastError();
   const int n_rt = (a.max_q * a.group + R * kTgRows - 1) / (R * kTgRows);
