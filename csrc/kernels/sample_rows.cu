@@ -10,18 +10,19 @@
 // order.  They have to be exact to far below an element's share, or another token comes out than exact arithmetic's: tokens are equal
 // but for a probability of about 2^-35 per kept element.
 //
-// A row's read is all the traffic, so it is read once, by a cluster whose CTAs hold a slice each in shared memory:
-//   1. the largest logit, over the cluster;
-//   2. a histogram of 1024 bins whose edges are even in the logit, 32 a factor of two in w (counts alone, 32 per logit, where k is small
-//      enough for the next step to take all of the first k): a bin's mass is its middle's weight times the sum of 2^-e, e the distance
-//      from the middle, by a polynomial, from a distance that is rounded to 2^-30 and not to a logit's 2^-20 (two numbers in 32 bits
-//      carry it); the sums are two 32-bit atomics (one of 64 bits is a loop: 20 times slower);
-//   3. the bins' sums, exchanged over the cluster; every CTA finds the bins where the limits and the token can lie;
-//   4. those bins' elements, or all up to there if that is what at most 2048 are, go to the first CTA, which sorts them, weighs them in 64
-//      bits and finds the place; one more such round for each limit whose elements are too many.
-// What that does not settle (a bin of more than 2048 elements, as with equal logits, a limit among weights below 2^-32, a
-// largest logit above 1e38) the first
-// CTA settles alone, digit by digit of the 64-bit number (image of the logit, ~index), whose unsigned order is the row's.
+// A row is read once from memory, by a cluster of up to 8 CTAs with a slice each, which few rows' CTAs hold in shared memory and many rows'
+// read again from L2 for the few elements of step 3:
+//   1. a histogram of each slice, 1024 bins down from about the slice's largest logit on a grid that is the same for the whole row, 16 bins
+//      a factor of two in w (counts alone, 16 bins per logit, where k is small enough for step 3 to take all of the first k): a bin's mass is
+//      its middle's weight times the sum of 2^e, e the distance from the middle in octaves, by a polynomial, from a distance that is
+//      good to 2^-30 (two numbers in 32 bits carry it); the sums are two 32-bit atomics (one of 64 bits in shared memory is a loop: 20
+//      times slower).  What weighs less than 2^-48 of the largest is left out;
+//   2. the bins' sums, exchanged over the cluster; every CTA finds the bins where the limits and the token can lie;
+//   3. those bins' elements, or all up to there if that is what at most 2048 are, go to the first CTA, which sorts them, weighs them in 64
+//      bits and finds the place; one more such round for each limit whose elements are too many.  The others leave before the last.
+// What that does not settle (a bin of more than 2048 elements, as with equal logits, a limit among weights that are left out, logits of
+// which a bin is less than 32 bits resolve) the first CTA settles alone, digit by digit of the 64-bit number (image of the logit, ~index),
+// whose unsigned order is the row's.
 #include "ptx.cuh"
 
 namespace xft {
@@ -45,7 +46,8 @@ typedef unsigned long long u64;
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 1024, kSampleList = 2048;
 constexpr float kSampleEdge = kSampleBins - 1.5f;        // from here on: the elements outside the bins
-constexpr int kSampleUnit = 28;                          // a weight's factor in its bin has so many bits behind the point
+constexpr int kSamplePer = 16;                           // bins an octave, or a logit
+constexpr int kSampleUnit = 27;                          // a weight's factor in its bin has so many bits behind the point
 
 // Unsigned order of the images is the order of the floats; NaN counts as -inf, -0 as 0
 __device__ __forceinline__ float logit(float x) { return x == x ? x + 0.f : -INFINITY; }
@@ -58,9 +60,9 @@ __device__ __forceinline__ u64 element(float x, unsigned i) { return (u64)image(
 
 struct SampleRow {
   const void* x;
-  int V, bf16, shift;
+  int V, bf16;
   float top;
-  double inv_t;
+  double inv_t, unit;                                    // mass of the weight 1
   __device__ float at(int i) const {
     return logit(bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i]) : static_cast<const float*>(x)[i]);
   }
@@ -70,7 +72,7 @@ struct SampleRow {
     if (v == -INFINITY || top == INFINITY) return 0.0;
     return exp((static_cast<double>(v) - static_cast<double>(top)) * inv_t);
   }
-  __device__ u64 mass(double w) const { return static_cast<u64>(__double2ll_rn(ldexp(w, shift))); }
+  __device__ u64 mass(double w) const { return __double2ull_rn(w * unit); }
 };
 
 struct SampleLimits { int k; float p, least, u; };
@@ -83,10 +85,12 @@ struct SampleShared {
   };
   u64 mass[kSampleBins];                                 // of the whole row
   unsigned cnt[kSampleBins];
-  u64 warps[kSampleWarps], found[4];
-  float top[16];                                         // of each CTA
-  unsigned first[16];
-  u64 over[16];
+  u64 warps[kSampleWarps], found[4], kept;
+  unsigned warp_counts[kSampleWarps];
+  float top[8], ref[8];                                  // of each CTA: its slice's largest logit, and where its bins begin
+  u64 first[8];
+  double root[kSamplePer];                               // 2^(-i / 16)
+  int above;
   unsigned n_list, at;
   int what, from, to;                                    // the next round: see Round
   u64 base;
@@ -115,10 +119,32 @@ __device__ void scan(u64 v, u64* warps, u64& before, u64& total) {
   __syncthreads();
 }
 
+// The same of a count and a mass
+__device__ void scan2(unsigned c, u64 m, SampleShared& sh, unsigned& before_c, u64& before_m, u64& total_m) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  unsigned sc = c;
+  u64 sm = m;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned tc = __shfl_up_sync(0xffffffffu, sc, o);
+    const u64 tm = __shfl_up_sync(0xffffffffu, sm, o);
+    if (lane >= o) { sc += tc; sm += tm; }
+  }
+  if (lane == 31) { sh.warps[w] = sm; sh.warp_counts[w] = sc; }
+  __syncthreads();
+  before_c = sc - c; before_m = sm - m; total_m = 0;
+#pragma unroll
+  for (int i = 0; i < kSampleWarps; ++i) {
+    if (i < w) { before_c += sh.warp_counts[i]; before_m += sh.warps[i]; }
+    total_m += sh.warps[i];
+  }
+  __syncthreads();
+}
+
 // -- alone --------------------------------------------------------------------------------------------------------------------------
 // The place where the running count reaches `want` (by_mass false) or the running mass exceeds it; returns the mass up to and with the
 // element there and its index.  `want` lies within the row's count or mass.
-__device__ void place(const SampleRow& r, SampleShared& sh, bool by_mass, u64 want, u64& upto, unsigned& index) {
+__device__ __noinline__ void place(const SampleRow& r, SampleShared& sh, bool by_mass, u64 want, u64& upto, unsigned& index) {
   const int tid = threadIdx.x;
   u64 prefix = 0, done_m = 0, done_c = 0;
   for (int bits = 0; bits < 64;) {
@@ -164,7 +190,7 @@ __device__ __forceinline__ u64 exceed(float u, u64 mass) {
   return min((u64)(fmin(u > 0.f ? (double)u : 0.0, 1.0 - 0x1p-24) * (double)mass), mass - 1);
 }
 
-__device__ unsigned alone(const SampleRow& r, SampleShared& sh, const SampleLimits& lim) {
+__device__ __noinline__ unsigned alone(const SampleRow& r, SampleShared& sh, const SampleLimits& lim) {
   u64 all = 0, over = 0, before;
   for (int i = threadIdx.x; i < r.V; i += kSampleThreads) {
     const double w = r.weight(r.at(i));
@@ -189,13 +215,28 @@ __device__ unsigned alone(const SampleRow& r, SampleShared& sh, const SampleLimi
 }
 
 // -- the elements of a round --------------------------------------------------------------------------------------------------------
+// One bitonic step between neighbours of a warp's 64 elements, 32 apart in the two registers
+__device__ __forceinline__ void sort_pair(u64& x, u64& y, bool down) {
+  if ((x < y) == down) { const u64 t = x; x = y; y = t; }
+}
+__device__ __forceinline__ void sort_steps(u64& x0, u64& x1, int i0, int run, int step) {
+  if (step == 32) { sort_pair(x0, x1, (i0 & run) == 0); step = 16; }
+  for (; step > 0; step >>= 1) {
+    const u64 y0 = __shfl_xor_sync(0xffffffffu, x0, step), y1 = __shfl_xor_sync(0xffffffffu, x1, step);
+    const bool low = (i0 & step) == 0;                   // the lower of two keeps the larger where the run goes down
+    x0 = ((x0 > y0) == (low == ((i0 & run) == 0))) ? x0 : y0;
+    x1 = ((x1 > y1) == (low == (((i0 + 32) & run) == 0))) ? x1 : y1;
+  }
+}
+// Largest first; a warp sorts 64 elements in registers, only longer distances go through shared memory
 __device__ void sort_list(u64* list, int n) {
   int size = 64;
   while (size < n) size <<= 1;
   for (int i = n + threadIdx.x; i < size; i += kSampleThreads) list[i] = 0;
   __syncthreads();
-  for (int run = 2; run <= size; run <<= 1)
-    for (int step = run >> 1; step > 0; step >>= 1) {
+  const int lane = threadIdx.x & 31;
+  for (int run = 64; run <= size; run <<= 1) {
+    for (int step = run >> 1; step >= 64; step >>= 1) {
       for (int i = threadIdx.x; i < size / 2; i += kSampleThreads) {
         const int a = 2 * step * (i / step) + i % step, b = a + step;
         const u64 x = list[a], y = list[b];
@@ -203,50 +244,107 @@ __device__ void sort_list(u64* list, int n) {
       }
       __syncthreads();
     }
+    for (int i = (threadIdx.x >> 5) * 64 + lane; i < size; i += 2 * kSampleThreads) {
+      u64 x0 = list[i], x1 = list[i + 32];
+      if (run == 64)
+        for (int r = 2; r < 64; r <<= 1) sort_steps(x0, x1, i, r, r >> 1);
+      sort_steps(x0, x1, i, run, 32);
+      list[i] = x0;
+      list[i + 32] = x1;
+    }
+    __syncthreads();
+  }
 }
 
-// Where the sorted list's running mass (behind `base`) first reaches `want`, or with `pass` exceeds it: place and mass up to there; the
-// last element if nowhere
+// A list of up to 128, largest first: an element's place is the number of larger ones, counted by four threads
+__device__ void sort_few(u64* list, int n) {
+  const int i = threadIdx.x >> 2, part = threadIdx.x & 3;
+  const u64 x = i < n ? list[i] : 0;
+  int at = 0;
+  for (int j = part; j < n; j += 4) at += list[j] > x;
+  at += __shfl_xor_sync(0xffffffffu, at, 1);
+  at += __shfl_xor_sync(0xffffffffu, at, 2);
+  __syncthreads();
+  if (part == 0 && i < n) list[at] = x;
+  __syncthreads();
+}
+
+// A sorted list's masses: E elements a thread, of one warp (lists of up to 128) or of the CTA.  Elements and masses that are asked for come
+// out the same in every thread.
+template <int E, bool WARP>
 struct ListMasses {
-  u64 m[4], c[4];                                        // of the thread's four elements, and up to and with each
+  u64 m[E], c[E];                                        // of the thread's elements, and up to and with each, behind `base`
+  double w[E];
   int n;
   u64 end;
-  __device__ ListMasses(const SampleRow& r, SampleShared& sh, int n_, u64 base, double* w) : n(n_) {
+  __device__ void sums(SampleShared& sh, u64 v, u64& before, u64& total) const {
+    if (WARP) {
+      u64 s = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xffffffffu, s, o);
+        if ((threadIdx.x & 31) >= o) s += t;
+      }
+      before = s - v;
+      total = __shfl_sync(0xffffffffu, s, 31);
+    } else {
+      scan(v, sh.warps, before, total);
+    }
+  }
+  __device__ ListMasses(const SampleRow& r, SampleShared& sh, int n_, u64 base) : n(n_) {
     u64 sum = 0, before;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = threadIdx.x * 4 + e;
+    for (int e = 0; e < E; ++e) {
+      const int i = threadIdx.x * E + e;
       w[e] = i < n ? r.weight(from_image((uint32_t)(sh.list[i] >> 32))) : 0.0;
       m[e] = i < n ? r.mass(w[e]) : 0;
       sum += m[e];
     }
-    scan(sum, sh.warps, before, end);
+    sums(sh, sum, before, end);
     end += base;
     before += base;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = before += m[e];
+    for (int e = 0; e < E; ++e) c[e] = before += m[e];
   }
-  // (the element, mass up to and with it), the same in every thread
+  __device__ u64 least(SampleShared& sh, float limit) const {            // mass of what weighs so much
+    u64 sum = 0, before, total;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e] >= (double)limit ? m[e] : 0;
+    sums(sh, sum, before, total);
+    return total;
+  }
+  // The first element whose place and running mass pass, and that mass; the last element if none does
   template <class F>
   __device__ void first(SampleShared& sh, F test, int& at, u64& upto) const {
-    if (threadIdx.x == 0) { sh.found[0] = n - 1; sh.found[1] = end; }
-    __syncthreads();
+    int mine = -1;
+    u64 mass = 0;
 #pragma unroll
-    for (int e = 3; e >= 0; --e) {
-      const int i = threadIdx.x * 4 + e;
-      // of neighbours that both pass, the one whose predecessor does not
-      if (i < n && test(i, c[e]) && !(i > 0 && test(i - 1, c[e] - m[e]))) { sh.found[0] = i; sh.found[1] = c[e]; }
+    for (int e = E - 1; e >= 0; --e) {
+      const int i = threadIdx.x * E + e;
+      if (i < n && test(i, c[e])) { mine = i; mass = c[e]; }
     }
-    __syncthreads();
-    at = (int)sh.found[0];
-    upto = sh.found[1];
-    __syncthreads();
+    if (WARP) {
+      const unsigned who = __ballot_sync(0xffffffffu, mine >= 0);
+      const int from = who ? __ffs(who) - 1 : 0;
+      at = __shfl_sync(0xffffffffu, mine, from);
+      upto = __shfl_sync(0xffffffffu, mass, from);
+      if (!who) { at = n - 1; upto = end; }
+    } else {
+      if (threadIdx.x == 0) { sh.found[0] = n - 1; sh.found[1] = end; }
+      __syncthreads();
+      // of neighbours that both pass, the one whose predecessor does not
+      if (mine >= 0 && (mine > threadIdx.x * E || mine == 0 || !test(mine - 1, c[0] - m[0]))) { sh.found[0] = mine; sh.found[1] = mass; }
+      __syncthreads();
+      at = (int)sh.found[0];
+      upto = sh.found[1];
+      __syncthreads();
+    }
   }
 };
 
 // The bin of the row's running mass: the first at whose end test(mass) holds; kSampleBins if none.  `before`: mass in front of it
-template <class F>
-__device__ int bin_of(SampleShared& sh, const u64 (&c)[2], const u64 (&m)[2], F test, u64& before) {
+template <class T, class F>
+__device__ int bin_of(SampleShared& sh, const T (&c)[2], const T (&m)[2], F test, u64& before) {
   if (threadIdx.x == 0) sh.found[2] = kSampleBins;
   __syncthreads();
 #pragma unroll
@@ -283,7 +381,7 @@ __device__ __forceinline__ uint32_t add_peer(const void* own, uint32_t rank, uin
 
 // C CTAs a row.  HELD: the slices fit in shared memory
 template <int C, bool HELD>
-__global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) float slice[];
   __shared__ SampleShared sh;
   grid_dep_launch();
@@ -294,7 +392,14 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
   SampleRow r;
   r.x = a.bf16 ? (const void*)(static_cast<const __nv_bfloat16*>(a.x) + row * a.ld) : (const void*)(static_cast<const float*>(a.x) + row * a.ld);
   r.V = a.V; r.bf16 = a.bf16;
-  r.shift = min(45, 62 - (32 - __clz(a.V)));
+  const int shift = min(45, 63 - (32 - __clz(a.V)));     // masses of a row stay below 2^64
+  const float t = a.temperature ? a.temperature[row] : a.t0;
+  SampleLimits lim;
+  lim.k = a.top_k ? a.top_k[row] : a.k0;
+  lim.p = a.top_p ? a.top_p[row] : a.p0;
+  lim.least = a.min_p ? a.min_p[row] : a.m0;
+  lim.u = a.uniform[row];
+  if (lim.k >= a.V) lim.k = 0;
   // the slice: groups of four that start on 16 bytes where the row's do; `skew` elements of the first group are in front of the row
   const int skew = a.bf16 ? 0 : (int)(reinterpret_cast<uintptr_t>(r.x) >> 2 & 3);
   const int groups = (a.V + skew + 3) / 4, per = (groups + C - 1) / C;
@@ -309,37 +414,85 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
     return make_float4(v[0], v[1], v[2], v[3]);
   };
   auto group = [&](int j) -> float4 { return HELD ? reinterpret_cast<const float4*>(slice)[j] : fetch(g0 + j); };
-  float top = -INFINITY;
+  if (tid < kSamplePer) sh.root[tid] = exp2(tid * (-1.0 / kSamplePer));
+  if (tid == 0) { sh.n_list = 0; sh.above = 0; }
+  auto clear = [&]() {
+    for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.own.cnt[i] = sh.own.lo[i] = sh.own.hi[i] = 0;
+  };
+  clear();
+  auto cta_max = [&](float v) -> float {
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (lane == 0) sh.warps[tid >> 5] = __float_as_uint(v);
+    __syncthreads();
+    for (int i = 0; i < kSampleWarps; ++i) v = fmaxf(v, __uint_as_float((uint32_t)sh.warps[i]));
+    __syncthreads();
+    return v + 0.f;
+  };
+  r.inv_t = 1.0 / (double)t;
+  const bool greedy = !(t > 0.f), counts = lim.k > 0 && lim.k <= kSampleList, both = lim.k > kSampleList;       // counts: all of the first k are sorted
+  const double per_logit = kSamplePer * 1.4426950408889634 * r.inv_t;
+  float kh = counts ? (float)kSamplePer : (float)per_logit;
+  const float kl = counts ? 0.f : (float)(per_logit - (double)kh);
+  // place on the grid, the same in every pass and slice: rounding does not change the order of two logits
+  auto grid = [&](float x) { return __fmul_rn(x, kh); };
+  constexpr float kMagic = 12582912.f, kGrid = 2097152.f;          // 1.5 * 2^23: what is added to it is rounded to a whole number
+  auto whole = [&](float p) { return __fsub_rn(__fadd_rn(p, kMagic), kMagic); };
+  float ref = -INFINITY;                                 // where the bins begin
+  bool above = false;                                    // an element was in front of them
+  auto put = [&](float x) {
+    const float p = grid(x), d = ref - p;
+    if (!(d < kSampleEdge)) return;
+    const float mid = __fadd_rn(p, kMagic);
+    const int n = (int)(__float_as_uint(__fadd_rn(ref, kMagic)) - __float_as_uint(mid));
+    if (n < 0) { above = true; return; }
+    if (!counts) {
+      // x in grid units is p + rest; off: its distance from the bin's middle
+      const float rest = fmaf(x, kl, fmaf(x, kh, -p)), off = __fadd_rn(__fsub_rn(p, __fsub_rn(mid, kMagic)), rest);
+      // 2^(off / 16) - 1, |off| <= 1/2: (ln2 / 16)^i / i! off^i
+      const float q = off * fmaf(off, fmaf(off, fmaf(off, 1.46760905e-7f, 1.35507817e-5f), 9.38384793e-4f), 4.33216988e-2f);
+      const unsigned w = __float_as_uint(fmaf(q, (float)(1 << kSampleUnit), kMagic)) - 0x4b400000u + (1u << kSampleUnit);
+      atomicAdd(&sh.own.lo[n], w & 0x3fffu);
+      atomicAdd(&sh.own.hi[n], w >> 14);
+      if (!both) return;
+    }
+    atomicAdd(&sh.own.cnt[n], 1u);
+  };
+  auto put4 = [&](const float4& v) { put(v.x); put(v.y); put(v.z); put(v.w); };
+  auto max4 = [](float m, const float4& v) { return fmaxf(fmaxf(fmaxf(m, v.x), fmaxf(v.y, v.z)), v.w); };
+  float top = -INFINITY;                                 // the slice's largest
+  constexpr int kAhead = 4;                              // groups that a thread has under way
+  auto ahead = [&](int j, float4 (&v)[kAhead]) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e)
+      v[e] = j + e * kSampleThreads < ng ? group(j + e * kSampleThreads) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  };
+  if (HELD) {
 #pragma unroll 8
-  for (int j = tid; j < ng; j += kSampleThreads) {
-    const float4 v = fetch(g0 + j);
-    if (HELD) reinterpret_cast<float4*>(slice)[j] = v;
-    top = fmaxf(fmaxf(fmaxf(top, v.x), fmaxf(v.y, v.z)), v.w);
+    for (int j = tid; j < ng; j += kSampleThreads) {
+      const float4 v = fetch(g0 + j);
+      reinterpret_cast<float4*>(slice)[j] = v;
+      top = max4(top, v);
+    }
+  } else {
+    // the bins begin well above the first groups' largest, so that the rest can be counted as it comes
+    float4 v[kAhead];
+    ahead(tid, v);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) top = max4(top, v[e]);
+    const float begin = grid(cta_max(top));
+    if (!greedy && fabsf(begin) < kGrid) ref = whole(begin) + (ng > kAhead * kSampleThreads ? 256.f : 0.f);
+    for (int j = tid; j < ng; j += kAhead * kSampleThreads) {
+      if (j != tid) ahead(j, v);
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        top = max4(top, v[e]);
+        if (ref > -INFINITY) put4(v[e]);
+      }
+    }
+    if (above) sh.above = 1;
   }
-  for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.own.cnt[i] = sh.own.lo[i] = sh.own.hi[i] = 0;
-  if (tid == 0) sh.n_list = 0;
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) sh.warps[tid >> 5] = __float_as_uint(top);
-  __syncthreads();
-  for (int i = 0; i < kSampleWarps; ++i) top = fmaxf(top, __uint_as_float((uint32_t)sh.warps[i]));
-  if (tid < C) st_peer(&sh.top[rank], tid, __float_as_uint(top));
-  cluster_barrier<C>();
-  for (int i = 0; i < C; ++i) top = fmaxf(top, sh.top[i]);
-  top += 0.f;
-  r.top = top;
-
-  const float t = a.temperature ? a.temperature[row] : a.t0;
-  SampleLimits lim;
-  lim.k = a.top_k ? a.top_k[row] : a.k0;
-  lim.p = a.top_p ? a.top_p[row] : a.p0;
-  lim.least = a.min_p ? a.min_p[row] : a.m0;
-  lim.u = a.uniform[row];
-  if (lim.k >= a.V) lim.k = 0;
-  if (top == -INFINITY) {
-    if (rank == 0 && tid == 0) a.out[row] = -1;
-    return;                                              // (no CTA looks into another's memory from here on)
-  }
-  if (!(t > 0.f)) {                                      // the first of the largest
+  top = cta_max(top);
+  if (greedy) {                                          // the first of the largest
     unsigned first = 0xffffffffu;
     for (int j = tid; j < ng; j += kSampleThreads) {
       const float4 v = group(j);
@@ -352,103 +505,103 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
     __syncthreads();
     if (tid == 0) {
       for (int i = 0; i < kSampleWarps; ++i) first = min(first, (unsigned)sh.warps[i]);
-      st_peer(&sh.first[rank], 0, first);
+      st_peer(&sh.first[rank], 0, element(top, first));
     }
     cluster_barrier<C>();
     if (rank == 0 && tid == 0) {
-      for (int i = 0; i < C; ++i) first = min(first, sh.first[i]);
-      a.out[row] = first;
+      u64 best = 0;
+      for (int i = 0; i < C; ++i) best = max(best, sh.first[i]);
+      a.out[row] = (uint32_t)(best >> 32) == image(-INFINITY) ? -1 : (long long)(0xffffffffu - (uint32_t)best);
     }
     return;
   }
-  r.inv_t = 1.0 / (double)t;
-  const bool counts = lim.k > 0 && lim.k <= kSampleList;           // all of the first k are sorted
-  const double per_octave = 32.0 * 1.4426950408889634 * r.inv_t;
-  const float kh = counts ? 32.f : (float)per_octave, kl = counts ? 0.f : (float)(per_octave - (double)kh);
-  // distance from the largest in bins, and the same in every pass: rounding does not change the order of two logits
-  auto distance = [&](float x) { return __fmul_rn(__fsub_rn(top, x), kh); };
-  constexpr float kMagic = 12582912.f;                   // 1.5 * 2^23: what is added to it is rounded to a whole number
-  auto bin_at = [&](float d) { return (int)(__float_as_uint(__fadd_rn(d, kMagic)) - 0x4b400000u); };
-  u64 over = 0;
-  const bool huge = top > 1e38f;                         // a difference can be above what 32 bits hold
-  if (huge) {
-    // settled alone
-  } else if (counts) {
-    for (int j = tid; j < ng; j += kSampleThreads) {
-      const float4 v = group(j);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float d = distance((&v.x)[e]);
-        if (d < kSampleEdge) atomicAdd(&sh.own.cnt[bin_at(d)], 1u);
-      }
+  const bool fits = fabsf(grid(top)) < kGrid;            // (a slice that does not fit has nothing to add where the row's largest does)
+  if (HELD || sh.above || ref == -INFINITY) {
+    if (!HELD) {
+      __syncthreads();
+      clear();
+      __syncthreads();
     }
-  } else {
-    const bool both = lim.k > 0;
-    for (int j = tid; j < ng; j += kSampleThreads) {
-      const float4 v = group(j);
+    ref = fits ? whole(grid(top)) : -INFINITY;
+    if (fits)
+      for (int j = tid; j < ng; j += kAhead * kSampleThreads) {
+        float4 v[kAhead];
+        ahead(j, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = (&v.x)[e], s = __fsub_rn(top, x), d = __fmul_rn(s, kh);
-        if (d < kSampleEdge) {
-          // s + low is top - x, d + rest that in bins
-          const float back = __fsub_rn(s, top), low = __fadd_rn(__fsub_rn(top, __fsub_rn(s, back)), __fsub_rn(-x, back));
-          const float rest = fmaf(low, kh, fmaf(s, kl, fmaf(s, kh, -d)));
-          const float whole = __fadd_rn(d, kMagic), off = __fadd_rn(__fsub_rn(d, __fsub_rn(whole, kMagic)), rest);
-          const int n = (int)(__float_as_uint(whole) - 0x4b400000u);
-          // 2^(-off / 32) - 1, |off| <= 1/2: (ln2 / 32)^i / i! off^i
-          const float q = off * fmaf(off, fmaf(off, fmaf(off, 9.17256e-9f, -1.69385098e-6f), 2.34596198e-4f), -2.16608494e-2f);
-          const unsigned w = __float_as_uint(fmaf(q, (float)(1 << kSampleUnit), kMagic)) - 0x4b400000u + (1u << kSampleUnit);
-          atomicAdd(&sh.own.lo[n], w & 0x3fffu);
-          atomicAdd(&sh.own.hi[n], w >> 14);
-          if (both) atomicAdd(&sh.own.cnt[n], 1u);
-        } else {
-          over += __float2uint_rn(exp2f((float)r.shift - d * (1.f / 32)));         // below 2^-31: a logit's rounding does not count
+        for (int e = 0; e < kAhead; ++e) put4(v[e]);
+      }
+  }
+  if (tid < C) {
+    st_peer(&sh.top[rank], tid, __float_as_uint(top));
+    st_peer(&sh.ref[rank], tid, __float_as_uint(ref));
+  }
+  cluster_barrier<C>();
+  float row_ref = -INFINITY;                             // where the row's bins begin
+  for (int i = 0; i < C; ++i) { top = fmaxf(top, sh.top[i]); row_ref = fmaxf(row_ref, sh.ref[i]); }
+  r.top = top;
+  if (top == -INFINITY) {
+    if (rank == 0 && tid == 0) a.out[row] = -1;
+    return;                                              // (no CTA looks into another's memory from here on)
+  }
+  const bool settled = fabsf(grid(top)) < kGrid - 4.f * kSampleBins;
+  // at low temperatures, whatever has weight lies within a few bins of 1 / 16 logit
+  const bool sharp = !settled && !counts && t <= 1.f && fabsf(top) * kSamplePer < kGrid - 4.f * kSampleBins;
+  if (sharp) { kh = kSamplePer; row_ref = whole(grid(top)); }
+  const float row_top = settled ? whole(grid(top)) : 0.f;
+  const int lead = settled ? (int)(row_ref - row_top) : 0;         // the largest logit's bin
+  // a mass is 2^shift for what lies in the middle of that bin
+  r.unit = ldexp(settled && !counts ? exp2(((double)top * per_logit - (double)row_top) * (1.0 / kSamplePer)) : 1.0, shift);
+  auto lower = [&](int c) {                              // by how many bins CTA c's begin below the row's
+    return (int)fminf(row_ref - sh.ref[c], 2.f * kSampleBins);
+  };
+  // 2^(e - n / 16)
+  auto middle = [&](int n, int e) -> double {
+    const double x = sh.root[n & (kSamplePer - 1)];
+    return __hiloint2double(__double2hiint(x) + ((e - (n >> 4)) << 20), __double2loint(x));
+  };
+  // every CTA sums its share of the bins over the cluster and hands it to all; P threads a bin
+  constexpr int P = C < 4 ? 1 : 4, kShareBins = kSampleBins / C;
+  if (settled)
+    for (int i = tid; i < kShareBins * P; i += kSampleThreads) {
+      const int n = rank * kShareBins + i / P, part = i % P;
+      unsigned cnt = 0;
+      u64 w = 0;
+#pragma unroll
+      for (int c = 0; c < C / P; ++c) {
+        const int from = part * (C / P) + c, by = C > 1 ? lower(from) : 0;
+        if (n >= by) {
+          cnt += ld_peer(&sh.own.cnt[n - by], from);
+          if (!counts) w += ((u64)ld_peer(&sh.own.hi[n - by], from) << 14) + ld_peer(&sh.own.lo[n - by], from);
         }
       }
-    }
-  }
-  for (int o = 16; o > 0; o >>= 1) over += __shfl_xor_sync(0xffffffffu, over, o);
-  if (lane == 0) sh.warps[tid >> 5] = over;
-  __syncthreads();
-  if (tid < C) {
-    over = 0;
-    for (int i = 0; i < kSampleWarps; ++i) over += sh.warps[i];
-    st_peer(&sh.over[rank], tid, over);
-  }
-  cluster_barrier<C>();
-  // every CTA sums its share of the bins over the cluster and hands it to all
-  for (int i = tid; i < kSampleBins / C; i += kSampleThreads) {
-    const int n = rank * (kSampleBins / C) + i;
-    unsigned cnt = 0;
-    u64 w = 0;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      cnt += ld_peer(&sh.own.cnt[n], c);
-      if (!counts) w += ((u64)ld_peer(&sh.own.hi[n], c) << 14) + ld_peer(&sh.own.lo[n], c);
-    }
-    const u64 m = counts ? 0 : (u64)__double2ll_rn(exp2((double)r.shift - kSampleUnit - n * (1.0 / 32)) * (double)w);
-    // without counts, what a bin holds at most: its weights' factors are within 1.1 % of one
-    if (!counts && lim.k <= 0) cnt = (unsigned)((w + (w >> 6) + (1u << (kSampleUnit - 1))) >> kSampleUnit);
+      for (int o = 1; o < P; o <<= 1) {
+        cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+        w += __shfl_xor_sync(0xffffffffu, w, o);
+      }
+      const u64 m = counts ? 0 : __double2ull_rn(middle(n - lead, shift - kSampleUnit) * (double)w);
+      // without counts, what a bin holds at most: its weights' factors are within 2.2 % of one
+      if (!counts && lim.k <= 0) cnt = (unsigned)((w + (w >> 5) + (1u << (kSampleUnit - 1))) >> kSampleUnit);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      st_peer(&sh.cnt[n], c, cnt);
-      st_peer(&sh.mass[n], c, m);
+      for (int c = 0; c < C / P; ++c) {
+        const int to = part * (C / P) + c;
+        st_peer(&sh.cnt[n], to, cnt);
+        if (!counts) st_peer(&sh.mass[n], to, m);
+      }
     }
-  }
   cluster_barrier<C>();
   // running counts and masses, two bins a thread
-  u64 mass[2], upto[2], cnt[2], count[2], before, total, many;
+  u64 mass[2], upto[2], before, total;
+  unsigned cnt[2], count[2], front;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) { mass[e] = sh.mass[2 * tid + e]; cnt[e] = sh.cnt[2 * tid + e]; }
-  scan(cnt[0] + cnt[1], sh.warps, before, many);
-  count[0] = before + cnt[0]; count[1] = count[0] + cnt[1];
-  scan(mass[0] + mass[1], sh.warps, before, total);
+  for (int e = 0; e < 2; ++e) { mass[e] = counts ? 0 : sh.mass[2 * tid + e]; cnt[e] = sh.cnt[2 * tid + e]; }
+  scan2(cnt[0] + cnt[1], mass[0] + mass[1], sh, front, before, total);
+  count[0] = front + cnt[0]; count[1] = count[0] + cnt[1];
   upto[0] = before + mass[0]; upto[1] = upto[0] + mass[1];
-  for (int i = 0; i < C; ++i) total += sh.over[i];
   u64 kept = total;                                      // (the first CTA's; the others know the first round only)
   // the bins in which an element that weighs `least` can be
   const float least = lim.least > 0.f ? fminf(lim.least, 1.f) : 0.f;
-  const float d_least = least > 0.f ? -32.f * log2f(least) : INFINITY;
+  const float d_least = least > 0.f ? (float)lead - kSamplePer * log2f(least) : INFINITY;
   const int n_least = d_least < kSampleEdge - 1.f ? (int)rintf(d_least) : kSampleBins;
   auto next = [&](int done) -> int4 {                    // the round behind `done`: (what, first bin, last bin), base in sh.base
     u64 base = 0;
@@ -488,86 +641,94 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
     __syncthreads();
     return make_int4(kPick, b, b, 0);
   };
+  // the first CTA: the mass that a round's sorted list leaves, and in the last round the token
+  auto settle = [&](const auto& l, const int4& todo) -> u64 {
+    const bool all = todo.x == kAll;
+    int at;
+    u64 some, left = sharp ? l.end : kept;
+    if (all && lim.k > 0) l.first(sh, [&](int i, u64) { return i + 1 >= lim.k; }, at, left);
+    if (todo.x == kFirst) l.first(sh, [&](int i, u64) { return i + 1 >= lim.k - todo.w; }, at, left);
+    some = left;
+    if ((all || todo.x == kShare) && lim.p < 1.f) {
+      const u64 want = max(reach(lim.p, left), (u64)1);
+      l.first(sh, [&](int, u64 c) { return c >= want; }, at, some);
+    }
+    if ((all || todo.x == kLeast) && least > 0.f) some = min(some, (all ? 0 : sh.base) + l.least(sh, least));
+    left = min(left, some);
+    if (all || todo.x == kPick) {
+      const u64 want = exceed(lim.u, left);
+      l.first(sh, [&](int, u64 c) { return c > want; }, at, some);
+      if (tid == 0) a.out[row] = 0xffffffffu - (unsigned)(sh.list[at] & 0xffffffffu);
+    }
+    return left;
+  };
   int4 todo;
-  if (huge) todo = make_int4(kAlone, 0, 0, 0);
-  else if (counts) {
+  if (!settled) {
+    todo = sharp ? make_int4(kAll, 0, min(kSampleBins - 1, (int)(t * 500.f) + 2), 0) : make_int4(kAlone, 0, 0, 0);          // 2^-45
+  } else if (counts) {
     u64 base;
     const int b = bin_of(sh, count, cnt, [&](u64 c) { return c >= (u64)lim.k; }, base);
     todo = b == kSampleBins ? make_int4(kAlone, 0, 0, 0) : make_int4(kAll, 0, b, 0);
-  } else todo = next(kDone);
+  } else {
+    todo = next(kDone);
+  }
   while (todo.x > kAlone) {
-    // the bins' elements go to the first CTA
-    for (int j0 = 0; j0 < ng; j0 += kSampleThreads) {
-      const int j = j0 + tid;
-      float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (j < ng) v = group(j);
+    // the bins' elements go to the first CTA, the others' by way of a list of their own
+    const float from = row_ref - (float)todo.z, to_grid = row_ref - (float)todo.y;
+    for (int j = tid; j < ng; j += kAhead * kSampleThreads) {
+      float4 v4[kAhead];
+      ahead(j, v4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float d = distance((&v.x)[e]);
-        bool in = d < kSampleEdge;
-        if (in) {
-          const int n = bin_at(d);
-          in = n >= todo.y && n <= todo.z;
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, in);
-        if (who) {
-          unsigned to = 0;
-          if (lane == 0) to = add_peer(&sh.n_list, 0, __popc(who));
-          to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1u));
-          if (in && to < kSampleList) st_peer(&sh.list[to], 0, element((&v.x)[e], 4 * (g0 + j) - skew + e));
+      for (int b = 0; b < kAhead; ++b) {
+        if (!(grid(max4(-INFINITY, v4[b])) >= from - 0.5f)) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = (&v4[b].x)[e], p = grid(x);
+          if (!(p >= from - 0.5f && p <= to_grid + 0.5f)) continue;
+          const float n = whole(p);
+          if (!(n >= from && n <= to_grid)) continue;
+          const unsigned to = atomicAdd(&sh.n_list, 1u);
+          if (to < kSampleList) sh.list[to] = element(x, 4 * (g0 + j + b * kSampleThreads) - skew + e);
         }
       }
     }
+    if (C > 1) {
+      __syncthreads();
+      if (rank != 0) {
+        const unsigned n = sh.n_list;
+        if (tid == 0 && n) sh.at = add_peer(&sh.n_list, 0, n);
+        __syncthreads();
+        for (unsigned i = tid; i < min(n, (unsigned)kSampleList); i += kSampleThreads)
+          if (sh.at + i < kSampleList) st_peer(&sh.list[sh.at + i], 0, sh.list[i]);
+        __syncthreads();
+        if (tid == 0) sh.n_list = 0;
+      }
+    }
     cluster_barrier<C>();
+    if (rank != 0 && (todo.x == kAll || todo.x == kPick)) return;          // (the last round, or the first CTA goes on alone)
+    const bool last = todo.x == kAll || todo.x == kPick;
     if (rank == 0) {
       const int n = (int)sh.n_list;
       if (n > kSampleList || n < 1) {
         todo = make_int4(kAlone, 0, 0, 0);
       } else {
-        sort_list(sh.list, n);
         const u64 base = todo.x == kAll ? 0 : sh.base;
-        double w[4];
-        const ListMasses l(r, sh, n, base, w);
-        int at;
-        u64 m;
-        if (todo.x == kAll) {
-          if (lim.k > 0) l.first(sh, [&](int i, u64) { return i + 1 >= lim.k; }, at, kept);
-          u64 some = kept;
-          if (lim.p < 1.f) {
-            const u64 want = max(reach(lim.p, kept), (u64)1);
-            l.first(sh, [&](int, u64 c) { return c >= want; }, at, some);
+        if (n <= 128) {
+          sort_few(sh.list, n);
+          if (tid < 32) {
+            const u64 left = settle(ListMasses<4, true>(r, sh, n, base), todo);
+            if (tid == 0) sh.kept = left;
           }
-          if (least > 0.f) {                             // mass of what weighs enough
-            u64 mine = 0, b4, over_m;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mine += w[e] >= (double)least ? l.m[e] : 0;
-            scan(mine, sh.warps, b4, over_m);
-            some = min(some, over_m);
-          }
-          kept = min(kept, some);
-        } else if (todo.x == kFirst) {
-          l.first(sh, [&](int i, u64) { return i + 1 >= lim.k - todo.w; }, at, kept);
-        } else if (todo.x == kShare) {
-          const u64 want = max(reach(lim.p, kept), (u64)1);
-          l.first(sh, [&](int, u64 c) { return c >= want; }, at, m);
-          kept = min(kept, m);
-        } else if (todo.x == kLeast) {
-          u64 mine = 0, b4, over_m;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mine += w[e] >= (double)least ? l.m[e] : 0;
-          scan(mine, sh.warps, b4, over_m);
-          kept = min(kept, base + over_m);
-        }
-        if (todo.x == kAll || todo.x == kPick) {
-          const u64 want = exceed(lim.u, kept);
-          l.first(sh, [&](int, u64 c) { return c > want; }, at, m);
-          if (tid == 0) a.out[row] = 0xffffffffu - (unsigned)(sh.list[at] & 0xffffffffu);
-          todo = make_int4(kDone, 0, 0, 0);
+          __syncthreads();
+          kept = sh.kept;
         } else {
-          todo = next(todo.x);
+          sort_list(sh.list, n);
+          kept = n <= kSampleThreads ? settle(ListMasses<1, false>(r, sh, n, base), todo) : settle(ListMasses<4, false>(r, sh, n, base), todo);
         }
+        todo = last ? make_int4(kDone, 0, 0, 0) : next(todo.x);
       }
       __syncthreads();
+      if (last) break;
       if (tid == 0) sh.n_list = 0;
       if (tid < C) {
         st_peer(&sh.what, tid, (uint32_t)todo.x);
@@ -617,9 +778,13 @@ extern "C" int xft_sample_rows(const char* packed, cudaStream_t st) {
   memcpy(&a, packed, sizeof(a));
   if (a.rows <= 0) return 0;
   if (a.V < 1 || a.V > (1 << 24) || a.rows > (1 << 27)) return -1;
-  // slices of at most 19 Ki elements leave room for two CTAs per SM; few rows are cut finer
-  if (a.V <= 4096) return launch<1, true>(a, st);
-  if (a.V <= 19456 && a.rows >= 296) return launch<1, true>(a, st);
-  if (a.V <= 8 * 45056) return launch<8, true>(a, st);
-  return launch<8, false>(a, st);
+  // CTAs of a row: as many as find room at a time, two an SM; their serial steps cost each row C times.  us, C = 8 / 4 / 2 / 1: see below
+  const int fit = a.rows <= 37 ? 8 : a.rows <= 74 ? 4 : a.rows <= 148 || a.V > 65536 ? 2 : 1;
+  const int c = a.V <= 4096 ? 1 : fit;
+  // slices of up to 19 Ki elements are held: two CTAs of them share an SM
+  const bool held = a.V <= c * 19456;
+  if (c == 8) return held ? launch<8, true>(a, st) : launch<8, false>(a, st);
+  if (c == 4) return held ? launch<4, true>(a, st) : launch<4, false>(a, st);
+  if (c == 2) return held ? launch<2, true>(a, st) : launch<2, false>(a, st);
+  return held ? launch<1, true>(a, st) : launch<1, false>(a, st);
 }
