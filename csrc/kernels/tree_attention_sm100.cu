@@ -1,5 +1,5 @@
 // Attention of the nodes of trees of drafted tokens on the 5th-generation tensor cores: bf16 cache in blocks of a multiple of 64, heads of
-// 64 or 128, no window and no cap (those: tree_attention.cu, where the formula is).
+// 64 or 128 (int8 cache: 128), no window and no cap (those: tree_attention.cu, where the formula is).
 //
 // The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile (two CTAs per
 // SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of 128 keys
@@ -15,6 +15,9 @@
 // The masks matter only in the last tiles, where the nodes' keys are: 128 bits of a row, shifted to the tile's place.  There two more
 // warps clear the values of keys that no node sees and of slots behind the last key, since 0 x NaN is NaN.
 //
+// Codes of an int8 cache are expanded on the way, by four warps between the ring that TMA fills and the one that the products read; they are
+// exact in bf16, a key's scale multiplies its score and a value's its weight, in 32 bits.
+//
 // Every wait is bounded and reports through the status word.
 #include "tree_attention.cuh"
 
@@ -26,14 +29,20 @@ namespace {
 
 constexpr int kTgKeys = 128, kTgRows = 128;
 
-// R row tiles of heads of 64 * H
-template <int H, int R>
+// G groups of four softmax warps and heads of 64 * H; I8: int8 cache.  The groups have a tile of rows each, or (TURNS) take turns at the
+// key tiles of one.
+template <int H, int G, bool I8, bool TURNS>
 struct TgShape {
+  static constexpr int R = TURNS ? 1 : G;                // row tiles
+  static constexpr int kLead = TURNS ? G : 1;            // S of so many tiles is ahead of P V
   static constexpr int kHalf = kTgKeys * 128;            // 64 features of a tile's 128 rows
   static constexpr int kTile = H * kHalf;
-  static constexpr int kStages = R == 1 ? 4 / H : 10 / H;            // 64 KB (two CTAs an SM), 160 KB
-  static constexpr int kSmem = (R + kStages) * kTile + 1024;
-  static constexpr int kThreads = 128 + 128 * R;
+  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : R == 1 ? 4 / H : 10 / H;       // 64 KB (two CTAs an SM), 160 KB
+  static constexpr int kRaw = I8 ? (TURNS ? 3 : 5) : 0, kRawTile = kTgKeys * 128;                    // codes as they come
+  static constexpr int kScales = I8 ? 4 : 0, kScaleBytes = 2 * kTgKeys * 4;            // of a tile's keys and values
+  static constexpr int kSmem = (R + kStages) * kTile + kRaw * kRawTile + kScales * kScaleBytes + 1024;
+  static constexpr int kThreads = 128 + 128 * G + (I8 ? 128 : 0);
+  static constexpr int kPerSm = G == 1 ? 2 : 1;
 };
 
 __device__ __forceinline__ float tg_max3(float a, float b, float c) {
@@ -55,6 +64,13 @@ __device__ __forceinline__ float2 tg_add2(float2 a, float2 b) {
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return d;
 }
+__device__ __forceinline__ float2 tg_mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
 __device__ __forceinline__ uint32_t tg_pack(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
@@ -72,6 +88,17 @@ __device__ __forceinline__ void tg_ld_wait32(uint32_t (&v)[32]) {
                  "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
 }
 
+// Four codes as bf16, exact: (128 + the low seven bits) - (128 + the sign's 128), each one byte behind the exponent of 128
+__device__ __forceinline__ uint32_t tg_sub2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint2 tg_codes(uint32_t c) {
+  const uint32_t x = __byte_perm(c, 0x43434343u, 0x5140), y = __byte_perm(c, 0x43434343u, 0x5342);
+  return make_uint2(tg_sub2(x & 0xff7fff7fu, x & 0xff80ff80u), tg_sub2(y & 0xff7fff7fu, y & 0xff80ff80u));
+}
+
 // Bits of 32 keys from key `first` on that a node with mask `m` (32-bit words) sees: the context's all, then the nodes'
 __device__ __forceinline__ uint32_t tg_sees(const uint32_t* m, int first, int ctx, int n) {
   const int o = first - ctx;
@@ -85,33 +112,39 @@ __device__ __forceinline__ uint32_t tg_sees(const uint32_t* m, int first, int ct
   return __funnelshift_r(word(o >> 5), word((o >> 5) + 1), o & 31);
 }
 
-template <int H, int R>
-__global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
+template <int H, int G, bool I8, bool TURNS>
+__global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H, G, I8, TURNS>::kPerSm)
     tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs p) {
-  using S = TgShape<H, R>;
-  constexpr int D = 64 * H, ST = S::kStages;
+  using S = TgShape<H, G, I8, TURNS>;
+  constexpr int D = 64 * H, ST = S::kStages, R = S::R, L = S::kLead;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                                    // R tiles
   uint8_t* sT = smem + R * S::kTile;                     // ring: keys and values of the tiles in turn
-  __shared__ uint64_t q_full, full[ST], empty[ST], v_here, v_clean, s_full[R], p_half[R], p_full[R], o_full[R];
+  uint8_t* sRaw = sT + ST * S::kTile;                    // I8: ring of codes, in the same order
+  float* s_scales = reinterpret_cast<float*>(sRaw + S::kRaw * S::kRawTile);           // I8: ring of tiles' scales
+  __shared__ uint64_t raw_full[S::kRaw + 1], raw_empty[S::kRaw + 1], c_full[S::kScales + 1], c_empty[S::kScales + 1];
+  __shared__ uint64_t q_full, full[ST], empty[ST], v_here, v_clean, s_full[G], p_half[G], p_full[G], o_full[G];
+  __shared__ float2 s_ml[TURNS ? kTgRows : 1];
   __shared__ uint32_t tmem_base_s, s_union[kTreeWords * 2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, b = blockIdx.z;
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 4 * R);
-    for (int s = 0; s < ST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(&q_full, 4 * R);                           // (TURNS: the first group brings the queries)
+    for (int s = 0; s < ST; ++s) { mbar_init(&full[s], I8 ? 4 : 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < S::kRaw; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 4); }
+    for (int s = 0; s < S::kScales; ++s) { mbar_init(&c_full[s], 1); mbar_init(&c_empty[s], TURNS ? 4 : 4 * G); }
     mbar_init(&v_here, 1);
     mbar_init(&v_clean, 2);
-    for (int g = 0; g < R; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_half[g], 4); mbar_init(&p_full[g], 4); mbar_init(&o_full[g], 1); }
+    for (int g = 0; g < G; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_half[g], 4); mbar_init(&p_full[g], 4); mbar_init(&o_full[g], 1); }
     fence_barrier_init();
     fence_proxy_async();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base_s, 256 * R);                   // of a row tile: S, whose first half becomes P, and O
+    tmem_alloc(&tmem_base_s, 256 * G);                   // of a group: S, whose first half becomes P, and O
     tmem_relinquish();
   }
   grid_dep_launch();
@@ -129,25 +162,65 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
   tcgen05_fence_after();
   const uint32_t tmem_base = tmem_base_s;
 
-  // registers at launch: R = 1 256 x 128, R = 2 384 x 168; from here on 128 x 40 + 128 x 216, 128 x 72 + 256 x 216
-  if (warp < 4) {
-    if (R == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  // registers at launch: 256 x 128, 384 x 168 or (int8) 512 x 128; from here on 128 x 40 + 128 x 216, 128 x 72 + 256 x 216 or 128 x 40 +
+  // 256 x 200 + 128 x 72
+  if (I8 && warp >= 4 + 4 * G) {
+    // ------------------------------------------------------------------ codes to bf16, a row of a tile per thread
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int r = threadIdx.x & 127;
+    Ring raw{0, 0}, ring{0, 1};
+    for (int i = 0; i < 2 * nt; ++i) {
+      if (!mbar_wait(&raw_full[raw.s], raw.ph, p.status, XFT_ERR_WAIT_FULL)) break;
+      if (!mbar_wait(&empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY)) break;
+      const uint8_t* from = sRaw + raw.s * S::kRawTile + r * 128;
+      uint8_t* to = sT + ring.s * S::kTile + r * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint4 w = *reinterpret_cast<const uint4*>(from + ((c ^ (r & 7)) << 4));
+        const uint2 a0 = tg_codes(w.x), a1 = tg_codes(w.y), a2 = tg_codes(w.z), a3 = tg_codes(w.w);
+        uint8_t* half = to + (c >> 2) * S::kHalf;
+        *reinterpret_cast<uint4*>(half + (((2 * c & 7) ^ (r & 7)) << 4)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
+        *reinterpret_cast<uint4*>(half + (((2 * c + 1 & 7) ^ (r & 7)) << 4)) = make_uint4(a2.x, a2.y, a3.x, a3.y);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&full[ring.s]); mbar_arrive(&raw_empty[raw.s]); }
+      raw.next(S::kRaw);
+      ring.next(ST);
+    }
+  } else if (warp < 4) {
+    if (G == 1 || I8) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
       // ------------------------------------------------------------------ TMA producer
       if (elect_one()) {
         const int n_pieces = (s.kv + 63) / 64;
         Ring ring{0, 1};
-        bool ok = true;
-        for (int j = 0; j < nt && ok; ++j) {
+        // one tile of keys or values, in the order that the products take them
+        auto load = [&](int j, bool v) -> bool {
           int at[2];
           for (int i = 0; i < 2; ++i) {                  // past the last keys they are read again
             const int piece = min(2 * (t0 + j) + i, n_pieces - 1), first = piece * 64;
             at[i] = (tree_block(p, b, first / p.bs) * p.hkv + kvh) * p.bs + first % p.bs;
           }
-          for (int v = 0; v < 2; ++v) {
-            ok = mbar_wait(&empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY);
-            if (!ok) break;
+          if constexpr (I8) {
+            if (!v) {
+              const int cs = j % S::kScales;
+              if (!mbar_wait(&c_empty[cs], (j / S::kScales & 1) ^ 1, p.status, XFT_ERR_WAIT_EMPTY)) return false;
+              float* to = s_scales + cs * 2 * kTgKeys;
+              mbar_expect_tx(&c_full[cs], S::kScaleBytes);
+              for (int i = 0; i < 2; ++i) {
+                bulk_load(to + i * 64, p.ks + at[i], 256, &c_full[cs]);
+                bulk_load(to + kTgKeys + i * 64, p.vs + at[i], 256, &c_full[cs]);
+              }
+            }
+            if (!mbar_wait(&raw_empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY)) return false;
+            mbar_expect_tx(&raw_full[ring.s], S::kRawTile);
+            for (int i = 0; i < 2; ++i)
+              tma_load_2d(sRaw + ring.s * S::kRawTile + i * 8192, v ? &tmV : &tmK, &raw_full[ring.s], 0, at[i], kEvictNormal);
+            ring.next(S::kRaw);
+          } else {
+            if (!mbar_wait(&empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY)) return false;
             uint8_t* to = sT + ring.s * S::kTile;
             mbar_expect_tx(&full[ring.s], S::kTile);
             for (int i = 0; i < 2; ++i)
@@ -155,7 +228,11 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
                 tma_load_2d(to + h * S::kHalf + i * 8192, v ? &tmV : &tmK, &full[ring.s], h * 64, at[i], kEvictNormal);
             ring.next(ST);
           }
-        }
+          return true;
+        };
+        bool ok = true;
+        for (int j = 0; j < min(L, nt) && ok; ++j) ok = load(j, false);
+        for (int j = 0; j < nt && ok; ++j) ok = load(j, true) && (j + L >= nt || load(j + L, false));
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA issuer
@@ -163,9 +240,9 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
         constexpr uint32_t IDESC_S = umma_idesc(128, kTgKeys, 1, 1, 1);
         constexpr uint32_t IDESC_O = umma_idesc(128, D, 1, 1, 1) | (1u << 16);       // B = V, MN-major
         Ring ring{0, 0};
-        bool ok = mbar_wait(&q_full, 0, p.status, XFT_ERR_WAIT_FULL) && mbar_wait(&full[0], 0, p.status, XFT_ERR_WAIT_FULL);
+        bool ok = mbar_wait(&q_full, 0, p.status, XFT_ERR_WAIT_FULL);
         auto scores = [&](int g, int st) {
-          const uint64_t qd = umma_desc_k128(smem_u32(sQ + g * S::kTile)), kd = umma_desc_k128(smem_u32(sT + st * S::kTile));
+          const uint64_t qd = umma_desc_k128(smem_u32(sQ + (TURNS ? 0 : g) * S::kTile)), kd = umma_desc_k128(smem_u32(sT + st * S::kTile));
           tcgen05_fence_after();
 #pragma unroll
           for (int k = 0; k < 4 * H; ++k) {
@@ -174,9 +251,11 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
           }
           tcgen05_commit(&s_full[g]);
         };
-        if (ok) {
-          for (int g = 0; g < R; ++g) scores(g, 0);
-          tcgen05_commit(&empty[0]);
+        for (int j = 0; j < min(L, nt) && ok; ++j) {
+          ok = mbar_wait(&full[ring.s], ring.ph, p.status, XFT_ERR_WAIT_FULL);
+          if (!ok) break;
+          for (int g = TURNS ? j : 0; g < (TURNS ? j + 1 : G); ++g) scores(g, ring.s);
+          tcgen05_commit(&empty[ring.s]);
           ring.next(ST);
         }
         int cleaned = 0;
@@ -184,40 +263,43 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
           const Ring vr = ring;
           ring.next(ST);
           const Ring kr = ring;
+          const bool more = j + L < nt;
+          if (more) ring.next(ST);
           ok = mbar_wait(&full[vr.s], vr.ph, p.status, XFT_ERR_WAIT_FULL);
-          if (ok && t0 + j >= tail) {
+          if (!I8 && ok && t0 + j >= tail) {
             mbar_arrive(&v_here);
             ok = mbar_wait(&v_clean, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL);
           }
           if (!ok) break;
           const uint64_t vd = umma_desc_mn128(smem_u32(sT + vr.s * S::kTile), S::kHalf);
-          for (int g = 0; g < R && ok; ++g) {
+          const int g0 = TURNS ? j % G : 0, g1 = TURNS ? g0 + 1 : G;
+          const uint32_t ph = (TURNS ? j / G : j) & 1;
+          for (int g = g0; g < g1; ++g) {
             const uint32_t pa = tmem_base + g * 256, oa = pa + 128;
-            ok = mbar_wait(&p_half[g], j & 1, p.status, XFT_ERR_WAIT_TMEM);
+            ok = mbar_wait(&p_half[g], ph, p.status, XFT_ERR_WAIT_TMEM);
             if (!ok) break;
             tcgen05_fence_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, j > 0 || k > 0);
-            ok = mbar_wait(&p_full[g], j & 1, p.status, XFT_ERR_WAIT_TMEM);
+            for (int k = 0; k < 4; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, j >= L || k > 0);
+            ok = mbar_wait(&p_full[g], ph, p.status, XFT_ERR_WAIT_TMEM);
             if (!ok) break;
             tcgen05_fence_after();
 #pragma unroll
             for (int k = 4; k < 8; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, 1);
-            if (g == R - 1) tcgen05_commit(&empty[vr.s]);
-            if (j + 1 < nt) {                            // the next S goes over P, behind the product that reads P
-              if (g == 0) ok = mbar_wait(&full[kr.s], kr.ph, p.status, XFT_ERR_WAIT_FULL);
+            if (g == g1 - 1) tcgen05_commit(&empty[vr.s]);
+            if (more) {                                  // the next S goes over P, behind the product that reads P
+              if (g == g0) ok = mbar_wait(&full[kr.s], kr.ph, p.status, XFT_ERR_WAIT_FULL);
               if (!ok) break;
               scores(g, kr.s);
-              if (g == R - 1) tcgen05_commit(&empty[kr.s]);
+              if (g == g1 - 1) tcgen05_commit(&empty[kr.s]);
             } else {
               tcgen05_commit(&o_full[g]);
             }
           }
-          ring.next(ST);
         }
       }
-    } else {
-      // ------------------------------------------------------------------ values that no node sees
+    } else if (!I8) {
+      // ------------------------------------------------------------------ values that no node sees (codes are finite, their scales below)
       if (t0 + nt > tail && nt > 0) {
         uint32_t seen[kTreeWords * 2] = {};
         const uint32_t* m = reinterpret_cast<const uint32_t*>(p.mask + (long long)s.q0 * p.words);
@@ -259,15 +341,16 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax: one row per thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (I8) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int g = (warp - 4) >> 2, qd = warp & 3;
-    const int r = qd * 32 + lane, row = row0 + g * kTgRows + r;
-    const bool mine = row < rows, busy = row0 + g * kTgRows + qd * 32 < rows;          // the row, some row of the warp
+    const int tile = TURNS ? 0 : g, r = qd * 32 + lane, row = row0 + tile * kTgRows + r;
+    const bool mine = row < rows, busy = row0 + tile * kTgRows + qd * 32 < rows;          // the row, some row of the warp
     const int node = mine ? row / heads : 0, h = h0 + (mine ? row - node * heads : 0);
     const long long at = (long long)(s.q0 + node) * p.hq + h;
-    if (nt > 0) {
+    if (nt > 0 && (!TURNS || g == 0)) {
       // this row of queries in the order that the product reads: 16-byte pieces exchanged with the row's low bits
-      uint8_t* to = sQ + g * S::kTile + r * 128;
+      uint8_t* to = sQ + tile * S::kTile + r * 128;
       uint4 v[8];
 #pragma unroll
       for (int half = 0; half < H; ++half) {
@@ -284,11 +367,17 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
     const float scale = p.scale * kTreeLog2e;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < nt; ++j) {
-      if (!mbar_wait(&s_full[g], j & 1, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
+    const int first = TURNS ? g : 0;                     // of this group's tiles
+    constexpr int kRing = I8 ? S::kScales : 1;
+    for (int j = first; j < nt; j += L) {
+      const int cs = j % kRing;
+      const uint32_t ph = (TURNS ? j / G : j) & 1;
+      const float* scales = s_scales + cs * 2 * kTgKeys;
+      if (I8 && !mbar_wait(&c_full[cs], j / kRing & 1, p.status, XFT_ERR_WAIT_FULL)) { ok = false; break; }
+      if (!mbar_wait(&s_full[g], ph, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
       tcgen05_fence_after();
       if (!busy) {
-        if (lane == 0) { mbar_arrive(&p_half[g]); mbar_arrive(&p_full[g]); }
+        if (lane == 0) { mbar_arrive(&p_half[g]); mbar_arrive(&p_full[g]); if (I8) mbar_arrive(&c_empty[cs]); }
         continue;
       }
       uint32_t x[4][32];
@@ -296,14 +385,32 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
       for (int c = 0; c < 4; ++c) tmem_ld32(sa + 32 * c, x[c]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) tg_ld_wait32(x[c]);
+      if constexpr (I8) {                                // a key's scale belongs to its scores
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 16) {
+            float4 f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = *reinterpret_cast<const float4*>(scales + 32 * c + i + 4 * e);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 y = tg_mul2(make_float2(__uint_as_float(x[c][i + e]), __uint_as_float(x[c][i + e + 1])),
+                                       make_float2((&f[e >> 2].x)[e & 3], (&f[e >> 2].x)[(e & 3) + 1]));
+              x[c][i + e] = __float_as_uint(y.x);
+              x[c][i + e + 1] = __float_as_uint(y.y);
+            }
+          }
+      }
+      uint32_t sees[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
       if (t0 + j >= tail) {
         const uint32_t* bits = reinterpret_cast<const uint32_t*>(p.mask + (long long)(s.q0 + node) * p.words);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t sees = tg_sees(bits, (t0 + j) * kTgKeys + 32 * c, s.ctx, s.n);
+          sees[c] = tg_sees(bits, (t0 + j) * kTgKeys + 32 * c, s.ctx, s.n);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (!(sees >> i & 1)) x[c][i] = 0xff800000u;
+            if (!(sees[c] >> i & 1)) x[c][i] = 0xff800000u;
         }
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -317,7 +424,7 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
         const float f = grown ? exp2f(m - mx) : 1.f;     // 0 where nothing has been seen yet
         if (grown) m = mx;
         l *= f;
-        if (j > 0) {
+        if (j > first) {
           uint32_t y[32];
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
@@ -334,13 +441,24 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t w[16];
+        float4 f[I8 ? 8 : 1];                            // the values' scales
+        if constexpr (I8)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float4*>(scales + kTgKeys + 32 * c + 4 * i);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float2 e = tg_fma2(make_float2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), make_float2(scale, scale), make_float2(off, off));
           e.x = exp2f(e.x);
           e.y = exp2f(e.y);
-          w[i >> 1] = tg_round(e.x, e.y);
           sum[(i >> 1) & 1] = tg_add2(sum[(i >> 1) & 1], e);
+          if constexpr (I8) {                            // a value's scale belongs to the product, not to the sum
+            e = tg_mul2(e, make_float2((&f[i >> 2].x)[i & 3], (&f[i >> 2].x)[(i & 3) + 1]));
+            if (sees[c] != 0xffffffffu) {                // (0 x the scale of a slot behind the last key may be NaN)
+              if (!(sees[c] >> i & 1)) e.x = 0.f;
+              if (!(sees[c] >> (i + 1) & 1)) e.y = 0.f;
+            }
+          }
+          w[i >> 1] = I8 ? tg_pack(e.x, e.y) : tg_round(e.x, e.y);           // (int8: the other instructions are what is short)
         }
         tmem_st16(sa + 16 * c, w);
         if (c == 1) {                                    // the product may begin with the first 64 keys
@@ -355,29 +473,69 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
       tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[g]);
+      if (lane == 0) { mbar_arrive(&p_full[g]); if (I8) mbar_arrive(&c_empty[cs]); }
     }
-    if (nt > 0 && ok && busy && mbar_wait(&o_full[g], 0, p.status, XFT_ERR_WAIT_TMEM)) {
-      tcgen05_fence_after();
-      float f = 1.f;
+    bool have = ok && busy && nt > first;                // the group has sums
+    for (int o = 0; o < G; ++o)                          // (TURNS: the ring is free for the exchange when both are through)
+      if (have && (TURNS ? o < nt : o == g)) have = mbar_wait(&o_full[o], 0, p.status, XFT_ERR_WAIT_TMEM);
+    tcgen05_fence_after();
+    float f = 1.f, f2 = 0.f;
+    if constexpr (TURNS) {
+      // the second group's sums go through shared memory, column after column
+      float* sO = reinterpret_cast<float*>(sT);
+      if (g == 1) {
+        s_ml[r] = have ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        if (have)
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t y[32];
+            tmem_ld32(oa + c, y);
+            tg_ld_wait32(y);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sO[(c + i) * kTgRows + r] = __uint_as_float(y[i]);
+          }
+      }
+      named_bar_sync(1, 256);
+      const float2 o = s_ml[r];
+      if (g == 0 && o.y != 0.f) {
+        const float mx = fmaxf(m, o.x);
+        f = m == -INFINITY ? 0.f : exp2f(m - mx);
+        f2 = o.x == -INFINITY ? 1.f : exp2f(o.x - mx);   // (a NaN among the sums stays one)
+        l = l * f + o.y * f2;
+        m = mx;
+      }
+      if (g == 1) have = false;
+    }
+    if (have) {
+      float all = 1.f;
       if (p.nsplit == 1) {
         float sum = l;
         if (p.sinks) {
           const float sink = p.sinks[h] * kTreeLog2e, mx = fmaxf(m, sink);
-          f = exp2f(m - mx);
-          sum = sum * f + exp2f(sink - mx);
+          all = exp2f(m - mx);
+          sum = sum * all + exp2f(sink - mx);
         }
-        f = l == 0.f ? 0.f : __fdividef(f, sum);         // a row that sees nothing
+        all = l == 0.f ? 0.f : __fdividef(all, sum);     // a row that sees nothing
       }
+      f *= all;
+      f2 *= all;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
         tmem_ld32(oa + c, y);
         tg_ld_wait32(y);
+        if (TURNS && f2 != 0.f) {
+          const float* sO = reinterpret_cast<const float*>(sT);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f + sO[(c + i) * kTgRows + r] * f2);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+        }
         if (mine && p.nsplit == 1) {
           uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = tg_pack(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
+          for (int i = 0; i < 16; ++i) w[i] = tg_pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
           st_global_256(p.out + at * D + c, w);
           st_global_256(p.out + at * D + c + 16, w + 8);
         } else if (mine) {
@@ -387,26 +545,28 @@ __global__ void __launch_bounds__(TgShape<H, R>::kThreads, R == 1 ? 2 : 1)
         }
       }
     }
-    if (mine && p.nsplit > 1) *reinterpret_cast<float2*>(p.part_ml + (at * p.nsplit + slice) * 2) = ok ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+    if (mine && p.nsplit > 1 && (!TURNS || g == 0))
+      *reinterpret_cast<float2*>(p.part_ml + (at * p.nsplit + slice) * 2) = have ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
   }
   __syncwarp();
   tcgen05_fence_before();
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem_base, 256 * R);
+    tmem_dealloc(tmem_base, 256 * G);
   }
 }
 
-template <int H, int R>
+template <int H, int G, bool I8, bool TURNS>
 int launch(const TreeAttnArgs& a, cudaStream_t st) {
-  using S = TgShape<H, R>;
+  using S = TgShape<H, G, I8, TURNS>;
   CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)a.num_blocks * a.hkv * a.bs;
-  if (encode_tensor_map(&tmK, a.kc, rows, a.D, a.D, 64, 2) || encode_tensor_map(&tmV, a.vc, rows, a.D, a.D, 64, 2)) return -4;
-  auto k = tree_attention_tc_kernel<H, R>;
+  const uint32_t size = I8 ? 1 : 2;
+  if (encode_tensor_map(&tmK, a.kc, rows, a.D, a.D, 64, size) || encode_tensor_map(&tmV, a.vc, rows, a.D, a.D, 64, size)) return -4;
+  auto k = tree_attention_tc_kernel<H, G, I8, TURNS>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return 3000 + (int)cudaGetLastError();
-  const int n_rt = (a.max_q * a.group + R * kTgRows - 1) / (R * kTgRows);
+  const int n_rt = (a.max_q * a.group + S::R * kTgRows - 1) / (S::R * kTgRows);
   const cudaError_t e = launch_pdl(k, dim3(n_rt * a.nsplit, a.hkv, a.B), dim3(S::kThreads), (size_t)S::kSmem, st, tmK, tmV, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
@@ -415,10 +575,14 @@ int launch(const TreeAttnArgs& a, cudaStream_t st) {
 
 // 0, -1 where the shape is not one of this kernel's, or an error
 int launch_tree_attention_tc(const TreeAttnArgs& a, cudaStream_t st) {
-  if (a.ks || a.bs % 64 || a.window > 0 || a.softcap > 0.f || !(a.scale > 0.f) || (a.D != 64 && a.D != 128)) return -1;
+  if (a.bs % 64 || a.window > 0 || a.softcap > 0.f || !(a.scale > 0.f) || (a.D != 64 && a.D != 128)) return -1;
   if ((long long)a.num_blocks * a.hkv * a.bs > 0x7fffffffll) return -1;
-  if (a.D == 64) return a.form == 2 ? launch<1, 2>(a, st) : launch<1, 1>(a, st);
-  return a.form == 2 ? launch<2, 2>(a, st) : launch<2, 1>(a, st);
+  if (a.ks) {
+    if (a.D != 128 || ((reinterpret_cast<uintptr_t>(a.ks) | reinterpret_cast<uintptr_t>(a.vs)) & 15)) return -1;
+    return a.form == 2 ? launch<2, 2, true, false>(a, st) : launch<2, 2, true, true>(a, st);
+  }
+  if (a.D == 64) return a.form == 2 ? launch<1, 2, false, false>(a, st) : launch<1, 1, false, false>(a, st);
+  return a.form == 2 ? launch<2, 2, false, false>(a, st) : launch<2, 1, false, false>(a, st);
 }
 
 }  // namespace xft

@@ -92,11 +92,11 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
     return mask, positions
 
 
-def _plan(B, hkv, rows, D, max_kv, tensor):
+def _plan(B, hkv, rows, D, max_kv, tensor, int8=False):
     """(form, slices that the keys are cut into): the kernel of csrc/kernels/tree_attention_sm100.cu with one or two tiles of 128 rows per
     CTA, or (form 0) that of tree_attention.cu."""
     form = 0 if not tensor else 1 if rows <= 128 else 2
-    keys, tall, slots = ((32 if D == 256 else 64), 64, 296) if not form else (128, 128 * form, 296 // form)
+    keys, tall, slots = ((32 if D == 256 else 64), 64, 296) if not form else (128, 128 * form, 148 if int8 else 296 // form)
     ctas = B * hkv * -(-rows // tall)
     tiles = -(-max_kv // keys)
     most = max(1, min(tiles // (1 if form else 4), 64))
@@ -121,6 +121,8 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     if q.dtype is not torch.bfloat16 or D not in (64, 128, 256) or kc.dtype is not (torch.bfloat16 if ks is None else torch.int8):
         raise N.KernelError(f"tree_attention: bf16 queries over a bf16 or int8 cache with heads of 64, 128 or 256, not {q.dtype} over {kc.dtype} "
                             f"with {D}")
+    if (kc.data_ptr() | vc.data_ptr()) % 16:
+        raise N.KernelError("tree_attention: caches start on 16 bytes")
     q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
     mask = mask if mask.is_contiguous() else mask.contiguous()
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
@@ -131,7 +133,8 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
         return out
     ws = N.Workspace.get(dev)
     form, n = _plan(B, hkv, most * group, D, longest,
-                    ks is None and D <= 128 and bs % 64 == 0 and window == 0 and softcap == 0 and scale > 0 and nb * hkv * bs < 2 ** 31)
+                    (D == 128 or D == 64 and ks is None) and bs % 64 == 0 and window == 0 and softcap == 0 and scale > 0
+                    and nb * hkv * bs < 2 ** 31 and (_ptr(ks) | _ptr(vs)) % 16 == 0, ks is not None)
     part = torch.empty(T * hq * n * (D + 2), dtype=torch.float32, device=dev) if n > 1 else None
     po = _ptr(part)
     a = ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), _ptr(ks), _ptr(vs), block_table.data_ptr(), cu.data_ptr(),
