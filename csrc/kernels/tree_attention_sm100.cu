@@ -1,5 +1,5 @@
-// Attention of the nodes of trees of drafted tokens on the 5th-generation tensor cores: bf16 cache in blocks of a multiple of 64, heads of
-// 64 or 128 (int8 cache: 128), no window and no cap (those: tree_attention.cu, where the formula is).
+// Attention of the nodes of trees of drafted tokens on the 5th-generation tensor cores: caches in blocks of a multiple of 64, heads of
+// 64, 128 or 256 (int8: 128).  The formula, and the kernel for what is left: tree_attention.cu.
 //
 // The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile (two CTAs per
 // SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of 128 keys
@@ -27,20 +27,22 @@ int encode_tensor_map(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t
 
 namespace {
 
-constexpr int kTgKeys = 128, kTgRows = 128;
+constexpr int kTgRows = 128;
 
 // G groups of four softmax warps and heads of 64 * H; I8: int8 cache.  The groups have a tile of rows each, or (TURNS) take turns at the
 // key tiles of one.
 template <int H, int G, bool I8, bool TURNS>
 struct TgShape {
+  static constexpr int kKeys = H == 4 ? 64 : 128;        // of a tile
   static constexpr int R = TURNS ? 1 : G;                // row tiles
   static constexpr int kLead = TURNS ? G : 1;            // S of so many tiles is ahead of P V
-  static constexpr int kHalf = kTgKeys * 128;            // 64 features of a tile's 128 rows
-  static constexpr int kTile = H * kHalf;
-  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : R == 1 ? 4 / H : 10 / H;       // 64 KB (two CTAs an SM), 160 KB
-  static constexpr int kRaw = I8 ? (TURNS ? 3 : 5) : 0, kRawTile = kTgKeys * 128;                    // codes as they come
-  static constexpr int kScales = I8 ? 4 : 0, kScaleBytes = 2 * kTgKeys * 4;            // of a tile's keys and values
-  static constexpr int kSmem = (R + kStages) * kTile + kRaw * kRawTile + kScales * kScaleBytes + 1024;
+  static constexpr int kQHalf = kTgRows * 128, kHalf = kKeys * 128;          // 64 features of a tile's rows
+  static constexpr int kQTile = H * kQHalf, kTile = H * kHalf;
+  static constexpr int kTmem = H == 4 ? 512 : 256 * G;   // columns: of a group S, whose first half becomes P, and 128 behind it O
+  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : R == 1 ? 4 / H : 10 / H;         // 64 KB (two CTAs an SM), 160 KB
+  static constexpr int kRaw = I8 ? (TURNS ? 3 : 5) : 0, kRawTile = kKeys * 128;                    // codes as they come
+  static constexpr int kScales = I8 ? 4 : 0, kScaleBytes = 2 * kKeys * 4;            // of a tile's keys and values
+  static constexpr int kSmem = R * kQTile + kStages * kTile + kRaw * kRawTile + kScales * kScaleBytes + 1024;
   static constexpr int kThreads = 128 + 128 * G + (I8 ? 128 : 0);
   static constexpr int kPerSm = G == 1 ? 2 : 1;
 };
@@ -112,15 +114,28 @@ __device__ __forceinline__ uint32_t tg_sees(const uint32_t* m, int first, int ct
   return __funnelshift_r(word(o >> 5), word((o >> 5) + 1), o & 31);
 }
 
-template <int H, int G, bool I8, bool TURNS>
+// Of the same bits those that a window leaves: `pos` is the node's position, `at` the positions of the sequence's nodes
+__device__ __forceinline__ uint32_t tg_window(uint32_t sees, int first, int ctx, int pos, const int* at, int window, int keep) {
+  auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
+  const uint32_t context = below(ctx - first);
+  sees &= ~context | ~below(pos - window + 1 - first) | below(keep - first);
+  for (uint32_t rest = sees & ~context; rest; rest &= rest - 1) {
+    const int i = __ffs(rest) - 1, k = at[first + i - ctx];
+    if (!((long long)pos - k < window || k < keep)) sees &= ~(1u << i);
+  }
+  return sees;
+}
+
+// EXT: windows with kept first keys (only tiles with a visible key are visited), and caps on the scores
+template <int H, int G, bool I8, bool TURNS, bool EXT>
 __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H, G, I8, TURNS>::kPerSm)
     tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs p) {
   using S = TgShape<H, G, I8, TURNS>;
-  constexpr int D = 64 * H, ST = S::kStages, R = S::R, L = S::kLead;
+  constexpr int D = 64 * H, ST = S::kStages, R = S::R, L = S::kLead, KT = S::kKeys, NC = KT / 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                                    // R tiles
-  uint8_t* sT = smem + R * S::kTile;                     // ring: keys and values of the tiles in turn
+  uint8_t* sT = smem + R * S::kQTile;                    // ring: keys and values of the tiles in turn
   uint8_t* sRaw = sT + ST * S::kTile;                    // I8: ring of codes, in the same order
   float* s_scales = reinterpret_cast<float*>(sRaw + S::kRaw * S::kRawTile);           // I8: ring of tiles' scales
   __shared__ uint64_t raw_full[S::kRaw + 1], raw_empty[S::kRaw + 1], c_full[S::kScales + 1], c_empty[S::kScales + 1];
@@ -144,7 +159,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
     tma_prefetch_desc(&tmV);
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base_s, 256 * G);                   // of a group: S, whose first half becomes P, and O
+    tmem_alloc(&tmem_base_s, S::kTmem);
     tmem_relinquish();
   }
   grid_dep_launch();
@@ -154,9 +169,19 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
   const int heads = tree_heads(p, kvh, h0), rows = s.n * heads;
   const int n_rt = (p.max_q * p.group + R * kTgRows - 1) / (R * kTgRows);
   const int row0 = (blockIdx.x % n_rt) * (R * kTgRows), slice = blockIdx.x / n_rt;
-  const int all = (s.kv + kTgKeys - 1) / kTgKeys, per = (all + p.nsplit - 1) / p.nsplit;
+  // tiles: those of the kept first keys, then those from the first key of the widest window
+  int lo = 0, n_keep = 0;
+  if (EXT && p.window > 0) {
+    int at = 0x7fffffff;
+    for (int i = lane; i < s.n; i += 32) at = min(at, p.positions[s.q0 + i]);
+    at = __reduce_min_sync(0xffffffffu, at);
+    lo = max(0, (int)min((long long)at - p.window + 1, (long long)s.ctx)) / KT;
+    n_keep = min((min(p.keep, s.kv) + KT - 1) / KT, lo);
+  }
+  const int all = n_keep + (s.kv + KT - 1) / KT - lo, per = (all + p.nsplit - 1) / p.nsplit;
   const int t0 = min(all, slice * per), nt = row0 < rows ? min(all, t0 + per) - t0 : 0;
-  const int tail = s.ctx / kTgKeys;                      // from this tile on there are keys that are not the context's
+  auto tile_at = [&](int j) -> int { return EXT && t0 + j >= n_keep ? t0 + j - n_keep + lo : t0 + j; };
+  const int tail = s.ctx / KT;                           // from this tile on there are keys that are not the context's
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
@@ -198,32 +223,32 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         Ring ring{0, 1};
         // one tile of keys or values, in the order that the products take them
         auto load = [&](int j, bool v) -> bool {
-          int at[2];
-          for (int i = 0; i < 2; ++i) {                  // past the last keys they are read again
-            const int piece = min(2 * (t0 + j) + i, n_pieces - 1), first = piece * 64;
+          int at[KT / 64];
+          for (int i = 0; i < KT / 64; ++i) {            // past the last keys they are read again
+            const int piece = min(KT / 64 * tile_at(j) + i, n_pieces - 1), first = piece * 64;
             at[i] = (tree_block(p, b, first / p.bs) * p.hkv + kvh) * p.bs + first % p.bs;
           }
           if constexpr (I8) {
             if (!v) {
               const int cs = j % S::kScales;
               if (!mbar_wait(&c_empty[cs], (j / S::kScales & 1) ^ 1, p.status, XFT_ERR_WAIT_EMPTY)) return false;
-              float* to = s_scales + cs * 2 * kTgKeys;
+              float* to = s_scales + cs * 2 * KT;
               mbar_expect_tx(&c_full[cs], S::kScaleBytes);
-              for (int i = 0; i < 2; ++i) {
+              for (int i = 0; i < KT / 64; ++i) {
                 bulk_load(to + i * 64, p.ks + at[i], 256, &c_full[cs]);
-                bulk_load(to + kTgKeys + i * 64, p.vs + at[i], 256, &c_full[cs]);
+                bulk_load(to + KT + i * 64, p.vs + at[i], 256, &c_full[cs]);
               }
             }
             if (!mbar_wait(&raw_empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY)) return false;
             mbar_expect_tx(&raw_full[ring.s], S::kRawTile);
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < KT / 64; ++i)
               tma_load_2d(sRaw + ring.s * S::kRawTile + i * 8192, v ? &tmV : &tmK, &raw_full[ring.s], 0, at[i], kEvictNormal);
             ring.next(S::kRaw);
           } else {
             if (!mbar_wait(&empty[ring.s], ring.ph, p.status, XFT_ERR_WAIT_EMPTY)) return false;
             uint8_t* to = sT + ring.s * S::kTile;
             mbar_expect_tx(&full[ring.s], S::kTile);
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < KT / 64; ++i)
               for (int h = 0; h < H; ++h)
                 tma_load_2d(to + h * S::kHalf + i * 8192, v ? &tmV : &tmK, &full[ring.s], h * 64, at[i], kEvictNormal);
             ring.next(ST);
@@ -237,17 +262,17 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA issuer
       if (nt > 0 && elect_one()) {
-        constexpr uint32_t IDESC_S = umma_idesc(128, kTgKeys, 1, 1, 1);
+        constexpr uint32_t IDESC_S = umma_idesc(128, KT, 1, 1, 1);
         constexpr uint32_t IDESC_O = umma_idesc(128, D, 1, 1, 1) | (1u << 16);       // B = V, MN-major
         Ring ring{0, 0};
         bool ok = mbar_wait(&q_full, 0, p.status, XFT_ERR_WAIT_FULL);
         auto scores = [&](int g, int st) {
-          const uint64_t qd = umma_desc_k128(smem_u32(sQ + (TURNS ? 0 : g) * S::kTile)), kd = umma_desc_k128(smem_u32(sT + st * S::kTile));
+          const uint64_t qd = umma_desc_k128(smem_u32(sQ + (TURNS ? 0 : g) * S::kQTile)), kd = umma_desc_k128(smem_u32(sT + st * S::kTile));
           tcgen05_fence_after();
 #pragma unroll
           for (int k = 0; k < 4 * H; ++k) {
-            const uint32_t off = ((k >> 2) * S::kHalf + (k & 3) * 32) / 16;
-            umma_bf16(tmem_base + g * 256, qd + off, kd + off, IDESC_S, k > 0);
+            const uint32_t q_off = ((k >> 2) * S::kQHalf + (k & 3) * 32) / 16, k_off = ((k >> 2) * S::kHalf + (k & 3) * 32) / 16;
+            umma_bf16(tmem_base + g * 256, qd + q_off, kd + k_off, IDESC_S, k > 0);
           }
           tcgen05_commit(&s_full[g]);
         };
@@ -266,7 +291,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
           const bool more = j + L < nt;
           if (more) ring.next(ST);
           ok = mbar_wait(&full[vr.s], vr.ph, p.status, XFT_ERR_WAIT_FULL);
-          if (!I8 && ok && t0 + j >= tail) {
+          if (!I8 && ok && tile_at(j) >= tail) {
             mbar_arrive(&v_here);
             ok = mbar_wait(&v_clean, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL);
           }
@@ -280,12 +305,12 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
             if (!ok) break;
             tcgen05_fence_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, j >= L || k > 0);
+            for (int k = 0; k < KT / 32; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, j >= L || k > 0);
             ok = mbar_wait(&p_full[g], ph, p.status, XFT_ERR_WAIT_TMEM);
             if (!ok) break;
             tcgen05_fence_after();
 #pragma unroll
-            for (int k = 4; k < 8; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, 1);
+            for (int k = KT / 32; k < KT / 16; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, 1);
             if (g == g1 - 1) tcgen05_commit(&empty[vr.s]);
             if (more) {                                  // the next S goes over P, behind the product that reads P
               if (g == g0) ok = mbar_wait(&full[kr.s], kr.ph, p.status, XFT_ERR_WAIT_FULL);
@@ -300,7 +325,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       }
     } else if (!I8) {
       // ------------------------------------------------------------------ values that no node sees (codes are finite, their scales below)
-      if (t0 + nt > tail && nt > 0) {
+      if (nt > 0 && tile_at(nt - 1) >= tail) {
         uint32_t seen[kTreeWords * 2] = {};
         const uint32_t* m = reinterpret_cast<const uint32_t*>(p.mask + (long long)s.q0 * p.words);
         for (int i = lane; i < s.n; i += 32)
@@ -320,16 +345,16 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         const int st = ring.s;
         const uint32_t ph = ring.ph;
         ring.next(ST);
-        if (t0 + j < tail) continue;
+        if (tile_at(j) < tail) continue;
         // (these warps do not hold the ring back, so they ask the issuer which round it is in)
         if (!mbar_wait(&v_here, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL)) break;
-        const int key = (warp - 2) * 64 + lane * 2;      // two keys a lane
-        const int k0 = (t0 + j) * kTgKeys;
+        const int key = (warp - 2) * (KT / 2) + lane * (KT / 64);            // one or two keys a lane
+        const int k0 = tile_at(j) * KT;
         const uint32_t sees = tg_sees(s_union, k0 + (key & ~31), s.ctx, s.n) >> (key & 31);
         if (!mbar_wait(&full[st], ph, p.status, XFT_ERR_WAIT_FULL)) break;
         uint8_t* v = sT + st * S::kTile;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < KT / 64; ++e)
           if (!(sees >> e & 1))
 #pragma unroll
             for (int c = 0; c < 8 * H; ++c)
@@ -350,21 +375,24 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
     const long long at = (long long)(s.q0 + node) * p.hq + h;
     if (nt > 0 && (!TURNS || g == 0)) {
       // this row of queries in the order that the product reads: 16-byte pieces exchanged with the row's low bits
-      uint8_t* to = sQ + tile * S::kTile + r * 128;
+      uint8_t* to = sQ + tile * S::kQTile + r * 128;
       uint4 v[8];
 #pragma unroll
       for (int half = 0; half < H; ++half) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c] = mine ? *reinterpret_cast<const uint4*>(p.q + at * D + half * 64 + c * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(to + half * S::kHalf + ((c ^ (r & 7)) << 4)) = v[c];
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(to + half * S::kQHalf + ((c ^ (r & 7)) << 4)) = v[c];
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
     }
     const uint32_t sa = tmem_base + g * 256 + (uint32_t(qd * 32) << 16), oa = sa + 128;
-    const float scale = p.scale * kTreeLog2e;
+    const bool caps = EXT && p.softcap > 0.f;
+    const float scale = caps ? 1.f : p.scale * kTreeLog2e;           // (capped scores are in octaves already)
+    const float cap = p.softcap * kTreeLog2e, inv_cap = caps ? p.scale / p.softcap : 0.f;
+    const int pos = EXT && p.window > 0 && nt > 0 ? p.positions[s.q0 + node] : 0;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     const int first = TURNS ? g : 0;                     // of this group's tiles
@@ -372,7 +400,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
     for (int j = first; j < nt; j += L) {
       const int cs = j % kRing;
       const uint32_t ph = (TURNS ? j / G : j) & 1;
-      const float* scales = s_scales + cs * 2 * kTgKeys;
+      const float* scales = s_scales + cs * 2 * KT;
       if (I8 && !mbar_wait(&c_full[cs], j / kRing & 1, p.status, XFT_ERR_WAIT_FULL)) { ok = false; break; }
       if (!mbar_wait(&s_full[g], ph, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
       tcgen05_fence_after();
@@ -380,14 +408,14 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         if (lane == 0) { mbar_arrive(&p_half[g]); mbar_arrive(&p_full[g]); if (I8) mbar_arrive(&c_empty[cs]); }
         continue;
       }
-      uint32_t x[4][32];
+      uint32_t x[NC][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(sa + 32 * c, x[c]);
+      for (int c = 0; c < NC; ++c) tmem_ld32(sa + 32 * c, x[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tg_ld_wait32(x[c]);
+      for (int c = 0; c < NC; ++c) tg_ld_wait32(x[c]);
       if constexpr (I8) {                                // a key's scale belongs to its scores
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 16) {
             float4 f[4];
@@ -402,20 +430,59 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
             }
           }
       }
-      uint32_t sees[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-      if (t0 + j >= tail) {
+      if (caps) {                                        // cap tanh(z), z = score / cap
+        float far = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            x[c][i] = __float_as_uint(__uint_as_float(x[c][i]) * inv_cap);
+            far = fmaxf(far, fabsf(__uint_as_float(x[c][i])));
+          }
+        if (__all_sync(0xffffffffu, far <= 1.f)) {
+          // tanh(z) / z as a polynomial in z^2, minimax on [0, 1] (off by less than 2e-7), away from the exponentials' unit
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float z = __uint_as_float(x[c][i]), y = z * z;
+              float q = 0.0010410224785f;
+              q = fmaf(q, y, -0.0062033790164f);
+              q = fmaf(q, y, 0.020289981738f);
+              q = fmaf(q, y, -0.053457029164f);
+              q = fmaf(q, y, 0.13325203957f);
+              q = fmaf(q, y, -0.33332839608f);
+              q = fmaf(q, y, 0.99999994040f);
+              x[c][i] = __float_as_uint(z * cap * q);
+            }
+        } else {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              x[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(fminf(__uint_as_float(x[c][i]) * 2.8853900817779268f, 120.f))));
+        }
+      }
+      const int k0 = tile_at(j) * KT;
+      uint32_t sees[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) sees[c] = 0xffffffffu;
+      const bool ends = k0 + KT > s.ctx;
+      if (ends || (EXT && p.window > 0)) {
         const uint32_t* bits = reinterpret_cast<const uint32_t*>(p.mask + (long long)(s.q0 + node) * p.words);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sees[c] = tg_sees(bits, (t0 + j) * kTgKeys + 32 * c, s.ctx, s.n);
+        for (int c = 0; c < NC; ++c) {
+          if (ends) sees[c] = tg_sees(bits, k0 + 32 * c, s.ctx, s.n);
+          if (EXT && p.window > 0) sees[c] = tg_window(sees[c], k0 + 32 * c, s.ctx, pos, p.positions + s.q0, p.window, p.keep);
+          if (__any_sync(0xffffffffu, sees[c] != 0xffffffffu))
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(sees[c] >> i & 1)) x[c][i] = 0xff800000u;
+            for (int i = 0; i < 32; ++i)
+              if (!(sees[c] >> i & 1)) x[c][i] = 0xff800000u;
         }
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = tg_max3(top[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
       const float mx = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale);
@@ -439,12 +506,12 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       const float off = m == -INFINITY ? 0.f : -m;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < NC; ++c) {
         uint32_t w[16];
         float4 f[I8 ? 8 : 1];                            // the values' scales
         if constexpr (I8)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float4*>(scales + kTgKeys + 32 * c + 4 * i);
+          for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float4*>(scales + KT + 32 * c + 4 * i);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float2 e = tg_fma2(make_float2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), make_float2(scale, scale), make_float2(off, off));
@@ -461,7 +528,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
           w[i >> 1] = I8 ? tg_pack(e.x, e.y) : tg_round(e.x, e.y);           // (int8: the other instructions are what is short)
         }
         tmem_st16(sa + 16 * c, w);
-        if (c == 1) {                                    // the product may begin with the first 64 keys
+        if (c == NC / 2 - 1) {                           // the product may begin with the first half of the keys
           tmem_st_wait();
           tcgen05_fence_before();
           __syncwarp();
@@ -553,36 +620,40 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_dealloc(tmem_base, 256 * G);
+    tmem_dealloc(tmem_base, S::kTmem);
   }
 }
 
-template <int H, int G, bool I8, bool TURNS>
+template <int H, int G, bool I8, bool TURNS, bool EXT>
 int launch(const TreeAttnArgs& a, cudaStream_t st) {
   using S = TgShape<H, G, I8, TURNS>;
   CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)a.num_blocks * a.hkv * a.bs;
   const uint32_t size = I8 ? 1 : 2;
   if (encode_tensor_map(&tmK, a.kc, rows, a.D, a.D, 64, size) || encode_tensor_map(&tmV, a.vc, rows, a.D, a.D, 64, size)) return -4;
-  auto k = tree_attention_tc_kernel<H, G, I8, TURNS>;
+  auto k = tree_attention_tc_kernel<H, G, I8, TURNS, EXT>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return 3000 + (int)cudaGetLastError();
   const int n_rt = (a.max_q * a.group + S::R * kTgRows - 1) / (S::R * kTgRows);
   const cudaError_t e = launch_pdl(k, dim3(n_rt * a.nsplit, a.hkv, a.B), dim3(S::kThreads), (size_t)S::kSmem, st, tmK, tmV, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
+template <bool EXT>
+int pick(const TreeAttnArgs& a, cudaStream_t st) {
+  if (a.ks) return a.form == 2 ? launch<2, 2, true, false, EXT>(a, st) : launch<2, 2, true, true, EXT>(a, st);
+  if (a.D == 64) return a.form == 2 ? launch<1, 2, false, false, EXT>(a, st) : launch<1, 1, false, false, EXT>(a, st);
+  if (a.D == 256) return launch<4, 1, false, false, EXT>(a, st);
+  return a.form == 2 ? launch<2, 2, false, false, EXT>(a, st) : launch<2, 1, false, false, EXT>(a, st);
+}
+
 }  // namespace
 
 // 0, -1 where the shape is not one of this kernel's, or an error
 int launch_tree_attention_tc(const TreeAttnArgs& a, cudaStream_t st) {
-  if (a.bs % 64 || a.window > 0 || a.softcap > 0.f || !(a.scale > 0.f) || (a.D != 64 && a.D != 128)) return -1;
+  if (a.bs % 64 || (!(a.scale > 0.f) && !(a.softcap > 0.f)) || (a.D != 64 && a.D != 128 && a.D != 256) || (a.D == 256 && a.form != 1)) return -1;
   if ((long long)a.num_blocks * a.hkv * a.bs > 0x7fffffffll) return -1;
-  if (a.ks) {
-    if (a.D != 128 || ((reinterpret_cast<uintptr_t>(a.ks) | reinterpret_cast<uintptr_t>(a.vs)) & 15)) return -1;
-    return a.form == 2 ? launch<2, 2, true, false>(a, st) : launch<2, 2, true, true>(a, st);
-  }
-  if (a.D == 64) return a.form == 2 ? launch<1, 2, false, false>(a, st) : launch<1, 1, false, false>(a, st);
-  return a.form == 2 ? launch<2, 2, false, false>(a, st) : launch<2, 1, false, false>(a, st);
+  if (a.ks && (a.D != 128 || ((reinterpret_cast<uintptr_t>(a.ks) | reinterpret_cast<uintptr_t>(a.vs)) & 15))) return -1;
+  return a.window > 0 || a.softcap > 0.f ? pick<true>(a, st) : pick<false>(a, st);
 }
 
 }  // namespace xft

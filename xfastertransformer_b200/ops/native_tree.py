@@ -79,8 +79,8 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
     parents = _i32(parents)
     cu, kv, B, most, _ = _arrays(cu_q, kv_lens, meta, dev)
     T, words = parents.numel(), max(1, -(-most // 64))
-    mask = torch.empty((T, words), dtype=torch.int64, device=dev)
-    positions = torch.empty(T, dtype=torch.int32, device=dev)
+    mask = parents.new_empty((T, words), dtype=torch.int64)
+    positions = torch.empty_like(parents)
     if T and B and most:
         ws = N.Workspace.get(dev)
         a = MASK_ARGS.pack(cu.data_ptr(), kv.data_ptr(), B, T, parents.data_ptr(), mask.data_ptr(), positions.data_ptr(), ws.status.data_ptr(),
@@ -95,8 +95,8 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
 def _plan(B, hkv, rows, D, max_kv, tensor, int8=False):
     """(form, slices that the keys are cut into): the kernel of csrc/kernels/tree_attention_sm100.cu with one or two tiles of 128 rows per
     CTA, or (form 0) that of tree_attention.cu."""
-    form = 0 if not tensor else 1 if rows <= 128 else 2
-    keys, tall, slots = ((32 if D == 256 else 64), 64, 296) if not form else (128, 128 * form, 148 if int8 else 296 // form)
+    form = 0 if not tensor else 1 if rows <= 128 or D == 256 else 2
+    keys, tall, slots = ((32 if D == 256 else 64), 64, 296) if not form else ((64 if D == 256 else 128), 128 * form, 148 if int8 or D == 256 else 296 // form)
     ctas = B * hkv * -(-rows // tall)
     tiles = -(-max_kv // keys)
     most = max(1, min(tiles // (1 if form else 4), 64))
@@ -132,14 +132,14 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     if not (T and B and most):
         return out
     ws = N.Workspace.get(dev)
-    form, n = _plan(B, hkv, most * group, D, longest,
-                    (D == 128 or D == 64 and ks is None) and bs % 64 == 0 and window == 0 and softcap == 0 and scale > 0
-                    and nb * hkv * bs < 2 ** 31 and (_ptr(ks) | _ptr(vs)) % 16 == 0, ks is not None)
-    part = torch.empty(T * hq * n * (D + 2), dtype=torch.float32, device=dev) if n > 1 else None
+    form, n = _plan(B, hkv, most * group, D, min(longest, window + keep_first + most + 256) if window else longest,
+                    (D == 128 or ks is None) and bs % 64 == 0 and (scale > 0 or softcap > 0) and nb * hkv * bs < 2 ** 31 and (_ptr(ks) | _ptr(vs)) % 16 == 0,
+                    ks is not None)
+    part = q.new_empty(T * hq * n * (D + 2), dtype=torch.float32) if n > 1 else None
     po = _ptr(part)
     a = ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), _ptr(ks), _ptr(vs), block_table.data_ptr(), cu.data_ptr(),
                        kv.data_ptr(), mask.data_ptr(), _ptr(positions), _ptr(sinks), po, po + T * hq * n * D * 4, ws.status.data_ptr(),
-                       block_table.stride(0), B, T, most, hq, hkv, group, q_off, D, bs, nb, block_table.shape[1], mask.shape[1], n, window,
+                       block_table.stride(0), B, T, most, hq, hkv, group, q_off, D, bs, nb, block_table.shape[1], mask.shape[1], n, min(window, 1 << 30),
                        keep_first, scale, softcap, form)
     rc = _lib().xft_tree_attention(a, _stream())
     if rc:
@@ -152,11 +152,11 @@ def _per_row(v, rows, dtype, dev):
     """(tensor or None, number): a parameter of every row, or one for all."""
     if not isinstance(v, torch.Tensor):
         return None, v
+    if v.dtype is dtype and v.numel() == rows and v.device == dev and v.is_contiguous():
+        return v, 0
     if v.numel() == 1 and rows != 1:
         v = v.reshape(1).expand(rows)
-    if v.dtype is not dtype or not v.is_contiguous() or v.device != dev:
-        v = v.to(device=dev, dtype=dtype).contiguous()
-    return v, 0
+    return v.to(device=dev, dtype=dtype).contiguous(), 0
 
 
 def sample(logits, temperature, top_k, top_p, min_p, uniform):
@@ -171,7 +171,7 @@ def sample(logits, temperature, top_k, top_p, min_p, uniform):
     if x.stride(1) != 1 and V > 1:
         x = x.contiguous()
     rows = x.shape[0]
-    out = torch.empty(rows, dtype=torch.int64, device=dev)
+    out = x.new_empty(rows, dtype=torch.int64)
     if rows:
         t, t0 = _per_row(temperature, rows, torch.float32, dev)
         k, k0 = _per_row(top_k, rows, torch.int32, dev)
@@ -209,9 +209,7 @@ def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table, pools, met
     tokens, sampled = (t if t.dtype is torch.int64 and t.is_contiguous() else t.long().contiguous() for t in (tokens, sampled))
     cu, kv, B, most, _ = _arrays(cu_q, kv_lens, meta, dev)
     T = tokens.numel()
-    emitted = torch.empty((B, most), dtype=torch.int64, device=dev)
-    path = torch.empty((B, most), dtype=torch.int32, device=dev)
-    count = torch.empty(B, dtype=torch.int32, device=dev)
+    emitted, path, count = tokens.new_empty((B, most)), parents.new_empty((B, most)), parents.new_empty(B)
     if B and most:
         if block_table is not None and block_table.stride(1) != 1:
             block_table = block_table.contiguous()
