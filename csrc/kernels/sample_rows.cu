@@ -18,9 +18,10 @@
 //      good to 2^-30 (two numbers in 32 bits carry it); the sums are two 32-bit atomics (one of 64 bits in shared memory is a loop: 20
 //      times slower).  What weighs less than 2^-48 of the largest is left out;
 //   2. the bins' sums, exchanged over the cluster; every CTA finds the bins where the limits and the token can lie;
-//   3. those bins' elements, or all up to there if that is what at most 2048 are, go to the first CTA, which sorts them, weighs them in 64
-//      bits and finds the place; one more such round for each limit whose elements are too many.  The others leave before the last.
-// What that does not settle (a bin of more than 2048 elements, as with equal logits, a limit among weights that are left out, logits of
+//   3. those bins' elements, or all up to there if those are at most 2048, go to the first CTA, which sorts them, weighs them in 64
+//      bits and finds the place; one more such round for each limit whose elements are too many.  A bin of more than 2048 is cut in 1024
+//      parts in the same way first.  The other CTAs leave before the last round.
+// What that does not settle (more than 2048 equal logits or nearly so, a limit among weights that are left out, logits of
 // which a bin is less than 32 bits resolve) the first CTA settles alone, digit by digit of the 64-bit number (image of the logit, ~index),
 // whose unsigned order is the row's.
 #include "ptx.cuh"
@@ -44,7 +45,7 @@ namespace {
 
 typedef unsigned long long u64;
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 1024, kSampleList = 2048;
+constexpr int kSampleBins = 1024, kSampleList = 2048, kSampleFirst = 1536;             // counts alone up to the last (bins come whole)
 constexpr float kSampleEdge = kSampleBins - 1.5f;        // from here on: the elements outside the bins
 constexpr int kSamplePer = 16;                           // bins an octave, or a logit
 constexpr int kSampleUnit = 27;                          // a weight's factor in its bin has so many bits behind the point
@@ -79,9 +80,10 @@ struct SampleLimits { int k; float p, least, u; };
 
 struct SampleShared {
   union {
-    struct { unsigned cnt[kSampleBins], lo[kSampleBins], hi[kSampleBins]; } own;       // this CTA's slice
+    struct { unsigned cnt[kSampleBins], lo[kSampleBins], hi[kSampleBins], zoom_cnt[kSampleBins]; u64 zoom_mass[kSampleBins]; } own;        // this CTA's
+                                                         // slice; the first CTA's: of one bin, cut into 1024
     u64 list[kSampleList];                               // the first CTA's, once the sums have been exchanged
-    u64 fine[kSampleBins];                               // place()
+    struct { unsigned lo[kSampleBins], hi[kSampleBins]; } fine;          // place()
   };
   u64 mass[kSampleBins];                                 // of the whole row
   unsigned cnt[kSampleBins];
@@ -92,7 +94,7 @@ struct SampleShared {
   double root[kSamplePer];                               // 2^(-i / 16)
   int above;
   unsigned n_list, at;
-  int what, from, to;                                    // the next round: see Round
+  int what, from, to, sub;                               // the next round: see Round
   u64 base;
 };
 
@@ -149,7 +151,7 @@ __device__ __noinline__ void place(const SampleRow& r, SampleShared& sh, bool by
   u64 prefix = 0, done_m = 0, done_c = 0;
   for (int bits = 0; bits < 64;) {
     const int take = min(10, 64 - bits), shift = 64 - bits - take;
-    for (int i = tid; i < kSampleBins; i += kSampleThreads) { sh.cnt[i] = 0; sh.fine[i] = 0; }
+    for (int i = tid; i < kSampleBins; i += kSampleThreads) { sh.cnt[i] = 0; sh.fine.lo[i] = sh.fine.hi[i] = 0; }
     __syncthreads();
     for (int i = tid; i < r.V; i += kSampleThreads) {
       const float v = r.at(i);
@@ -158,11 +160,15 @@ __device__ __noinline__ void place(const SampleRow& r, SampleShared& sh, bool by
       const int bin = kSampleBins - 1 - (int)((c >> shift) & ((1u << take) - 1));         // descending order: bin 0 is the first
       atomicAdd(&sh.cnt[bin], 1u);
       const u64 m = r.mass(r.weight(v));
-      if (m) atomicAdd(&sh.fine[bin], m);
+      if (m) {
+        const unsigned add = (unsigned)m, old = atomicAdd(&sh.fine.lo[bin], add);
+        const unsigned up = (unsigned)(m >> 32) + (old + add < add);
+        if (up) atomicAdd(&sh.fine.hi[bin], up);
+      }
     }
     __syncthreads();
     const unsigned c0 = sh.cnt[2 * tid], c1 = sh.cnt[2 * tid + 1];
-    const u64 m0 = sh.fine[2 * tid], m1 = sh.fine[2 * tid + 1];
+    const u64 m0 = (u64)sh.fine.hi[2 * tid] << 32 | sh.fine.lo[2 * tid], m1 = (u64)sh.fine.hi[2 * tid + 1] << 32 | sh.fine.lo[2 * tid + 1];
     u64 bc, bm, tc, tm;
     scan(c0 + c1, sh.warps, bc, tc);
     scan(m0 + m1, sh.warps, bm, tm);
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     return v + 0.f;
   };
   r.inv_t = 1.0 / (double)t;
-  const bool greedy = !(t > 0.f), counts = lim.k > 0 && lim.k <= kSampleList, both = lim.k > kSampleList;       // counts: all of the first k are sorted
+  const bool greedy = !(t > 0.f), counts = lim.k > 0 && lim.k <= kSampleFirst, both = lim.k > kSampleFirst;     // counts: all of the first k are sorted
   const double per_logit = kSamplePer * 1.4426950408889634 * r.inv_t;
   float kh = counts ? (float)kSamplePer : (float)per_logit;
   const float kl = counts ? 0.f : (float)(per_logit - (double)kh);
@@ -439,21 +445,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   auto whole = [&](float p) { return __fsub_rn(__fadd_rn(p, kMagic), kMagic); };
   float ref = -INFINITY;                                 // where the bins begin
   bool above = false;                                    // an element was in front of them
+  // distance from the middle of x's bin: in grid units x is p + rest.  Its order in a bin is that of the logits too
+  auto beside = [&](float x, float p, float mid) -> float {
+    const float rest = fmaf(x, kl, fmaf(x, kh, -p));
+    return __fadd_rn(__fsub_rn(p, __fsub_rn(mid, kMagic)), rest);
+  };
+  auto part_of = [](float off) -> int { return max(0, min(kSampleBins - 1, (int)((0.5f - off) * kSampleBins))); };
+  int zoom = -1;                                         // >= 0: only elements of this bin are counted, in 1024 parts of it
   auto put = [&](float x) {
     const float p = grid(x), d = ref - p;
     if (!(d < kSampleEdge)) return;
     const float mid = __fadd_rn(p, kMagic);
-    const int n = (int)(__float_as_uint(__fadd_rn(ref, kMagic)) - __float_as_uint(mid));
+    int n = (int)(__float_as_uint(__fadd_rn(ref, kMagic)) - __float_as_uint(mid));
     if (n < 0) { above = true; return; }
+    if (zoom >= 0 && n != zoom) return;
     if (!counts) {
-      // x in grid units is p + rest; off: its distance from the bin's middle
-      const float rest = fmaf(x, kl, fmaf(x, kh, -p)), off = __fadd_rn(__fsub_rn(p, __fsub_rn(mid, kMagic)), rest);
+      const float off = beside(x, p, mid);
+      if (zoom >= 0) n = part_of(off);
       // 2^(off / 16) - 1, |off| <= 1/2: (ln2 / 16)^i / i! off^i
       const float q = off * fmaf(off, fmaf(off, fmaf(off, 1.46760905e-7f, 1.35507817e-5f), 9.38384793e-4f), 4.33216988e-2f);
       const unsigned w = __float_as_uint(fmaf(q, (float)(1 << kSampleUnit), kMagic)) - 0x4b400000u + (1u << kSampleUnit);
       atomicAdd(&sh.own.lo[n], w & 0x3fffu);
       atomicAdd(&sh.own.hi[n], w >> 14);
-      if (!both) return;
+      if (!both && zoom < 0) return;
     }
     atomicAdd(&sh.own.cnt[n], 1u);
   };
@@ -673,6 +687,61 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     todo = next(kDone);
   }
   while (todo.x > kAlone) {
+    // a bin of too many elements: its 1024 parts are counted as the bins were, and the part is taken that the place lies in
+    int part = -1;
+    if ((todo.x == kFirst || todo.x == kShare || todo.x == kPick) && todo.y == todo.z && sh.cnt[todo.y] > kSampleList) {
+      __syncthreads();
+      clear();
+      __syncthreads();
+      zoom = todo.y;
+      ref = row_ref;                                     // (the row's bins)
+      for (int j = tid; j < ng; j += kAhead * kSampleThreads) {
+        float4 v[kAhead];
+        ahead(j, v);
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) put4(v[e]);
+      }
+      cluster_barrier<C>();
+      for (int i = tid; i < kShareBins; i += kSampleThreads) {
+        const int n = rank * kShareBins + i;
+        unsigned c = 0;
+        u64 w = 0;
+#pragma unroll
+        for (int from = 0; from < C; ++from) {
+          c += ld_peer(&sh.own.cnt[n], from);
+          w += ((u64)ld_peer(&sh.own.hi[n], from) << 14) + ld_peer(&sh.own.lo[n], from);
+        }
+        st_peer(&sh.own.zoom_cnt[n], 0, c);
+        st_peer(&sh.own.zoom_mass[n], 0, __double2ull_rn(middle(todo.y - lead, shift - kSampleUnit) * (double)w));
+      }
+      cluster_barrier<C>();
+      if (rank == 0) {
+        u64 m2[2], u2[2], b2, all2;
+        unsigned c2[2], f2;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { m2[e] = sh.own.zoom_mass[2 * tid + e]; c2[e] = sh.own.zoom_cnt[2 * tid + e]; }
+        scan2(c2[0] + c2[1], m2[0] + m2[1], sh, f2, b2, all2);
+        unsigned k2[2] = {f2 + c2[0], f2 + c2[0] + c2[1]};
+        u2[0] = sh.base + b2 + m2[0]; u2[1] = u2[0] + m2[1];
+        u64 front, want = todo.x == kShare ? max(reach(lim.p, kept), (u64)1) : exceed(lim.u, kept);
+        int s2;
+        if (todo.x == kFirst) s2 = bin_of(sh, k2, c2, [&](unsigned c) { return c >= (unsigned)(lim.k - todo.w); }, front);
+        else s2 = bin_of(sh, u2, m2, [&](u64 c) { return todo.x == kShare ? c >= want : c > want; }, front);
+        if (s2 == kSampleBins) {                         // (rounding: the place is the bin's last element's)
+          if (tid == kSampleThreads - 1) sh.found[0] = k2[1];
+          __syncthreads();
+          const unsigned every = (unsigned)sh.found[0];
+          s2 = bin_of(sh, k2, c2, [&](unsigned c) { return c >= every; }, front);
+        }
+        if (2 * tid <= s2 && s2 < 2 * tid + 2) { sh.base = u2[s2 & 1] - m2[s2 & 1]; sh.found[0] = k2[s2 & 1] - c2[s2 & 1]; }
+        __syncthreads();
+        todo.w += (int)sh.found[0];
+        __syncthreads();
+        if (tid < C) st_peer(&sh.sub, tid, (uint32_t)s2);
+      }
+      cluster_barrier<C>();
+      part = sh.sub;
+    }
     // the bins' elements go to the first CTA, the others' by way of a list of their own
     const float from = row_ref - (float)todo.z, to_grid = row_ref - (float)todo.y;
     for (int j = tid; j < ng; j += kAhead * kSampleThreads) {
@@ -687,6 +756,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
           if (!(p >= from - 0.5f && p <= to_grid + 0.5f)) continue;
           const float n = whole(p);
           if (!(n >= from && n <= to_grid)) continue;
+          if (part >= 0 && part_of(beside(x, p, __fadd_rn(p, kMagic))) != part) continue;
           const unsigned to = atomicAdd(&sh.n_list, 1u);
           if (to < kSampleList) sh.list[to] = element(x, 4 * (g0 + j + b * kSampleThreads) - skew + e);
         }
@@ -705,7 +775,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
       }
     }
     cluster_barrier<C>();
-    if (rank != 0 && (todo.x == kAll || todo.x == kPick)) return;          // (the last round, or the first CTA goes on alone)
+    if (rank != 0 && (todo.x == kAll || todo.x == kPick)) return;          // (the last round; what is still too much the first CTA settles alone)
     const bool last = todo.x == kAll || todo.x == kPick;
     if (rank == 0) {
       const int n = (int)sh.n_list;
@@ -723,7 +793,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
           kept = sh.kept;
         } else {
           sort_list(sh.list, n);
-          kept = n <= kSampleThreads ? settle(ListMasses<1, false>(r, sh, n, base), todo) : settle(ListMasses<4, false>(r, sh, n, base), todo);
+          kept = n <= kSampleThreads ? settle(ListMasses<1, false>(r, sh, n, base), todo)
+                                     : settle(ListMasses<4, false>(r, sh, n, base), todo);
         }
         todo = last ? make_int4(kDone, 0, 0, 0) : next(todo.x);
       }
@@ -781,8 +852,8 @@ extern "C" int xft_sample_rows(const char* packed, cudaStream_t st) {
   // CTAs of a row: as many as find room at a time, two an SM; their serial steps cost each row C times.  us, C = 8 / 4 / 2 / 1: see below
   const int fit = a.rows <= 37 ? 8 : a.rows <= 74 ? 4 : a.rows <= 148 || a.V > 65536 ? 2 : 1;
   const int c = a.V <= 4096 ? 1 : fit;
-  // slices of up to 19 Ki elements are held: two CTAs of them share an SM
-  const bool held = a.V <= c * 19456;
+  // slices of up to 18 Ki elements are held: two CTAs of them share an SM
+  const bool held = a.V <= c * 18432;
   if (c == 8) return held ? launch<8, true>(a, st) : launch<8, false>(a, st);
   if (c == 4) return held ? launch<4, true>(a, st) : launch<4, false>(a, st);
   if (c == 2) return held ? launch<2, true>(a, st) : launch<2, false>(a, st);

@@ -273,6 +273,26 @@ def test_all_logits_equal(V):
         assert torch.equal(ops.sample(x.cuda(), 1.0, k, p, 0.0, u.cuda()).cpu(), R.sample(x, 1.0, k, p, 0.0, u))
 
 
+@pytest.mark.parametrize("V,width", [(20000, 0.02), (151936, 0.05), (200003, 0.3), (100000, 1e-6)])
+def test_crowded_logits(V, width):
+    g = torch.Generator().manual_seed(V)
+    x = 5 + width * torch.randn(14, V, generator=g)
+    u = torch.rand(14, generator=g)
+    for T, k, p, m in ((1.0, 0, 1.0, 0.0), (2.5, 0, 0.6, 0.0), (0.8, 5000, 0.9, 0.0), (1.3, V // 2, 1.0, 0.0), (0.02, 0, 0.7, 0.3), (1.0, 700, 0.5, 0.0)):
+        assert torch.equal(ops.sample(x.cuda(), T, k, p, m, u.cuda()).cpu(), R.sample(x, T, k, p, m, u)), (T, k, p, m)
+
+
+@pytest.mark.parametrize("T", [1e-6, 1e-4, 2e-3, 0.02])
+def test_low_temperatures(T):
+    g = torch.Generator().manual_seed(8)
+    x = 3 * torch.randn(20, 50257, generator=g)
+    x[::2] = (200 * x[::2]).round() / 200                  # largest logits that come more than once, or nearly
+    x[3, :9000] = x[3].max()
+    u = torch.rand(20, generator=g)
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.1), (3, 0.5, 0.0), (0, 1.0, 0.5)):
+        assert torch.equal(ops.sample(x.cuda(), T, k, p, m, u.cuda()).cpu(), R.sample(x, T, k, p, m, u)), (k, p, m)
+
+
 def test_frequencies():
     w = torch.tensor([0.5, 0.25, 0.125, 0.125])
     n = 4096
