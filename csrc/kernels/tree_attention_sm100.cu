@@ -2,15 +2,19 @@
 // 64, 128 or 256 (int8: 128).  The formula, and the kernel for what is left: tree_attention.cu.
 //
 // The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile (two CTAs per
-// SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of 128 keys
+// SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of 64 keys (int8: 128)
 //
-//   S = Q K^T   tcgen05.mma, both operands from shared memory; the keys come by TMA, two blocks of 64 by the block table
+//   S = Q K^T   tcgen05.mma, both operands from shared memory; the keys come by TMA, in pieces of 64 by the block table
 //   P = exp2(S - m) as bf16 over S, whole rows in registers; the sum of a row beside it
 //   O += P V    tcgen05.mma, P from TMEM, V as it lies in the cache (MN-major)
 //
+// There are two tiles of S, so that one is made while the softmax is at the other: its exponentials, 16 a cycle and SM, and the products
+// are then what bounds many rows over a key (with one tile of 128 keys, S, softmax and P V of a group followed one another: 1.85 us for
+// 256 rows x 128 keys).
+//
 // O stays in TMEM.  m is the largest score only up to a factor of 2^8: O is multiplied again when a row's maximum has grown by more than
-// that, in the time between S and P when no product with V is under way, which after the first tiles hardly ever happens; P and its sum
-// stay below 2^8 per key, and their quotient does not depend on m.
+// that, behind the product with V that is under way, which after the first tiles hardly ever happens; P and its sum stay below 2^8 per
+// key, and their quotient does not depend on m.
 //
 // The masks matter only in the last tiles, where the nodes' keys are: 128 bits of a row, shifted to the tile's place.  There two more
 // warps clear the values of keys that no node sees and of slots behind the last key, since 0 x NaN is NaN.
@@ -33,13 +37,14 @@ constexpr int kTgRows = 128;
 // key tiles of one.
 template <int H, int G, bool I8, bool TURNS>
 struct TgShape {
-  static constexpr int kKeys = H == 4 ? 64 : 128;        // of a tile
+  static constexpr int kKeys = I8 ? 128 : 64;            // of a tile
+  static constexpr int kBufs = I8 ? 1 : 2;               // of S, of a group
   static constexpr int R = TURNS ? 1 : G;                // row tiles
-  static constexpr int kLead = TURNS ? G : 1;            // S of so many tiles is ahead of P V
+  static constexpr int kLead = TURNS ? G : kBufs;        // S of so many tiles is ahead of P V
   static constexpr int kQHalf = kTgRows * 128, kHalf = kKeys * 128;          // 64 features of a tile's rows
   static constexpr int kQTile = H * kQHalf, kTile = H * kHalf;
-  static constexpr int kTmem = H == 4 ? 512 : 256 * G;   // columns: of a group S, whose first half becomes P, and 128 behind it O
-  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : R == 1 ? 4 / H : 10 / H;         // 64 KB (two CTAs an SM), 160 KB
+  static constexpr int kTmem = H == 4 ? 512 : 256 * G;   // columns: of a group 128 of S, half of which becomes P, and O
+  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : G == 1 ? 8 / H : 20 / H;         // 64 KB (two CTAs an SM), 160 KB
   static constexpr int kRaw = I8 ? (TURNS ? 3 : 5) : 0, kRawTile = kKeys * 128;                    // codes as they come
   static constexpr int kScales = I8 ? 4 : 0, kScaleBytes = 2 * kKeys * 4;            // of a tile's keys and values
   static constexpr int kSmem = R * kQTile + kStages * kTile + kRaw * kRawTile + kScales * kScaleBytes + 1024;
@@ -131,7 +136,7 @@ template <int H, int G, bool I8, bool TURNS, bool EXT>
 __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H, G, I8, TURNS>::kPerSm)
     tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs p) {
   using S = TgShape<H, G, I8, TURNS>;
-  constexpr int D = 64 * H, ST = S::kStages, R = S::R, L = S::kLead, KT = S::kKeys, NC = KT / 32;
+  constexpr int D = 64 * H, ST = S::kStages, R = S::R, L = S::kLead, KT = S::kKeys, NC = KT / 32, NB = S::kBufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                                    // R tiles
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
   uint8_t* sRaw = sT + ST * S::kTile;                    // I8: ring of codes, in the same order
   float* s_scales = reinterpret_cast<float*>(sRaw + S::kRaw * S::kRawTile);           // I8: ring of tiles' scales
   __shared__ uint64_t raw_full[S::kRaw + 1], raw_empty[S::kRaw + 1], c_full[S::kScales + 1], c_empty[S::kScales + 1];
-  __shared__ uint64_t q_full, full[ST], empty[ST], v_here, v_clean, s_full[G], p_half[G], p_full[G], o_full[G];
+  __shared__ uint64_t q_full, full[ST], empty[ST], v_here, v_clean, s_full[G * S::kBufs], p_half[G], p_full[G * S::kBufs], o_step[G], o_full[G];
   __shared__ float2 s_ml[TURNS ? kTgRows : 1];
   __shared__ uint32_t tmem_base_s, s_union[kTreeWords * 2];
 
@@ -152,7 +157,8 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
     for (int s = 0; s < S::kScales; ++s) { mbar_init(&c_full[s], 1); mbar_init(&c_empty[s], TURNS ? 4 : 4 * G); }
     mbar_init(&v_here, 1);
     mbar_init(&v_clean, 2);
-    for (int g = 0; g < G; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_half[g], 4); mbar_init(&p_full[g], 4); mbar_init(&o_full[g], 1); }
+    for (int g = 0; g < G; ++g) { mbar_init(&p_half[g], 4); mbar_init(&o_step[g], 1); mbar_init(&o_full[g], 1); }
+    for (int i = 0; i < G * NB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
     fence_barrier_init();
     fence_proxy_async();
     tma_prefetch_desc(&tmK);
@@ -266,20 +272,20 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         constexpr uint32_t IDESC_O = umma_idesc(128, D, 1, 1, 1) | (1u << 16);       // B = V, MN-major
         Ring ring{0, 0};
         bool ok = mbar_wait(&q_full, 0, p.status, XFT_ERR_WAIT_FULL);
-        auto scores = [&](int g, int st) {
+        auto scores = [&](int g, int j, int st) {
           const uint64_t qd = umma_desc_k128(smem_u32(sQ + (TURNS ? 0 : g) * S::kQTile)), kd = umma_desc_k128(smem_u32(sT + st * S::kTile));
           tcgen05_fence_after();
 #pragma unroll
           for (int k = 0; k < 4 * H; ++k) {
             const uint32_t q_off = ((k >> 2) * S::kQHalf + (k & 3) * 32) / 16, k_off = ((k >> 2) * S::kHalf + (k & 3) * 32) / 16;
-            umma_bf16(tmem_base + g * 256, qd + q_off, kd + k_off, IDESC_S, k > 0);
+            umma_bf16(tmem_base + g * 256 + j % NB * KT, qd + q_off, kd + k_off, IDESC_S, k > 0);
           }
-          tcgen05_commit(&s_full[g]);
+          tcgen05_commit(&s_full[g * NB + j % NB]);
         };
         for (int j = 0; j < min(L, nt) && ok; ++j) {
           ok = mbar_wait(&full[ring.s], ring.ph, p.status, XFT_ERR_WAIT_FULL);
           if (!ok) break;
-          for (int g = TURNS ? j : 0; g < (TURNS ? j + 1 : G); ++g) scores(g, ring.s);
+          for (int g = TURNS ? j : 0; g < (TURNS ? j + 1 : G); ++g) scores(g, j, ring.s);
           tcgen05_commit(&empty[ring.s]);
           ring.next(ST);
         }
@@ -298,27 +304,30 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
           if (!ok) break;
           const uint64_t vd = umma_desc_mn128(smem_u32(sT + vr.s * S::kTile), S::kHalf);
           const int g0 = TURNS ? j % G : 0, g1 = TURNS ? g0 + 1 : G;
-          const uint32_t ph = (TURNS ? j / G : j) & 1;
+          const uint32_t ph = j / L & 1;
           for (int g = g0; g < g1; ++g) {
-            const uint32_t pa = tmem_base + g * 256, oa = pa + 128;
-            ok = mbar_wait(&p_half[g], ph, p.status, XFT_ERR_WAIT_TMEM);
+            const uint32_t pa = tmem_base + g * 256 + j % NB * KT, oa = tmem_base + g * 256 + 128;
+            const bool sum = TURNS ? j >= G : j > 0;
+            if (NB == 1) {                               // the product may begin with the first half of the keys
+              ok = mbar_wait(&p_half[g], ph, p.status, XFT_ERR_WAIT_TMEM);
+              if (!ok) break;
+              tcgen05_fence_after();
+#pragma unroll
+              for (int k = 0; k < KT / 32; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, sum || k > 0);
+            }
+            ok = mbar_wait(&p_full[g * NB + j % NB], ph, p.status, XFT_ERR_WAIT_TMEM);
             if (!ok) break;
             tcgen05_fence_after();
 #pragma unroll
-            for (int k = 0; k < KT / 32; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, j >= L || k > 0);
-            ok = mbar_wait(&p_full[g], ph, p.status, XFT_ERR_WAIT_TMEM);
-            if (!ok) break;
-            tcgen05_fence_after();
-#pragma unroll
-            for (int k = KT / 32; k < KT / 16; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, 1);
+            for (int k = NB == 1 ? KT / 32 : 0; k < KT / 16; ++k) umma_bf16_ta(oa, pa + k * 8, vd + k * (2048 / 16), IDESC_O, sum || k > 0);
             if (g == g1 - 1) tcgen05_commit(&empty[vr.s]);
+            if (NB > 1) tcgen05_commit(&o_step[g]);
+            if (TURNS ? !more : j == nt - 1) tcgen05_commit(&o_full[g]);
             if (more) {                                  // the next S goes over P, behind the product that reads P
               if (g == g0) ok = mbar_wait(&full[kr.s], kr.ph, p.status, XFT_ERR_WAIT_FULL);
               if (!ok) break;
-              scores(g, kr.s);
+              scores(g, j + L, kr.s);
               if (g == g1 - 1) tcgen05_commit(&empty[kr.s]);
-            } else {
-              tcgen05_commit(&o_full[g]);
             }
           }
         }
@@ -339,13 +348,10 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         }
       }
       named_bar_sync(1, 64);
-      Ring ring{0, 0};
       for (int j = 0, cleaned = 0; j < nt; ++j) {
-        ring.next(ST);
-        const int st = ring.s;
-        const uint32_t ph = ring.ph;
-        ring.next(ST);
         if (tile_at(j) < tail) continue;
+        const int i = min(j + L, nt) + j, st = i % ST;   // of the ring's tiles, in order
+        const uint32_t ph = i / ST & 1;
         // (these warps do not hold the ring back, so they ask the issuer which round it is in)
         if (!mbar_wait(&v_here, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL)) break;
         const int key = (warp - 2) * (KT / 2) + lane * (KT / 64);            // one or two keys a lane
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
     }
-    const uint32_t sa = tmem_base + g * 256 + (uint32_t(qd * 32) << 16), oa = sa + 128;
+    const uint32_t base = tmem_base + g * 256 + (uint32_t(qd * 32) << 16), oa = base + 128;
     const bool caps = EXT && p.softcap > 0.f;
     const float scale = caps ? 1.f : p.scale * kTreeLog2e;           // (capped scores are in octaves already)
     const float cap = p.softcap * kTreeLog2e, inv_cap = caps ? p.scale / p.softcap : 0.f;
@@ -397,15 +403,16 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
     bool ok = true;
     const int first = TURNS ? g : 0;                     // of this group's tiles
     constexpr int kRing = I8 ? S::kScales : 1;
-    for (int j = first; j < nt; j += L) {
+    for (int j = first; j < nt; j += TURNS ? G : 1) {
       const int cs = j % kRing;
-      const uint32_t ph = (TURNS ? j / G : j) & 1;
+      const int buf = j % NB, box = g * NB + buf;
+      const uint32_t ph = j / L & 1, sa = base + buf * KT;
       const float* scales = s_scales + cs * 2 * KT;
       if (I8 && !mbar_wait(&c_full[cs], j / kRing & 1, p.status, XFT_ERR_WAIT_FULL)) { ok = false; break; }
-      if (!mbar_wait(&s_full[g], ph, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
+      if (!mbar_wait(&s_full[box], ph, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
       tcgen05_fence_after();
       if (!busy) {
-        if (lane == 0) { mbar_arrive(&p_half[g]); mbar_arrive(&p_full[g]); if (I8) mbar_arrive(&c_empty[cs]); }
+        if (lane == 0) { if (NB == 1) mbar_arrive(&p_half[g]); mbar_arrive(&p_full[box]); if (I8) mbar_arrive(&c_empty[cs]); }
         continue;
       }
       uint32_t x[NC][32];
@@ -492,6 +499,10 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         if (grown) m = mx;
         l *= f;
         if (j > first) {
+          // NB = 2: of the products with V, the last one may be under way (the one before it is not, S came behind that: two phases are
+          // possible here, which a parity can tell apart); NB = 1: S came behind the last one
+          if (NB > 1 && !mbar_wait(&o_step[g], (j - 1) & 1, p.status, XFT_ERR_WAIT_TMEM)) { ok = false; break; }
+          tcgen05_fence_after();
           uint32_t y[32];
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
@@ -528,7 +539,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
           w[i >> 1] = I8 ? tg_pack(e.x, e.y) : tg_round(e.x, e.y);           // (int8: the other instructions are what is short)
         }
         tmem_st16(sa + 16 * c, w);
-        if (c == NC / 2 - 1) {                           // the product may begin with the first half of the keys
+        if (NB == 1 && c == NC / 2 - 1) {                // the product may begin with the first half of the keys
           tmem_st_wait();
           tcgen05_fence_before();
           __syncwarp();
@@ -540,7 +551,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) { mbar_arrive(&p_full[g]); if (I8) mbar_arrive(&c_empty[cs]); }
+      if (lane == 0) { mbar_arrive(&p_full[box]); if (I8) mbar_arrive(&c_empty[cs]); }
     }
     bool have = ok && busy && nt > first;                // the group has sums
     for (int o = 0; o < G; ++o)                          // (TURNS: the ring is free for the exchange when both are through)

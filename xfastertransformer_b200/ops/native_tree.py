@@ -96,10 +96,10 @@ def _plan(B, hkv, rows, D, max_kv, tensor, int8=False):
     """(form, slices that the keys are cut into): the kernel of csrc/kernels/tree_attention_sm100.cu with one or two tiles of 128 rows per
     CTA, or (form 0) that of tree_attention.cu."""
     form = 0 if not tensor else 1 if rows <= 128 or D == 256 else 2
-    keys, tall, slots = ((32 if D == 256 else 64), 64, 296) if not form else ((64 if D == 256 else 128), 128 * form, 148 if int8 or D == 256 else 296 // form)
+    tall, slots = (64, 296) if not form else (128 * form, 148 if int8 or D == 256 else 296 // form)
     ctas = B * hkv * -(-rows // tall)
-    tiles = -(-max_kv // keys)
-    most = max(1, min(tiles // (1 if form else 4), 64))
+    tiles = -(-max_kv // 128)
+    most = max(1, min(tiles // (1 if form else 2), 64))
     best = None
     for waves in (1, 2, 3):                               # slices that fill the SMs once, twice, ...; a CTA costs as much as two tiles beside its own
         n = max(1, min(waves * slots // ctas, most))
