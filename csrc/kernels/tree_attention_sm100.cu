@@ -2,15 +2,14 @@
 // 64, 128 or 256 (int8: 128).  The formula, and the kernel for what is left: tree_attention.cu.
 //
 // The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile (two CTAs per
-// SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of 64 keys (int8: 128)
+// SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of keys
 //
 //   S = Q K^T   tcgen05.mma, both operands from shared memory; the keys come by TMA, in pieces of 64 by the block table
 //   P = exp2(S - m) as bf16 over S, whole rows in registers; the sum of a row beside it
 //   O += P V    tcgen05.mma, P from TMEM, V as it lies in the cache (MN-major)
 //
-// There are two tiles of S, so that one is made while the softmax is at the other: its exponentials, 16 a cycle and SM, and the products
-// are then what bounds many rows over a key (with one tile of 128 keys, S, softmax and P V of a group followed one another: 1.85 us for
-// 256 rows x 128 keys).
+// Bound, for many rows over a key, by the exponentials (16 a cycle and SM), the products and the steps between them; for few by the
+// keys' bytes.
 //
 // O stays in TMEM.  m is the largest score only up to a factor of 2^8: O is multiplied again when a row's maximum has grown by more than
 // that, behind the product with V that is under way, which after the first tiles hardly ever happens; P and its sum stay below 2^8 per
@@ -37,14 +36,16 @@ constexpr int kTgRows = 128;
 // key tiles of one.
 template <int H, int G, bool I8, bool TURNS>
 struct TgShape {
-  static constexpr int kKeys = I8 ? 128 : 64;            // of a tile
-  static constexpr int kBufs = I8 ? 1 : 2;               // of S, of a group
+  // one group makes the next tile's S while the softmax is at this one's; two, whose products keep the tensor cores busy in turns, are
+  // faster with whole tiles (256 rows x 128 keys 1.83 us, in halves 2.07; 128 rows 1.74 and 1.62)
+  static constexpr int kBufs = I8 || G == 2 ? 1 : 2;     // tiles of S of a group
+  static constexpr int kKeys = 128 / kBufs;              // of a tile
   static constexpr int R = TURNS ? 1 : G;                // row tiles
   static constexpr int kLead = TURNS ? G : kBufs;        // S of so many tiles is ahead of P V
   static constexpr int kQHalf = kTgRows * 128, kHalf = kKeys * 128;          // 64 features of a tile's rows
   static constexpr int kQTile = H * kQHalf, kTile = H * kHalf;
   static constexpr int kTmem = H == 4 ? 512 : 256 * G;   // columns: of a group 128 of S, half of which becomes P, and O
-  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : G == 1 ? 8 / H : 20 / H;         // 64 KB (two CTAs an SM), 160 KB
+  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : G == 1 ? 8 / H : 10 / H;         // 64 KB (two CTAs an SM), 160 KB
   static constexpr int kRaw = I8 ? (TURNS ? 3 : 5) : 0, kRawTile = kKeys * 128;                    // codes as they come
   static constexpr int kScales = I8 ? 4 : 0, kScaleBytes = 2 * kKeys * 4;            // of a tile's keys and values
   static constexpr int kSmem = R * kQTile + kStages * kTile + kRaw * kRawTile + kScales * kScaleBytes + 1024;
@@ -107,13 +108,15 @@ __device__ __forceinline__ uint2 tg_codes(uint32_t c) {
 }
 
 // Bits of 32 keys from key `first` on that a node with mask `m` (32-bit words) sees: the context's all, then the nodes'
-__device__ __forceinline__ uint32_t tg_sees(const uint32_t* m, int first, int ctx, int n) {
+// (of the words, the first two come in registers)
+__device__ __forceinline__ uint32_t tg_sees(unsigned long long m01, const uint32_t* m, int first, int ctx, int n) {
   const int o = first - ctx;
   if (o <= -32) return 0xffffffffu;
   auto word = [&](int i) -> uint32_t {
     const int left = n - 32 * i;
     if (left <= 0) return 0;
-    return left >= 32 ? m[i] : m[i] & ((1u << left) - 1);
+    const uint32_t w = i == 0 ? (uint32_t)m01 : i == 1 ? (uint32_t)(m01 >> 32) : m[i];
+    return left >= 32 ? w : w & ((1u << left) - 1);
   };
   if (o < 0) return (word(0) << -o) | ((1u << -o) - 1);
   return __funnelshift_r(word(o >> 5), word((o >> 5) + 1), o & 31);
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
         if (!mbar_wait(&v_here, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL)) break;
         const int key = (warp - 2) * (KT / 2) + lane * (KT / 64);            // one or two keys a lane
         const int k0 = tile_at(j) * KT;
-        const uint32_t sees = tg_sees(s_union, k0 + (key & ~31), s.ctx, s.n) >> (key & 31);
+        const uint32_t sees = tg_sees((unsigned long long)s_union[1] << 32 | s_union[0], s_union, k0 + (key & ~31), s.ctx, s.n) >> (key & 31);
         if (!mbar_wait(&full[st], ph, p.status, XFT_ERR_WAIT_FULL)) break;
         uint8_t* v = sT + st * S::kTile;
 #pragma unroll
@@ -395,6 +398,8 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       if (lane == 0) mbar_arrive(&q_full);
     }
     const uint32_t base = tmem_base + g * 256 + (uint32_t(qd * 32) << 16), oa = base + 128;
+    const uint32_t* bits = reinterpret_cast<const uint32_t*>(p.mask + (long long)(s.q0 + node) * p.words);
+    const unsigned long long first_bits = nt > 0 && tile_at(nt - 1) >= tail ? p.mask[(long long)(s.q0 + node) * p.words] : 0;
     const bool caps = EXT && p.softcap > 0.f;
     const float scale = caps ? 1.f : p.scale * kTreeLog2e;           // (capped scores are in octaves already)
     const float cap = p.softcap * kTreeLog2e, inv_cap = caps ? p.scale / p.softcap : 0.f;
@@ -476,10 +481,9 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       for (int c = 0; c < NC; ++c) sees[c] = 0xffffffffu;
       const bool ends = k0 + KT > s.ctx;
       if (ends || (EXT && p.window > 0)) {
-        const uint32_t* bits = reinterpret_cast<const uint32_t*>(p.mask + (long long)(s.q0 + node) * p.words);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          if (ends) sees[c] = tg_sees(bits, k0 + 32 * c, s.ctx, s.n);
+          if (ends) sees[c] = tg_sees(first_bits, bits, k0 + 32 * c, s.ctx, s.n);
           if (EXT && p.window > 0) sees[c] = tg_window(sees[c], k0 + 32 * c, s.ctx, pos, p.positions + s.q0, p.window, p.keep);
           if (__any_sync(0xffffffffu, sees[c] != 0xffffffffu))
 #pragma unroll
