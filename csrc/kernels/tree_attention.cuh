@@ -23,7 +23,7 @@ struct TreeAttnArgs {
   long long table_ld;
   int B, T, max_q, hq, hkv, group, q_off, D, bs, num_blocks, table_w, words, nsplit, window, keep;
   float scale, softcap;
-  int form;                                  // row tiles of a CTA in tree_attention_sm100.cu, 0: tree_attention.cu
+  int form;                                  // row tiles of a CTA in tree_attention_sm100.cu (2: int8 only), 0: tree_attention.cu
 };
 
 // One sequence's rows and keys, cut to what the arrays hold; n = 0 where the lengths cannot be right

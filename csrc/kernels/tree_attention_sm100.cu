@@ -1,8 +1,9 @@
 // Attention of the nodes of trees of drafted tokens on the 5th-generation tensor cores: caches in blocks of a multiple of 64, heads of
 // 64, 128 or 256 (int8: 128).  The formula, and the kernel for what is left: tree_attention.cu.
 //
-// The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile (two CTAs per
-// SM) or two (one CTA, each key tile read once for 256 rows) per CTA.  For each tile of keys
+// The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile a CTA, two CTAs
+// an SM (heads of 256: one).  CTAs with other rows over the same keys run beside one another and find them in L2; two tiles of rows in a
+// CTA over the same keys were no faster (512 rows x 65600 keys, 8 heads: 147 us, one tile 146).  For each tile of keys
 //
 //   S = Q K^T   tcgen05.mma, both operands from shared memory; the keys come by TMA, in pieces of 64 by the block table
 //   P = exp2(S - m) as bf16 over S, whole rows in registers; the sum of a row beside it
@@ -32,20 +33,20 @@ namespace {
 
 constexpr int kTgRows = 128;
 
-// G groups of four softmax warps and heads of 64 * H; I8: int8 cache.  The groups have a tile of rows each, or (TURNS) take turns at the
-// key tiles of one.
+// Heads of 64 * H; I8: int8 cache.  G groups of four softmax warps, two over an int8 cache, which have a tile of rows each, or (TURNS) take
+// turns at the key tiles of one.
 template <int H, int G, bool I8, bool TURNS>
 struct TgShape {
-  // one group makes the next tile's S while the softmax is at this one's; two, whose products keep the tensor cores busy in turns, are
-  // faster with whole tiles (256 rows x 128 keys 1.83 us, in halves 2.07; 128 rows 1.74 and 1.62)
-  static constexpr int kBufs = I8 || G == 2 ? 1 : 2;     // tiles of S of a group
+  // tiles of S of a group: with two of 64 keys the next one is made while the softmax is at this one (128 rows x 128 keys 1.62 us, with one
+  // of 128 keys 1.74)
+  static constexpr int kBufs = I8 ? 1 : 2;
   static constexpr int kKeys = 128 / kBufs;              // of a tile
   static constexpr int R = TURNS ? 1 : G;                // row tiles
   static constexpr int kLead = TURNS ? G : kBufs;        // S of so many tiles is ahead of P V
   static constexpr int kQHalf = kTgRows * 128, kHalf = kKeys * 128;          // 64 features of a tile's rows
   static constexpr int kQTile = H * kQHalf, kTile = H * kHalf;
   static constexpr int kTmem = H == 4 ? 512 : 256 * G;   // columns: of a group 128 of S, half of which becomes P, and O
-  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : G == 1 ? 8 / H : 10 / H;         // 64 KB (two CTAs an SM), 160 KB
+  static constexpr int kStages = I8 ? (TURNS ? 4 : 2) : H == 4 ? 5 : 8 / H;              // 64 KB: two CTAs an SM, one with heads of 256
   static constexpr int kRaw = I8 ? (TURNS ? 3 : 5) : 0, kRawTile = kKeys * 128;                    // codes as they come
   static constexpr int kScales = I8 ? 4 : 0, kScaleBytes = 2 * kKeys * 4;            // of a tile's keys and values
   static constexpr int kSmem = R * kQTile + kStages * kTile + kRaw * kRawTile + kScales * kScaleBytes + 1024;
@@ -196,8 +197,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
   tcgen05_fence_after();
   const uint32_t tmem_base = tmem_base_s;
 
-  // registers at launch: 256 x 128, 384 x 168 or (int8) 512 x 128; from here on 128 x 40 + 128 x 216, 128 x 72 + 256 x 216 or 128 x 40 +
-  // 256 x 200 + 128 x 72
+  // registers at launch: 256 x 128, int8 512 x 128; from here on 128 x 40 + 128 x 216, int8 128 x 40 + 256 x 200 + 128 x 72
   if (I8 && warp >= 4 + 4 * G) {
     // ------------------------------------------------------------------ codes to bf16, a row of a tile per thread
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -223,8 +223,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       ring.next(ST);
     }
   } else if (warp < 4) {
-    if (G == 1 || I8) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ------------------------------------------------------------------ TMA producer
       if (elect_one()) {
@@ -656,16 +655,14 @@ int launch(const TreeAttnArgs& a, cudaStream_t st) {
 template <bool EXT>
 int pick(const TreeAttnArgs& a, cudaStream_t st) {
   if (a.ks) return a.form == 2 ? launch<2, 2, true, false, EXT>(a, st) : launch<2, 2, true, true, EXT>(a, st);
-  if (a.D == 64) return a.form == 2 ? launch<1, 2, false, false, EXT>(a, st) : launch<1, 1, false, false, EXT>(a, st);
-  if (a.D == 256) return launch<4, 1, false, false, EXT>(a, st);
-  return a.form == 2 ? launch<2, 2, false, false, EXT>(a, st) : launch<2, 1, false, false, EXT>(a, st);
+  return a.D == 64 ? launch<1, 1, false, false, EXT>(a, st) : a.D == 128 ? launch<2, 1, false, false, EXT>(a, st) : launch<4, 1, false, false, EXT>(a, st);
 }
 
 }  // namespace
 
 // 0, -1 where the shape is not one of this kernel's, or an error
 int launch_tree_attention_tc(const TreeAttnArgs& a, cudaStream_t st) {
-  if (a.bs % 64 || (!(a.scale > 0.f) && !(a.softcap > 0.f)) || (a.D != 64 && a.D != 128 && a.D != 256) || (a.D == 256 && a.form != 1)) return -1;
+  if (a.bs % 64 || (!(a.scale > 0.f) && !(a.softcap > 0.f)) || (a.D != 64 && a.D != 128 && a.D != 256) || (!a.ks && a.form != 1)) return -1;
   if ((long long)a.num_blocks * a.hkv * a.bs > 0x7fffffffll) return -1;
   if (a.ks && (a.D != 128 || ((reinterpret_cast<uintptr_t>(a.ks) | reinterpret_cast<uintptr_t>(a.vs)) & 15))) return -1;
   return a.window > 0 || a.softcap > 0.f ? pick<true>(a, st) : pick<false>(a, st);

@@ -92,18 +92,21 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
     return mask, positions
 
 
-def _plan(B, hkv, rows, D, max_kv, tensor, int8=False):
-    """(form, slices that the keys are cut into): the kernel of csrc/kernels/tree_attention_sm100.cu with one or two tiles of 128 rows per
-    CTA, or (form 0) that of tree_attention.cu."""
-    form = 0 if not tensor else 1 if rows <= 128 or D == 256 else 2
-    tall, slots = (64, 296) if not form else (128 * form, 148 if int8 or D == 256 else 296 // form)
+def _plan(B, hkv, rows, total, D, max_kv, tensor, int8=False):
+    """(form, slices that the keys are cut into): the kernel of csrc/kernels/tree_attention_sm100.cu with one tile of 128 rows per CTA or
+    (int8: codes are expanded once for both) two, or (form 0) that of tree_attention.cu.  `rows` over a key, `total` of all sequences and heads."""
+    form = 0 if not tensor else 2 if int8 and rows > 128 else 1
+    tall, slots = (64, 296) if not form else (128 * form, 148 if int8 or D == 256 else 296)
     ctas = B * hkv * -(-rows // tall)
     tiles = -(-max_kv // 128)
     most = max(1, min(tiles // (1 if form else 2), 64))
     best = None
-    for waves in (1, 2, 3):                               # slices that fill the SMs once, twice, ...; a CTA costs as much as two tiles beside its own
-        n = max(1, min(waves * slots // ctas, most))
-        cost = -(-ctas * n // slots) * (-(-tiles // n) + 2) + (2 if n > 1 else 0)
+    # slices that fill the SMs by half, once, twice, ...  us: a tile of 128 keys 1.6 to 1.9, 3 where two CTAs of an SM share its part of the
+    # memory's rate; a CTA's start and end 3; the second launch 2.5, and 0.27 ns for each row and slice that it joins
+    for k in (0.5, 1, 2, 3):
+        n = max(1, min(int(k * slots) // ctas, most))
+        tile = (3.0 if int8 else 1.9) if form != 1 or slots == 148 else 1.6 if ctas * n <= 148 else 3.0
+        cost = -(-ctas * n // slots) * (-(-tiles // n) * tile + 3) + (2.5 + 2.7e-4 * total * n if n > 1 else 0)
         if best is None or cost < best[0]:
             best = cost, n
     return form, best[1]
@@ -132,7 +135,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     if not (T and B and most):
         return out
     ws = N.Workspace.get(dev)
-    form, n = _plan(B, hkv, most * group, D, min(longest, window + keep_first + most + 256) if window else longest,
+    form, n = _plan(B, hkv, most * group, T * hq, D, min(longest, window + keep_first + most + 256) if window else longest,
                     (D == 128 or ks is None) and bs % 64 == 0 and (scale > 0 or softcap > 0) and nb * hkv * bs < 2 ** 31 and (_ptr(ks) | _ptr(vs)) % 16 == 0,
                     ks is not None)
     part = q.new_empty(T * hq * n * (D + 2), dtype=torch.float32) if n > 1 else None
