@@ -82,34 +82,42 @@ struct TreeAcceptArgs {
 };
 
 constexpr int kAcceptThreads = 256;
-constexpr int kAcceptMoves = 8;                // rows that a thread has under way at a time
+constexpr int kAcceptMoves = 2, kAcceptPieces = 4;           // rows that a thread has under way at a time, and pieces of each
 
 template <typename V>
 __device__ __forceinline__ void move_rows(char* pool, long long head_rows, int heads, int row_bytes, const int* src, const int* dst, const int* blk_src,
                                           const int* blk_dst, int n) {
   const int pieces = row_bytes / (int)sizeof(V), all = heads * pieces;
-  for (int i = threadIdx.x & 31; i < all; i += 32) {
-    const int h = i / pieces, at = (i - h * pieces) * (int)sizeof(V);
+  for (int i0 = threadIdx.x & 31; i0 < all; i0 += 32 * kAcceptPieces) {
     for (int j0 = 0; j0 < n; j0 += kAcceptMoves) {
-      V v[kAcceptMoves];
+      V v[kAcceptPieces][kAcceptMoves];
+      auto each = [&](const int* blk, const int* row, auto use) {
 #pragma unroll
-      for (int j = 0; j < kAcceptMoves; ++j)
-        if (j0 + j < n)
-          v[j] = *reinterpret_cast<const V*>(pool + (((long long)blk_src[j0 + j] * heads + h) * head_rows + src[j0 + j]) * row_bytes + at);
+        for (int e = 0; e < kAcceptPieces; ++e) {
+          const int i = i0 + 32 * e, h = i / pieces, at = (i - h * pieces) * (int)sizeof(V);
 #pragma unroll
-      for (int j = 0; j < kAcceptMoves; ++j)
-        if (j0 + j < n)
-          *reinterpret_cast<V*>(pool + (((long long)blk_dst[j0 + j] * heads + h) * head_rows + dst[j0 + j]) * row_bytes + at) = v[j];
+          for (int j = 0; j < kAcceptMoves; ++j)
+            if (i < all && j0 + j < n)
+              use(v[e][j], reinterpret_cast<V*>(pool + (((long long)blk[j0 + j] * heads + h) * head_rows + row[j0 + j]) * row_bytes + at));
+        }
+      };
+      each(blk_src, src, [](V& x, const V* from) { x = *from; });
+      each(blk_dst, dst, [](const V& x, V* to) { *to = x; });
     }
   }
 }
 
 __global__ void __launch_bounds__(kAcceptThreads) tree_accept_kernel(const TreeAcceptArgs a) {
   __shared__ int path[kTreeNodes], src[kTreeNodes], dst[kTreeNodes], blk_src[kTreeNodes], blk_dst[kTreeNodes];
+  __shared__ long long says[kTreeNodes];
   __shared__ int s_count, s_moves;
   grid_dep_launch();
   grid_dep_wait();
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pool = blockIdx.x * (kAcceptThreads / 32) + warp;
+  long long place[3] = {};
+  if (pool < a.n_pools)
+    for (int i = 0; i < 3; ++i) place[i] = a.pools[3 * pool + i];
   int q0, n;
   bool bad = !tree_rows(a.t, b, q0, n);
   if (n > a.width) { bad = true; n = 0; }
@@ -126,16 +134,18 @@ __global__ void __launch_bounds__(kAcceptThreads) tree_accept_kernel(const TreeA
       const int i = lane + 32 * e;
       up[e] = i < n ? a.parents[q0 + i] : -1;
       tok[e] = i < n ? a.tokens[q0 + i] : 0;
+      if (i < n) says[i] = a.sampled[q0 + i];              // (a step that reads it from memory takes ten times as long)
     }
+    __syncwarp();
     for (int at = n > 0 ? 0 : -1; at >= 0;) {
       if (lane == 0) path[count] = at;
       ++count;
-      const long long says = a.sampled[q0 + at];
+      const long long said = says[at];
       unsigned next = 0xffffffffu;
 #pragma unroll
       for (int e = kTreeNodes / 32 - 1; e >= 0; --e) {
         const int i = lane + 32 * e;
-        if (i > at && up[e] == at && tok[e] == says) next = i;
+        if (i > at && up[e] == at && tok[e] == said) next = i;
       }
       next = __reduce_min_sync(0xffffffffu, next);
       at = next == 0xffffffffu ? -1 : (int)next;
@@ -168,15 +178,13 @@ __global__ void __launch_bounds__(kAcceptThreads) tree_accept_kernel(const TreeA
   if (blockIdx.x == 0) {
     for (int j = threadIdx.x; j < a.width; j += kAcceptThreads) {
       a.path[(long long)b * a.width + j] = j < count ? path[j] : -1;
-      a.emitted[(long long)b * a.width + j] = j < count ? a.sampled[q0 + path[j]] : -1;
+      a.emitted[(long long)b * a.width + j] = j < count ? says[path[j]] : -1;
     }
     if (threadIdx.x == 0) a.count[b] = count;
   }
-  if (!moves) return;
-  const int pool = blockIdx.x * (kAcceptThreads / 32) + warp;
-  if (pool >= a.n_pools) return;
-  char* base = reinterpret_cast<char*>(a.pools[3 * pool]);
-  const int heads = (int)a.pools[3 * pool + 1], row = (int)a.pools[3 * pool + 2];
+  if (!moves || pool >= a.n_pools) return;
+  char* base = reinterpret_cast<char*>(place[0]);
+  const int heads = (int)place[1], row = (int)place[2];
   if (row % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0) move_rows<uint4>(base, a.bs, heads, row, src, dst, blk_src, blk_dst, moves);
   else move_rows<uint16_t>(base, a.bs, heads, row, src, dst, blk_src, blk_dst, moves);
 }

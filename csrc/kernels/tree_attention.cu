@@ -31,7 +31,7 @@ __device__ __forceinline__ __nv_bfloat16* ta_at(__nv_bfloat16* t, int row, int p
 template <int D>
 constexpr int kTaKeys = D == 256 ? 32 : 64;
 template <int D>
-constexpr int kTaSmem = (kTaRows + 4 * kTaKeys<D>) * D * 2 + 4 * kTaKeys<D> * 4;
+constexpr int kTaSmem = (kTaRows + 4 * kTaKeys<D>) * D * 2 + 8 * kTaKeys<D> * 4;
 
 template <int D, bool INT8>
 __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAttnArgs p) {
@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
   __nv_bfloat16* sK = sQ + kTaRows * D;                  // two tiles
   __nv_bfloat16* sV = sK + 2 * KT * D;                   // two tiles
   float* s_scale = reinterpret_cast<float*>(sV + 2 * KT * D);          // int8: [2][keys | values][KT]
+  long long* s_at = reinterpret_cast<long long*>(s_scale + 4 * KT);    // [2][KT]: where a tile's keys are, and whether they are seen
   __shared__ unsigned long long s_mask[kTaRows][kTreeWords], s_union[kTreeWords];
   __shared__ int s_pos[kTreeMaxNodes], s_first;
   grid_dep_launch();
@@ -85,16 +86,22 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
   }
   const int nt = n_keep + end - lo, per = (nt + p.nsplit - 1) / p.nsplit;
   const int t_end = min(nt, (slice + 1) * per);
+  // rows of a tile's keys: twice the place in the cache, plus one where some node sees the key; below zero behind the last one
+  auto locate = [&](int t, int buf) {
+    if (tid >= KT) return;
+    const int key = (t < n_keep ? t : t - n_keep + lo) * KT + tid;
+    const bool in = key < s.kv;
+    const bool seen = in && (key < s.ctx || (s_union[(key - s.ctx) >> 6] >> ((key - s.ctx) & 63) & 1));
+    const int block = key / p.bs;
+    s_at[buf * KT + tid] = in ? 2 * (((long long)tree_block(p, b, block) * p.hkv + kvh) * p.bs + key - block * p.bs) + seen : -1;
+  };
   auto fetch = [&](int t, int buf) {
-    const int k0 = (t < n_keep ? t : t - n_keep + lo) * KT;
     __nv_bfloat16 *dk = sK + buf * KT * D, *dv = sV + buf * KT * D;
     constexpr int per_row = INT8 ? D / 16 : D / 8;
     for (int i = tid; i < KT * per_row; i += kTaThreads) {
-      const int r = i / per_row, c = i % per_row, key = k0 + r;
-      const bool in = key < s.kv;
-      const bool seen = in && (key < s.ctx || (s_union[(key - s.ctx) >> 6] >> ((key - s.ctx) & 63) & 1));
-      long long at = 0;
-      if (in) at = ((long long)tree_block(p, b, key / p.bs) * p.hkv + kvh) * p.bs + key % p.bs;
+      const int r = i / per_row, c = i % per_row;
+      const long long where = s_at[buf * KT + r], at = where < 0 ? 0 : where >> 1;
+      const bool in = where >= 0, seen = in && (where & 1);
       if constexpr (INT8) {
         uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (in) raw[0] = *reinterpret_cast<const uint4*>(static_cast<const int8_t*>(p.kc) + at * D + c * 16);
@@ -128,7 +135,12 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
   const int nd[2] = {min(r0, rows - 1) / heads, min(r0 + 8, rows - 1) / heads};
   const int pos[2] = {p.window > 0 ? s_pos[nd[0]] : 0, p.window > 0 ? s_pos[nd[1]] : 0};
   const bool busy = row0 + warp * 16 < rows;
-  if (slice * per < t_end) fetch(slice * per, 0);
+  if (slice * per < t_end) {
+    locate(slice * per, 0);
+    if (slice * per + 1 < t_end) locate(slice * per + 1, 1);
+    __syncthreads();
+    fetch(slice * per, 0);
+  }
   for (int t = slice * per, it = 0; t < t_end; ++t, ++it) {
     const int buf = it & 1;
     if (t + 1 < t_end) { fetch(t + 1, buf ^ 1); ta_wait<1>(); } else ta_wait<0>();
@@ -216,6 +228,7 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
         }
       }
     }
+    if (t + 2 < t_end) locate(t + 2, buf);
     __syncthreads();
   }
 #pragma unroll

@@ -101,12 +101,12 @@ def _plan(B, hkv, rows, total, D, max_kv, tensor, int8=False):
     tiles = -(-max_kv // 128)
     most = max(1, min(tiles // (1 if form else 2), 64))
     best = None
-    # slices that fill the SMs by half, once, twice, ...  us: a tile of 128 keys 1.6 to 1.9, 3 where two CTAs of an SM share its part of the
-    # memory's rate; a CTA's start and end 3; the second launch 2.5, and 0.27 ns for each row and slice that it joins
+    # slices that fill the SMs by half, once, twice, ...  us: a tile of 128 keys in a CTA that is alone on its SM, or one of two; a CTA's start
+    # and end 3; the second launch 2.5, and 0.27 ns for each row and slice that it joins
+    one, two = (3.0, 3.0) if int8 or not form else (1.4, 1.7) if D == 64 else (2.0, 2.8) if D == 128 else (2.6, 2.6)
     for k in (0.5, 1, 2, 3):
         n = max(1, min(int(k * slots) // ctas, most))
-        tile = (3.0 if int8 else 1.9) if form != 1 or slots == 148 else 1.6 if ctas * n <= 148 else 3.0
-        cost = -(-ctas * n // slots) * (-(-tiles // n) * tile + 3) + (2.5 + 2.7e-4 * total * n if n > 1 else 0)
+        cost = -(-ctas * n // slots) * (-(-tiles // n) * (one if ctas * n <= 148 else two) + 3) + (2.5 + 2.7e-4 * total * n if n > 1 else 0)
         if best is None or cost < best[0]:
             best = cost, n
     return form, best[1]
