@@ -406,14 +406,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   lim.least = a.min_p ? a.min_p[row] : a.m0;
   lim.u = a.uniform[row];
   if (lim.k >= a.V) lim.k = 0;
-  // the slice: groups of four that start on 16 bytes where the row's do; `skew` elements of the first group are in front of the row
-  const int skew = a.bf16 ? 0 : (int)(reinterpret_cast<uintptr_t>(r.x) >> 2 & 3);
+  // the slice: groups of four that start on 16 (bf16: 8) bytes; `skew` elements of the row's first group are in front of it
+  const int skew = (int)(reinterpret_cast<uintptr_t>(r.x) >> (a.bf16 ? 1 : 2) & 3);
   const int groups = (a.V + skew + 3) / 4, per = (groups + C - 1) / C;
   const int g0 = min(groups, (int)rank * per), ng = min(groups, g0 + per) - g0;
-  const float* xf = static_cast<const float*>(r.x) - skew;
   auto fetch = [&](int g) -> float4 {                    // group g of the row; what is not the row's is -inf
     const int i = 4 * g - skew;
-    if (!a.bf16 && i >= 0 && i + 4 <= a.V) return __ldg(reinterpret_cast<const float4*>(xf + 4 * g));
+    if (i >= 0 && i + 4 <= a.V) {
+      if (!a.bf16) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(r.x) + i));
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(r.x) + i));
+      return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+    }
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < a.V ? r.at(i + e) : -INFINITY;

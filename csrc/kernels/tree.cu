@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kTreeNodes) tree_mask_kernel(const TreeMaskArg
   const int b = blockIdx.x, i = threadIdx.x;
   int q0, n;
   bool bad = !tree_rows(a.t, b, q0, n);
-  if (n > 64 * a.words) { bad = true; n = 0; }
+  if (n > 64 * a.words || n > (int)blockDim.x) { bad = true; n = 0; }
   if (i < n) {
     const int p = a.parents[q0 + i];
     up[i] = p < i ? p : -1;                    // a parent comes before its children: the walk ends

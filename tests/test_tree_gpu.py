@@ -38,6 +38,21 @@ def test_masks(lens):
     _ok()
 
 
+def test_batches_that_understate_their_trees_are_reported():
+    from xfastertransformer_b200.ops import native as N
+    cu, kv = [0, 40], [50]
+    meta = _meta(cu, kv, None)
+    meta.max_q = 5
+    up = torch.arange(-1, 39, dtype=torch.int32, device="cuda")
+    c = torch.zeros(1, 1, 64, 128, dtype=torch.bfloat16, device="cuda")
+    bits, table = torch.zeros(40, 1, dtype=torch.int64, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    for f in (lambda: ops.tree_mask(up, cu, kv, meta), lambda: ops.tree_accept(up, up, up, cu, kv, meta=meta),
+              lambda: ops.tree_attention(torch.zeros(40, 2, 128, device="cuda").bfloat16(), c, c, table, cu, kv, bits, 0.1, meta=meta)):
+        f()
+        with pytest.raises(N.KernelError):
+            N.Workspace.get(torch.device("cuda", 0)).check_status()
+
+
 def test_a_parent_behind_its_child_is_reported():
     from xfastertransformer_b200.ops import native as N
     mask, pos = ops.tree_mask(torch.tensor([-1, 2, 0], dtype=torch.int32, device="cuda"), [0, 3], [5])
@@ -248,6 +263,10 @@ def test_one_number_for_all_rows_and_other_shapes():
     wide = torch.zeros(12, 600, device="cuda")
     wide[:, 3:503] = x.view(12, 500).cuda()
     assert torch.equal(ops.sample(wide[:, 3:503], torch.full((12,), 0.8), 30, torch.tensor([0.9]), 0.01, u).cpu(), want.view(-1))
+    for n in (1, 2, 3):                                    # bf16 rows that start anywhere in 8 bytes
+        wide = torch.zeros(12, 507, device="cuda", dtype=torch.bfloat16)
+        wide[:, n:n + 500] = x.view(12, 500).bfloat16().cuda()
+        assert torch.equal(ops.sample(wide[:, n:n + 500], 0.8, 30, 0.9, 0.01, u.cuda()).cpu(), R.sample(x.view(12, 500).bfloat16(), 0.8, 30, 0.9, 0.01, u))
     turned = x.view(12, 500).cuda().t().contiguous().t()
     assert torch.equal(ops.sample(turned, 0.8, 30, 0.9, 0.01, u.cuda()).cpu(), want.view(-1))
     assert ops.sample(x[:0].cuda(), 0.8, 30, 0.9, 0.01, u[:0].cuda()).shape == (0, 4)

@@ -388,9 +388,14 @@ def paged_attention(q, kc, vc, block_table, cu_q, kv_lens, scale, ks=None, vs=No
 MAX_TREE_NODES = 256
 
 
+_tree = None
+
+
 def _native_tree():
-    from . import native_tree
-    return native_tree
+    global _tree
+    if _tree is None:
+        from . import native_tree as _tree
+    return _tree
 
 
 def _check_trees(what, T, cu_q, kv_lens, meta, device):
