@@ -26,6 +26,8 @@
 // whose unsigned order is the row's.
 #include "ptx.cuh"
 
+#include <type_traits>
+
 namespace xft {
 
 struct SampleArgs {
@@ -385,8 +387,20 @@ __device__ __forceinline__ uint32_t add_peer(const void* own, uint32_t rank, uin
   return old;
 }
 
-// C CTAs a row.  HELD: the slices fit in shared memory
-template <int C, bool HELD>
+// Four logits at an end of the row (out of line, where it does not lengthen the loops over the others)
+template <bool BF16>
+__device__ __noinline__ float4 end_group(const void* x, int i, int V) {
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool in = i + e >= 0 && i + e < V;
+    v[e] = !in ? -INFINITY : BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i + e]) : static_cast<const float*>(x)[i + e];
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// C CTAs a row of fp32 or BF16 logits.  HELD: the slices fit in shared memory
+template <int C, bool HELD, bool BF16>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) float slice[];
   __shared__ SampleShared sh;
@@ -396,8 +410,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   const int row = blockIdx.x / C;
   const uint32_t rank = C > 1 ? cluster_ctarank() : 0;
   SampleRow r;
-  r.x = a.bf16 ? (const void*)(static_cast<const __nv_bfloat16*>(a.x) + row * a.ld) : (const void*)(static_cast<const float*>(a.x) + row * a.ld);
-  r.V = a.V; r.bf16 = a.bf16;
+  r.x = BF16 ? (const void*)(static_cast<const __nv_bfloat16*>(a.x) + row * a.ld) : (const void*)(static_cast<const float*>(a.x) + row * a.ld);
+  r.V = a.V; r.bf16 = BF16;
   const int shift = min(45, 63 - (32 - __clz(a.V)));     // masses of a row stay below 2^64
   const float t = a.temperature ? a.temperature[row] : a.t0;
   SampleLimits lim;
@@ -407,20 +421,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   lim.u = a.uniform[row];
   if (lim.k >= a.V) lim.k = 0;
   // the slice: groups of four that start on 16 (bf16: 8) bytes; `skew` elements of the row's first group are in front of it
-  const int skew = (int)(reinterpret_cast<uintptr_t>(r.x) >> (a.bf16 ? 1 : 2) & 3);
+  const int skew = (int)(reinterpret_cast<uintptr_t>(r.x) >> (BF16 ? 1 : 2) & 3);
   const int groups = (a.V + skew + 3) / 4, per = (groups + C - 1) / C;
   const int g0 = min(groups, (int)rank * per), ng = min(groups, g0 + per) - g0;
+  const float* xf = static_cast<const float*>(r.x) - skew;
   auto fetch = [&](int g) -> float4 {                    // group g of the row; what is not the row's is -inf
     const int i = 4 * g - skew;
-    if (i >= 0 && i + 4 <= a.V) {
-      if (!a.bf16) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(r.x) + i));
+    const bool in = i >= 0 && i + 4 <= a.V;
+    if (!BF16 && in) return __ldg(reinterpret_cast<const float4*>(xf + 4 * g));
+    if (BF16 && in) {
       const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(r.x) + i));
       return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
     }
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < a.V ? r.at(i + e) : -INFINITY;
-    return make_float4(v[0], v[1], v[2], v[3]);
+    return end_group<BF16>(r.x, i, a.V);
   };
   auto group = [&](int j) -> float4 { return HELD ? reinterpret_cast<const float4*>(slice)[j] : fetch(g0 + j); };
   if (tid < kSamplePer) sh.root[tid] = exp2(tid * (-1.0 / kSamplePer));
@@ -454,27 +467,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     return __fadd_rn(__fsub_rn(p, __fsub_rn(mid, kMagic)), rest);
   };
   auto part_of = [](float off) -> int { return max(0, min(kSampleBins - 1, (int)((0.5f - off) * kSampleBins))); };
-  int zoom = -1;                                         // >= 0: only elements of this bin are counted, in 1024 parts of it
-  auto put = [&](float x) {
+  int zoom = -1;                                         // the bin whose elements alone are counted, in 1024 parts of it (`zooms`)
+  auto put = [&](float x, auto zooms) {
+    constexpr bool kZooms = decltype(zooms)::value;
     const float p = grid(x), d = ref - p;
     if (!(d < kSampleEdge)) return;
     const float mid = __fadd_rn(p, kMagic);
     int n = (int)(__float_as_uint(__fadd_rn(ref, kMagic)) - __float_as_uint(mid));
     if (n < 0) { above = true; return; }
-    if (zoom >= 0 && n != zoom) return;
+    if (kZooms && n != zoom) return;
     if (!counts) {
       const float off = beside(x, p, mid);
-      if (zoom >= 0) n = part_of(off);
+      if (kZooms) n = part_of(off);
       // 2^(off / 16) - 1, |off| <= 1/2: (ln2 / 16)^i / i! off^i
       const float q = off * fmaf(off, fmaf(off, fmaf(off, 1.46760905e-7f, 1.35507817e-5f), 9.38384793e-4f), 4.33216988e-2f);
       const unsigned w = __float_as_uint(fmaf(q, (float)(1 << kSampleUnit), kMagic)) - 0x4b400000u + (1u << kSampleUnit);
       atomicAdd(&sh.own.lo[n], w & 0x3fffu);
       atomicAdd(&sh.own.hi[n], w >> 14);
-      if (!both && zoom < 0) return;
+      if (!kZooms && !both) return;
     }
     atomicAdd(&sh.own.cnt[n], 1u);
   };
-  auto put4 = [&](const float4& v) { put(v.x); put(v.y); put(v.z); put(v.w); };
+  auto put4 = [&](const float4& v, auto zooms) { put(v.x, zooms); put(v.y, zooms); put(v.z, zooms); put(v.w, zooms); };
   auto max4 = [](float m, const float4& v) { return fmaxf(fmaxf(fmaxf(m, v.x), fmaxf(v.y, v.z)), v.w); };
   float top = -INFINITY;                                 // the slice's largest
   constexpr int kAhead = 4;                              // groups that a thread has under way
@@ -503,7 +517,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
         top = max4(top, v[e]);
-        if (ref > -INFINITY) put4(v[e]);
+        if (ref > -INFINITY) put4(v[e], std::false_type());
       }
     }
     if (above) sh.above = 1;
@@ -545,7 +559,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
         float4 v[kAhead];
         ahead(j, v);
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e) put4(v[e]);
+        for (int e = 0; e < kAhead; ++e) put4(v[e], std::false_type());
       }
   }
   if (tid < C) {
@@ -702,7 +716,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
         float4 v[kAhead];
         ahead(j, v);
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e) put4(v[e]);
+        for (int e = 0; e < kAhead; ++e) put4(v[e], std::true_type());
       }
       cluster_barrier<C>();
       for (int i = tid; i < kShareBins; i += kSampleThreads) {
@@ -822,7 +836,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
 
 template <int C, bool HELD>
 int launch(const SampleArgs& a, cudaStream_t st) {
-  auto k = sample_rows_kernel<C, HELD>;
+  auto k = a.bf16 ? sample_rows_kernel<C, HELD, true> : sample_rows_kernel<C, HELD, false>;
   const int groups = (a.V + 3 + 3) / 4, bytes = HELD ? (groups + C - 1) / C * 16 : 0;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 3000 + (int)cudaGetLastError();
   cudaLaunchConfig_t cfg = {};
@@ -852,8 +866,10 @@ extern "C" int xft_sample_rows(const char* packed, cudaStream_t st) {
   memcpy(&a, packed, sizeof(a));
   if (a.rows <= 0) return 0;
   if (a.V < 1 || a.V > (1 << 24) || a.rows > (1 << 27)) return -1;
-  // CTAs of a row: as many as find room at a time, two an SM; their serial steps cost each row C times.  us, C = 8 / 4 / 2 / 1: see below
-  const int fit = a.rows <= 37 ? 8 : a.rows <= 74 ? 4 : a.rows <= 148 || a.V > 65536 ? 2 : 1;
+  // CTAs of a row: as many as find room at a time, two an SM; their serial steps cost a row C times.  us, top-k (top-p), rows of 151936, C = 8 /
+  // 4 / 2 / 1: 1 row 15 / 19 / 33 / 51 (31 / 37 / 68 / 107), 64 rows 39 / 31 / 37 / 55 (87 / 73 / 88 / 129), 512 rows 279 / 213 / 179 / 165
+  // (491 / 371 / 323 / 313)
+  const int fit = a.rows <= 37 ? 8 : a.rows <= 74 ? 4 : a.rows <= 148 ? 2 : 1;
   const int c = a.V <= 4096 ? 1 : fit;
   // slices of up to 18 Ki elements are held: two CTAs of them share an SM
   const bool held = a.V <= c * 18432;
