@@ -24,6 +24,9 @@
 // What that does not settle (more than 2048 equal logits or nearly so, a limit among weights that are left out, logits of
 // which a bin is less than 32 bits resolve) the first CTA settles alone, digit by digit of the 64-bit number (image of the logit, ~index),
 // whose unsigned order is the row's.
+//
+// Bound by the serial steps of a cluster where rows are few (a row of 32000 10 us), by instructions and the atomics where they are many (512
+// rows of 151936, top-p, 289 us; their bytes take 48).
 #include "ptx.cuh"
 
 #include <type_traits>

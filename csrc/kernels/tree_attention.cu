@@ -7,6 +7,10 @@
 // mma.sync.m16n8k16, keys in tiles through cp.async, two in flight.  Long caches are cut into slices whose sums a second kernel joins.
 // Masks matter in the last tiles alone, where the nodes' keys are.  Values of keys that no node sees and of slots behind the last key count
 // as zero: 0 x what a slot happens to hold may be NaN.
+//
+// This is the kernel for what tree_attention_sm100.cu does not take: blocks that are no multiple of 64, int8 caches with heads of 64 or
+// 256, scales of zero or below.  Bound by the instructions around mma.sync, of one warp where few rows share a key.  us: 8 trees of 13
+// nodes, 32 and 8 heads of 64, int8, 4000 keys 86 (its bytes take 5).
 #include "tree_attention.cuh"
 #include "mma_sync.cuh"
 

@@ -37,11 +37,11 @@ MAX_BODY_BYTES = 16 << 20          # a request body larger than this is refused 
 class Request:
     def __init__(self, prompt_ids: List[int], max_tokens: int, temperature: float, top_p: float, top_k: int,
                  stop_ids: List[int], seed: Optional[int], repetition_penalty: float = 1.0,
-                 logprobs: Optional[int] = None, stop_fn=None):
+                 logprobs: Optional[int] = None, stop_fn=None, min_p: float = 0.0):
         self.id = uuid.uuid4().hex[:24]
         self.prompt_ids = prompt_ids
         self.max_tokens = max(1, max_tokens)
-        self.temperature, self.top_p, self.top_k = temperature, top_p, top_k
+        self.temperature, self.top_p, self.top_k, self.min_p = temperature, top_p, top_k, min_p
         self.stop_ids = set(stop_ids)
         self.seed = seed
         self.repetition_penalty = float(repetition_penalty)
@@ -155,6 +155,10 @@ class Scheduler(threading.Thread):
         torch = self.torch
         if req.temperature <= 1e-5:
             return int(row.argmax())
+        if req.min_p > 0.0:
+            from xfastertransformer_b200 import ops
+            g = None if req.seed is None else torch.Generator().manual_seed(req.seed + len(req.generated))
+            return max(0, int(ops.sample(row[None], req.temperature, req.top_k, req.top_p, req.min_p, torch.rand(1, generator=g))))
         logits = row / req.temperature
         if req.top_k > 0 and req.top_k < logits.numel():
             kth = torch.topk(logits, req.top_k).values[-1]
@@ -477,7 +481,7 @@ def make_handler(sched: Scheduler, tok: Tokenizer, model_name: str):
                         seed = q.get("seed")
                         reqs.append(Request(ids, int(q.get("max_tokens", 16)), temp, float(q.get("top_p", 1.0)),
                                             int(q.get("top_k", 0)), stop_ids, None if seed is None else int(seed) + 7919 * k,
-                                            float(q.get("repetition_penalty", 1.0)), lp, stop_fn))
+                                            float(q.get("repetition_penalty", 1.0)), lp, stop_fn, float(q.get("min_p", 0.0))))
             except Exception as e:
                 return self._json(400, {"error": {"message": str(e), "type": "invalid_request_error"}})
             if sched.max_queue > 0 and sched.waiting.qsize() + len(reqs) > sched.max_queue:

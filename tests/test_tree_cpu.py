@@ -144,6 +144,18 @@ def test_sampling_of_odd_logits():
     assert pick(0.4, T=inf) == [-1, 2, 0, -1, 1, 1]
 
 
+def test_the_server_samples_with_min_p():
+    from types import SimpleNamespace
+    from serving.openai_server import Request, Scheduler
+    row = 3 * torch.randn(50, generator=torch.Generator().manual_seed(1))
+    pick = lambda seed, **kw: Scheduler._pick(SimpleNamespace(torch=torch), Request([1], 4, 0.8, kw.pop("top_p", 0.9), 20, [], seed, **kw), row)
+    assert {pick(s, min_p=1.0) for s in range(20)} == {int(row.argmax())}
+    for s in range(20):
+        u = torch.rand(1, generator=torch.Generator().manual_seed(s))
+        assert pick(s, min_p=0.05) == int(ops.sample(row[None], 0.8, 20, 0.9, 0.05, u))
+    assert len({pick(s, top_p=1.0) for s in range(40)}) > 1 and pick(3) == pick(3)
+
+
 def test_refusals():
     z = torch.zeros
     up = z(4, dtype=torch.int32) - 1
