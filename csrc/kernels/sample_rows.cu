@@ -868,12 +868,13 @@ extern "C" int xft_sample_rows(const char* packed, cudaStream_t st) {
   SampleArgs a;
   memcpy(&a, packed, sizeof(a));
   if (a.rows <= 0) return 0;
-  if (a.V < 1 || a.V > (1 << 24) || a.rows > (1 << 27)) return -1;
+  if (a.V < 1 || a.V > (1 << 21) || a.rows > (1 << 27)) return -1;
   // CTAs of a row: as many as find room at a time, two an SM; their serial steps cost a row C times.  us, top-k (top-p), rows of 151936, C = 8 /
   // 4 / 2 / 1: 1 row 15 / 19 / 33 / 51 (31 / 37 / 68 / 107), 64 rows 39 / 31 / 37 / 55 (87 / 73 / 88 / 129), 512 rows 279 / 213 / 179 / 165
   // (491 / 371 / 323 / 313)
   const int fit = a.rows <= 37 ? 8 : a.rows <= 74 ? 4 : a.rows <= 148 ? 2 : 1;
-  const int c = a.V <= 4096 ? 1 : fit;
+  int c = a.V <= 4096 ? 1 : fit;
+  while (c * (1 << 18) < a.V) c *= 2;                    // (a slice's sums of 14-bit parts stay below 2^32)
   // slices of up to 18 Ki elements are held: two CTAs of them share an SM
   const bool held = a.V <= c * 18432;
   if (c == 8) return held ? launch<8, true>(a, st) : launch<8, false>(a, st);

@@ -167,6 +167,7 @@ def test_refusals():
         lambda: ops.tree_mask(torch.arange(4, dtype=torch.int32), [0, 4], [9]),
         lambda: ops.tree_mask(z(300, dtype=torch.int32), [0, 300], [400]),
         lambda: ops.sample(z(2, 0), 1.0, 0, 1.0, 0.0, z(2)),
+        lambda: ops.sample(z(1).expand(1, (1 << 21) + 1), 1.0, 0, 1.0, 0.0, z(1)),
         lambda: ops.sample(z(2, 5, dtype=torch.int32), 1.0, 0, 1.0, 0.0, z(2)),
         lambda: ops.sample(z(2, 5), z(3), 0, 1.0, 0.0, z(2)),
         lambda: ops.sample(z(2, 5), 1.0, 0, 1.0, 0.0, 0.5),

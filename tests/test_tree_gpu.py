@@ -292,13 +292,24 @@ def test_all_logits_equal(V):
         assert torch.equal(ops.sample(x.cuda(), 1.0, k, p, 0.0, u.cuda()).cpu(), R.sample(x, 1.0, k, p, 0.0, u))
 
 
-@pytest.mark.parametrize("V,width", [(20000, 0.02), (151936, 0.05), (200003, 0.3), (100000, 1e-6)])
+@pytest.mark.parametrize("V,width", [(20000, 0.02), (151936, 0.05), (200003, 0.3), (100000, 1e-6), (1 << 21, 0.01)])
 def test_crowded_logits(V, width):
     g = torch.Generator().manual_seed(V)
-    x = 5 + width * torch.randn(14, V, generator=g)
-    u = torch.rand(14, generator=g)
+    rows = 14 if V < 1 << 20 else 3
+    x = 5 + width * torch.randn(rows, V, generator=g)
+    u = torch.rand(rows, generator=g)
     for T, k, p, m in ((1.0, 0, 1.0, 0.0), (2.5, 0, 0.6, 0.0), (0.8, 5000, 0.9, 0.0), (1.3, V // 2, 1.0, 0.0), (0.02, 0, 0.7, 0.3), (1.0, 700, 0.5, 0.0)):
         assert torch.equal(ops.sample(x.cuda(), T, k, p, m, u.cuda()).cpu(), R.sample(x, T, k, p, m, u)), (T, k, p, m)
+
+
+def test_many_rows_of_a_wide_vocabulary():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = 0.01 * torch.randn(160, 300001, generator=g, device="cuda")         # one bin: a slice's sums stay whole
+    u = torch.rand(160, generator=g, device="cuda")
+    got = ops.sample(x, 1.0, 0, 1.0, 0.0, u).cpu()
+    few = [0, 1, 77, 159]
+    assert torch.equal(got[few], R.sample(x[few].cpu(), 1.0, 0, 1.0, 0.0, u[few].cpu()))
+    assert torch.equal(ops.sample(x[:1], 1e39, 0, 1.0, 0.0, u[:1]).cpu(), R.sample(x[:1].cpu(), 1e39, 0, 1.0, 0.0, u[:1].cpu()))
 
 
 @pytest.mark.parametrize("T", [1e-6, 1e-4, 2e-3, 0.02])

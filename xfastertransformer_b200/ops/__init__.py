@@ -876,7 +876,7 @@ def sample_top_k_top_p(logits, top_k, top_p, temperature, uniform):
     return R.sample_top_k_top_p(logits, top_k, top_p, temperature, uniform)
 
 
-MAX_SAMPLE_VOCAB = 1 << 24
+MAX_SAMPLE_VOCAB = 1 << 21
 
 
 def sample(logits, temperature, top_k, top_p, min_p, uniform):

@@ -6,13 +6,13 @@ the device of their rows, on that device's current stream."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 
 import torch
 
 from . import native as N
 
-MAX_NODES = 256                # of one tree (csrc/kernels/tree_attention.cuh:kTreeMaxNodes)
 
 # csrc/kernels/tree.cu:TreeMaskArgs: cu_q, kv_lens | B, T | parents, mask, positions, status | words
 MASK_ARGS = struct.Struct("@2P2i4Pi4x")
@@ -143,7 +143,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     a = ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), _ptr(ks), _ptr(vs), block_table.data_ptr(), cu.data_ptr(),
                        kv.data_ptr(), mask.data_ptr(), _ptr(positions), _ptr(sinks), po, po + T * hq * n * D * 4, ws.status.data_ptr(),
                        block_table.stride(0), B, T, most, hq, hkv, group, q_off, D, bs, nb, block_table.shape[1], mask.shape[1], n, min(window, 1 << 30),
-                       keep_first, scale, softcap, form)
+                       min(keep_first, 1 << 30), scale, softcap, form)
     rc = _lib().xft_tree_attention(a, _stream())
     if rc:
         N._check(rc, "tree_attention")
@@ -154,7 +154,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
 def _per_row(v, rows, dtype, dev):
     """(tensor or None, number): a parameter of every row, or one for all."""
     if not isinstance(v, torch.Tensor):
-        return None, v
+        return None, v if dtype is torch.int32 or not abs(v) > 3.4e38 else math.copysign(math.inf, v)
     if v.dtype is dtype and v.numel() == rows and v.device == dev and v.is_contiguous():
         return v, 0
     if v.numel() == 1 and rows != 1:
