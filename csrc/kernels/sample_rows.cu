@@ -641,11 +641,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     u64 base = 0;
     if (done < kFirst && lim.k > 0) {
       const int b = bin_of(sh, count, cnt, [&](u64 c) { return c >= (u64)lim.k; }, base);
-      if (b == kSampleBins) return make_int4(kAlone, 0, 0, 0);
       const int in = (int)base;
       if (2 * tid <= b && b < 2 * tid + 2) sh.base = upto[b & 1] - mass[b & 1];
       __syncthreads();
-      return make_int4(kFirst, b, b, in);
+      if (b < kSampleBins) return make_int4(kFirst, b, b, in);         // (else fewer than k have weight)
     }
     if (done < kShare && lim.p < 1.f) {
       const u64 want = max(reach(lim.p, kept), (u64)1);
@@ -702,7 +701,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   } else if (counts) {
     u64 base;
     const int b = bin_of(sh, count, cnt, [&](u64 c) { return c >= (u64)lim.k; }, base);
-    todo = b == kSampleBins ? make_int4(kAlone, 0, 0, 0) : make_int4(kAll, 0, b, 0);
+    // fewer than k in the bins, as where most of a row is masked: what is 64 logits below the largest has no weight, unless T is above 1.9
+    todo = b < kSampleBins ? make_int4(kAll, 0, b, 0) : t <= 1.9f ? make_int4(kAll, 0, kSampleBins - 1, 0) : make_int4(kAlone, 0, 0, 0);
   } else {
     todo = next(kDone);
   }

@@ -208,6 +208,14 @@ def test_strided_inputs_and_lists():
     assert torch.equal(got, want)
     more = ops.tree_attention(torch.cat([q, q[:3]]), kc, vc, table.cuda(), cu, kv, torch.cat([bits, bits[:3]]), 0.1)
     assert torch.equal(more[:13], want) and not bool(more[13:].any())
+    padded = torch.cat([flat, flat[:3]]).cuda()
+    for meta in (None, _meta(cu, kv, table)):             # rows behind the last sequence
+        m, p = ops.tree_mask(padded, cu, kv, meta)
+        assert torch.equal(m[:13], bits) and not bool(m[13:].any()) and not bool(p[13:].any())
+        more = ops.tree_attention(torch.cat([q, q[:3]]), kc, vc, table.cuda(), cu, kv, m, 0.1, meta=meta)
+        assert torch.equal(more[:13], want) and not bool(more[13:].any())
+    emitted, path, count = ops.tree_accept(padded, padded, padded, cu, kv)
+    assert emitted.shape == (2, 9) and count.shape == (2,)
     _ok()
 
 
@@ -300,6 +308,19 @@ def test_crowded_logits(V, width):
     u = torch.rand(rows, generator=g)
     for T, k, p, m in ((1.0, 0, 1.0, 0.0), (2.5, 0, 0.6, 0.0), (0.8, 5000, 0.9, 0.0), (1.3, V // 2, 1.0, 0.0), (0.02, 0, 0.7, 0.3), (1.0, 700, 0.5, 0.0)):
         assert torch.equal(ops.sample(x.cuda(), T, k, p, m, u.cuda()).cpu(), R.sample(x, T, k, p, m, u)), (T, k, p, m)
+
+
+@pytest.mark.parametrize("masked", [-math.inf, torch.finfo(torch.float32).min, -1e4])
+@pytest.mark.parametrize("V", [1000, 128256])
+def test_rows_that_are_masked_but_for_a_few(V, masked):
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((16, V), masked)
+    for r in range(16):
+        x[r, torch.randperm(V, generator=g)[:r + 1]] = 3 * torch.randn(r + 1, generator=g)
+    u = torch.rand(16, generator=g)
+    for T in (0.5, 1.0, 1.9, 2.5):
+        for k, p, m in ((50, 1.0, 0.0), (50, 0.9, 0.0), (900, 0.7, 0.05), (5000, 0.9, 0.0), (5000, 1.0, 0.2), (0, 0.9, 0.0), (0, 1.0, 0.1), (3, 1.0, 0.0)):
+            assert torch.equal(ops.sample(x.cuda(), T, k, p, m, u.cuda()).cpu(), R.sample(x, T, k, p, m, u)), (T, k, p, m)
 
 
 def test_many_rows_of_a_wide_vocabulary():

@@ -71,6 +71,11 @@ def _arrays(cu_q, kv_lens, meta, dev):
     return cu, kv, kv.numel(), max(n, default=0), max(kv_lens, default=0)
 
 
+def _padded(cu_q, T) -> bool:
+    """Whether there are rows behind the last sequence."""
+    return isinstance(cu_q, (list, tuple)) and len(cu_q) > 0 and cu_q[-1] < T
+
+
 def tree_mask(parents, cu_q, kv_lens, meta=None):
     dev = parents.device
     if _foreign(dev):
@@ -79,8 +84,10 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
     parents = _i32(parents)
     cu, kv, B, most, _ = _arrays(cu_q, kv_lens, meta, dev)
     T, words = parents.numel(), max(1, -(-most // 64))
-    mask = parents.new_empty((T, words), dtype=torch.int64)
-    positions = torch.empty_like(parents)
+    if _padded(cu_q, T):
+        mask, positions = parents.new_zeros((T, words), dtype=torch.int64), torch.zeros_like(parents)
+    else:
+        mask, positions = parents.new_empty((T, words), dtype=torch.int64), torch.empty_like(parents)
     if T and B and most:
         ws = N.Workspace.get(dev)
         a = MASK_ARGS.pack(cu.data_ptr(), kv.data_ptr(), B, T, parents.data_ptr(), mask.data_ptr(), positions.data_ptr(), ws.status.data_ptr(),
@@ -130,8 +137,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     mask = mask if mask.is_contiguous() else mask.contiguous()
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     cu, kv, B, most, longest = _arrays(cu_q, kv_lens, meta, dev)
-    whole = meta is not None or not len(cu_q) or cu_q[-1] >= T
-    out = torch.empty_like(q) if whole else torch.zeros_like(q)
+    out = torch.zeros_like(q) if _padded(cu_q, T) else torch.empty_like(q)
     if not (T and B and most):
         return out
     ws = N.Workspace.get(dev)
