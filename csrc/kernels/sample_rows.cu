@@ -412,6 +412,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   const int tid = threadIdx.x, lane = tid & 31;
   const int row = blockIdx.x / C;
   const uint32_t rank = C > 1 ? cluster_ctarank() : 0;
+  if (C > 1) cluster_arrive();                           // another CTA's shared memory is there from its start on: see all_here
   SampleRow r;
   r.x = BF16 ? (const void*)(static_cast<const __nv_bfloat16*>(a.x) + row * a.ld) : (const void*)(static_cast<const float*>(a.x) + row * a.ld);
   r.V = a.V; r.bf16 = BF16;
@@ -441,6 +442,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   auto group = [&](int j) -> float4 { return HELD ? reinterpret_cast<const float4*>(slice)[j] : fetch(g0 + j); };
   if (tid < kSamplePer) sh.root[tid] = exp2(tid * (-1.0 / kSamplePer));
   if (tid == 0) { sh.n_list = 0; sh.above = 0; }
+  // in front of the first store to another CTA; that all have started is long known here, their slices have been read in between
+  auto all_here = [&]() {
+    if (C > 1) { __syncwarp(); cluster_wait(); }
+  };
   auto clear = [&]() {
     for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.own.cnt[i] = sh.own.lo[i] = sh.own.hi[i] = 0;
   };
@@ -537,6 +542,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.warps[tid >> 5] = first;
     __syncthreads();
+    all_here();
     if (tid == 0) {
       for (int i = 0; i < kSampleWarps; ++i) first = min(first, (unsigned)sh.warps[i]);
       st_peer(&sh.first[rank], 0, element(top, first));
@@ -565,6 +571,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
         for (int e = 0; e < kAhead; ++e) put4(v[e], std::false_type());
       }
   }
+  all_here();
   if (tid < C) {
     st_peer(&sh.top[rank], tid, __float_as_uint(top));
     st_peer(&sh.ref[rank], tid, __float_as_uint(ref));
