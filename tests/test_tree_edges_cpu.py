@@ -21,3 +21,11 @@ def test_no_store_to_another_cta_before_all_have_started():
     end_of_greedy = body.index("return;", body.index("if (greedy) {"))
     for start, end in ((0, end_of_greedy), (end_of_greedy, len(body))):       # rows at temperature 0 leave early
         assert [w for w in waits if start < w < end][0] < [p for p in peers if start < p < end][0]
+
+
+def test_attention_refuses_a_cache_without_blocks():
+    q, m, t = torch.zeros(4, 4, 64), torch.ones(4, 1, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int32)
+    for c in (torch.zeros(0, 2, 64, 64), torch.zeros(2, 2, 0, 64)):
+        with pytest.raises(ValueError):                   # there is no block that an index outside the pool could be read as
+            ops.tree_attention(q, c, c, t, [0, 4], [70], m, 0.1)
+        assert ops.tree_attention(q[:0], c, c, t, [0, 0], [0], m[:0], 0.1).shape == (0, 4, 64)

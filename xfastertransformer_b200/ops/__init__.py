@@ -453,6 +453,8 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     if mask.dim() != 2 or mask.shape[0] != T or mask.dtype is not torch.int64 or not 1 <= mask.shape[1] <= MAX_TREE_NODES // 64:
         raise ValueError(f"tree_attention: the mask is int64 [{T}, words], up to {MAX_TREE_NODES // 64} of them, not {tuple(mask.shape)} in {mask.dtype}")
     most = meta.max_q if meta is not None and getattr(meta, "max_q", 0) else max([b - a for a, b in zip(cu_q, cu_q[1:])], default=0)
+    if most and nb * bs == 0:
+        raise ValueError(f"tree_attention: {most} nodes over a cache {tuple(kc.shape)}, which has no blocks")
     if most > 64 * mask.shape[1]:
         raise ValueError(f"tree_attention: a mask of {mask.shape[1]} words for trees of {most} nodes")
     B = meta.kv_lens_dev.numel() if meta is not None and getattr(meta, "kv_lens_dev", None) is not None else len(kv_lens)
