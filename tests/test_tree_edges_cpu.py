@@ -29,3 +29,10 @@ def test_attention_refuses_a_cache_without_blocks():
         with pytest.raises(ValueError):                   # there is no block that an index outside the pool could be read as
             ops.tree_attention(q, c, c, t, [0, 4], [70], m, 0.1)
         assert ops.tree_attention(q[:0], c, c, t, [0, 0], [0], m[:0], 0.1).shape == (0, 4, 64)
+
+
+def test_pools_start_on_an_even_byte():
+    odd = torch.zeros(2 * 64 * 4 + 1, dtype=torch.int8)[1:].view(2, 1, 64, 4)          # rows move in pieces of two bytes at least
+    assert odd.data_ptr() % 2 == 1 and odd.is_contiguous()
+    with pytest.raises(ValueError):
+        ops.cache_pools([odd])

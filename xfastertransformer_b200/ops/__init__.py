@@ -488,6 +488,8 @@ def cache_pools(k, v=None, ks=None, vs=None):
             raise ValueError("cache_pools: pools of different numbers or sizes of blocks")
         if p.element_size() * (p.shape[3] if p.dim() == 4 else 1) % 2:
             raise ValueError(f"cache_pools: rows of an even number of bytes, not {tuple(p.shape)} in {p.dtype}")
+        if p.data_ptr() % 2:
+            raise ValueError(f"cache_pools: pools start on an even byte, not {p.data_ptr():#x}")
     _same_device("cache_pools", *pools)
     return _native_tree().CachePools(pools)
 
