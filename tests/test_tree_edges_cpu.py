@@ -36,3 +36,29 @@ def test_pools_start_on_an_even_byte():
     assert odd.data_ptr() % 2 == 1 and odd.is_contiguous()
     with pytest.raises(ValueError):
         ops.cache_pools([odd])
+
+
+def chain_with_gaps(dev="cpu"):
+    """A tree whose accepted path is 0, 2, 4, 5: (tokens, parents, sampled, cu_q, kv_lens, table)."""
+    t = lambda *x: torch.tensor(x, device=dev)
+    return t(0, 9, 2, 9, 4, 5), t(-1, 0, 0, 2, 2, 4).int(), t(2, 0, 4, 0, 5, 7), [0, 6], [16], t(0).int()[None]
+
+
+def test_a_pool_that_several_layers_read_moves_once():
+    for dtype in (torch.float32, torch.int8):
+        pools = [torch.arange(64).view(1, 1, 64, 1).repeat(1, 2, 1, 4).to(dtype) for _ in range(2)]
+        scales = torch.arange(64.0).view(1, 1, 64)
+        k = [pools[0], pools[1], pools[0], pools[0].view(1, 2, 64, 4)]
+        *_, count = ops.tree_accept(*chain_with_gaps(), ops.cache_pools(k, ks=[scales, None, scales, scales]))
+        assert int(count[0]) == 4
+        for p in (*pools, scales[..., None]):
+            assert p[0, 0, 10:14, 0].tolist() == [10, 12, 14, 15]
+
+
+def test_pools_that_overlap_are_refused():
+    flat = torch.zeros(3 * 64 * 4)
+    a, b, c = flat[:512].view(2, 1, 64, 4), flat[256:].view(2, 1, 64, 4), torch.zeros(2, 1, 64, 4)
+    for pools in ([a, b], [a, c, a.view(torch.int32)], [a, flat[:256].view(2, 1, 64, 2)]):
+        with pytest.raises(ValueError):
+            ops.cache_pools(pools)
+    ops.cache_pools([flat[:256].view(2, 1, 64, 2), flat[256:512].view(2, 1, 64, 2)], [c], None)          # neighbours do not

@@ -42,3 +42,14 @@ def test_clusters_of_short_rows_beside_other_work(rows, T):
     torch.cuda.synchronize()
     for got in outs:
         assert torch.equal(got.cpu(), want)
+
+
+def test_a_pool_that_several_layers_read_moves_once():
+    from test_tree_edges_cpu import chain_with_gaps
+    pools = [torch.arange(64.0, device="cuda").view(1, 1, 64, 1).repeat(1, 2, 1, 128).bfloat16() for _ in range(3)]
+    handle = ops.cache_pools([pools[i % 3] for i in range(80)])
+    *_, count = ops.tree_accept(*chain_with_gaps("cuda"), handle)
+    assert int(count[0]) == 4
+    for p in pools:
+        assert p[0, 1, 10:14, 5].tolist() == [10, 12, 14, 15]
+    _ok()

@@ -476,7 +476,8 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
 
 def cache_pools(k, v=None, ks=None, vs=None):
     """The pools of all layers as `tree_accept` takes them: lists of keys and values [blocks, heads, block, D] (None or a None entry: a layer
-    without) and of an int8 cache's scales [blocks, heads, block].  Made once; it holds the pools, and belongs to them for as long as they
+    without) and of an int8 cache's scales [blocks, heads, block].  A pool that several layers read may be listed for each of them: its rows
+    move once.  Pools that overlap in another way are refused.  Made once; it holds the pools, and belongs to them for as long as they
     stay where they are (`PagedKVCache.pools` makes one for a cache)."""
     pools = [p for group in (k, v, ks, vs) for p in (group or []) if p is not None]
     if not pools:
@@ -491,6 +492,11 @@ def cache_pools(k, v=None, ks=None, vs=None):
         if p.data_ptr() % 2:
             raise ValueError(f"cache_pools: pools start on an even byte, not {p.data_ptr():#x}")
     _same_device("cache_pools", *pools)
+    # moving is no idempotent step: the second time, a row that has come to a place would be taken from there
+    pools = list({(p.data_ptr(), p.shape, p.dtype): p for p in pools}.values())
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in pools if p.numel())
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+        raise ValueError("cache_pools: pools that overlap")
     return _native_tree().CachePools(pools)
 
 
