@@ -62,3 +62,29 @@ def test_pools_that_overlap_are_refused():
         with pytest.raises(ValueError):
             ops.cache_pools(pools)
     ops.cache_pools([flat[:256].view(2, 1, 64, 2), flat[256:512].view(2, 1, 64, 2)], [c], None)          # neighbours do not
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int8"])
+def test_the_handle_of_a_cache_is_made_once_and_refused_when_its_pools_have_moved(dtype):
+    import gc
+    import weakref
+    from xfastertransformer_b200.runtime.kv_cache import PagedKVCache
+    c = PagedKVCache(2, 2, 8, 8, dtype, torch.device("cpu"))
+    c.ensure_blocks(2)
+    handle = c.pools()
+    assert c.pools() is handle and len(handle.pools) == (8 if dtype == "int8" else 4)
+    c.k[1][0, :, 10:16] = torch.arange(10, 16)[:, None]
+    ops.tree_accept(*chain_with_gaps(), handle)
+    assert c.k[1][0, 1, 10:14, 3].tolist() == [10, 12, 14, 15]
+    was = weakref.ref(c.k[0])
+    c.ensure_blocks(9)                                    # grows: the rows are elsewhere now
+    gc.collect()
+    assert was() is None                                  # and the memory that they were in is free
+    for pools in (handle, handle):
+        with pytest.raises(ValueError):
+            ops.tree_accept(*chain_with_gaps(), pools)
+    new = c.pools()
+    assert new is not handle and c.pools() is new and not bool(handle.table.any())
+    c.k[1][0, :, 10:16] = torch.arange(10, 16)[:, None]
+    ops.tree_accept(*chain_with_gaps(), new)
+    assert c.k[1][0, 1, 10:14, 3].tolist() == [10, 12, 14, 15]

@@ -53,3 +53,29 @@ def test_a_pool_that_several_layers_read_moves_once():
     for p in pools:
         assert p[0, 1, 10:14, 5].tolist() == [10, 12, 14, 15]
     _ok()
+
+
+def test_a_graph_captured_before_its_cache_grew_moves_nothing():
+    from test_tree_edges_cpu import chain_with_gaps
+    from xfastertransformer_b200.runtime.kv_cache import PagedKVCache
+    c = PagedKVCache(3, 2, 128, 128, "bf16", torch.device("cuda", 0))
+    c.ensure_blocks(2)
+    pools, args = c.pools(), chain_with_gaps("cuda")
+    meta = _meta(args[3], args[4], args[5])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert c.pools() is pools                         # (made already: nothing waits here)
+        count = ops.tree_accept(*args, pools, meta=meta)[2]
+    fill = torch.arange(64.0, device="cuda").bfloat16()[:, None]
+    for l in range(3):
+        c.k[l][0, :] = fill
+    graph.replay()
+    assert int(count[0]) == 4 and all(k[0, 1, 10:14, 7].tolist() == [10, 12, 14, 15] for k in c.k)
+    old = c.k[2]                                          # (held, so that what a late move would write can be seen)
+    c.ensure_blocks(64)
+    for k in (old, *c.k):
+        k[0, :] = fill
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(count[0]) == 4 and all(k[0, 1, 10:14, 7].tolist() == [10, 11, 12, 13] for k in (old, *c.k))
+    _ok()

@@ -477,8 +477,9 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
 def cache_pools(k, v=None, ks=None, vs=None):
     """The pools of all layers as `tree_accept` takes them: lists of keys and values [blocks, heads, block, D] (None or a None entry: a layer
     without) and of an int8 cache's scales [blocks, heads, block].  A pool that several layers read may be listed for each of them: its rows
-    move once.  Pools that overlap in another way are refused.  Made once; it holds the pools, and belongs to them for as long as they
-    stay where they are (`PagedKVCache.pools` makes one for a cache)."""
+    move once.  Pools that overlap in another way are refused.  Made once, outside of a capture; it holds the pools, and
+    belongs to them for as long as they stay where they are.  (`PagedKVCache.pools` has the one of a cache, which `tree_accept` refuses once
+    the cache's pools have been replaced.)"""
     pools = [p for group in (k, v, ks, vs) for p in (group or []) if p is not None]
     if not pools:
         raise ValueError("cache_pools: no pools")
@@ -511,6 +512,8 @@ def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table=None, pools
             raise ValueError(f"tree_accept: {name} are int32 or int64 [{T}], not {tuple(t.shape)} in {t.dtype}")
     _check_trees("tree_accept", T, cu_q, kv_lens, meta, tokens.device)
     if pools is not None:
+        if pools.retired:
+            raise ValueError("tree_accept: the cache's pools have been replaced since `pools` was made")
         B = meta.kv_lens_dev.numel() if meta is not None and getattr(meta, "kv_lens_dev", None) is not None else len(kv_lens)
         if block_table is None or block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] < B:
             raise ValueError(f"tree_accept: moving rows needs the block table, int32 [{B}, blocks]")

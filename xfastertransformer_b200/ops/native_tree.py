@@ -207,6 +207,12 @@ class CachePools:
                                   dtype=torch.int64).to(first.device)
         if first.is_cuda:
             torch.cuda.current_stream(first.device).synchronize()       # other streams may read it from now on
+        self.retired = False
+
+    def retire(self):
+        """The pools are replaced: lets them go.  `tree_accept` refuses the handle from now on, and a graph captured with it moves nothing."""
+        self.retired, self.pools = True, []
+        self.table.zero_()                                               # no heads, rows of no bytes
 
 
 def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table, pools, meta=None):

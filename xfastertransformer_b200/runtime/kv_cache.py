@@ -169,6 +169,7 @@ class PagedKVCache:
         self.tables: Dict[int, List[int]] = {}
         self.lens: Dict[int, int] = {}
         self.version = 0                         # bumped when pools are reallocated
+        self._handle = None                      # of the present k, v, ks and vs, see pools()
         self.prefix_index: Optional[PrefixIndex] = None      # set by the engine when automatic prefix reuse is on
         self.state_geometry = list(states)       # (shape of one slot, type) of every state pool
         self.max_states = max_states             # > 0: the state pools never grow past this many slots
@@ -243,6 +244,9 @@ class PagedKVCache:
 
     def _grow_pools(self, total: int) -> None:
         old = self.alloc.num_blocks
+        if self._handle is not None:
+            self._handle.retire()
+            self._handle = None
         mk = lambda H, d: torch.zeros(total, H, self.block, d, dtype=self.dtype, device=self.device)
         nk, nv, nks, nvs = [], [], [], []
         for l in range(self.L):
@@ -272,9 +276,12 @@ class PagedKVCache:
         self.k, self.v, self.ks, self.vs = nk, nv, nks, nvs
 
     def pools(self):
-        """Every layer's pools for `ops.tree_accept`; good until `version` changes, which happens when the pools are replaced."""
-        from .. import ops
-        return ops.cache_pools(self.k, self.v, self.ks, self.vs)
+        """Every layer's pools for `ops.tree_accept`: the same handle until they are replaced, then refused.  Making it waits for the stream,
+        so a program asks for it before it captures a step."""
+        if self._handle is None:
+            from .. import ops
+            self._handle = ops.cache_pools(self.k, self.v, self.ks, self.vs)
+        return self._handle
 
     def blocks_for(self, n_tokens: int) -> int:
         return (n_tokens + self.block - 1) // self.block
