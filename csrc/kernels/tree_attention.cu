@@ -5,8 +5,8 @@
 //
 // All rows (node, query head) of one kv head read the same keys: 64 of them per CTA, 16 a warp, flash attention with
 // mma.sync.m16n8k16, keys in tiles through cp.async, two in flight.  Long caches are cut into slices whose sums a second kernel joins.
-// Masks matter in the last tiles alone, where the nodes' keys are.  Values of keys that no node sees and of slots behind the last key count
-// as zero: 0 x what a slot happens to hold may be NaN.
+// Masks matter in the last tiles alone, where the nodes' keys are.  Values of keys that no node sees (for its mask or the window) and of slots
+// behind the last key count as zero: 0 x what a slot happens to hold may be NaN.
 //
 // This is the kernel for what tree_attention_sm100.cu does not take: blocks that are no multiple of 64, int8 caches with heads of 64 or
 // 256, scales of zero or below.  Bound by the instructions around mma.sync, of one warp where few rows share a key.  us: 8 trees of 13
@@ -62,16 +62,18 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
   if (tid < kTreeWords) s_union[tid] = 0;
   if (tid == 0) s_first = 0x7fffffff;
   __syncthreads();
-  for (int i = tid; i < s.n * p.words; i += kTaThreads) {
-    const int nd = i / p.words, w = i - nd * p.words;
-    const unsigned long long m = p.mask[(long long)(s.q0 + nd) * p.words + w];
-    if (m) atomicOr(&s_union[w], m);
-    if (nd >= node0 && nd - node0 < kTaRows) s_mask[nd - node0][w] = m;
-  }
   if (p.window > 0) {
     int first = 0x7fffffff;
     for (int i = tid; i < s.n; i += kTaThreads) first = min(first, s_pos[i] = p.positions[s.q0 + i]);
     atomicMin(&s_first, first);
+    __syncthreads();
+  }
+  for (int i = tid; i < s.n * p.words; i += kTaThreads) {
+    const int nd = i / p.words, w = i - nd * p.words;
+    unsigned long long m = p.mask[(long long)(s.q0 + nd) * p.words + w];
+    if (nd >= node0 && nd - node0 < kTaRows) s_mask[nd - node0][w] = m;
+    if (p.window > 0) m = tree_within(m, 64 * w, s.n, s_pos[nd], s_pos, p.window, p.keep);
+    if (m) atomicOr(&s_union[w], m);
   }
   // rows of queries, 16 bytes at a time; rows behind the last one are zero
   for (int i = tid; i < kTaRows * (D / 8); i += kTaThreads) {
@@ -83,9 +85,10 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
   __syncthreads();
   // tiles: those of the kept first keys, then those from the first key of the widest window
   const int end = (s.kv + KT - 1) / KT;
-  int lo = 0, n_keep = 0;
+  int lo = 0, n_keep = 0, first_key = 0;
   if (p.window > 0) {
-    lo = min(max(0, (int)min((long long)s_first - p.window + 1, (long long)s.ctx)) / KT, end);
+    first_key = tree_first(p, s, s_first);
+    lo = min(first_key / KT, end);
     n_keep = min((min(p.keep, s.kv) + KT - 1) / KT, lo);
   }
   const int nt = n_keep + end - lo, per = (nt + p.nsplit - 1) / p.nsplit;
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(kTaThreads) tree_attention_kernel(const TreeAt
     if (tid >= KT) return;
     const int key = (t < n_keep ? t : t - n_keep + lo) * KT + tid;
     const bool in = key < s.kv;
-    const bool seen = in && (key < s.ctx || (s_union[(key - s.ctx) >> 6] >> ((key - s.ctx) & 63) & 1));
+    const bool seen = in && (key < s.ctx ? key >= first_key || key < p.keep : (bool)(s_union[(key - s.ctx) >> 6] >> ((key - s.ctx) & 63) & 1));
     const int block = key / p.bs;
     s_at[buf * KT + tid] = in ? 2 * (((long long)tree_block(p, b, block) * p.hkv + kvh) * p.bs + key - block * p.bs) + seen : -1;
   };

@@ -57,6 +57,21 @@ __device__ __forceinline__ int tree_block(const TreeAttnArgs& p, int b, int i) {
   return blk;
 }
 
+// Of a mask's bits for nodes first .. first + 63, those whose nodes the window leaves to a node at `pos`; `at`: positions of the sequence's n nodes
+__device__ __forceinline__ unsigned long long tree_within(unsigned long long m, int first, int n, int pos, const int* at, int window, int keep) {
+  if (n - first < 64) m &= n > first ? (1ull << (n - first)) - 1 : 0;
+  for (unsigned long long rest = m; rest; rest &= rest - 1) {
+    const int i = __ffsll(rest) - 1, k = at[first + i];
+    if (!((long long)pos - k < window || k < keep)) m &= ~(1ull << i);
+  }
+  return m;
+}
+
+// The first key of the context that a window leaves to some node, `at` the lowest position of the nodes
+__device__ __forceinline__ int tree_first(const TreeAttnArgs& p, const TreeSeq& s, int at) {
+  return (int)max(0ll, min((long long)at - p.window + 1, (long long)s.ctx));
+}
+
 constexpr float kTreeLog2e = 1.4426950408889634f;
 
 int launch_tree_join(const TreeAttnArgs& a, cudaStream_t st);                 // tree_attention.cu

@@ -17,8 +17,8 @@
 // that, behind the product with V that is under way, which after the first tiles hardly ever happens; P and its sum stay below 2^8 per
 // key, and their quotient does not depend on m.
 //
-// The masks matter only in the last tiles, where the nodes' keys are: 128 bits of a row, shifted to the tile's place.  There two more
-// warps clear the values of keys that no node sees and of slots behind the last key, since 0 x NaN is NaN.
+// The masks matter only in the last tiles, where the nodes' keys are: 128 bits of a row, shifted to the tile's place.  There, and in the tiles
+// that a window cuts, two more warps clear the values of keys that no node sees and of slots behind the last key, since 0 x NaN is NaN.
 //
 // Codes of an int8 cache are expanded on the way, by four warps between the ring that TMA fills and the one that the products read; they are
 // exact in bf16, a key's scale multiplies its score and a value's its weight, in 32 bits.  Bound by shared memory: codes, values and the
@@ -126,11 +126,16 @@ __device__ __forceinline__ uint32_t tg_sees(unsigned long long m01, const uint32
   return __funnelshift_r(word(o >> 5), word((o >> 5) + 1), o & 31);
 }
 
+__device__ __forceinline__ uint32_t tg_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+// All of 32 keys from key `first` on but those of the context in front of key `from` that are not among the first `keep`
+__device__ __forceinline__ uint32_t tg_context(int first, int ctx, int from, int keep) {
+  return ~tg_below(ctx - first) | ~tg_below(from - first) | tg_below(keep - first);
+}
+
 // Of the same bits those that a window leaves: `pos` is the node's position, `at` the positions of the sequence's nodes
 __device__ __forceinline__ uint32_t tg_window(uint32_t sees, int first, int ctx, int pos, const int* at, int window, int keep) {
-  auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
-  const uint32_t context = below(ctx - first);
-  sees &= ~context | ~below(pos - window + 1 - first) | below(keep - first);
+  const uint32_t context = tg_below(ctx - first);
+  sees &= tg_context(first, ctx, pos - window + 1, keep);
   for (uint32_t rest = sees & ~context; rest; rest &= rest - 1) {
     const int i = __ffs(rest) - 1, k = at[first + i - ctx];
     if (!((long long)pos - k < window || k < keep)) sees &= ~(1u << i);
@@ -183,18 +188,24 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
   const int n_rt = (p.max_q * p.group + R * kTgRows - 1) / (R * kTgRows);
   const int row0 = (blockIdx.x % n_rt) * (R * kTgRows), slice = blockIdx.x / n_rt;
   // tiles: those of the kept first keys, then those from the first key of the widest window
-  int lo = 0, n_keep = 0;
+  int lo = 0, n_keep = 0, first_key = 0;
   if (EXT && p.window > 0) {
     int at = 0x7fffffff;
     for (int i = lane; i < s.n; i += 32) at = min(at, p.positions[s.q0 + i]);
     at = __reduce_min_sync(0xffffffffu, at);
-    lo = max(0, (int)min((long long)at - p.window + 1, (long long)s.ctx)) / KT;
+    first_key = tree_first(p, s, at);
+    lo = first_key / KT;
     n_keep = min((min(p.keep, s.kv) + KT - 1) / KT, lo);
   }
   const int all = n_keep + (s.kv + KT - 1) / KT - lo, per = (all + p.nsplit - 1) / p.nsplit;
   const int t0 = min(all, slice * per), nt = row0 < rows ? min(all, t0 + per) - t0 : 0;
   auto tile_at = [&](int j) -> int { return EXT && t0 + j >= n_keep ? t0 + j - n_keep + lo : t0 + j; };
   const int tail = s.ctx / KT;                           // from this tile on there are keys that are not the context's
+  // tile j has keys that no node may see: those that are not the context's, and the ones that the window leaves to none
+  auto unseen = [&](int j) -> bool {
+    const int t = tile_at(j), k0 = t * KT;
+    return t >= tail || (EXT && max(k0, p.keep) < min(k0 + KT, first_key));
+  };
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
@@ -302,7 +313,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
           const bool more = j + L < nt;
           if (more) ring.next(ST);
           ok = mbar_wait(&full[vr.s], vr.ph, p.status, XFT_ERR_WAIT_FULL);
-          if (!I8 && ok && tile_at(j) >= tail) {
+          if (!I8 && ok && unseen(j)) {
             mbar_arrive(&v_here);
             ok = mbar_wait(&v_clean, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL);
           }
@@ -342,10 +353,21 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       if (nt > 0 && tile_at(nt - 1) >= tail) {
         uint32_t seen[kTreeWords * 2] = {};
         const uint32_t* m = reinterpret_cast<const uint32_t*>(p.mask + (long long)s.q0 * p.words);
-        for (int i = lane; i < s.n; i += 32)
+        for (int i = lane; i < s.n; i += 32) {
+          if (EXT && p.window > 0) {
+            const int* at = p.positions + s.q0;
+            for (int w = 0; w < p.words; ++w) {
+              const unsigned long long x = tree_within(p.mask[(long long)(s.q0 + i) * p.words + w], 64 * w, s.n, at[i], at, p.window, p.keep);
+#pragma unroll
+              for (int e = 0; e < kTreeWords; ++e)
+                if (e == w) { seen[2 * e] |= (uint32_t)x; seen[2 * e + 1] |= (uint32_t)(x >> 32); }
+            }
+            continue;
+          }
 #pragma unroll
           for (int w = 0; w < kTreeWords * 2; ++w)
             if (w < 2 * p.words) seen[w] |= m[(long long)i * p.words * 2 + w];
+        }
 #pragma unroll
         for (int w = 0; w < kTreeWords * 2; ++w) {
           const uint32_t x = __reduce_or_sync(0xffffffffu, seen[w]);
@@ -354,14 +376,17 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
       }
       named_bar_sync(1, 64);
       for (int j = 0, cleaned = 0; j < nt; ++j) {
-        if (tile_at(j) < tail) continue;
+        if (!unseen(j)) continue;
         const int i = min(j + L, nt) + j, st = i % ST;   // of the ring's tiles, in order
         const uint32_t ph = i / ST & 1;
         // (these warps do not hold the ring back, so they ask the issuer which round it is in)
         if (!mbar_wait(&v_here, cleaned++ & 1, p.status, XFT_ERR_WAIT_FULL)) break;
         const int key = (warp - 2) * (KT / 2) + lane * (KT / 64);            // one or two keys a lane
         const int k0 = tile_at(j) * KT;
-        const uint32_t sees = tg_sees((unsigned long long)s_union[1] << 32 | s_union[0], s_union, k0 + (key & ~31), s.ctx, s.n) >> (key & 31);
+        const int k32 = k0 + (key & ~31);
+        uint32_t sees = tg_sees((unsigned long long)s_union[1] << 32 | s_union[0], s_union, k32, s.ctx, s.n);
+        if (EXT && p.window > 0) sees &= tg_context(k32, s.ctx, first_key, p.keep);
+        sees >>= key & 31;
         if (!mbar_wait(&full[st], ph, p.status, XFT_ERR_WAIT_FULL)) break;
         uint8_t* v = sT + st * S::kTile;
 #pragma unroll

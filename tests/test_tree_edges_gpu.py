@@ -79,3 +79,80 @@ def test_a_graph_captured_before_its_cache_grew_moves_nothing():
     torch.cuda.synchronize()
     assert int(count[0]) == 4 and all(k[0, 1, 10:14, 7].tolist() == [10, 11, 12, 13] for k in (old, *c.k))
     _ok()
+
+
+# -- attention --------------------------------------------------------------------------------------------------------
+def _close(got, q, kc, vc, table, cu, kv, bits, scale, ks=None, vs=None, **kw):
+    """`got` against 64 bits.  A weight is rounded to bf16 once, 2^-8 of it; the sum that divides has the rounded weights (the same again) or
+    the whole ones; the result is rounded to bf16.  Scores in 32 bits: D + 8 roundings of 2^-24 of sums of |q k| <= |q| |k|, which move a weight
+    and the denominator by as much; 2^-12: exponentials and divisions, far below."""
+    f64 = torch.float64
+    args = (table, cu, kv, bits, scale, ks, vs)
+    want = R.tree_attention(q, kc, vc, *args, dtype=f64, **kw)
+    size = R.tree_attention(q, kc, vc.abs(), *args, dtype=f64, **kw)
+    k = kc.double() * (1.0 if ks is None else ks.double()[..., None])
+    norms = float(q.double().norm(dim=-1).max()) * float(k.nan_to_num(0, 0, 0).norm(dim=-1).max())
+    score = 2 * (q.shape[2] + 8) * 2.0 ** -24 * norms * abs(scale)
+    bound = (2 * BF16 + score + 2.0 ** -12) * size + BF16 * 1.02 * want.abs() + 1e-30
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= bound).all()), (float((err / bound.clamp_min(1e-20)).max()), float(err.max()))
+
+
+def _where(table, p, bs):
+    return int(table[p // bs]), p % bs
+
+
+HEADS = [(64, 64, False), (128, 64, False), (256, 64, False), (128, 16, False), (128, 64, True), (64, 64, True), (256, 192, True)]
+
+
+@pytest.mark.parametrize("D,bs,int8", HEADS)
+@pytest.mark.parametrize("window,keep", [(7, 0), (100, 5), (64, 64), (130, 70), (1, 0), (1000, 3)])
+@pytest.mark.parametrize("spoil", [math.nan, math.inf])
+def test_values_that_a_window_leaves_to_no_node(D, bs, int8, window, keep, spoil):
+    lens = [(9, 300), (4, 0), (17, 64), (1, 700), (70, 130)]
+    g = torch.Generator().manual_seed(D + window)
+    _, flat, cu, kv, table, blocks = batch(lens, D + window, bs)
+    kc, vc, ks, vs = caches(g, blocks, 2, D, bs, int8)
+    q = torch.randn(cu[-1], 6, D, generator=g).bfloat16()
+    bits, pos = R.tree_mask(flat, cu, kv)
+    hidden = 0
+    for b, (n, c) in enumerate(lens):
+        first = int(pos[cu[b]:cu[b + 1]].min()) - window + 1
+        for p in range(c):
+            if p < first and p >= keep:
+                blk, off = _where(table[b], p, bs)
+                for t in (ks, vs) if int8 else (kc, vc):
+                    t[blk, :, off] = spoil
+                hidden += 1
+    assert hidden > 0 or window == 1000
+    c = lambda t: None if t is None else t.cuda()
+    got = ops.tree_attention(c(q), c(kc), c(vc), c(table), cu, kv, c(bits), D ** -0.5, c(ks), c(vs), window=window, keep_first=keep,
+                             positions=c(pos), meta=_meta(cu, kv, table))
+    _ok()
+    assert bool(torch.isfinite(got).all())
+    _close(got, q, kc, vc, table, cu, kv, bits, D ** -0.5, ks, vs, group=3, window=window, keep_first=keep, positions=pos)
+
+
+@pytest.mark.parametrize("D,bs,int8", HEADS)
+@pytest.mark.parametrize("ctx", [0, 3, 61, 200])
+def test_nodes_that_only_the_window_hides(D, bs, int8, ctx):
+    n, window = 70, 3
+    g = torch.Generator().manual_seed(D + ctx)
+    _, _, cu, kv, table, blocks = batch([(n, ctx)], 4, bs)
+    kc, vc, ks, vs = caches(g, blocks, 2, D, bs, int8)
+    q = torch.randn(n, 6, D, generator=g).bfloat16()
+    bits = torch.full((n, 2), -1, dtype=torch.int64)       # every node sees every one, but for the window
+    bits[[5, 66]] = 0                                      # these two see none, themselves neither
+    for j in (5, 66):
+        blk, off = _where(table[0], ctx + j, bs)
+        for t in (ks, vs) if int8 else (kc, vc):
+            t[blk, :, off] = math.nan
+    c = lambda t: None if t is None else t.cuda()
+    for keep in (0, 2):
+        pos = ctx + 10 + torch.arange(n, dtype=torch.int32) // 2
+        pos[[5, 66]] = keep                                # far behind all others, and not among the kept ones
+        got = ops.tree_attention(c(q), c(kc), c(vc), c(table), cu, kv, c(bits), D ** -0.5, c(ks), c(vs), window=window, keep_first=keep,
+                                 positions=c(pos), meta=_meta(cu, kv, table))
+        _ok()
+        assert bool(torch.isfinite(got).all())
+        _close(got, q, kc, vc, table, cu, kv, bits, D ** -0.5, ks, vs, group=3, window=window, keep_first=keep, positions=pos)
