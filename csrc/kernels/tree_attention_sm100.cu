@@ -62,6 +62,11 @@ __device__ __forceinline__ float tg_max3(float a, float b, float c) {
   asm("max.ftz.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float tg_min(float a, float b) {              // NaN where one of them is
+  float d;
+  asm("min.NaN.ftz.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float2 tg_fma2(float2 a, float2 b, float2 c) {
   float2 d;
   asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
@@ -499,7 +504,7 @@ __global__ void __launch_bounds__(TgShape<H, G, I8, TURNS>::kThreads, TgShape<H,
           for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              x[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(fminf(__uint_as_float(x[c][i]) * 2.8853900817779268f, 120.f))));
+              x[c][i] = __float_as_uint(cap - __fdividef(2.f * cap, 1.f + exp2f(tg_min(__uint_as_float(x[c][i]) * 2.8853900817779268f, 120.f))));
         }
       }
       const int k0 = tile_at(j) * KT;

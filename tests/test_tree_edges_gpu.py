@@ -156,3 +156,26 @@ def test_nodes_that_only_the_window_hides(D, bs, int8, ctx):
         _ok()
         assert bool(torch.isfinite(got).all())
         _close(got, q, kc, vc, table, cu, kv, bits, D ** -0.5, ks, vs, group=3, window=window, keep_first=keep, positions=pos)
+
+
+@pytest.mark.parametrize("D,bs,int8", HEADS)
+@pytest.mark.parametrize("gain", [0.01, 30.0])                 # scores far below the cap, and far above it
+@pytest.mark.parametrize("kw", [{}, {"softcap": 5.0}, {"softcap": 5.0, "sinks": True}])
+def test_a_key_that_is_not_a_number_makes_its_rows_so(D, bs, int8, gain, kw):
+    g = torch.Generator().manual_seed(D)
+    _, flat, cu, kv, table, blocks = batch([(9, 300), (12, 40)], 6, bs)
+    kc, vc, ks, vs = caches(g, blocks, 2, D, bs, int8)
+    q = (gain * torch.randn(cu[-1], 6, D, generator=g)).bfloat16()
+    bits, _ = R.tree_mask(flat, cu, kv)
+    seen = [torch.ones(9, dtype=torch.bool), (bits[9:, 0] >> 4 & 1).bool()]
+    for b, p in ((0, 77), (1, 40 + 4)):                    # a key of the context, and one that a branch sees
+        blk, off = _where(table[b], p, bs)
+        (ks if int8 else kc)[blk, 1, off] = math.nan       # of one head
+    kw = dict(kw, sinks=torch.randn(6, generator=g)) if "sinks" in kw else kw
+    c = lambda t: t.cuda() if isinstance(t, torch.Tensor) else t
+    got = ops.tree_attention(c(q), c(kc), c(vc), c(table), cu, kv, c(bits), 0.3, c(ks), c(vs), meta=_meta(cu, kv, table),
+                             **{n: c(v) for n, v in kw.items()}).cpu()
+    _ok()
+    assert 0 < int(seen[1].sum()) < 12
+    assert bool(torch.isfinite(got[:, :3]).all())
+    assert torch.equal(torch.isnan(got[:, 3:]).all(-1).all(-1), torch.cat(seen)) and bool(torch.isfinite(got[:, 3:][~torch.cat(seen)]).all())
