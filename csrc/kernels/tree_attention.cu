@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeAttnArgs p) {
   grid_dep_wait();
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (row >= (long long)min(p.T, p.cu_q[p.B]) * p.hq) return;
+  if (row < (long long)p.cu_q[0] * p.hq || row >= (long long)min(p.T, p.cu_q[p.B]) * p.hq) return;          // of no sequence
   float2 ml[2];                                          // slices lane and lane + 32
   float mx = -INFINITY;
 #pragma unroll

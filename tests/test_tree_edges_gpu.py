@@ -179,3 +179,30 @@ def test_a_key_that_is_not_a_number_makes_its_rows_so(D, bs, int8, gain, kw):
     assert 0 < int(seen[1].sum()) < 12
     assert bool(torch.isfinite(got[:, :3]).all())
     assert torch.equal(torch.isnan(got[:, 3:]).all(-1).all(-1), torch.cat(seen)) and bool(torch.isfinite(got[:, 3:][~torch.cat(seen)]).all())
+
+
+@pytest.mark.parametrize("lens", [[(9, 40), (4, 70)], [(9, 9000), (4, 70)], [(1, 3)]])         # (the second: several slices, joined)
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("with_meta", [False, True])
+def test_rows_in_front_of_the_first_sequence(lens, bs, with_meta):
+    g = torch.Generator().manual_seed(bs)
+    _, flat, cu, kv, table, blocks = batch(lens, 3, bs)
+    kc, vc, _, _ = caches(g, blocks, 2, 128, bs)
+    q = torch.randn(cu[-1] + 8, 8, 128, generator=g).bfloat16().cuda()
+    kc, vc, table = kc.cuda(), vc.cuda(), table.cuda()
+    n, up = cu[-1], torch.cat([torch.full((5,), 7, dtype=torch.int32), flat, torch.full((3,), 7, dtype=torch.int32)]).cuda()
+    later = [x + 5 for x in cu]
+    meta = _meta(later, kv, table) if with_meta else None
+    want, want_pos = ops.tree_mask(flat.cuda(), cu, kv)
+    for _ in range(4):
+        torch.full((1 << 22,), math.nan, device="cuda")    # what a fresh output may find in its memory
+        mask, pos = ops.tree_mask(up, later, kv, meta)
+        assert torch.equal(mask[5:n + 5], want) and torch.equal(pos[5:n + 5], want_pos)
+        assert not any(bool(t[rows].any()) for t in (mask, pos) for rows in (slice(0, 5), slice(n + 5, None)))
+        got = ops.tree_attention(q, kc, vc, table, later, kv, mask, 0.1, meta=meta)
+        assert torch.equal(got[5:n + 5], ops.tree_attention(q[5:n + 5].contiguous(), kc, vc, table, cu, kv, want, 0.1))
+        assert not bool(got[:5].any()) and not bool(got[n + 5:].any())
+    tokens = torch.zeros(n + 8, dtype=torch.long, device="cuda")
+    _, path, count = ops.tree_accept(tokens, up, tokens, later, kv, meta=meta)
+    assert torch.equal(path.cpu(), R.tree_accept(tokens.cpu(), up.cpu(), tokens.cpu(), later, kv)[1])
+    _ok()

@@ -420,7 +420,7 @@ def tree_mask(parents, cu_q, kv_lens, meta=None):
     """What the nodes of trees see of each other, and where they stand: (mask int64 [T, words], bit j of word j // 64 for every node j on the
     way from a node to its root, itself included; positions int32 [T], context + distance from the root).  `parents` [T]: index of a node's
     parent in its own tree, before the node; below zero: a root.  A GPU reports a parent that comes later in the status word and takes the
-    node as a root.  Rows behind the last sequence (of the lists) are zero."""
+    node as a root.  Rows of no sequence (of the lists) are zero."""
     if parents.dim() != 1 or parents.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tree_mask: parents are int32 or int64 [T], not {tuple(parents.shape)} in {parents.dtype}")
     _check_trees("tree_mask", parents.numel(), cu_q, kv_lens, meta, parents.device)
@@ -434,7 +434,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     """Attention of trees' nodes q [T, Hq, D] over the paged cache: a node sees the context before the tree and the nodes that its `mask`
     (int64 [T, words], see tree_mask; any other choice of nodes will do) has; one that sees nothing gives zeros.  Other arguments as in
     paged_attention; `window` counts in `positions` (int32 [T], needed with it).  A GPU takes bf16 queries over bf16 or int8 caches, D
-    64, 128 or 256.  Of keys that some node sees, the values are finite.  Rows behind the last sequence (of the lists) are zero."""
+    64, 128 or 256.  Of keys that some node sees, the values are finite.  Rows of no sequence (of the lists) are zero."""
     if q.dim() != 3 or kc.dim() != 4 or vc.shape != kc.shape or q.shape[2] != kc.shape[3]:
         raise ValueError(f"tree_attention: queries {tuple(q.shape)} over keys {tuple(kc.shape)} and values {tuple(vc.shape)}")
     T, hq, D = q.shape

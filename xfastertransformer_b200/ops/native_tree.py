@@ -72,8 +72,8 @@ def _arrays(cu_q, kv_lens, meta, dev):
 
 
 def _padded(cu_q, T) -> bool:
-    """Whether there are rows behind the last sequence."""
-    return isinstance(cu_q, (list, tuple)) and len(cu_q) > 0 and cu_q[-1] < T
+    """Whether there are rows in front of the first sequence or behind the last one."""
+    return isinstance(cu_q, (list, tuple)) and len(cu_q) > 0 and (cu_q[0] > 0 or cu_q[-1] < T)
 
 
 def tree_mask(parents, cu_q, kv_lens, meta=None):
