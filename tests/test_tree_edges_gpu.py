@@ -206,3 +206,15 @@ def test_rows_in_front_of_the_first_sequence(lens, bs, with_meta):
     _, path, count = ops.tree_accept(tokens, up, tokens, later, kv, meta=meta)
     assert torch.equal(path.cpu(), R.tree_accept(tokens.cpu(), up.cpu(), tokens.cpu(), later, kv)[1])
     _ok()
+
+
+# -- sampling ---------------------------------------------------------------------------------------------------------
+def test_limits_beyond_32_bits():
+    g = torch.Generator().manual_seed(6)
+    x, u = torch.randn(8, 500, generator=g), torch.rand(8, generator=g)
+    k = torch.tensor([2 ** 32 + 5, 2 ** 31, 2 ** 31 - 1, -2 ** 31 - 1, -2 ** 32 + 3, 5, 2 ** 62, -2 ** 63])
+    want = R.sample(x, 1.0, k, 1.0, 0.0, u)
+    assert torch.equal(ops.sample(x.cuda(), 1.0, k.cuda(), 1.0, 0.0, u.cuda()).cpu(), want)
+    for n in k.tolist():
+        for one in (n, torch.tensor(n), torch.tensor([n], device="cuda")):
+            assert torch.equal(ops.sample(x.cuda(), 1.0, one, 1.0, 0.0, u.cuda()).cpu(), R.sample(x, 1.0, n, 1.0, 0.0, u))

@@ -894,7 +894,7 @@ MAX_SAMPLE_VOCAB = 1 << 21
 
 def sample(logits, temperature, top_k, top_p, min_p, uniform):
     """A token id (int64) per row of `logits` [.., V], every row with its own parameters (tensors with one number per row, or one number
-    for all, taken as fp32 and int32).  A row is ordered by logit, equal ones by index, and weighed w = exp((x - max) / temperature).  Kept
+    for all, taken as fp32 and whole numbers).  A row is ordered by logit, equal ones by index, and weighed w = exp((x - max) / temperature).  Kept
     are the first `top_k` (<= 0: all), of these the ones with less than `top_p` of their mass in front of them (>= 1: all), of these the
     ones with w >= `min_p` (<= 0: all), the first in any case; the token is the first one up to which more than `uniform` (in [0, 1)) of the
     kept mass lies.  A temperature <= 0 gives the first of the row.  A logit that is NaN counts as -inf; a row without another gives -1."""

@@ -165,6 +165,8 @@ def _per_row(v, rows, dtype, dev):
         return v, 0
     if v.numel() == 1 and rows != 1:
         v = v.reshape(1).expand(rows)
+    if dtype is torch.int32 and v.dtype is torch.int64:                 # (beyond 32 bits: as good as none, and not the low 32 bits)
+        v = v.clamp(-1, 2 ** 31 - 1)
     return v.to(device=dev, dtype=dtype).contiguous(), 0
 
 
