@@ -81,6 +81,23 @@ def test_a_graph_captured_before_its_cache_grew_moves_nothing():
     _ok()
 
 
+def test_parents_beyond_32_bits():
+    from xfastertransformer_b200.ops import native as N
+    up = torch.tensor([-2 ** 40, 0, -2 ** 32, 1, -2 ** 32 + 1])
+    cu, kv = [0, 5], [9]
+    mask, pos = ops.tree_mask(up.cuda(), cu, kv)
+    want = R.tree_mask(up, cu, kv)
+    assert torch.equal(mask.cpu(), want[0]) and torch.equal(pos.cpu(), want[1])
+    tokens, sampled = torch.zeros(5, dtype=torch.long), torch.zeros(5, dtype=torch.long)
+    for a, b in zip(ops.tree_accept(tokens.cuda(), up.cuda(), sampled.cuda(), cu, kv), R.tree_accept(tokens, up, sampled, cu, kv)):
+        assert torch.equal(a.cpu(), b)
+    _ok()
+    mask, _ = ops.tree_mask(torch.tensor([-1, 2 ** 32, 1], device="cuda"), [0, 3], [3])
+    assert mask[:, 0].tolist() == [1, 2, 6]               # reported, and taken as a root
+    with pytest.raises(N.KernelError):
+        N.Workspace.get(torch.device("cuda", 0)).check_status()
+
+
 # -- attention --------------------------------------------------------------------------------------------------------
 def _close(got, q, kc, vc, table, cu, kv, bits, scale, ks=None, vs=None, **kw):
     """`got` against 64 bits.  A weight is rounded to bf16 once, 2^-8 of it; the sum that divides has the rounded weights (the same again) or

@@ -55,7 +55,8 @@ def _ptr(t) -> int:
 
 
 def _i32(t):
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.int().contiguous()
+    """Parents as the kernels take them: of int64 ones, those beyond 32 bits stay below zero or behind every node."""
+    return t.contiguous() if t.dtype is torch.int32 else t.clamp(-1, 2 ** 31 - 1).int().contiguous()
 
 
 def _arrays(cu_q, kv_lens, meta, dev):
