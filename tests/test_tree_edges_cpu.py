@@ -88,3 +88,12 @@ def test_the_handle_of_a_cache_is_made_once_and_refused_when_its_pools_have_move
     c.k[1][0, :, 10:16] = torch.arange(10, 16)[:, None]
     ops.tree_accept(*chain_with_gaps(), new)
     assert c.k[1][0, 1, 10:14, 3].tolist() == [10, 12, 14, 15]
+
+
+def test_attention_of_a_share_without_heads():
+    m, t = torch.ones(4, 1, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int32)
+    for hkv in (0, 2):
+        c = torch.zeros(2, hkv, 64, 64)
+        assert ops.tree_attention(torch.zeros(4, 0, 64), c, c, t, [0, 4], [70], m, 0.1).shape == (4, 0, 64)
+    with pytest.raises(ValueError):                       # queries that have no keys
+        ops.tree_attention(torch.zeros(4, 2, 64), torch.zeros(2, 0, 64, 64), torch.zeros(2, 0, 64, 64), t, [0, 4], [70], m, 0.1)

@@ -225,6 +225,17 @@ def test_rows_in_front_of_the_first_sequence(lens, bs, with_meta):
     _ok()
 
 
+@pytest.mark.parametrize("hkv", [0, 2])
+@pytest.mark.parametrize("ctx", [10, 9000])
+def test_a_share_without_heads(hkv, ctx):
+    _, _, cu, kv, table, blocks = batch([(9, ctx)], 3)
+    q, c = torch.zeros(9, 0, 128, device="cuda").bfloat16(), torch.zeros(blocks, hkv, 64, 128, device="cuda").bfloat16()
+    bits = torch.ones(9, 1, dtype=torch.int64, device="cuda")
+    assert ops.tree_attention(q, c, c, table.cuda(), cu, kv, bits, 0.1).shape == (9, 0, 128)
+    assert torch.ones(3, device="cuda").sum().item() == 3   # no error is left behind
+    _ok()
+
+
 # -- sampling ---------------------------------------------------------------------------------------------------------
 def test_limits_beyond_32_bits():
     g = torch.Generator().manual_seed(6)

@@ -439,7 +439,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
         raise ValueError(f"tree_attention: queries {tuple(q.shape)} over keys {tuple(kc.shape)} and values {tuple(vc.shape)}")
     T, hq, D = q.shape
     nb, hkv, bs, _ = kc.shape
-    group = group or max(hq // hkv, 1)
+    group = group or max(hq // max(hkv, 1), 1)
     if group < 1 or q_off < 0 or (hq and (hq - 1 + q_off) // group >= hkv):
         raise ValueError(f"tree_attention: {hq} query heads from {q_off} on in groups of {group} over {hkv} heads of keys")
     if not kc.is_contiguous() or not vc.is_contiguous() or kc.dtype != vc.dtype:

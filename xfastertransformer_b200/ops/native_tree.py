@@ -139,7 +139,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     cu, kv, B, most, longest = _arrays(cu_q, kv_lens, meta, dev)
     out = torch.zeros_like(q) if _padded(cu_q, T) else torch.empty_like(q)
-    if not (T and B and most):
+    if not (T and hq and B and most):
         return out
     ws = N.Workspace.get(dev)
     form, n = _plan(B, hkv, most * group, T * hq, D, min(longest, window + keep_first + most + 256) if window else longest,
