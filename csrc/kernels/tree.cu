@@ -210,7 +210,7 @@ extern "C" int xft_tree_accept(const char* packed, cudaStream_t st) {
   TreeAcceptArgs a;
   memcpy(&a, packed, sizeof(a));
   if (a.t.B <= 0) return 0;
-  if (a.width < 1 || a.n_pools < 0 || (a.n_pools > 0 && (a.bs < 1 || !a.table))) return -1;
+  if (a.t.B > 65535 || a.width < 1 || a.n_pools < 0 || (a.n_pools > 0 && (a.bs < 1 || !a.table))) return -1;
   const int per = kAcceptThreads / 32;
   const cudaError_t e = launch_pdl(tree_accept_kernel, dim3(a.n_pools ? (a.n_pools + per - 1) / per : 1, a.t.B), dim3(kAcceptThreads), 0, st, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();

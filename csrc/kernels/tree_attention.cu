@@ -361,8 +361,8 @@ extern "C" int xft_tree_attention(const char* packed, cudaStream_t st) {
   TreeAttnArgs a;
   memcpy(&a, packed, sizeof(a));
   if (a.B <= 0 || a.T <= 0 || a.max_q <= 0) return 0;
-  if (a.max_q > 64 * a.words || a.words > kTreeWords || a.group < 1 || a.nsplit < 1 || a.nsplit > 64 || (a.nsplit > 1 && (!a.part_o || !a.part_ml)) ||
-      (a.window > 0 && !a.positions) || a.bs < 1)
+  if (a.B > 65535 || a.max_q > 64 * a.words || a.words > kTreeWords || a.group < 1 || a.nsplit < 1 || a.nsplit > 64 ||
+      (a.nsplit > 1 && (!a.part_o || !a.part_ml)) || (a.window > 0 && !a.positions) || a.bs < 1)
     return -1;
   int rc = -1;
   const bool i8 = a.ks != nullptr;

@@ -236,6 +236,25 @@ def test_a_share_without_heads(hkv, ctx):
     _ok()
 
 
+def test_more_sequences_than_a_grid_has_rows():
+    from xfastertransformer_b200.ops import native as N
+    B = 65536
+    cu, kv = list(range(B + 1)), [1] * B
+    up, tokens = torch.full((B,), -1, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.long, device="cuda")
+    mask, pos = ops.tree_mask(up, cu, kv)
+    assert bool((mask == 1).all()) and not bool(pos.any())
+    c, table = torch.ones(1, 1, 64, 64, device="cuda").bfloat16(), torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    q = torch.zeros(B, 1, 64, device="cuda").bfloat16()
+    for f in (lambda: ops.tree_accept(tokens, up, tokens, cu, kv), lambda: ops.tree_attention(q, c, c, table, cu, kv, mask, 0.1)):
+        with pytest.raises(N.KernelError):
+            f()
+        assert torch.ones(3, device="cuda").sum().item() == 3           # no error is left behind
+    count = ops.tree_accept(tokens[1:], up[1:], tokens[1:], cu[:-1], kv[1:])[2]
+    assert bool((count == 1).all())
+    assert bool((ops.tree_attention(q[1:], c, c, table[1:], cu[:-1], kv[1:], mask[1:], 0.1) == 1).all())
+    _ok()
+
+
 # -- sampling ---------------------------------------------------------------------------------------------------------
 def test_limits_beyond_32_bits():
     g = torch.Generator().manual_seed(6)

@@ -72,6 +72,14 @@ def _arrays(cu_q, kv_lens, meta, dev):
     return cu, kv, kv.numel(), max(n, default=0), max(kv_lens, default=0)
 
 
+MAX_SEQUENCES = 65535                # of one launch: the grid has a row of CTAs for each
+
+
+def _few(what, B):
+    if B > MAX_SEQUENCES:
+        raise N.KernelError(f"{what}: up to {MAX_SEQUENCES} sequences at a time, not {B}")
+
+
 def _padded(cu_q, T) -> bool:
     """Whether there are rows in front of the first sequence or behind the last one."""
     return isinstance(cu_q, (list, tuple)) and len(cu_q) > 0 and (cu_q[0] > 0 or cu_q[-1] < T)
@@ -141,6 +149,7 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     out = torch.zeros_like(q) if _padded(cu_q, T) else torch.empty_like(q)
     if not (T and hq and B and most):
         return out
+    _few("tree_attention", B)
     ws = N.Workspace.get(dev)
     form, n = _plan(B, hkv, most * group, T * hq, D, min(longest, window + keep_first + most + 256) if window else longest,
                     (D == 128 or ks is None) and bs % 64 == 0 and (scale > 0 or softcap > 0) and nb * hkv * bs < 2 ** 31 and (_ptr(ks) | _ptr(vs)) % 16 == 0,
@@ -226,6 +235,7 @@ def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table, pools, met
     parents = _i32(parents)
     tokens, sampled = (t if t.dtype is torch.int64 and t.is_contiguous() else t.long().contiguous() for t in (tokens, sampled))
     cu, kv, B, most, _ = _arrays(cu_q, kv_lens, meta, dev)
+    _few("tree_accept", B)
     T = tokens.numel()
     emitted, path, count = tokens.new_empty((B, most)), parents.new_empty((B, most)), parents.new_empty(B)
     if B and most:
