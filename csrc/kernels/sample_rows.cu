@@ -101,6 +101,7 @@ struct SampleShared {
   unsigned n_list, at;
   int what, from, to, sub;                               // the next round: see Round
   u64 base;
+  u64 rest;                                              // of the bins' mass, beside the first round's elements
 };
 
 enum Round { kDone, kAlone, kAll, kFirst, kShare, kLeast, kPick };
@@ -195,11 +196,19 @@ __device__ __noinline__ void place(const SampleRow& r, SampleShared& sh, bool by
   upto = done_m + r.mass(r.weight(r.at((int)index)));
 }
 
-// Mass that a share of it has to reach, and that a token's running mass has to exceed
-__device__ __forceinline__ u64 reach(float p, u64 mass) { return (u64)ceil(fmax((double)p, 0.0) * (double)mass); }
-__device__ __forceinline__ u64 exceed(float u, u64 mass) {
-  return min((u64)(fmin(u > 0.f ? (double)u : 0.0, 1.0 - 0x1p-24) * (double)mass), mass - 1);
+// f * mass, 0 <= f < 1, in whole numbers: down, or up.  (A product in 64-bit floats is off by more than nothing where a share ends between two of
+// many equal logits, and that decides which of them it is.)
+__device__ u64 share(float f, u64 mass, bool up) {
+  const uint32_t bits = __float_as_uint(f), e = max(bits >> 23, 1u), digits = bits >> 23 ? (bits & 0x7fffffu) | 0x800000u : bits;
+  const u64 lo = mass * digits, hi = __umul64hi(mass, digits);             // f = digits 2^(e - 150)
+  const int by = 150 - (int)e;                           // at least 24, and hi is below 2^24
+  const u64 whole = by < 64 ? hi << (64 - by) | lo >> by : by < 128 ? hi >> (by - 64) : 0;
+  const u64 rest = by < 64 ? lo << (64 - by) : by == 64 ? lo : by < 128 ? lo | hi << (128 - by) : lo | hi;
+  return whole + (up && rest != 0);
 }
+// Mass that a share of it has to reach, and that a token's running mass has to exceed
+__device__ __forceinline__ u64 reach(float p, u64 mass) { return p > 0.f ? share(p, mass, true) : 0; }
+__device__ __forceinline__ u64 exceed(float u, u64 mass) { return u > 0.f ? share(fminf(u, 1.f - 0x1p-24f), mass, false) : 0; }
 
 __device__ __noinline__ unsigned alone(const SampleRow& r, SampleShared& sh, const SampleLimits& lim) {
   u64 all = 0, over = 0, before;
@@ -682,10 +691,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     return make_int4(kPick, b, b, 0);
   };
   // the first CTA: the mass that a round's sorted list leaves, and in the last round the token
+  bool first = settled && !counts;                       // (else there are no masses of bins)
   auto settle = [&](const auto& l, const int4& todo) -> u64 {
     const bool all = todo.x == kAll;
     int at;
-    u64 some, left = sharp ? l.end : kept;
+    // in the first round the elements' own masses take the place of their bins', which are good to 2^-27 of each
+    u64 some, left = sharp ? l.end : first ? sh.rest + l.end - (all ? 0 : sh.base) : kept;
     if (all && lim.k > 0) l.first(sh, [&](int i, u64) { return i + 1 >= lim.k; }, at, left);
     if (todo.x == kFirst) l.first(sh, [&](int i, u64) { return i + 1 >= lim.k - todo.w; }, at, left);
     some = left;
@@ -712,6 +723,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     todo = b < kSampleBins ? make_int4(kAll, 0, b, 0) : t <= 1.9f ? make_int4(kAll, 0, kSampleBins - 1, 0) : make_int4(kAlone, 0, 0, 0);
   } else {
     todo = next(kDone);
+    const u64 base = todo.x == kAll ? 0 : sh.base;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (todo.x > kAlone && 2 * tid + e == todo.z) sh.rest = kept - (upto[e] - base);
+    __syncthreads();
   }
   while (todo.x > kAlone) {
     // a bin of too many elements: its 1024 parts are counted as the bins were, and the part is taken that the place lies in
@@ -760,7 +776,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
           const unsigned every = (unsigned)sh.found[0];
           s2 = bin_of(sh, k2, c2, [&](unsigned c) { return c >= every; }, front);
         }
-        if (2 * tid <= s2 && s2 < 2 * tid + 2) { sh.base = u2[s2 & 1] - m2[s2 & 1]; sh.found[0] = k2[s2 & 1] - c2[s2 & 1]; }
+        if (2 * tid <= s2 && s2 < 2 * tid + 2) {
+          sh.base = u2[s2 & 1] - m2[s2 & 1];
+          sh.rest = kept - m2[s2 & 1];
+          sh.found[0] = k2[s2 & 1] - c2[s2 & 1];
+        }
         __syncthreads();
         todo.w += (int)sh.found[0];
         __syncthreads();
@@ -823,6 +843,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
           kept = n <= kSampleThreads ? settle(ListMasses<1, false>(r, sh, n, base), todo)
                                      : settle(ListMasses<4, false>(r, sh, n, base), todo);
         }
+        first = false;
         todo = last ? make_int4(kDone, 0, 0, 0) : next(todo.x);
       }
       __syncthreads();

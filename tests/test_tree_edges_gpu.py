@@ -265,3 +265,34 @@ def test_limits_beyond_32_bits():
     for n in k.tolist():
         for one in (n, torch.tensor(n), torch.tensor([n], device="cuda")):
             assert torch.equal(ops.sample(x.cuda(), 1.0, one, 1.0, 0.0, u.cuda()).cpu(), R.sample(x, 1.0, n, 1.0, 0.0, u))
+
+
+def _equal_rows(n, k, p, u):
+    """Place of the token in a row of n equal logits, in whole numbers: the first ceil(p min(k, n)), of them the one behind a share u."""
+    from fractions import Fraction
+    n = min(k, n) if k > 0 else n
+    if p < 1:
+        n = max(1, math.ceil(Fraction(p) * n))
+    return int(Fraction(u) * n)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 8, 100, 128, 1000, 1024, 1536, 2048, 2049, 5000, 8192, 32000, 1 << 18])
+@pytest.mark.parametrize("fill", [None, -math.inf, -1e4])      # nothing else in the row, or what weighs nothing
+def test_equal_logits_at_the_borders_of_equal_shares(n, fill):
+    u = torch.arange(0, 64) / 64.0
+    u[-1] = 1 - 2.0 ** -24
+    V = n if fill is None else 2 * n + 5
+    for top in (1.25, -3.7, 0.0, 41.3):
+        x = torch.full((64, V), top)
+        at = torch.arange(n)
+        if fill is not None:
+            at = torch.randperm(V, generator=torch.Generator().manual_seed(n))[:n].sort().values
+            x = torch.full((64, V), fill)
+            x[:, at] = top
+        x = x.cuda()
+        for T, k, p, m in ((1.0, 0, 1.0, 0.0), (0.7, 0, 0.5, 0.0), (1.0, 0, 0.375, 0.2), (3.0, 0, 0.75, 0.0), (0.9, 0, 1.0, 0.5), (1.1, n // 2, 1.0, 0.0),
+                           (0.6, n // 2, 0.5, 0.0), (1.3, 40, 0.25, 0.1), (0.01, 0, 0.5, 0.0), (1.0, 1600, 0.625, 0.0), (2.1, 1, 0.5, 0.0)):
+            if T > 2 and fill == -1e4:
+                continue
+            got = ops.sample(x, T, k, p, m, u.cuda()).tolist()
+            assert got == [int(at[_equal_rows(n, k, p, v)]) for v in u.tolist()], (top, T, k, p, m)
