@@ -481,7 +481,7 @@ def make_handler(sched: Scheduler, tok: Tokenizer, model_name: str):
                         seed = q.get("seed")
                         reqs.append(Request(ids, int(q.get("max_tokens", 16)), temp, float(q.get("top_p", 1.0)),
                                             int(q.get("top_k", 0)), stop_ids, None if seed is None else int(seed) + 7919 * k,
-                                            float(q.get("repetition_penalty", 1.0)), lp, stop_fn, float(q.get("min_p", 0.0))))
+                                            float(q.get("repetition_penalty", 1.0)), lp, stop_fn, float(q.get("min_p") or 0.0)))
             except Exception as e:
                 return self._json(400, {"error": {"message": str(e), "type": "invalid_request_error"}})
             if sched.max_queue > 0 and sched.waiting.qsize() + len(reqs) > sched.max_queue:

@@ -97,3 +97,25 @@ def test_attention_of_a_share_without_heads():
         assert ops.tree_attention(torch.zeros(4, 0, 64), c, c, t, [0, 4], [70], m, 0.1).shape == (4, 0, 64)
     with pytest.raises(ValueError):                       # queries that have no keys
         ops.tree_attention(torch.zeros(4, 2, 64), torch.zeros(2, 0, 64, 64), torch.zeros(2, 0, 64, 64), t, [0, 4], [70], m, 0.1)
+
+
+def test_the_server_takes_a_min_p_of_null(tmp_path, monkeypatch):
+    import json
+    import urllib.request
+    import xfastertransformer_b200 as xft
+    from serving import openai_server
+    from xfastertransformer_b200.tools.synthetic import preset, write_synthetic_checkpoint
+    monkeypatch.setenv("XFT_ENGINE", "CPU")
+    write_synthetic_checkpoint(str(tmp_path), preset("tiny-llama", vocab_size=500), seed=3, dtype="fp32", std=0.1)
+    httpd, sched, port = openai_server.serve(xft.AutoModel.from_pretrained(str(tmp_path), dtype="bf16"), 0, max_batch=4, model_name="tiny")
+
+    def post(**body):
+        body = json.dumps({"prompt": [5, 9, 100], "max_tokens": 4, **body}).encode()
+        req = urllib.request.Request(f"http://127.0.0.1:{port}/v1/completions", data=body, headers={"Content-Type": "application/json"})
+        return json.loads(urllib.request.urlopen(req, timeout=120).read())["choices"][0]["text"]
+    try:
+        assert post(min_p=None) == post()                 # as without it, which is what it was before the field had a meaning
+        assert post(min_p=1.0, temperature=0.9, seed=1, top_k=-1) == post()
+    finally:
+        sched.shutdown()
+        httpd.shutdown()
