@@ -119,3 +119,10 @@ def test_the_server_takes_a_min_p_of_null(tmp_path, monkeypatch):
     finally:
         sched.shutdown()
         httpd.shutdown()
+
+
+def test_a_limit_of_any_size():
+    x, u = torch.randn(3, 50, generator=torch.Generator().manual_seed(1)), torch.tensor([0.1, 0.5, 0.9])
+    want = ops.sample(x, 1.0, 0, 0.9, 0.01, u)
+    for k in (50, 2 ** 31, 2 ** 63, 10 ** 30, -2 ** 63 - 1, -10 ** 30):          # a request's number may be any
+        assert torch.equal(ops.sample(x, 1.0, k, 0.9, 0.01, u), want)

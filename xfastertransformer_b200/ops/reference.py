@@ -962,7 +962,7 @@ def sample(logits: torch.Tensor, temperature, top_k, top_p, min_p, uniform) -> t
     rows = l2.shape[0]
     row = lambda v, t: torch.as_tensor(v, dtype=t).reshape(-1, 1).expand(rows, 1)
     T, p, m, u = (row(v, torch.float32).double() for v in (temperature, top_p, min_p, uniform))
-    k = row(top_k, torch.int64)
+    k = row(top_k if isinstance(top_k, torch.Tensor) else max(-1, min(int(top_k), V)), torch.int64)
     x, idx = torch.sort(torch.where(l2.isnan(), -torch.inf, l2).double() + 0.0, dim=1, descending=True, stable=True)
     top = x[:, :1]
     z = (x - top) / torch.where(T > 0, T, 1.0)
