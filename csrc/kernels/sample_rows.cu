@@ -7,11 +7,14 @@
 // Each limit keeps a beginning of that order, so the smallest of the three masses is the mass of what all keep, and the token is the
 // element of the whole row at which the running mass passes u times that.  Everything comes down to finding the place in the order
 // where a count or a mass is reached; the row is never sorted.  Masses are whole numbers, 2^shift w, so their sums do not depend on an
-// order.  They have to be exact to far below an element's share, or another token comes out than exact arithmetic's: tokens are equal
-// but for a probability of about 2^-35 per kept element.
+// order, and shares of them are taken in whole numbers, so that equal logits share evenly.  They have to be exact to far below an element's
+// share, or another token comes out than exact arithmetic's.  A weight of an element that a round gathers is one of 64 bits; the other bins'
+// sums are off by up to 2^-27.4 of each weight, by the same in a bin of equal logits, less the more different ones there are.  Of 5.5 million
+// rows of 1 to 2 million logits, a tenth of them with u within 10^-6 of 1, where borders are dense, 84 tokens were others than in 64 bits: those whose
+// border lay within 2^-34 of the kept mass from u, and one, in a row of a million logits of few values, 2^-30.
 //
-// A row is read once from memory, by a cluster of up to 8 CTAs with a slice each, which few rows' CTAs hold in shared memory and many rows'
-// read again from L2 for the few elements of step 3:
+// A row is read from memory by a cluster of up to 8 CTAs with a slice each, which few rows' CTAs hold in shared memory.  Many rows' read
+// theirs again for the few elements of step 3, from L2 as far as it holds them (512 rows of 151936, top-p: 717 MB from HBM for 311 MB):
 //   1. a histogram of each slice, 1024 bins down from about the slice's largest logit on a grid that is the same for the whole row, 16 bins
 //      a factor of two in w (counts alone, 16 bins per logit, where k is small enough for step 3 to take all of the first k): a bin's mass is
 //      its middle's weight times the sum of 2^e, e the distance from the middle in octaves, by a polynomial, from a distance that is
@@ -19,14 +22,17 @@
 //      times slower).  What weighs less than 2^-48 of the largest is left out;
 //   2. the bins' sums, exchanged over the cluster; every CTA finds the bins where the limits and the token can lie;
 //   3. those bins' elements, or all up to there if those are at most 2048, go to the first CTA, which sorts them, weighs them in 64
-//      bits and finds the place; one more such round for each limit whose elements are too many.  A bin of more than 2048 is cut in 1024
-//      parts in the same way first.  The other CTAs leave before the last round.
-// What that does not settle (more than 2048 equal logits or nearly so, a limit among weights that are left out, logits of
-// which a bin is less than 32 bits resolve) the first CTA settles alone, digit by digit of the 64-bit number (image of the logit, ~index),
-// whose unsigned order is the row's.
+//      bits and finds the place; one more such round for each limit whose elements are too many.  A bin of more than 2048 at the place of a
+//      k above 1536, of a share or of the token is cut in 1024 parts in the same way first.  The other CTAs leave before the last round.
+// What that does not settle the first CTA settles alone, digit by digit of the 64-bit number (image of the logit, ~index), whose unsigned
+// order is the row's: more than 2048 equal logits or nearly so at such a place; more than 2048 within 1/16 of a logit where a k of up to 1536
+// ends; more than 2048 in the three bins around the weight min_p; a limit among weights that are left out; logits of which a bin is
+// less than 32 bits resolve.  us: a row of 32000 equal logits 260, of 152064 1210; min-p of 0.02 to 0.1 at T = 2 to 3 over 128256
+// normal logits of deviation 2.2, whose border is so crowded, 680, 64 such rows 790 (T = 1.5: 28 and 63).
 //
-// Bound by the serial steps of a cluster where rows are few (a row of 32000 10 us), by instructions and the atomics where they are many (512
-// rows of 151936, top-p, 289 us; their bytes take 48).
+// Bound by the serial steps of a cluster where rows are few (a row of 32000 10.7 us), by instructions and the atomics where they are many (512
+// rows of 151936, top-p, 295 us, their bytes take 48: 75 instructions a logit in all, of which its place in the bins and its weight there take 27, the
+// rest are the atomics, the search for the largest and two more passes for the elements of the share and of the token).
 #include "ptx.cuh"
 
 #include <type_traits>
@@ -719,7 +725,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   } else if (counts) {
     u64 base;
     const int b = bin_of(sh, count, cnt, [&](u64 c) { return c >= (u64)lim.k; }, base);
-    // fewer than k in the bins, as where most of a row is masked: what is 64 logits below the largest has no weight, unless T is above 1.9
+    // fewer than k in the bins, as where most of a row is masked: what is 64 logits below the largest (48, where the bins begin above it) has no
+    // weight, unless T is above 1.9: the k elements that are left out, at most 1536, weigh less than 2^-48 (2^-36) of it each, together less
+    // than a third of the step between two numbers u below 1
     todo = b < kSampleBins ? make_int4(kAll, 0, b, 0) : t <= 1.9f ? make_int4(kAll, 0, kSampleBins - 1, 0) : make_int4(kAlone, 0, 0, 0);
   } else {
     todo = next(kDone);

@@ -3,13 +3,13 @@
 //
 // The rows (node, query head) of one kv head share its keys: 128 rows a tile, one row per TMEM lane and thread, one tile a CTA, two CTAs
 // an SM (heads of 256: one).  CTAs with other rows over the same keys run beside one another and find them in L2; two tiles of rows in a
-// CTA over the same keys were no faster (512 rows x 65600 keys, 8 heads: 147 us, one tile 146).  For each tile of keys
+// CTA over the same keys were no faster (512 rows x 65600 keys, 8 heads: 137 to 147 us, one tile 143 to 147).  For each tile of keys
 //
 //   S = Q K^T   tcgen05.mma, both operands from shared memory; the keys come by TMA, in pieces of 64 by the block table
 //   P = exp2(S - m) as bf16 over S, whole rows in registers; the sum of a row beside it
 //   O += P V    tcgen05.mma, P from TMEM, V as it lies in the cache (MN-major)
 //
-// Bound, for many rows over a key, by the steps between products and softmax (512 rows x 65600 keys, 8 heads, 143 us: tensor pipe and
+// Bound, for many rows over a key, by the steps between products and softmax (512 rows x 65600 keys, 8 heads, 147 us: tensor pipe and
 // exponentials are at work half of the time each; 256 rows x 2100 keys, 16 sequences, 47 us); for few by the keys' bytes and some 4 us of a
 // CTA's start and end (8 rows x 1080 keys, 32 sequences of 32 heads, 509 MB, 92 us: 5.5 TB/s).
 //
