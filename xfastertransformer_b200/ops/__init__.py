@@ -435,7 +435,8 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
     """Attention of trees' nodes q [T, Hq, D] over the paged cache: a node sees the context before the tree and the nodes that its `mask`
     (int64 [T, words], see tree_mask; any other choice of nodes will do) has; one that sees nothing gives zeros.  Other arguments as in
     paged_attention; `window` counts in `positions` (int32 [T], needed with it).  A GPU takes bf16 queries over bf16 or int8 caches, D
-    64, 128 or 256.  Of keys that some node sees, the values are finite; what its mask and the window leave to no node may hold anything.  Rows of no sequence (of the lists) are zero."""
+    64, 128 or 256.  Of keys that some node sees, the values are finite; keys that masks and window leave to no node may hold anything.
+    Rows of no sequence (of the lists) are zero."""
     if q.dim() != 3 or kc.dim() != 4 or vc.shape != kc.shape or q.shape[2] != kc.shape[3]:
         raise ValueError(f"tree_attention: queries {tuple(q.shape)} over keys {tuple(kc.shape)} and values {tuple(vc.shape)}")
     T, hq, D = q.shape
