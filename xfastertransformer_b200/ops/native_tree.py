@@ -224,7 +224,7 @@ class CachePools:
     def retire(self):
         """The pools are replaced: lets them go.  `tree_accept` refuses the handle from now on, and a graph captured with it moves nothing."""
         self.retired, self.pools = True, []
-        self.table.zero_()                                               # no heads, rows of no bytes
+        self.table[:, 1:].zero_()                                        # no heads, rows of no bytes (a launch under way may still use an address)
 
 
 def tree_accept(tokens, parents, sampled, cu_q, kv_lens, block_table, pools, meta=None):
