@@ -126,3 +126,17 @@ def test_a_limit_of_any_size():
     want = ops.sample(x, 1.0, 0, 0.9, 0.01, u)
     for k in (50, 2 ** 31, 2 ** 63, 10 ** 30, -2 ** 63 - 1, -10 ** 30):          # a request's number may be any
         assert torch.equal(ops.sample(x, 1.0, k, 0.9, 0.01, u), want)
+
+
+def test_tables_of_replaced_pools_stay_for_the_graphs_that_read_them():
+    import gc
+    import weakref
+    from xfastertransformer_b200.runtime.kv_cache import PagedKVCache
+    c = PagedKVCache(2, 2, 8, 8, "bf16", torch.device("cpu"))
+    tables = []
+    for blocks in (2, 9, 30):
+        c.ensure_blocks(blocks)
+        tables.append(weakref.ref(c.pools().table))       # the program keeps none of the handles
+    gc.collect()
+    assert all(t() is not None for t in tables)
+    assert [bool(t()[:, 1:].any()) for t in tables] == [False, False, True]

@@ -170,6 +170,7 @@ class PagedKVCache:
         self.lens: Dict[int, int] = {}
         self.version = 0                         # bumped when pools are reallocated
         self._handle = None                      # of the present k, v, ks and vs, see pools()
+        self._retired = []                       # handles of pools that have been replaced: a captured graph may still read their tables
         self.prefix_index: Optional[PrefixIndex] = None      # set by the engine when automatic prefix reuse is on
         self.state_geometry = list(states)       # (shape of one slot, type) of every state pool
         self.max_states = max_states             # > 0: the state pools never grow past this many slots
@@ -246,6 +247,7 @@ class PagedKVCache:
         old = self.alloc.num_blocks
         if self._handle is not None:
             self._handle.retire()
+            self._retired.append(self._handle)
             self._handle = None
         mk = lambda H, d: torch.zeros(total, H, self.block, d, dtype=self.dtype, device=self.device)
         nk, nv, nks, nvs = [], [], [], []
