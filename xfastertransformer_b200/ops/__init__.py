@@ -479,9 +479,9 @@ def tree_attention(q, kc, vc, block_table, cu_q, kv_lens, mask, scale, ks=None, 
 def cache_pools(k, v=None, ks=None, vs=None):
     """The pools of all layers as `tree_accept` takes them: lists of keys and values [blocks, heads, block, D] (None or a None entry: a layer
     without) and of an int8 cache's scales [blocks, heads, block].  A pool that several layers read may be listed for each of them: its rows
-    move once.  Pools that overlap in another way are refused.  Made once, outside of a capture; it holds the pools,
-    belongs to them for as long as they stay where they are, and is kept as long as a graph that was captured with it.  (`PagedKVCache.pools` has the one of a cache, which `tree_accept` refuses once
-    the cache's pools have been replaced.)"""
+    move once.  Pools that overlap in another way are refused.  Made once, outside of a capture; it holds the pools, belongs to them for as
+    long as they stay where they are, and is kept as long as a graph that was captured with it.  (`PagedKVCache.pools` has the one of a
+    cache, which `tree_accept` refuses once the cache's pools have been replaced.)"""
     pools = [p for group in (k, v, ks, vs) for p in (group or []) if p is not None]
     if not pools:
         raise ValueError("cache_pools: no pools")
